@@ -21,10 +21,12 @@ from typing import Callable, Optional, Sequence
 import numpy as np
 
 from . import _lib
+from .operators import Q4Weight, attention_causal, attention_prefix, linear_q4
 
 __all__ = ["EmbeddingModel", "EmbedOptions", "LoadOptions", "ImageEmbedOptions", "MultimodalEmbedOptions", "AudioEmbedOptions",
            "AudioInput", "audio_tokens", "audio_to_mono16k", "decode_wav", "Embedding",
-           "EmbeddingProgress", "ModelInfo", "GemmaEmbedError", "TaskPrefix", "Tokenizer", "ALLOWED_DIMENSIONS"]
+           "EmbeddingProgress", "ModelInfo", "GemmaEmbedError", "TaskPrefix", "Tokenizer", "ALLOWED_DIMENSIONS",
+           "attention_causal", "attention_prefix", "linear_q4", "Q4Weight"]
 
 ALLOWED_DIMENSIONS = (768, 512, 256, 128)
 

@@ -75,6 +75,13 @@ class GeInfo(ctypes.Structure):
                                       "audio_projection_dim")] + [("graph_captures", ctypes.c_int64)]
 
 
+class GeAttentionShape(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int32) for n in ("dtype", "heads", "kv_heads", "head_dim")] + [
+        ("scale", ctypes.c_float), ("window", ctypes.c_int32)] + [
+        (n, ctypes.c_int64) for n in ("q_stride", "k_stride", "v_stride", "prefix_k_stride", "prefix_v_stride",
+                                      "out_stride")]
+
+
 class GeKernelTime(ctypes.Structure):
     _fields_ = [("name", ctypes.c_char * 32), ("ms_per_launch", ctypes.c_double), ("flops_per_launch", ctypes.c_double),
                 ("bytes_per_launch", ctypes.c_double), ("launches_per_forward", ctypes.c_int32)]
@@ -105,6 +112,19 @@ SIGNATURES = {
                     ctypes.c_int32, i32p], ctypes.c_int),
     "ge_pool_head_noalloc": ([ctypes.c_void_p, ctypes.c_int32, ctypes.c_void_p, ctypes.c_int32, ctypes.c_void_p,
                               ctypes.c_int32, ctypes.c_void_p, ctypes.c_void_p], ctypes.c_int),
+    "ge_attention_workspace": ([ctypes.c_int32, P(GeAttentionShape), ctypes.c_int32, ctypes.c_int32, i64p], ctypes.c_int),
+    "ge_attention_causal": ([ctypes.c_int32, P(GeAttentionShape)] + [ctypes.c_void_p] * 3 + [
+        ctypes.c_int32, ctypes.c_void_p, ctypes.c_int32, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p],
+        ctypes.c_int),
+    "ge_attention_prefix": ([ctypes.c_int32, P(GeAttentionShape), ctypes.c_void_p, ctypes.c_int32, ctypes.c_void_p,
+                             ctypes.c_void_p, ctypes.c_int32, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int32,
+                             ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int32, ctypes.c_void_p, ctypes.c_void_p,
+                             ctypes.c_int64, ctypes.c_void_p], ctypes.c_int),
+    "ge_q4_repack": ([P(ctypes.c_uint8), ctypes.c_int32, ctypes.c_int64, ctypes.c_int64, P(ctypes.c_uint8), u16p, u16p],
+                     ctypes.c_int),
+    "ge_linear_q4": ([ctypes.c_int32, ctypes.c_int32, ctypes.c_void_p, ctypes.c_int64, ctypes.c_int32, ctypes.c_int32,
+                      ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int32, ctypes.c_int32, ctypes.c_void_p,
+                      ctypes.c_int64, ctypes.c_void_p], ctypes.c_int),
     "ge_batches": ([i64p, ctypes.c_int32, ctypes.c_int32, ctypes.c_int32, i64p, i32p, i32p], ctypes.c_int),
     "ge_finish": ([f32p, ctypes.c_int32, ctypes.c_int32, ctypes.c_int32, f32p], ctypes.c_int),
     "ge_tokenizer_load": ([ctypes.c_char_p, P(ctypes.c_void_p)], ctypes.c_int),

@@ -48,6 +48,17 @@ namespace {
 
 thread_local std::string t_last_error;
 
+}  // namespace
+
+namespace ge {
+int set_thread_error(int code, const std::string& msg) {
+    t_last_error = msg;
+    return code;
+}
+}  // namespace ge
+
+namespace {
+
 // Checks that `seqs` tile [0, ntok) in order with lengths 1..max_tokens, that every id is a
 // token of the vocabulary (negative ids are the reference's vector rows, which only the image
 // and audio towers produce) and that positions index the RoPE table.

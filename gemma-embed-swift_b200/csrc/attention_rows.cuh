@@ -1,0 +1,89 @@
+// attention_rows.cuh -- one attention row of ge_attention_causal / ge_attention_prefix by one warp,
+// straight from the definition: lane l holds dims [l * D / 32, (l + 1) * D / 32) of the row, and the
+// running maximum m (log2 units), sum l and unnormalised output of a softmax are kept in fp32
+// over one key at a time.  It reads the visible keys and values only, so nothing a masked place
+// holds can reach the row.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <stdint.h>
+
+#include "ptx.cuh"
+
+namespace ge {
+
+template <typename T>
+__device__ __forceinline__ float2 pair_to_float(uint32_t u);
+template <>
+__device__ __forceinline__ float2 pair_to_float<__half>(uint32_t u) {
+    return __half22float2(*reinterpret_cast<const __half2*>(&u));
+}
+template <>
+__device__ __forceinline__ float2 pair_to_float<__nv_bfloat16>(uint32_t u) {
+    return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&u));
+}
+template <typename T>
+__device__ __forceinline__ uint32_t float_to_pair(float a, float b);
+template <>
+__device__ __forceinline__ uint32_t float_to_pair<__half>(float a, float b) {
+    return pack_half2(a, b);
+}
+template <>
+__device__ __forceinline__ uint32_t float_to_pair<__nv_bfloat16>(float a, float b) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+template <int D>
+struct RowState {
+    static constexpr int kPer = D / 32;  // dims of one lane
+    float q[kPer], o[kPer], m, l;
+};
+
+template <typename T, int D>
+__device__ __forceinline__ void row_load(const T* p, int lane, float (&x)[D / 32]) {
+    const uint32_t* w = reinterpret_cast<const uint32_t*>(p + lane * (D / 32));
+#pragma unroll
+    for (int i = 0; i < D / 64; i++) {
+        const float2 f = pair_to_float<T>(w[i]);
+        x[2 * i] = f.x;
+        x[2 * i + 1] = f.y;
+    }
+}
+
+// q is the row's query; the state starts empty (m = -inf).
+template <typename T, int D>
+__device__ __forceinline__ void row_begin(RowState<D>& s, const T* q, int lane) {
+    row_load<T, D>(q, lane, s.q);
+#pragma unroll
+    for (int i = 0; i < D / 32; i++) s.o[i] = 0.f;
+    s.m = -INFINITY;
+    s.l = 0.f;
+}
+
+// Adds keys [0, n) at k, v (rows `k_stride`, `v_stride` elements apart).
+template <typename T, int D>
+__device__ void row_keys(RowState<D>& s, const T* k, const T* v, int64_t k_stride, int64_t v_stride, int n,
+                         float scale_log2e, int lane) {
+    for (int j = 0; j < n; j++) {
+        float x[D / 32];
+        row_load<T, D>(k + int64_t(j) * k_stride, lane, x);
+        float d = 0.f;
+#pragma unroll
+        for (int i = 0; i < D / 32; i++) d = fmaf(s.q[i], x[i], d);
+        d = warp_sum(d) * scale_log2e;
+        const float m = fmaxf(s.m, d);
+        const float alpha = s.m == m ? 1.0f : ex2_approx(s.m - m);
+        // A score of -inf under a finite maximum weighs 0; with no finite score yet it counts
+        // nothing either (m stays -inf).
+        const float p = m == -INFINITY ? 0.f : ex2_approx(d - m);
+        row_load<T, D>(v + int64_t(j) * v_stride, lane, x);
+        s.l = fmaf(s.l, alpha, p);
+#pragma unroll
+        for (int i = 0; i < D / 32; i++) s.o[i] = fmaf(s.o[i], alpha, p * x[i]);
+        s.m = isnan(d) ? d : m;
+    }
+}
+
+}  // namespace ge

@@ -286,4 +286,6 @@ void store_graph(Device& d, const GraphKey& k, cudaGraphExec_t exec, int64_t lau
 bool seen_before(Device& d, const GraphKey& k);
 void clear_graphs(Device& d);
 int set_error(ge_model* m, int code, const std::string& msg);
+// The message ge_last_error(NULL) gives the calling thread (calls without a model); returns `code`.
+int set_thread_error(int code, const std::string& msg);
 }  // namespace ge

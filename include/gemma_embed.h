@@ -482,6 +482,79 @@ GE_API int ge_embed_multimodal(ge_model* model, const ge_multimodal_input* input
 GE_API int ge_pool_head_noalloc(ge_model* model, int32_t device_ordinal, const float* d_hidden, int32_t ntok,
                                 const uint32_t* d_seqs, int32_t nseq, float* d_out, void* stream);
 
+/* ---- Operators on device tensors (no counterpart in the reference) -------------------------
+ *
+ * Building blocks of an embedding tower with a causal mask, and of single queries, beside the
+ * bidirectional forward above.  They need no model: every pointer is a device pointer of
+ * `device_ordinal` unless said otherwise, work is enqueued on `stream` (a cudaStream_t; NULL is the
+ * legacy default stream) without synchronising, and nothing is allocated or kept between calls, so
+ * calls may be captured into CUDA graphs.  The calling thread's current device is left as it was.
+ * Messages of failed calls come from ge_last_error(NULL) on the calling thread. */
+
+typedef enum ge_dtype { GE_F16 = 0, GE_BF16 = 1 } ge_dtype;
+
+/* The layout of an attention call: token-major rows, heads of head_dim values side by side in a row
+ * (a row may be a column range of a wider one, as of a fused projection). */
+typedef struct ge_attention_shape {
+    int32_t dtype;     /* ge_dtype of every tensor */
+    int32_t heads;     /* query heads, a multiple of kv_heads (at most 128 times) */
+    int32_t kv_heads;
+    int32_t head_dim;  /* 64, 128 or 256 */
+    float scale;       /* of q . k, positive and finite */
+    int32_t window;    /* ge_attention_causal: keys a query sees, itself included; 0: all before it */
+    /* Elements between rows, multiples of 8; every tensor starts on a 16-byte boundary. */
+    int64_t q_stride, k_stride, v_stride, prefix_k_stride, prefix_v_stride, out_stride;
+} ge_attention_shape;
+
+/* Bytes of device workspace the attention calls below need for `ntok` query rows behind a prefix of
+ * `prefix_len` rows (0 for ge_attention_causal).  The workspace must be 256-byte aligned; what it
+ * holds is free again once the call's work has completed, and calls that may overlap on the GPU
+ * (other streams, captured graphs replayed at the same time) need one each. */
+GE_API int ge_attention_workspace(int32_t device_ordinal, const ge_attention_shape* shape, int32_t ntok,
+                                  int32_t prefix_len, int64_t* bytes);
+
+/* Causal attention over packed prompts: for row i of a sequence, out[i] = sum_j softmax_j(scale
+ * q[i] . k[j]) v[j] over the rows j <= i of its sequence (j > i - window under a window), head h
+ * reading KV head h / (heads / kv_heads).  q and out are [ntok][heads][head_dim], k and v
+ * [ntok][kv_heads][head_dim]; d_seqs holds nseq (start, length) pairs on the device.  Ranges are cut
+ * at ntok, empty ones are allowed, ranges that share rows are not (their rows hold one or the
+ * other); rows of `out` in no range are left as they were.  Scores, sums and maxima are fp32,
+ * probabilities are rounded to dtype before their product with v, the result once to dtype. */
+GE_API int ge_attention_causal(int32_t device_ordinal, const ge_attention_shape* shape, const void* d_q, const void* d_k,
+                               const void* d_v, int32_t ntok, const uint32_t* d_seqs, int32_t nseq, void* d_out,
+                               void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Attention of texts behind one shared prefix, whose keys and values exist once: every query sees
+ * all prefix_len rows of d_prefix_k / d_prefix_v, and the keys of its own sequence up to its place.
+ * Sequence s has the query rows d_q_seqs[s] = (start, n) of q (ntok rows) and the key rows
+ * d_kv_seqs[s] = (start, m) of k and v (nkv rows); the queries stand at the end, so query i sees the
+ * own keys j <= m - n + i (none where that is negative).  n = 1 is the step of a single token.
+ * Key ranges may be shared, in any order (fastest in the order of the queries).  A row that sees no
+ * key at all gives zeros.  Otherwise as ge_attention_causal; a window is refused. */
+GE_API int ge_attention_prefix(int32_t device_ordinal, const ge_attention_shape* shape, const void* d_q, int32_t ntok,
+                               const void* d_k, const void* d_v, int32_t nkv, const void* d_prefix_k,
+                               const void* d_prefix_v, int32_t prefix_len, const uint32_t* d_q_seqs,
+                               const uint32_t* d_kv_seqs, int32_t nseq, void* d_out, void* workspace,
+                               int64_t workspace_bytes, void* stream);
+
+typedef enum ge_q4_type { GE_Q4_0 = 2, GE_Q4_1 = 3 } ge_q4_type; /* the GGUF tensor type ids */
+
+/* Splits n rows of k 4-bit weights as a GGUF file stores them (blocks of 32: Q4_0 18 bytes, Q4_1 20)
+ * into the planes ge_linear_q4 reads with group 32, all on the host: values [n][k / 2], scales and
+ * (Q4_1) mins [n][k / 32] fp16.  Host code only. */
+GE_API int ge_q4_repack(const uint8_t* blocks, int32_t type, int64_t n, int64_t k, uint8_t* values, uint16_t* scales,
+                        uint16_t* mins);
+
+/* A linear layer over a few rows (0 .. 64) with 4-bit weights: out[r][i] = sum_j x[r][j] w[i][j],
+ * where w[i][j] = scale (q - 8) without d_mins and scale q + min with it, q the 4-bit value (element
+ * 2 j in the low half of byte j) and scale and min those of group j / group (32, 64 or 128 weights).
+ * x is [rows][k] of `dtype` (16-byte aligned, row stride a multiple of 8), d_values [n][k / 2]
+ * (16-byte aligned), d_scales and d_mins [n][k / group] fp16, out [rows][n] of `dtype`.  Sums are
+ * fp32 over exact products, the result is rounded once.  k is a multiple of group, at most 65536. */
+GE_API int ge_linear_q4(int32_t device_ordinal, int32_t dtype, const void* d_x, int64_t x_stride, int32_t rows, int32_t k,
+                        const uint8_t* d_values, const uint16_t* d_scales, const uint16_t* d_mins, int32_t group,
+                        int32_t n, void* d_out, int64_t out_stride, void* stream);
+
 /* EmbeddingModel.batches (EmbeddingModel.swift:200-215): splits `n` items with `ncost` costs
  * each (row-major costs[n][ncost]) into consecutive ranges, by count when batch_size > 0,
  * otherwise before the item that would take any summed cost past its budget.  Writes

@@ -1,0 +1,161 @@
+"""Operators on device tensors, what needs no GPU: refusals of the C entry points (every argument is
+checked before a device is touched) and the repacking of GGUF's 4-bit blocks."""
+import ctypes
+import importlib
+
+import numpy as np
+import pytest
+
+FAKE = 1 << 20  # a pointer that is never followed: the calls below are refused, or have no rows
+
+
+@pytest.fixture(scope="module")
+def lib(ge):
+    return importlib.import_module("gemma-embed-swift_b200._lib")
+
+
+def shape(lib, **over):
+    s = lib.GeAttentionShape()
+    base = dict(dtype=0, heads=4, kv_heads=2, head_dim=64, scale=0.125, window=0, q_stride=256, k_stride=128, v_stride=128,
+                prefix_k_stride=128, prefix_v_stride=128, out_stride=256)
+    for n, v in {**base, **over}.items():
+        setattr(s, n, v)
+    return s
+
+
+def causal(lib, s, **over):
+    a = dict(q=FAKE, k=FAKE, v=FAKE, ntok=8, seqs=FAKE, nseq=1, out=FAKE, ws=FAKE, nbytes=1 << 30)
+    a.update(over)
+    L = lib.lib()
+    rc = L.ge_attention_causal(0, ctypes.byref(s), a["q"], a["k"], a["v"], a["ntok"], a["seqs"], a["nseq"], a["out"],
+                               a["ws"], a["nbytes"], None)
+    return rc, (L.ge_last_error(None) or b"").decode()
+
+
+def prefix(lib, s, **over):
+    a = dict(q=FAKE, ntok=8, k=FAKE, v=FAKE, nkv=8, pk=FAKE, pv=FAKE, plen=4, qs=FAKE, ks=FAKE, nseq=1, out=FAKE, ws=FAKE,
+             nbytes=1 << 30)
+    a.update(over)
+    L = lib.lib()
+    rc = L.ge_attention_prefix(0, ctypes.byref(s), a["q"], a["ntok"], a["k"], a["v"], a["nkv"], a["pk"], a["pv"], a["plen"],
+                               a["qs"], a["ks"], a["nseq"], a["out"], a["ws"], a["nbytes"], None)
+    return rc, (L.ge_last_error(None) or b"").decode()
+
+
+@pytest.mark.parametrize("over", [
+    dict(dtype=2), dict(dtype=-1), dict(head_dim=96), dict(head_dim=0), dict(heads=5), dict(heads=0), dict(kv_heads=0),
+    dict(heads=-4, kv_heads=-2), dict(heads=258, kv_heads=2), dict(heads=65536 * 2, kv_heads=2), dict(scale=0.0),
+    dict(scale=-1.0), dict(scale=float("nan")), dict(scale=float("inf")), dict(window=-1), dict(q_stride=248),
+    dict(q_stride=260), dict(k_stride=64), dict(v_stride=0), dict(out_stride=257), dict(q_stride=1 << 40)])
+def test_attention_refuses_bad_shapes(lib, over):
+    rc, msg = causal(lib, shape(lib, **over))
+    assert rc == 9 and msg.startswith("invalid options: ")
+
+
+@pytest.mark.parametrize("over", [dict(q=None), dict(k=None), dict(v=None), dict(out=None), dict(seqs=None), dict(seqs=FAKE + 2),
+                                  dict(q=FAKE + 2), dict(k=FAKE + 8), dict(v=FAKE + 4), dict(out=FAKE + 2), dict(ntok=-1),
+                                  dict(nseq=-1), dict(ntok=(1 << 30) + 1)])
+def test_causal_refuses_bad_arguments(lib, over):
+    rc, msg = causal(lib, shape(lib), **over)
+    assert rc == 9 and msg.startswith("invalid options: ")
+
+
+@pytest.mark.parametrize("over", [dict(q=None), dict(pk=None), dict(pv=None), dict(pk=FAKE + 2), dict(pv=FAKE + 8), dict(k=None),
+                                  dict(qs=None), dict(ks=None), dict(ks=FAKE + 1), dict(plen=-1), dict(nkv=-1), dict(ntok=-2),
+                                  dict(plen=(1 << 30) + 1)])
+def test_prefix_refuses_bad_arguments(lib, over):
+    rc, msg = prefix(lib, shape(lib), **over)
+    assert rc == 9 and msg.startswith("invalid options: ")
+
+
+def test_prefix_refuses_a_window(lib):
+    rc, msg = prefix(lib, shape(lib, window=16))
+    assert rc == 9 and "window" in msg
+
+
+def test_null_shape_is_refused(lib):
+    L = lib.lib()
+    assert L.ge_attention_causal(0, None, FAKE, FAKE, FAKE, 8, FAKE, 1, FAKE, FAKE, 1 << 30, None) == 9
+    n = ctypes.c_int64(0)
+    assert L.ge_attention_workspace(0, None, 8, 0, ctypes.byref(n)) == 9
+    assert L.ge_attention_workspace(0, ctypes.byref(shape(lib)), 8, 0, None) == 9
+    assert L.ge_attention_workspace(0, ctypes.byref(shape(lib)), -1, 0, ctypes.byref(n)) == 9
+
+
+def test_calls_without_rows_do_nothing(lib):
+    """No rows or no sequences: accepted with whatever pointers, and no device is touched."""
+    assert causal(lib, shape(lib), ntok=0, q=None, k=None, v=None, out=None)[0] == 0
+    assert causal(lib, shape(lib), nseq=0, seqs=None)[0] == 0
+    assert prefix(lib, shape(lib), ntok=0, q=None, out=None)[0] == 0
+    assert lib.lib().ge_linear_q4(0, 0, None, 32, 0, 32, None, None, None, 32, 8, None, 8, None) == 0
+    assert lib.lib().ge_linear_q4(0, 0, None, 32, 1, 32, None, None, None, 32, 0, None, 8, None) == 0
+
+
+@pytest.mark.parametrize("over", [
+    dict(dtype=2), dict(rows=-1), dict(rows=65), dict(group=16), dict(group=0), dict(k=48), dict(k=0), dict(k=65536 + 32),
+    dict(n=-1), dict(x=None), dict(values=None), dict(scales=None), dict(out=None), dict(x=FAKE + 8), dict(values=FAKE + 4),
+    dict(scales=FAKE + 1), dict(mins=FAKE + 1), dict(out=FAKE + 1), dict(x_stride=56), dict(x_stride=68), dict(out_stride=7)])
+def test_linear_q4_refuses_bad_arguments(lib, over):
+    a = dict(dtype=0, x=FAKE, x_stride=64, rows=2, k=64, values=FAKE, scales=FAKE, mins=None, group=32, n=8, out=FAKE, out_stride=8)
+    a.update(over)
+    L = lib.lib()
+    rc = L.ge_linear_q4(0, a["dtype"], a["x"], a["x_stride"], a["rows"], a["k"], a["values"], a["scales"], a["mins"], a["group"],
+                        a["n"], a["out"], a["out_stride"], None)
+    assert rc == 9 and (L.ge_last_error(None) or b"").startswith(b"invalid options: ")
+
+
+def repack(lib, blocks, kind, n, k):
+    values, scales, mins = np.zeros((n, k // 2), np.uint8), np.zeros((n, k // 32), np.uint16), np.zeros((n, k // 32), np.uint16)
+    u8, u16 = ctypes.POINTER(ctypes.c_uint8), ctypes.POINTER(ctypes.c_uint16)
+    rc = lib.lib().ge_q4_repack(blocks.ctypes.data_as(u8), kind, n, k, values.ctypes.data_as(u8), scales.ctypes.data_as(u16),
+                                mins.ctypes.data_as(u16))
+    assert rc == 0
+    return values, scales, mins
+
+
+@pytest.mark.parametrize("kind,per", [(2, 18), (3, 20)])
+@pytest.mark.parametrize("n,k", [(1, 32), (3, 96), (5, 256)])
+def test_q4_repack_matches_the_block_layout(lib, kind, per, n, k):
+    """GGUF's Q4_0 (fp16 scale, 16 bytes) and Q4_1 (scale, min, 16 bytes) blocks: byte j holds elements j and
+    j + 16 of the block."""
+    rng = np.random.default_rng(n * k + kind)
+    blocks = rng.integers(0, 256, (n, k // 32, per), dtype=np.uint8)
+    values, scales, mins = repack(lib, np.ascontiguousarray(blocks), kind, n, k)
+    assert np.array_equal(scales, blocks[..., :2].copy().view(np.uint16)[..., 0])
+    if kind == 3:
+        assert np.array_equal(mins, blocks[..., 2:4].copy().view(np.uint16)[..., 0])
+    q = blocks[..., per - 16:]
+    want = np.concatenate([q & 15, q >> 4], -1).reshape(n, k)
+    got = np.stack([values & 15, values >> 4], -1).reshape(n, k)
+    assert np.array_equal(got, want)
+
+
+def test_q4_repack_refusals(lib):
+    u8, u16 = ctypes.POINTER(ctypes.c_uint8), ctypes.POINTER(ctypes.c_uint16)
+    b = np.zeros(64, np.uint8)
+    p8, p16 = b.ctypes.data_as(u8), b.ctypes.data_as(u16)
+    call = lib.lib().ge_q4_repack
+    assert call(p8, 8, 1, 32, p8, p16, None) == 3  # Q8_0
+    assert call(p8, 2, 1, 31, p8, p16, None) == 9
+    assert call(p8, 2, -1, 32, p8, p16, None) == 9
+    assert call(p8, 3, 1, 32, p8, p16, None) == 9  # Q4_1 without room for the mins
+    assert call(None, 2, 1, 32, p8, p16, None) == 9
+    assert call(None, 2, 0, 32, None, None, None) == 0
+
+
+def test_python_wrappers_refuse_host_tensors(ge):
+    import torch
+    q = torch.zeros(4, 2, 64, dtype=torch.float16)
+    seqs = torch.zeros(1, 2, dtype=torch.int32)
+    for call in (lambda: ge.attention_causal(q, q, q, seqs), lambda: ge.attention_prefix(q, q, q, seqs, seqs, q, q),
+                 lambda: ge.Q4Weight(torch.zeros(4, 16, dtype=torch.uint8), torch.zeros(4, 1, dtype=torch.float16)),
+                 lambda: ge.attention_prefix(q, q, q, seqs, seqs, None, None)):
+        with pytest.raises(ge.GemmaEmbedError) as e:
+            call()
+        assert e.value.case == "invalidOptions"
+    with pytest.raises(ge.GemmaEmbedError) as e:
+        ge.Q4Weight.from_blocks(b"", "Q8_0", 1, 32)
+    assert e.value.case == "unsupportedTensorType"
+    with pytest.raises(ge.GemmaEmbedError) as e:
+        ge.Q4Weight.from_blocks(b"\0" * 17, "Q4_0", 1, 32)
+    assert e.value.case == "invalidOptions"
