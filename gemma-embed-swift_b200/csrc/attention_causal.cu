@@ -1,12 +1,43 @@
 // attention_causal.cu -- ge_attention_causal and ge_attention_prefix: attention of query rows over a
-// shared prefix and over their own sequences' keys up to their own place.
+// shared prefix and over their own sequences' keys up to their own place, on the tensor cores.
 //
 // Every query row r reduces to a pair of key ranges: the prefix rows [0, P), the same for every row,
 // and its own key rows [lo(r), hi(r)):
 //   query i of n in a sequence whose own keys are rows [s, s + m):  hi = s + m - n + i + 1 (cut to
 //   [s, s + m]), lo = s, or max(s, hi - window) under a window.
-// A causal prompt is the case P = 0, m = n.  k_causal_ranges writes (lo, hi) per query row to the
-// workspace, (0, -1) for rows of no sequence, which are never stored.
+// A causal prompt is the case P = 0, m = n.  With that, sequences need no tiles of their own: a tile is
+// T = 128 / G consecutive query rows (G = heads / KV heads) with all G heads that read one KV head, row
+// t * G + g of its 128, whatever sequences its rows belong to.  Short texts fill a tile together, and
+// the prefix' tiles serve the rows of many sequences at once.
+//
+// Three kernels, each waiting for the one before (programmatic dependent launch):
+//   k_causal_plan   one CTA: (lo, hi) per row, per tile the disjoint key segments its rows see, and the
+//                   list of work pieces, costliest first.  When the tiles of all KV heads do not fill
+//                   the GPU, a tile's key blocks are cut into pieces that do.
+//   k_causal_tc     persistent, one CTA per SM: walks the pieces in turn (below)
+//   k_causal_merge  only where tiles were cut: joins the pieces' partial rows by their maxima and sums
+// The result of a row depends only on its own ranges and, through the pieces, on the call's sizes:
+// which CTA takes a piece changes nothing.
+//
+// k_causal_tc.  A work item is NT = 2 neighbouring tiles (head dims 64, 128; NT = 1 for 256, whose O
+// takes half of tensor memory), one KV head and a run of key blocks of 128, each K and V tile serving
+// both tiles' products.  Per tile x and block j: S = Q K^T (128 x 128, fp32 in tensor memory); a warpgroup
+// per tile, one thread per row, turns S into P = 2^(S scale log2e - m) in 16 bits, written over S; O += P V
+// (fp32 in tensor memory).  One warp issues every product, in the order PV_0(j - 1), S_0(j), PV_1(j - 1),
+// S_1(j), so that one tile's softmax runs under the other tile's products; head dim 256 has two S
+// buffers instead and runs S(j) ahead of PV(j - 1).  The running maximum of a row is moved (and its O
+// rescaled) only when it grows by more than 2^8; until then every term of the row shares the old one, so
+// the result is exact and P stays within 2^8.  P in 16 bits is the operand the product takes; sums are
+// taken over the unrounded fp32 values.
+//   warp 0   TMA producer of Q and K      warp 1   MMA issuer
+//   warp 2   TMA producer of V            warp 3   owns tensor memory
+//   warps 4-7 (and 8-11 for tile 1)       softmax, then O / l to the output (or the partial rows)
+// K and V blocks come in boxes of 32 rows, so a short segment loads few rows it does not need; rows of
+// the V block past its last key, up to the product's step of 16, are zeroed, so whatever lies behind a
+// segment never meets the product.  Keys masked for some rows of a tile only (later tokens, other
+// sequences) do meet it, with P = 0: where their values are infinite or NaN, 0 x V leaves NaN in rows that
+// must not see it, and the epilogue recomputes rows with non-finite outputs from the definition
+// (attention_rows.cuh), key by key.
 #include <algorithm>
 
 #include "attention_rows.cuh"
@@ -17,92 +48,910 @@ namespace ge {
 namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kGrow = 8.0f;  // log2 units a row's maximum may grow before it is moved
+constexpr int kKeys = 128;     // keys of a block
+constexpr int kMaxPieces = 64;
+constexpr int kBuckets = 1024;
 
-struct RangeParams {
-    const uint32_t* q_seqs;
-    const uint32_t* kv_seqs;
-    int nseq, ntok, nkv, window;
-    int2* rng;
+// ------------------------------------------------------------------------------------ sizes
+constexpr int tiles_per_item(int hd) { return hd == 256 ? 1 : 2; }
+
+struct Sizes {
+    int group, T, TI, tiles, lmax;  // TI = rows of an item
+};
+Sizes sizes_of(const CausalLaunch& a) {
+    Sizes s;
+    s.group = a.heads / a.kv_heads;
+    s.T = 128 / s.group;
+    s.TI = s.T * tiles_per_item(a.hd);
+    s.tiles = (a.ntok + s.TI - 1) / s.TI;
+    // Pieces a tile may be cut into: enough for two rounds of the SMs, one where the tiles fill them.
+    const int64_t units = std::max<int64_t>(int64_t(s.tiles) * a.kv_heads, 1);
+    s.lmax = units >= a.num_sms ? 1 : int(std::min<int64_t>(kMaxPieces, (2 * a.num_sms + units - 1) / units));
+    return s;
+}
+
+struct Header {
+    int err;    // a wait that gave up
+    int nwork;  // pieces in the work list
+};
+struct TileInfo {
+    int nblk, nseg, pieces, live;  // key blocks, own-key segments, pieces; bit x: tile x has rows of a sequence
+    int lo0, hi0, lo1, hi1;        // per tile the hull of its rows' own keys
+};
+struct Work {
+    int tile, b0, b1, piece;    // blocks [b0, b1) of the tile; piece -1: the whole tile, straight to the output
+    int seg, pos, nseg, live;   // where b0's own keys start
 };
 
-__global__ void __launch_bounds__(1024) k_causal_ranges(RangeParams p) {
+struct Layout {
+    Header* head;
+    int2 *rng, *segs;
+    TileInfo* info;
+    Work* work;
+    float* o;    // [piece][row][head][hd]
+    float2* ml;  // [piece][row][head]: maximum (log2 units), sum
+    size_t bytes;
+};
+Layout layout_of(const CausalLaunch& a, const Sizes& s) {
+    Layout l;
+    size_t at = 0;
+    const auto take = [&](size_t n) {
+        char* p = static_cast<char*>(a.workspace) + at;
+        at += (n + 255) / 256 * 256;
+        return p;
+    };
+    l.head = reinterpret_cast<Header*>(take(sizeof(Header)));
+    l.rng = reinterpret_cast<int2*>(take(size_t(a.ntok) * sizeof(int2)));
+    l.segs = reinterpret_cast<int2*>(take(size_t(s.tiles) * s.TI * sizeof(int2)));
+    l.info = reinterpret_cast<TileInfo*>(take(size_t(s.tiles) * sizeof(TileInfo)));
+    // With pieces, (pieces of all tiles) x (KV heads) stays within the SMs (k_causal_plan).
+    l.work = reinterpret_cast<Work*>(take(size_t(std::max(s.tiles, s.lmax > 1 ? a.num_sms : 0)) * sizeof(Work)));
+    const size_t part = s.lmax > 1 ? size_t(s.lmax) * a.ntok * a.heads : 0;
+    l.ml = reinterpret_cast<float2*>(take(part * sizeof(float2)));
+    l.o = reinterpret_cast<float*>(take(part * a.hd * sizeof(float)));
+    l.bytes = at;
+    return l;
+}
+
+// ------------------------------------------------------------------------------------ plan
+struct PlanParams {
+    const uint32_t* q_seqs;
+    const uint32_t* kv_seqs;
+    int nseq, ntok, nkv, window, T, TI, tiles, kv_heads, prefix_blocks, lmax, sms;
+    Header* head;
+    int2 *rng, *segs;
+    TileInfo* info;
+    Work* work;
+};
+
+__device__ __forceinline__ int warp_max_i(int v) { return __reduce_max_sync(0xffffffffu, v); }
+__device__ __forceinline__ int warp_min_i(int v) { return __reduce_min_sync(0xffffffffu, v); }
+
+__global__ void __launch_bounds__(1024) k_causal_plan(PlanParams p) {
+    __shared__ int hist[kBuckets], warp_sum_s[32];
+    __shared__ int s_max, s_chunk;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     pdl_wait();
-    for (int r = threadIdx.x; r < p.ntok; r += blockDim.x) p.rng[r] = make_int2(0, -1);
+    pdl_launch();
+    if (tid == 0) {
+        p.head->err = 0;
+        s_max = 0;
+    }
+    hist[tid] = 0;
+    // (lo, hi) per row; (0, -1) for rows of no sequence, which are never stored.
+    for (int r = tid; r < p.ntok; r += blockDim.x) p.rng[r] = make_int2(0, -1);
     __syncthreads();
-    for (int s = threadIdx.x >> 5; s < p.nseq; s += int(blockDim.x >> 5)) {
+    for (int s = warp; s < p.nseq; s += 32) {
         const int64_t q0 = p.q_seqs[2 * s], n = p.q_seqs[2 * s + 1];
         const int64_t k0 = p.kv_seqs[2 * s], m = p.kv_seqs[2 * s + 1];
         // Ranges past the tensors are cut; a key range that starts outside holds no key.
         const int64_t q1 = min(q0 + n, int64_t(p.ntok));
         const int64_t ks = min(k0, int64_t(p.nkv)), ke = min(k0 + m, int64_t(p.nkv));
-        for (int64_t r = q0 + (threadIdx.x & 31); r < q1; r += 32) {
+        for (int64_t r = q0 + lane; r < q1; r += 32) {
             const int64_t see = k0 + m - n + (r - q0) + 1;
             const int64_t hi = max(ks, min(see, ke));
             const int64_t lo = p.window > 0 ? min(hi, max(ks, see - p.window)) : ks;
             p.rng[r] = make_int2(int(lo), int(hi));
         }
     }
+    __syncthreads();
+    // Per tile: its rows' own keys as disjoint ascending segments, when the rows' ranges come in
+    // ascending order (lo never falls); else one segment over all of them, the masks doing the rest.
+    for (int t = warp; t < p.tiles; t += 32) {
+        int2* seg = p.segs + int64_t(t) * p.TI;
+        int lo_x[2] = {INT_MAX, INT_MAX}, hi_x[2] = {0, 0}, live = 0;
+        int end = -1, low = -1, nseg = 0;  // running maximum of hi and lo over the rows so far
+        bool sorted = true;
+        for (int i0 = 0; i0 < p.TI; i0 += 32) {
+            const int i = i0 + lane, r = t * p.TI + i;
+            const int2 rg = i < p.TI && r < p.ntok ? p.rng[r] : make_int2(0, -1);
+            const bool in = rg.y >= 0, some = rg.y > rg.x;
+            const int x = i >= p.T ? 1 : 0;
+#pragma unroll
+            for (int y = 0; y < 2; y++) {
+                lo_x[y] = min(lo_x[y], warp_min_i(some && x == y ? rg.x : INT_MAX));
+                hi_x[y] = max(hi_x[y], warp_max_i(some && x == y ? rg.y : 0));
+                if (__any_sync(0xffffffffu, in && x == y)) live |= 1 << y;
+            }
+            // Inclusive running maxima over the lanes, then those of the rows before each lane's.
+            int e = some ? rg.y : -1, l = some ? rg.x : -1;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int pe = __shfl_up_sync(0xffffffffu, e, o), pl = __shfl_up_sync(0xffffffffu, l, o);
+                if (lane >= o) {
+                    e = max(e, pe);
+                    l = max(l, pl);
+                }
+            }
+            int be = __shfl_up_sync(0xffffffffu, e, 1), bl = __shfl_up_sync(0xffffffffu, l, 1);
+            be = lane ? max(be, end) : end;
+            bl = lane ? max(bl, low) : low;
+            if (__any_sync(0xffffffffu, some && rg.x < bl)) sorted = false;
+            const bool fresh = some && rg.x > be;  // keys between be and lo are no row's
+            const unsigned fm = __ballot_sync(0xffffffffu, fresh);
+            if (fresh) {
+                const int at = nseg + __popc(fm & ((1u << lane) - 1));
+                seg[at].x = rg.x;
+                if (at > 0) seg[at - 1].y = be;
+            }
+            nseg += __popc(fm);
+            end = max(end, __shfl_sync(0xffffffffu, e, 31));
+            low = max(low, __shfl_sync(0xffffffffu, l, 31));
+        }
+        __syncwarp();
+        if (!sorted) {
+            nseg = 1;
+            if (lane == 0) seg[0] = make_int2(min(lo_x[0], lo_x[1]), max(hi_x[0], hi_x[1]));
+        } else if (nseg > 0 && lane == 0) {
+            seg[nseg - 1].y = end;
+        }
+        __syncwarp();
+        int nblk = 0;
+        for (int i = lane; i < nseg; i += 32) nblk += (seg[i].y - seg[i].x + kKeys - 1) / kKeys;
+        nblk = __reduce_add_sync(0xffffffffu, nblk) + (live ? p.prefix_blocks : 0);
+        if (lane == 0) {
+            p.info[t] = TileInfo{nblk, nseg, live ? 1 : 0, live, lo_x[0], hi_x[0], lo_x[1], hi_x[1]};
+            atomicMax(&s_max, nblk);
+        }
+    }
+    __syncthreads();
+    // Blocks per piece: the fewest for which the pieces of all tiles and KV heads still fit one round of
+    // the SMs (a second, short round would cost as much as the first).
+    if (warp == 0) {
+        int lo = max(1, s_max);
+        if (p.lmax > 1) {
+            int hi = lo;  // fits: one piece per tile
+            lo = max(1, (s_max + p.lmax - 1) / p.lmax);
+            while (lo < hi) {
+                const int mid = (lo + hi) >> 1;
+                int n = 0;
+                for (int t = lane; t < p.tiles; t += 32) n += max(p.info[t].live ? 1 : 0, (p.info[t].nblk + mid - 1) / mid);
+                n = __reduce_add_sync(0xffffffffu, n);
+                if (int64_t(n) * p.kv_heads <= p.sms) hi = mid;
+                else lo = mid + 1;
+            }
+        }
+        if (lane == 0) s_chunk = lo;
+    }
+    __syncthreads();
+    const int chunk = s_chunk;
+    // Costliest pieces first (a counting sort by blocks; the order within a bucket does not matter).
+    for (int t = tid; t < p.tiles; t += blockDim.x) {
+        TileInfo* f = p.info + t;
+        if (!f->live) continue;
+        const int pieces = max(1, (f->nblk + chunk - 1) / chunk), sz = (f->nblk + pieces - 1) / pieces;
+        // The last piece may come out shorter, or empty and dropped.
+        const int used = sz ? (f->nblk + sz - 1) / sz : 1;
+        f->pieces = used;
+        atomicAdd(&hist[min(sz, kBuckets - 1)], used);
+    }
+    __syncthreads();
+    // Exclusive sums from the costliest bucket down: thread i holds bucket kBuckets - 1 - i.
+    {
+        const int v = hist[kBuckets - 1 - tid];
+        int inc = v;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int u = __shfl_up_sync(0xffffffffu, inc, o);
+            if (lane >= o) inc += u;
+        }
+        if (lane == 31) warp_sum_s[warp] = inc;
+        __syncthreads();
+        int before = 0;
+        for (int w = 0; w < warp; w++) before += warp_sum_s[w];
+        hist[kBuckets - 1 - tid] = before + inc - v;
+        if (tid == blockDim.x - 1) p.head->nwork = before + inc;
+    }
+    __syncthreads();
+    for (int t = tid; t < p.tiles; t += blockDim.x) {
+        const TileInfo f = p.info[t];
+        if (!f.live) continue;
+        const int sz = (f.nblk + f.pieces - 1) / f.pieces;
+        int at = atomicAdd(&hist[min(sz, kBuckets - 1)], f.pieces);
+        const int2* seg = p.segs + int64_t(t) * p.TI;
+        int s = 0, first = p.prefix_blocks;  // segment s starts at block `first`
+        for (int i = 0; i < f.pieces; i++, at++) {
+            const int b0 = i * sz, b1 = min(f.nblk, b0 + sz);
+            int pos = 0;
+            if (f.nseg > 0) {
+                while (s + 1 < f.nseg) {
+                    const int n = (seg[s].y - seg[s].x + kKeys - 1) / kKeys;
+                    if (b0 < first + n) break;
+                    first += n;
+                    s++;
+                }
+                pos = seg[s].x + max(0, b0 - first) * kKeys;
+            }
+            p.work[at] = Work{t, b0, b1, f.pieces > 1 ? i : -1, s, pos, f.nseg, f.live};
+        }
+    }
 }
 
-struct RowParams {
+// ------------------------------------------------------------------------------------ main kernel
+template <int D>
+struct Cfg {
+    static constexpr int NT = tiles_per_item(D);
+    static constexpr int DS = D < 128 ? D : 128;         // dims of a K or V stage
+    static constexpr int DH = D / DS;                    // stages of a block
+    static constexpr int QC = D / 64, SC = DS / 64;      // 64-dim chunks of [128 rows][128 bytes]
+    static constexpr int ST = D == 64 ? 4 : 2;           // ring depth, K and V each
+    static constexpr int kChunk = 128 * 128;
+    static constexpr int kStage = SC * kChunk;
+    static constexpr int kQ = NT * QC * kChunk;
+    static constexpr int kOffK = kQ, kOffV = kOffK + ST * kStage, kOffBar = kOffV + ST * kStage;
+    static constexpr int kSmem = kOffBar + 512 + 1024;
+    static constexpr int kThreads = 128 + 128 * NT;
+    static constexpr uint32_t kTmemS = 256;              // O in [0, 256), S and P in [256, 512)
+};
+
+struct TcParams {
     const void *q, *k, *v, *pk, *pv;
     void* out;
     int64_t q_stride, k_stride, v_stride, pk_stride, pv_stride, out_stride;
-    int heads, group, ntok, prefix;
+    int heads, kv_heads, group, T, TI, ntok, prefix, prefix_blocks;
     float scale_log2e;
-    const int2* rng;
+    Header* head;
+    const int2 *rng, *segs;
+    const TileInfo* info;
+    const Work* work;
+    float* o;
+    float2* ml;
 };
 
-// One warp per (row, head).
-template <typename T, int D>
-__global__ void __launch_bounds__(256) k_causal_rows(RowParams p) {
-    pdl_wait();
-    const int64_t id = int64_t(blockIdx.x) * 8 + (threadIdx.x >> 5);
-    const int lane = threadIdx.x & 31;
-    if (id >= int64_t(p.ntok) * p.heads) return;
-    const int64_t r = id / p.heads;
-    const int h = int(id - r * p.heads), kh = h / p.group;
-    const int2 rng = p.rng[r];
-    if (rng.y < 0) return;
-    RowState<D> s;
-    row_begin<T, D>(s, static_cast<const T*>(p.q) + r * p.q_stride + int64_t(h) * D, lane);
-    if (p.prefix > 0)
-        row_keys<T, D>(s, static_cast<const T*>(p.pk) + int64_t(kh) * D, static_cast<const T*>(p.pv) + int64_t(kh) * D,
-                       p.pk_stride, p.pv_stride, p.prefix, p.scale_log2e, lane);
-    row_keys<T, D>(s, static_cast<const T*>(p.k) + rng.x * p.k_stride + int64_t(kh) * D,
-                   static_cast<const T*>(p.v) + rng.x * p.v_stride + int64_t(kh) * D, p.k_stride, p.v_stride,
-                   rng.y - rng.x, p.scale_log2e, lane);
-    const float inv = s.l == 0.f ? 0.f : 1.0f / s.l;
-    uint32_t* o = reinterpret_cast<uint32_t*>(static_cast<T*>(p.out) + r * p.out_stride + int64_t(h) * D + lane * (D / 32));
-#pragma unroll
-    for (int i = 0; i < D / 64; i++) o[i] = float_to_pair<T>(s.o[2 * i] * inv, s.o[2 * i + 1] * inv);
+__device__ __forceinline__ bool elect_one() {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "elect.sync _|p, 0xffffffff;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok));
+    return ok != 0;
 }
 
-template <typename T, int D>
-cudaError_t launch_rows(const CausalLaunch& a, const RowParams& p, cudaStream_t stream) {
-    const int64_t blocks = (int64_t(a.ntok) * a.heads + 7) / 8;
-    return launch_kernel(k_causal_rows<T, D>, dim3(unsigned(blocks)), dim3(256), 0, stream, 1, p);
+// A piece of work as every role walks it.
+struct Piece {
+    int tile, kvh, b0, b1, piece, nseg, live;
+    int lo[2], hi[2];
+    int seg0, pos0;
+    const int2* segs;
+};
+__device__ __forceinline__ Piece load_piece(const TcParams& p, int id) {
+    const int w = id / p.kv_heads;
+    const int4* src = reinterpret_cast<const int4*>(p.work + w);
+    const int4 a = src[0], b = src[1];
+    const int4 h = reinterpret_cast<const int4*>(p.info + a.x)[1];
+    Piece s;
+    s.kvh = id - w * p.kv_heads;
+    s.tile = a.x, s.b0 = a.y, s.b1 = a.z, s.piece = a.w;
+    s.seg0 = b.x, s.pos0 = b.y, s.nseg = b.z, s.live = b.w;
+    s.lo[0] = h.x, s.hi[0] = h.y, s.lo[1] = h.z, s.hi[1] = h.w;
+    s.segs = p.segs + int64_t(a.x) * p.TI;
+    return s;
+}
+// Walks a piece's key blocks: prefix blocks, then blocks of the own-key segments.
+struct Cursor {
+    int b, seg, pos, end;
+    bool prefix;
+    int row, nv;  // the block's first row and its keys
+    __device__ __forceinline__ void set(const TcParams& p) {
+        prefix = b < p.prefix_blocks;
+        row = prefix ? b * kKeys : pos;
+        nv = min(kKeys, (prefix ? p.prefix : end) - row);
+    }
+    __device__ __forceinline__ Cursor(const TcParams& p, const Piece& s) {
+        b = s.b0;
+        seg = s.seg0;
+        pos = s.pos0;
+        end = s.nseg > 0 ? s.segs[seg].y : 0;
+        set(p);
+    }
+    __device__ __forceinline__ void next(const TcParams& p, const Piece& s) {
+        if (!prefix) {
+            pos += kKeys;
+            if (pos >= end && b + 1 < s.b1) {
+                const int2 g = s.segs[++seg];
+                pos = g.x;
+                end = g.y;
+            }
+        }
+        b++;
+        set(p);
+    }
+    // Whether tile x has a row that may see a key of the block.
+    __device__ __forceinline__ bool active(const Piece& s, int x) const {
+        return prefix ? (s.live >> x) & 1 : (row < s.hi[x] && row + nv > s.lo[x]);
+    }
+};
+// Pieces are taken in turn, every second round backwards, so that the CTA with a round's costliest
+// piece gets the next round's cheapest.
+__device__ __forceinline__ int piece_id(int round) {
+    const int g = int(gridDim.x), c = int(blockIdx.x);
+    return round * g + ((round & 1) ? g - 1 - c : c);
+}
+
+__device__ __forceinline__ void drain(uint64_t* bar, uint32_t parity) {
+    const uint64_t t0 = globaltimer();
+    while (!mbar_test(bar, parity) && globaltimer() - t0 < kWaitLimitNs) {
+    }
+}
+
+template <typename T>
+__host__ __device__ constexpr uint32_t idesc_of(int M, int N, int b_mn);
+template <>
+__host__ __device__ constexpr uint32_t idesc_of<__half>(int M, int N, int b_mn) {
+    return idesc_f16(M, N, 0, b_mn);
+}
+template <>
+__host__ __device__ constexpr uint32_t idesc_of<__nv_bfloat16>(int M, int N, int b_mn) {
+    return idesc_f16(M, N, 0, b_mn) | (1u << 7) | (1u << 10);  // A and B: bf16
+}
+
+// One row of a piece from the definition, by a whole warp; stored like the epilogue does.
+template <typename E, int D>
+__device__ __noinline__ void exact_row(const TcParams& p, const Piece& s, int row, int head, int2 rg) {
+    const int lane = threadIdx.x & 31;
+    RowState<D> st;
+    row_begin<E, D>(st, static_cast<const E*>(p.q) + row * p.q_stride + int64_t(head) * D, lane);
+    const int64_t col = int64_t(s.kvh) * D;
+    Cursor c(p, s);
+    for (; c.b < s.b1; c.next(p, s)) {
+        const int j0 = c.prefix ? c.row : max(c.row, rg.x), j1 = c.prefix ? c.row + c.nv : min(c.row + c.nv, rg.y);
+        if (j0 >= j1) continue;
+        const E* k = static_cast<const E*>(c.prefix ? p.pk : p.k) + j0 * (c.prefix ? p.pk_stride : p.k_stride) + col;
+        const E* v = static_cast<const E*>(c.prefix ? p.pv : p.v) + j0 * (c.prefix ? p.pv_stride : p.v_stride) + col;
+        row_keys<E, D>(st, k, v, c.prefix ? p.pk_stride : p.k_stride, c.prefix ? p.pv_stride : p.v_stride, j1 - j0,
+                       p.scale_log2e, lane);
+    }
+    if (s.piece < 0) {
+        const float inv = st.l == 0.f ? 0.f : 1.0f / st.l;
+        uint32_t* o = reinterpret_cast<uint32_t*>(static_cast<E*>(p.out) + row * p.out_stride + int64_t(head) * D + lane * (D / 32));
+#pragma unroll
+        for (int i = 0; i < D / 64; i++) o[i] = float_to_pair<E>(st.o[2 * i] * inv, st.o[2 * i + 1] * inv);
+    } else {
+        const int64_t at = (int64_t(s.piece) * p.ntok + row) * p.heads + head;
+        if (lane == 0) p.ml[at] = make_float2(st.m, st.l);
+        float2* o = reinterpret_cast<float2*>(p.o + at * D + lane * (D / 32));
+#pragma unroll
+        for (int i = 0; i < D / 64; i++) o[i] = make_float2(st.o[2 * i], st.o[2 * i + 1]);
+    }
+}
+
+template <typename E, int D>
+__global__ void __launch_bounds__(Cfg<D>::kThreads, 1)
+    k_causal_tc(const __grid_constant__ CUtensorMap mapQ, const __grid_constant__ CUtensorMap mapK,
+                const __grid_constant__ CUtensorMap mapV, const __grid_constant__ CUtensorMap mapPK,
+                const __grid_constant__ CUtensorMap mapPV, const __grid_constant__ TcParams p) {
+    using C = Cfg<D>;
+    constexpr int NT = C::NT, ST = C::ST, DH = C::DH;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::kOffBar);
+    uint64_t *q_full = bars, *q_empty = bars + 1;
+    uint64_t *k_full = bars + 2, *k_empty = k_full + ST, *v_full = k_empty + ST, *v_empty = v_full + ST;
+    uint64_t *s_full = v_empty + ST, *p_full = s_full + 2;  // per S buffer
+    uint64_t *o_full = p_full + 2, *o_empty = o_full + 2;   // per tile
+    uint64_t *pv_done = o_empty + 2, *idle = pv_done + 1;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(idle + 1);
+    int* err = &p.head->err;
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int live_rows = p.group * p.T;
+    if (threadIdx.x == 0) {
+        mbar_init(q_full, 1);
+        mbar_init(q_empty, 1);
+        for (int i = 0; i < ST; i++) {
+            mbar_init(&k_full[i], 1);
+            mbar_init(&k_empty[i], 1);
+            mbar_init(&v_full[i], 1);
+            mbar_init(&v_empty[i], 1);
+        }
+        for (int i = 0; i < 2; i++) {
+            mbar_init(&s_full[i], 1);
+            mbar_init(&p_full[i], 4);
+            mbar_init(&o_full[i], 1);
+            mbar_init(&o_empty[i], 4);
+        }
+        mbar_init(pv_done, 1);
+        mbar_init(idle, 1);
+        fence_mbar_init();
+    }
+    if (warp == 0 && lane == 0) {
+        tma_prefetch(&mapQ);
+        tma_prefetch(&mapK);
+        tma_prefetch(&mapV);
+    }
+    if (warp == 3) {
+        tmem_alloc(tmem_slot, 512);
+        tmem_relinquish();
+    }
+    // Rows [live_rows, 128) of the Q chunks are never loaded: zeroed once, their scores stay finite.
+    {
+        const int dead = 128 - live_rows;
+        for (int i = threadIdx.x; i < NT * C::QC * dead * 8; i += C::kThreads) {
+            const int c = i / (dead * 8), rr = live_rows + (i / 8) % dead;
+            *reinterpret_cast<uint4*>(smem + c * C::kChunk + rr * 128 + (i & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
+        }
+        fence_proxy_async_smem();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    pdl_wait();
+    pdl_launch();
+    const int total = p.head->nwork * p.kv_heads;
+
+    if (warp == 0 || warp == 2) {
+        // ---------------------------------------------------------- TMA producers (Q and K; V)
+        if (lane == 0) {
+            const bool keys = warp == 0;
+            uint64_t *full = keys ? k_full : v_full, *empty = keys ? k_empty : v_empty;
+            uint8_t* ring = smem + (keys ? C::kOffK : C::kOffV);
+            const CUtensorMap* own = keys ? &mapK : &mapV;
+            const CUtensorMap* shared = keys ? &mapPK : &mapPV;
+            bool ok = true;
+            int issued = 0, issued_q = 0;
+            for (int round = 0, id; ok && (id = piece_id(round)) < total; round++) {
+                const Piece s = load_piece(p, id);
+                if (s.b0 >= s.b1) continue;
+                if (keys) {
+                    if (!mbar_wait_sleep(q_empty, uint32_t(issued_q & 1) ^ 1u, err, 32)) break;
+                    mbar_expect_tx(q_full, uint32_t(NT * C::QC * 128 * live_rows));
+                    for (int x = 0; x < NT; x++)
+                        for (int c = 0; c < C::QC; c++)
+                            tma_load_3d(smem + (x * C::QC + c) * C::kChunk, &mapQ, q_full, c * 64, s.kvh * p.group,
+                                        s.tile * p.TI + x * p.T);
+                    issued_q++;
+                }
+                for (Cursor c(p, s); ok && c.b < s.b1; c.next(p, s)) {
+                    const int boxes = (c.nv + 31) / 32;
+                    const CUtensorMap* map = c.prefix ? shared : own;
+                    for (int h = 0; h < DH; h++) {
+                        const int st = issued % ST;
+                        if (!mbar_wait_sleep(&empty[st], uint32_t((issued / ST) & 1) ^ 1u, err, 32)) {
+                            ok = false;
+                            break;
+                        }
+                        mbar_expect_tx(&full[st], uint32_t(boxes * C::SC * 4096));
+                        for (int ch = 0; ch < C::SC; ch++)
+                            for (int b = 0; b < boxes; b++)
+                                tma_load_2d(ring + st * C::kStage + ch * C::kChunk + b * 4096, map, &full[st],
+                                            s.kvh * D + h * C::DS + ch * 64, c.row + b * 32);
+                        issued++;
+                    }
+                }
+            }
+            // Every issued load lands before the CTA exits, also after an error.
+            if (issued_q > 0) drain(q_full, uint32_t((issued_q - 1) & 1));
+            for (int st = 0; st < ST; st++) {
+                const int n = issued / ST + (st < issued % ST ? 1 : 0);
+                if (n > 0) drain(&full[st], uint32_t((n - 1) & 1));
+            }
+        }
+    } else if (warp == 1) {
+        // ---------------------------------------------------------- MMA issuer (the whole warp walks along)
+        const uint32_t id_s = idesc_of<E>(128, kKeys, 0);      // K-major Q and K
+        const uint32_t id_o = idesc_of<E>(128, C::DS, 1);      // P from tensor memory, MN-major V
+        const uint32_t q_addr = smem_u32(smem), k_addr = smem_u32(smem + C::kOffK), v_addr = smem_u32(smem + C::kOffV);
+        bool ok = true;
+        auto wait = [&](uint64_t* bar, uint32_t parity) {
+            ok = __all_sync(0xffffffffu, ok && mbar_wait(bar, parity, err));
+            return ok;
+        };
+        int nq = 0, nk = 0, nv = 0;            // Q tiles, K stages and V stages used so far
+        int ns[2] = {0, 0}, np[2] = {0, 0};    // S and PV products per S buffer (NT 2) or in all (NT 1, [0])
+        int no[2] = {0, 0};                    // items with an O, per tile
+        for (int round = 0, id; ok && (id = piece_id(round)) < total; round++) {
+            const Piece s = load_piece(p, id);
+            if (s.b0 >= s.b1) continue;
+            if (!wait(q_full, uint32_t(nq & 1))) break;
+            nq++;
+            tc_fence_after();
+            Cursor c(p, s);
+            int prev = 0, prev_nv = 0;  // the block before: the tiles it is active for, its keys
+            int used = 0;               // tiles with an O in this item
+            for (;;) {
+                const bool more = c.b < s.b1;
+                int act = 0;
+                if (more)
+                    for (int x = 0; x < NT; x++) act |= c.active(s, x) ? 1 << x : 0;
+                // S of tile x (of head dim 256: into S buffer b)
+                auto scores = [&](int x, int b) {
+                    for (int h = 0; h < DH; h++) {
+                        const int st = (nk + h) % ST;
+                        if (!wait(&k_full[st], uint32_t(((nk + h) / ST) & 1))) return;
+                        tc_fence_after();
+                        if (elect_one()) {
+#pragma unroll
+                            for (int kk = 0; kk < C::DS / 16; kk++) {
+                                const uint64_t ad = sw128_desc(
+                                    q_addr + (x * C::QC + h * C::SC + (kk >> 2)) * C::kChunk + (kk & 3) * 32, 16, 1024);
+                                const uint64_t bd =
+                                    sw128_desc(k_addr + st * C::kStage + (kk >> 2) * C::kChunk + (kk & 3) * 32, 16, 1024);
+                                umma_f16(tmem + C::kTmemS + uint32_t(b * kKeys), ad, bd, id_s, (h | kk) != 0);
+                            }
+                            if (NT == 1) umma_commit(&k_empty[st]);
+                            if (h == DH - 1) umma_commit(&s_full[b]);
+                        }
+                        __syncwarp();
+                    }
+                };
+                // O of tile x += P of S buffer b times the block before's V
+                bool cleared = false;
+                auto values = [&](int x, int b, uint32_t parity) {
+                    if (!wait(&p_full[b], parity)) return;
+                    if (!((used >> x) & 1) && no[x] > 0 && !wait(&o_empty[x], uint32_t((no[x] - 1) & 1))) return;
+                    const int steps = (prev_nv + 15) / 16;
+                    for (int h = 0; h < DH; h++) {
+                        const int st = (nv + h) % ST;
+                        if (!wait(&v_full[st], uint32_t(((nv + h) / ST) & 1))) return;
+                        if (!cleared && (prev_nv & 15)) {
+                            // Rows behind the block's last key, up to the product's step.
+                            for (int i = lane; i < (steps * 16 - prev_nv) * C::SC * 8; i += 32) {
+                                const int rr = prev_nv + i / (C::SC * 8), ch = (i >> 3) % C::SC;
+                                *reinterpret_cast<uint4*>(smem + C::kOffV + st * C::kStage + ch * C::kChunk + rr * 128 +
+                                                          (i & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
+                            }
+                            fence_proxy_async_smem();
+                            __syncwarp();
+                        }
+                        tc_fence_after();
+                        if (elect_one()) {
+                            for (int kk = 0; kk < steps; kk++) {
+                                const uint64_t bd = sw128_desc(v_addr + st * C::kStage + kk * 2048, C::kChunk, 1024);
+                                umma_f16_ta(tmem + uint32_t(x * D + h * C::DS), tmem + C::kTmemS + uint32_t(b * kKeys + kk * 8),
+                                            bd, id_o, ((used >> x) & 1) | (kk != 0));
+                            }
+                            if (NT == 1) {
+                                umma_commit(&v_empty[st]);
+                                if (h == DH - 1) umma_commit(pv_done);
+                            }
+                        }
+                        __syncwarp();
+                    }
+                    if (NT == 2) cleared = true;
+                    if (!((used >> x) & 1)) no[x]++;
+                    used |= 1 << x;
+                };
+                if constexpr (NT == 2) {
+                    for (int x = 0; x < 2 && ok; x++) {
+                        if ((prev >> x) & 1) {
+                            values(x, x, uint32_t(np[x] & 1));
+                            np[x]++;
+                        }
+                        if (!more && ok && ((used >> x) & 1) && elect_one()) umma_commit(&o_full[x]);
+                        __syncwarp();
+                        if (ok && ((act >> x) & 1)) scores(x, x);
+                    }
+                    // A block no tile sees (between key ranges in falling order) is passed by once it has landed.
+                    if (ok && more && !act) wait(&k_full[nk % ST], uint32_t((nk / ST) & 1));
+                    if (ok && prev_nv && !prev) wait(&v_full[nv % ST], uint32_t((nv / ST) & 1));
+                    if (!ok) break;
+                    if (elect_one()) {
+                        if (prev_nv) umma_commit(&v_empty[nv % ST]);
+                        if (more) umma_commit(&k_empty[nk % ST]);
+                    }
+                    __syncwarp();
+                    if (prev_nv) nv++;
+                    if (more) nk++;
+                } else {
+                    if (more) {
+                        scores(0, ns[0] & 1);
+                        ns[0]++;
+                        nk += DH;
+                    }
+                    if (ok && prev_nv) {
+                        values(0, np[0] & 1, uint32_t((np[0] >> 1) & 1));
+                        np[0]++;
+                        nv += DH;
+                    }
+                    if (!ok) break;
+                    if (!more && elect_one()) umma_commit(&o_full[0]);
+                    __syncwarp();
+                }
+                if (!more) break;
+                prev = act;
+                prev_nv = c.nv;
+                c.next(p, s);
+                // Every S of the item has read Q.
+                if (c.b >= s.b1 && elect_one()) umma_commit(q_empty);
+                __syncwarp();
+            }
+        }
+        // The products in flight end before the CTA gives its memory back.
+        if (elect_one()) {
+            umma_commit(idle);
+            drain(idle, 0);
+        }
+        __syncwarp();
+    } else if (warp >= 4) {
+        // ---------------------------------------------------------- softmax and output, one thread per row
+        const int x = NT == 2 ? (warp - 4) >> 2 : 0;
+        const int quad = warp & 3, r = quad * 32 + lane;
+        const uint32_t lane_base = tmem + (uint32_t(quad * 32) << 16);
+        const int token = r / p.group;
+        bool ok = true;
+        auto wait = [&](uint64_t* bar, uint32_t parity) {
+            ok = __all_sync(0xffffffffu, ok && mbar_wait(bar, parity, err));
+            return ok;
+        };
+        int nb = 0, no = 0;  // blocks and items with an O so far
+        for (int round = 0, id; ok && (id = piece_id(round)) < total; round++) {
+            const Piece s = load_piece(p, id);
+            const int row = s.tile * p.TI + x * p.T + token;
+            const bool query = r < live_rows && row < p.ntok;
+            const int2 rg = query ? p.rng[row] : make_int2(0, -1);
+            float m = -INFINITY, l = 0.f;
+            int count = 0;
+            for (Cursor c(p, s); c.b < s.b1; c.next(p, s)) {
+                if (NT == 2 && !c.active(s, x)) continue;
+                const int b = NT == 2 ? x : nb & 1;
+                if (!wait(&s_full[b], uint32_t((NT == 2 ? nb : nb >> 1) & 1))) break;
+                nb++;
+                count++;
+                tc_fence_after();
+                const uint32_t scol = lane_base + C::kTmemS + uint32_t(b * kKeys);
+                uint32_t sr[128];
+#pragma unroll
+                for (int i = 0; i < 4; i++) tmem_ld32(scol + i * 32, *reinterpret_cast<uint32_t(*)[32]>(&sr[i * 32]));
+                tmem_wait_ld();
+                // The row's keys among the block's nv (a later segment's may start within 128 rows of this
+                // one's end).  Rows without a query take every score: finite, never stored.
+                const int lo = c.prefix || !query ? 0 : rg.x - c.row;
+                const int hi = !query ? kKeys : c.prefix ? c.nv : min(rg.y - c.row, c.nv);
+                if (__any_sync(0xffffffffu, lo > 0 || hi < kKeys)) {
+#pragma unroll
+                    for (int i = 0; i < 128; i++)
+                        if (i < lo || i >= hi) sr[i] = __float_as_uint(-INFINITY);
+                }
+                float mp[8];
+#pragma unroll
+                for (int i = 0; i < 8; i++) mp[i] = __uint_as_float(sr[i]);
+#pragma unroll
+                for (int i = 8; i < 128; i++) mp[i & 7] = fmaxf(mp[i & 7], __uint_as_float(sr[i]));
+                const float mb = fmaxf(fmaxf(fmaxf(mp[0], mp[1]), fmaxf(mp[2], mp[3])),
+                                       fmaxf(fmaxf(mp[4], mp[5]), fmaxf(mp[6], mp[7]))) * p.scale_log2e;
+                const bool grow = mb > m + kGrow && m != -INFINITY;
+                if (__any_sync(0xffffffffu, grow)) {
+                    // O holds every product before this block's (of head dim 256: once the last has completed).
+                    if (NT == 1 && !wait(pv_done, uint32_t((nb - 2) & 1))) break;
+                    tc_fence_after();
+                    const float alpha = grow ? ex2_approx(m - mb) : 1.0f;
+#pragma unroll 1
+                    for (int i = 0; i < D / 32; i++) {
+                        uint32_t o[32];
+                        tmem_ld32(lane_base + uint32_t(x * D + i * 32), o);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int e = 0; e < 32; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+                        tmem_st32(lane_base + uint32_t(x * D + i * 32), o);
+                    }
+                    if (grow) {
+                        l *= alpha;
+                        m = mb;
+                    }
+                }
+                if (m == -INFINITY) m = mb;  // the row's first visible key: O and l are still 0
+                const float mu = m == -INFINITY ? 0.f : m;
+                float ps[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    uint32_t pk[32];
+#pragma unroll
+                    for (int e = 0; e < 32; e++) {
+                        const float p0 = ex2_approx(fmaf(__uint_as_float(sr[h * 64 + 2 * e]), p.scale_log2e, -mu));
+                        const float p1 = ex2_approx(fmaf(__uint_as_float(sr[h * 64 + 2 * e + 1]), p.scale_log2e, -mu));
+                        ps[(2 * e) & 7] += p0;
+                        ps[(2 * e + 1) & 7] += p1;
+                        pk[e] = float_to_pair<E>(p0, p1);
+                    }
+                    tmem_st32(scol + h * 32, pk);
+                }
+                l += ((ps[0] + ps[1]) + (ps[2] + ps[3])) + ((ps[4] + ps[5]) + (ps[6] + ps[7]));
+                tmem_wait_st();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&p_full[b]);
+            }
+            if (!ok) break;
+            // ---- output
+            const bool in = rg.y >= 0;
+            const int head = s.kvh * p.group + (r - token * p.group);
+            const int64_t at = (int64_t(s.piece) * p.ntok + row) * p.heads + head;  // of a partial row
+            const float inv = s.piece >= 0 ? 1.0f : l == 0.f ? 0.f : 1.0f / l;
+            if (in && s.piece >= 0) p.ml[at] = make_float2(m, l);
+            bool bad = false;
+            if (count) {
+                if (!wait(&o_full[x], uint32_t(no & 1))) break;
+                no++;
+                tc_fence_after();
+            }
+#pragma unroll 1
+            for (int i = 0; i < D / 32; i++) {
+                uint32_t o[32];
+                if (count) {
+                    tmem_ld32(lane_base + uint32_t(x * D + i * 32), o);
+                    tmem_wait_ld();
+                    if (i == D / 32 - 1) {
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(&o_empty[x]);
+                    }
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 32; e++) o[e] = 0u;
+                }
+                float z = 0.f;
+#pragma unroll
+                for (int e = 0; e < 32; e++) z = fmaf(__uint_as_float(o[e]), 0.f, z);
+                bad |= z != 0.f;  // NaN: a value is infinite or NaN
+                if (in && s.piece < 0) {
+                    uint4* dst = reinterpret_cast<uint4*>(static_cast<E*>(p.out) + row * p.out_stride + int64_t(head) * D + i * 32);
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        uint32_t w[4];
+#pragma unroll
+                        for (int f = 0; f < 4; f++)
+                            w[f] = float_to_pair<E>(__uint_as_float(o[8 * e + 2 * f]) * inv, __uint_as_float(o[8 * e + 2 * f + 1]) * inv);
+                        dst[e] = make_uint4(w[0], w[1], w[2], w[3]);
+                    }
+                } else if (in) {
+                    uint4* dst = reinterpret_cast<uint4*>(p.o + at * D + i * 32);
+#pragma unroll
+                    for (int e = 0; e < 8; e++) dst[e] = make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+                }
+                __syncwarp();
+            }
+            unsigned redo = __ballot_sync(0xffffffffu, in && bad);
+            __syncwarp();
+            while (redo) {
+                const int src = __ffs(redo) - 1;
+                redo &= redo - 1;
+                const int2 g = make_int2(__shfl_sync(0xffffffffu, rg.x, src), __shfl_sync(0xffffffffu, rg.y, src));
+                exact_row<E, D>(p, s, __shfl_sync(0xffffffffu, row, src), __shfl_sync(0xffffffffu, head, src), g);
+            }
+        }
+    }
+
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 3) {
+        tc_fence_after();
+        tmem_dealloc(tmem, 512);
+    }
+}
+
+// ------------------------------------------------------------------------------------ merge
+struct MergeParams {
+    void* out;
+    int64_t out_stride;
+    int heads, ntok, TI;
+    const int2* rng;
+    const TileInfo* info;
+    const float* o;
+    const float2* ml;
+};
+
+// One warp per (row, head): out = sum_c 2^(m_c - m) O_c / sum_c 2^(m_c - m) l_c, m the largest m_c.
+template <typename E, int D>
+__global__ void __launch_bounds__(128) k_causal_merge(MergeParams p) {
+    pdl_wait();
+    pdl_launch();
+    const int64_t id = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 5);
+    const int lane = threadIdx.x & 31;
+    if (id >= int64_t(p.ntok) * p.heads) return;
+    const int row = int(id / p.heads);
+    const int n = p.info[row / p.TI].pieces;
+    if (n <= 1 || p.rng[row].y < 0) return;
+    const int64_t step = int64_t(p.ntok) * p.heads;
+    float2 a = lane < n ? p.ml[lane * step + id] : make_float2(-INFINITY, 0.f);
+    float2 b = lane + 32 < n ? p.ml[(lane + 32) * step + id] : make_float2(-INFINITY, 0.f);
+    const bool nan = __any_sync(0xffffffffu, isnan(a.x) || isnan(b.x));
+    const float m = warp_max(fmaxf(a.x, b.x));
+    float wa = a.x == -INFINITY ? 0.f : ex2_approx(a.x - m), wb = b.x == -INFINITY ? 0.f : ex2_approx(b.x - m);
+    const float l = warp_sum(wa * a.y + wb * b.y);
+    const float inv = nan ? NAN : l == 0.f ? 0.f : 1.0f / l;
+    float acc[D / 32];
+#pragma unroll
+    for (int i = 0; i < D / 32; i++) acc[i] = 0.f;
+    for (int c = 0; c < n; c++) {
+        const float w = c < 32 ? __shfl_sync(0xffffffffu, wa, c) : __shfl_sync(0xffffffffu, wb, c - 32);
+        if (w == 0.f) continue;  // a piece without a visible key left no row
+        const float2* src = reinterpret_cast<const float2*>(p.o + (c * step + id) * D + lane * (D / 32));
+#pragma unroll
+        for (int i = 0; i < D / 64; i++) {
+            const float2 v = src[i];
+            acc[2 * i] = fmaf(w, v.x, acc[2 * i]);
+            acc[2 * i + 1] = fmaf(w, v.y, acc[2 * i + 1]);
+        }
+    }
+    uint32_t* o = reinterpret_cast<uint32_t*>(static_cast<E*>(p.out) + row * p.out_stride + int64_t(id - int64_t(row) * p.heads) * D +
+                                              lane * (D / 32));
+#pragma unroll
+    for (int i = 0; i < D / 64; i++) o[i] = float_to_pair<E>(acc[2 * i] * inv, acc[2 * i + 1] * inv);
+}
+
+// ------------------------------------------------------------------------------------ launch
+// Always with programmatic stream serialisation: every kernel here waits for its predecessor first.
+template <typename... KArgs, typename... Args>
+cudaError_t launch_pdl(void (*kern)(KArgs...), unsigned grid, unsigned block, size_t smem, cudaStream_t stream, Args&&... args) {
+    const bool was = programmatic_launch();
+    set_programmatic_launch(true);
+    const cudaError_t e = launch_kernel(kern, dim3(grid), dim3(block), smem, stream, 1, std::forward<Args>(args)...);
+    set_programmatic_launch(was);
+    return e;
+}
+
+template <typename E, int D>
+cudaError_t launch_t(const CausalLaunch& a, const Sizes& s, const Layout& l, cudaStream_t stream) {
+    using C = Cfg<D>;
+    // Per device the kernel needs its shared-memory limit raised; the call is cheap and may run during a capture.
+    cudaError_t e = cudaFuncSetAttribute(k_causal_tc<E, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
+    if (e != cudaSuccess) return e;
+    const __half *q = static_cast<const __half*>(a.q), *k = static_cast<const __half*>(a.k), *v = static_cast<const __half*>(a.v);
+    const __half *pk = static_cast<const __half*>(a.pk), *pv = static_cast<const __half*>(a.pv);
+    CUtensorMap mq, mk, mv, mpk, mpv;
+    const uint64_t kw = uint64_t(a.kv_heads) * D;
+    if (!encode_fp16_map_3d(&mq, q, D, uint64_t(a.heads), uint64_t(a.ntok), 64, uint32_t(s.group), uint32_t(s.T), uint64_t(a.q_stride)))
+        return cudaErrorInvalidValue;
+    mk = mv = mpk = mpv = mq;  // never read where there are no rows
+    if (a.nkv > 0 && (!encode_fp16_map(&mk, k, kw, uint64_t(a.nkv), 64, 32, uint64_t(a.k_stride)) ||
+                      !encode_fp16_map(&mv, v, kw, uint64_t(a.nkv), 64, 32, uint64_t(a.v_stride))))
+        return cudaErrorInvalidValue;
+    if (a.prefix > 0 && (!encode_fp16_map(&mpk, pk, kw, uint64_t(a.prefix), 64, 32, uint64_t(a.pk_stride)) ||
+                         !encode_fp16_map(&mpv, pv, kw, uint64_t(a.prefix), 64, 32, uint64_t(a.pv_stride))))
+        return cudaErrorInvalidValue;
+    TcParams p{a.q, a.k, a.v, a.pk, a.pv, a.out, a.q_stride, a.k_stride, a.v_stride, a.pk_stride, a.pv_stride, a.out_stride,
+               a.heads, a.kv_heads, s.group, s.T, s.TI, a.ntok, a.prefix, (a.prefix + kKeys - 1) / kKeys, a.scale * kLog2e,
+               l.head, l.rng, l.segs, l.info, l.work, l.o, l.ml};
+    const int64_t most = s.lmax > 1 ? a.num_sms : int64_t(s.tiles) * a.kv_heads;
+    e = launch_pdl(k_causal_tc<E, D>, unsigned(std::min<int64_t>(a.num_sms, most)), C::kThreads, size_t(C::kSmem), stream, mq, mk, mv,
+                   mpk, mpv, p);
+    if (e != cudaSuccess || s.lmax == 1) return e;
+    MergeParams mp{a.out, a.out_stride, a.heads, a.ntok, s.TI, l.rng, l.info, l.o, l.ml};
+    return launch_pdl(k_causal_merge<E, D>, unsigned((int64_t(a.ntok) * a.heads + 3) / 4), 128, 0, stream, mp);
+}
+
+template <typename E>
+cudaError_t launch_e(const CausalLaunch& a, const Sizes& s, const Layout& l, cudaStream_t stream) {
+    if (a.hd == 64) return launch_t<E, 64>(a, s, l, stream);
+    if (a.hd == 128) return launch_t<E, 128>(a, s, l, stream);
+    return launch_t<E, 256>(a, s, l, stream);
 }
 
 }  // namespace
 
-size_t causal_workspace(const CausalLaunch& a) { return (size_t(a.ntok) * sizeof(int2) + 255) / 256 * 256; }
+size_t causal_workspace(const CausalLaunch& a) { return layout_of(a, sizes_of(a)).bytes; }
 
 cudaError_t launch_causal(const CausalLaunch& a, cudaStream_t stream) {
-    int2* rng = static_cast<int2*>(a.workspace);
-    RangeParams rp{a.q_seqs, a.kv_seqs, a.nseq, a.ntok, a.nkv, a.window, rng};
-    cudaError_t e = launch_kernel(k_causal_ranges, dim3(1), dim3(1024), 0, stream, 1, rp);
+    const Sizes s = sizes_of(a);
+    const Layout l = layout_of(a, s);
+    PlanParams pp{a.q_seqs, a.kv_seqs, a.nseq, a.ntok, a.nkv, a.window, s.T, s.TI, s.tiles, a.kv_heads,
+                  (a.prefix + kKeys - 1) / kKeys, s.lmax, a.num_sms, l.head, l.rng, l.segs, l.info, l.work};
+    const cudaError_t e = launch_pdl(k_causal_plan, 1, 1024, 0, stream, pp);
     if (e != cudaSuccess) return e;
-    RowParams p{a.q, a.k, a.v, a.pk, a.pv, a.out, a.q_stride, a.k_stride, a.v_stride, a.pk_stride, a.pv_stride, a.out_stride,
-                a.heads, a.heads / a.kv_heads, a.ntok, a.prefix, a.scale * kLog2e, rng};
-    if (a.bf16) {
-        if (a.hd == 64) return launch_rows<__nv_bfloat16, 64>(a, p, stream);
-        if (a.hd == 128) return launch_rows<__nv_bfloat16, 128>(a, p, stream);
-        return launch_rows<__nv_bfloat16, 256>(a, p, stream);
-    }
-    if (a.hd == 64) return launch_rows<__half, 64>(a, p, stream);
-    if (a.hd == 128) return launch_rows<__half, 128>(a, p, stream);
-    return launch_rows<__half, 256>(a, p, stream);
+    return a.bf16 ? launch_e<__nv_bfloat16>(a, s, l, stream) : launch_e<__half>(a, s, l, stream);
 }
 
 }  // namespace ge
