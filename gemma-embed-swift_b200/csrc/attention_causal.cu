@@ -893,16 +893,6 @@ __global__ void __launch_bounds__(128) k_causal_merge(MergeParams p) {
 }
 
 // ------------------------------------------------------------------------------------ launch
-// Always with programmatic stream serialisation: every kernel here waits for its predecessor first.
-template <typename... KArgs, typename... Args>
-cudaError_t launch_pdl(void (*kern)(KArgs...), unsigned grid, unsigned block, size_t smem, cudaStream_t stream, Args&&... args) {
-    const bool was = programmatic_launch();
-    set_programmatic_launch(true);
-    const cudaError_t e = launch_kernel(kern, dim3(grid), dim3(block), smem, stream, 1, std::forward<Args>(args)...);
-    set_programmatic_launch(was);
-    return e;
-}
-
 template <typename E, int D>
 cudaError_t launch_t(const CausalLaunch& a, const Sizes& s, const Layout& l, cudaStream_t stream) {
     using C = Cfg<D>;

@@ -9,6 +9,17 @@
 
 namespace ge {
 
+// Launches with programmatic stream serialisation whatever the calling thread's policy: every kernel
+// of the operators waits for its predecessor (pdl_wait) before it touches memory.
+template <typename... KArgs, typename... Args>
+cudaError_t launch_pdl(void (*kern)(KArgs...), unsigned grid, unsigned block, size_t smem, cudaStream_t stream, Args&&... args) {
+    const bool was = programmatic_launch();
+    set_programmatic_launch(true);
+    const cudaError_t e = launch_kernel(kern, dim3(grid), dim3(block), smem, stream, 1, std::forward<Args>(args)...);
+    set_programmatic_launch(was);
+    return e;
+}
+
 // ------------------------------------------------------------------ causal and shared-prefix attention
 // Query row r of head h attends to the prefix rows [0, prefix) and to its own key rows [lo, hi),
 // which the ranges of its sequence give.
