@@ -12,7 +12,9 @@ tensors' device -- and returns without synchronising; it may be captured into a 
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
+import functools
 import math
 from dataclasses import dataclass
 from typing import Any, Optional
@@ -23,6 +25,7 @@ from . import _lib
 
 __all__ = ["attention_causal", "attention_prefix", "linear_q4", "Q4Weight"]
 
+_HERE = contextlib.nullcontext()
 Q4_TYPES = {"Q4_0": 2, "Q4_1": 3}  # GGUF tensor type ids (ge_q4_type)
 
 
@@ -40,110 +43,125 @@ def _call(rc: int):
         raise _error(rc, (_lib.lib().ge_last_error(None) or b"").decode())
 
 
+@functools.cache
+def _torch():
+    import torch
+    return torch, {torch.float16: 0, torch.bfloat16: 1}
+
+
 def _dtype(t) -> int:
-    import torch
-    if t.dtype == torch.float16:
-        return 0
-    if t.dtype == torch.bfloat16:
-        return 1
-    raise _invalid(f"tensors must be float16 or bfloat16, got {t.dtype}")
+    code = _torch()[1].get(t.dtype)
+    if code is None:
+        raise _invalid(f"tensors must be float16 or bfloat16, got {t.dtype}")
+    return code
 
 
-def _on_device(name: str, t, like=None):
-    import torch
-    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+def _on_device(name: str, t, device: Optional[int] = None) -> int:
+    """The ordinal of the CUDA device that holds `t` (and has to be `device`, when given)."""
+    if not isinstance(t, _torch()[0].Tensor) or not t.is_cuda:
         raise _invalid(f"{name} must be a CUDA tensor")
-    if like is not None and t.device != like.device:
-        raise _invalid(f"{name} is on {t.device}, not on {like.device}")
+    d = t.get_device()
+    if device is not None and d != device:
+        raise _invalid(f"{name} is on cuda:{d}, not on cuda:{device}")
+    return d
 
 
-def _heads(name: str, t, like, heads: Optional[int], dim: int) -> int:
-    """Checks a [rows, heads, dim] tensor and gives the elements between its rows."""
-    _on_device(name, t, like)
-    if t.dtype != like.dtype:
-        raise _invalid(f"{name} is {t.dtype}, not {like.dtype}")
-    if t.dim() != 3 or t.shape[2] != dim or (heads is not None and t.shape[1] != heads):
+def _heads(name: str, t, device: int, dtype, heads: Optional[int], dim: int):
+    """Checks a [rows, heads, dim] tensor; gives its rows, heads and the elements between its rows."""
+    _on_device(name, t, device)
+    if t.dtype != dtype:
+        raise _invalid(f"{name} is {t.dtype}, not {dtype}")
+    shape = t.shape
+    if len(shape) != 3 or shape[2] != dim or (heads is not None and shape[1] != heads):
         want = f"[rows, {heads if heads is not None else 'heads'}, {dim}]"
-        raise _invalid(f"{name} must be {want}, got {list(t.shape)}")
-    if (dim > 1 and t.stride(2) != 1) or (t.shape[1] > 1 and t.stride(1) != dim):
+        raise _invalid(f"{name} must be {want}, got {list(shape)}")
+    rows, n, _ = shape
+    s0, s1, s2 = t.stride()
+    if (dim > 1 and s2 != 1) or (n > 1 and s1 != dim):
         raise _invalid(f"{name}'s heads must lie side by side in a row (strides {t.stride()})")
-    width = t.shape[1] * dim
-    return t.stride(0) if t.shape[0] > 1 else width
+    return rows, n, s0 if rows > 1 else n * dim
 
 
-def _ranges(name: str, t, like) -> int:
-    import torch
-    _on_device(name, t, like)
+def _ranges(name: str, t, device: int) -> int:
+    torch = _torch()[0]
+    _on_device(name, t, device)
     if t.dtype not in (torch.int32, torch.uint32) or t.dim() != 2 or t.shape[1] != 2 or not t.is_contiguous():
         raise _invalid(f"{name} must be a contiguous [sequences, 2] int32 tensor of (start, length)")
     return t.shape[0]
 
 
-def _stream(stream, device):
-    """The stream's handle, and a torch stream to allocate on."""
-    import torch
+def _stream(stream, device: int):
+    """The stream's handle, and a context in which torch allocates on it (None: already so)."""
+    torch = _torch()[0]
     if stream is None:
-        s = torch.cuda.current_stream(device)
-        return s.cuda_stream, s
+        return torch.cuda.current_stream(device).cuda_stream, None
     if hasattr(stream, "cuda_stream"):
-        if stream.device != device:
-            raise _invalid(f"the stream is on {stream.device}, not on {device}")
-        return stream.cuda_stream, stream
+        if stream.device.index != device:
+            raise _invalid(f"the stream is on {stream.device}, not on cuda:{device}")
+        return stream.cuda_stream, torch.cuda.stream(stream)
     handle = int(stream)
-    if handle == 0:
-        return 0, torch.cuda.default_stream(device)
-    return handle, torch.cuda.ExternalStream(handle, device=device)
+    s = torch.cuda.ExternalStream(handle, device=device) if handle else torch.cuda.default_stream(device)
+    return handle, torch.cuda.stream(s)
+
+
+@functools.lru_cache(maxsize=1024)
+def _workspace_bytes(device: int, dtype: int, heads: int, kv_heads: int, dim: int, scale: float, window: int, ntok: int,
+                     prefix: int) -> int:
+    s = _lib.GeAttentionShape(dtype, heads, kv_heads, dim, scale, window)
+    n = ctypes.c_int64(0)
+    _call(_lib.lib().ge_attention_workspace(device, ctypes.byref(s), ntok, prefix, ctypes.byref(n)))
+    return n.value
 
 
 def _attention(q, k, v, prefix_k, prefix_v, q_seqs, kv_seqs, scale, window, out, stream):
-    import torch
-    _on_device("q", q)
+    torch = _torch()[0]
+    device = _on_device("q", q)
+    dtype = q.dtype
+    code = _dtype(q)
     if q.dim() != 3:
         raise _invalid(f"q must be [rows, heads, dim], got {list(q.shape)}")
     dim = q.shape[2]
-    kv_heads = k.shape[1] if hasattr(k, "dim") and k.dim() == 3 else None
-    s = _lib.GeAttentionShape()
-    s.dtype = _dtype(q)
-    s.heads, s.head_dim = q.shape[1], dim
-    s.q_stride = _heads("q", q, q, None, dim)
-    s.k_stride = _heads("k", k, q, None, dim)
-    s.v_stride = _heads("v", v, q, kv_heads, dim)
-    s.kv_heads = kv_heads
-    if k.shape[0] != v.shape[0]:
-        raise _invalid(f"k has {k.shape[0]} rows, v {v.shape[0]}")
-    nseq = _ranges("q_seqs" if prefix_k is not None else "seqs", q_seqs, q)
+    ntok, heads, q_stride = _heads("q", q, device, dtype, None, dim)
+    nkv, kv_heads, k_stride = _heads("k", k, device, dtype, None, dim)
+    rows, _, v_stride = _heads("v", v, device, dtype, kv_heads, dim)
+    if rows != nkv:
+        raise _invalid(f"k has {nkv} rows, v {rows}")
+    nseq = _ranges("seqs" if prefix_k is None else "q_seqs", q_seqs, device)
+    prefix = pk_stride = pv_stride = 0
     if prefix_k is None:
-        if k.shape[0] != q.shape[0]:
-            raise _invalid(f"q has {q.shape[0]} rows, k and v {k.shape[0]}")
+        if nkv != ntok:
+            raise _invalid(f"q has {ntok} rows, k and v {nkv}")
     else:
-        s.prefix_k_stride = _heads("prefix_k", prefix_k, q, kv_heads, dim)
-        s.prefix_v_stride = _heads("prefix_v", prefix_v, q, kv_heads, dim)
-        if prefix_k.shape[0] != prefix_v.shape[0]:
-            raise _invalid(f"prefix_k has {prefix_k.shape[0]} rows, prefix_v {prefix_v.shape[0]}")
-        if _ranges("kv_seqs", kv_seqs, q) != nseq:
+        prefix, _, pk_stride = _heads("prefix_k", prefix_k, device, dtype, kv_heads, dim)
+        rows, _, pv_stride = _heads("prefix_v", prefix_v, device, dtype, kv_heads, dim)
+        if rows != prefix:
+            raise _invalid(f"prefix_k has {prefix} rows, prefix_v {rows}")
+        if _ranges("kv_seqs", kv_seqs, device) != nseq:
             raise _invalid(f"q_seqs names {nseq} sequences, kv_seqs {kv_seqs.shape[0]}")
-    s.scale = 1.0 / math.sqrt(dim) if scale is None else float(scale)
-    s.window = int(window)
-    device = q.device
+    scale = 1.0 / math.sqrt(dim) if scale is None else float(scale)
+    window = int(window)
     handle, on = _stream(stream, device)
-    ntok, prefix = q.shape[0], 0 if prefix_k is None else prefix_k.shape[0]
-    L = _lib.lib()
-    nbytes = ctypes.c_int64(0)
-    with torch.cuda.stream(on):
+    nbytes = _workspace_bytes(device, code, heads, kv_heads, dim, scale, window, ntok, prefix)
+    with on or _HERE:
         if out is None:
-            out = torch.empty((ntok, s.heads, dim), dtype=q.dtype, device=device)
-        s.out_stride = _heads("out", out, q, s.heads, dim)
-        if out.shape[0] != ntok:
-            raise _invalid(f"q has {ntok} rows, out {out.shape[0]}")
-        _call(L.ge_attention_workspace(device.index, ctypes.byref(s), ntok, prefix, ctypes.byref(nbytes)))
-        ws = torch.empty(max(nbytes.value, 1), dtype=torch.uint8, device=device)
-        if prefix_k is None:
-            _call(L.ge_attention_causal(device.index, ctypes.byref(s), q.data_ptr(), k.data_ptr(), v.data_ptr(), ntok,
-                                        q_seqs.data_ptr(), nseq, out.data_ptr(), ws.data_ptr(), nbytes.value, handle))
+            out = torch.empty((ntok, heads, dim), dtype=dtype, device=q.device)
+            out_stride = heads * dim
         else:
-            _call(L.ge_attention_prefix(device.index, ctypes.byref(s), q.data_ptr(), ntok, k.data_ptr(), v.data_ptr(),
-                                        k.shape[0], prefix_k.data_ptr(), prefix_v.data_ptr(), prefix, q_seqs.data_ptr(),
-                                        kv_seqs.data_ptr(), nseq, out.data_ptr(), ws.data_ptr(), nbytes.value, handle))
+            rows, _, out_stride = _heads("out", out, device, dtype, heads, dim)
+            if rows != ntok:
+                raise _invalid(f"q has {ntok} rows, out {rows}")
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
+    s = _lib.GeAttentionShape(code, heads, kv_heads, dim, scale, window, q_stride, k_stride, v_stride, pk_stride, pv_stride,
+                              out_stride)
+    L = _lib.lib()
+    if prefix_k is None:
+        rc = L.ge_attention_causal(device, s, q.data_ptr(), k.data_ptr(), v.data_ptr(), ntok, q_seqs.data_ptr(), nseq,
+                                   out.data_ptr(), ws.data_ptr(), nbytes, handle)
+    else:
+        rc = L.ge_attention_prefix(device, s, q.data_ptr(), ntok, k.data_ptr(), v.data_ptr(), nkv, prefix_k.data_ptr(),
+                                   prefix_v.data_ptr(), prefix, q_seqs.data_ptr(), kv_seqs.data_ptr(), nseq, out.data_ptr(),
+                                   ws.data_ptr(), nbytes, handle)
+    _call(rc)
     return out
 
 
@@ -180,14 +198,14 @@ class Q4Weight:
     mins: Any = None
 
     def __post_init__(self):
-        import torch
-        _on_device("values", self.values)
+        torch = _torch()[0]
+        device = _on_device("values", self.values)
         if self.values.dtype != torch.uint8 or self.values.dim() != 2 or not self.values.is_contiguous():
             raise _invalid("values must be a contiguous [n, k / 2] uint8 tensor")
         for name, t in (("scales", self.scales), ("mins", self.mins)):
             if t is None and name == "mins":
                 continue
-            _on_device(name, t, self.values)
+            _on_device(name, t, device)
             if t.dtype != torch.float16 or t.dim() != 2 or t.shape[0] != self.n or not t.is_contiguous():
                 raise _invalid(f"{name} must be a contiguous [{self.n}, k / group] float16 tensor")
         if self.mins is not None and self.mins.shape != self.scales.shape:
@@ -233,23 +251,33 @@ class Q4Weight:
 def linear_q4(x, weight: Q4Weight, out=None, stream=None):
     """x [rows, k] times the 4-bit weights (ge_linear_q4): out [rows, n] in x's type (float16 or
     bfloat16), for 0 to 64 rows.  x's rows may be a column range of a wider tensor."""
-    import torch
-    _on_device("x", x, weight.values)
-    if x.dim() != 2 or x.shape[1] != weight.k:
-        raise _invalid(f"x must be [rows, {weight.k}], got {list(x.shape)}")
+    torch = _torch()[0]
+    values, mins = weight.values, weight.mins
+    device = _on_device("x", x)
+    if values.get_device() != device:
+        raise _invalid(f"x is on cuda:{device}, the weight on {values.device}")
     dtype = _dtype(x)
-    if x.stride(1) != 1:
+    n, k = values.shape
+    k *= 2
+    shape = x.shape
+    if len(shape) != 2 or shape[1] != k:
+        raise _invalid(f"x must be [rows, {k}], got {list(shape)}")
+    rows = shape[0]
+    x_stride, step = x.stride()
+    if step != 1:
         raise _invalid("x's columns must lie side by side")
-    rows, n = x.shape[0], weight.n
-    handle, on = _stream(stream, x.device)
-    with torch.cuda.stream(on):
-        if out is None:
+    handle, on = _stream(stream, device)
+    out_stride = n
+    if out is None:
+        with on or _HERE:
             out = torch.empty((rows, n), dtype=x.dtype, device=x.device)
-        _on_device("out", out, x)
+    else:
+        _on_device("out", out, device)
         if out.dtype != x.dtype or out.shape != (rows, n) or (n > 1 and out.stride(1) != 1):
             raise _invalid(f"out must be a [{rows}, {n}] {x.dtype} tensor with its columns side by side")
-        _call(_lib.lib().ge_linear_q4(
-            x.device.index, dtype, x.data_ptr(), x.stride(0) if rows > 1 else weight.k, rows, weight.k,
-            weight.values.data_ptr(), weight.scales.data_ptr(), None if weight.mins is None else weight.mins.data_ptr(),
-            weight.group, n, out.data_ptr(), out.stride(0) if rows > 1 else n, handle))
+        if rows > 1:
+            out_stride = out.stride(0)
+    _call(_lib.lib().ge_linear_q4(device, dtype, x.data_ptr(), x_stride if rows > 1 else k, rows, k, values.data_ptr(),
+                                  weight.scales.data_ptr(), None if mins is None else mins.data_ptr(), weight.group, n,
+                                  out.data_ptr(), out_stride, handle))
     return out
