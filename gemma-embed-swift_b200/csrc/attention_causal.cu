@@ -50,8 +50,9 @@ namespace {
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kGrow = 8.0f;  // log2 units a row's maximum may grow before it is moved
 constexpr int kKeys = 128;     // keys of a block
-constexpr int kMaxPieces = 64;
+constexpr int kMaxPieces = 128;
 constexpr int kBuckets = 1024;
+constexpr size_t kPlanSmem = 200 * 1024;
 
 // ------------------------------------------------------------------------------------ sizes
 constexpr int tiles_per_item(int hd) { return hd == 256 ? 1 : 2; }
@@ -75,9 +76,13 @@ struct Header {
     int err;    // a wait that gave up
     int nwork;  // pieces in the work list
 };
-struct TileInfo {
+// An item: NT neighbouring tiles.
+struct alignas(16) TileInfo {
     int nblk, nseg, pieces, live;  // key blocks, own-key segments, pieces; bit x: tile x has rows of a sequence
     int lo0, hi0, lo1, hi1;        // per tile the hull of its rows' own keys
+    // Items inside one sequence (simple): row i sees [ks, ke) up to key see + i, as own_range has it; the
+    // others' rows have theirs in rng.
+    int simple, see, ks, ke;
 };
 struct Work {
     int tile, b0, b1, piece;    // blocks [b0, b1) of the tile; piece -1: the whole tile, straight to the output
@@ -118,7 +123,7 @@ Layout layout_of(const CausalLaunch& a, const Sizes& s) {
 struct PlanParams {
     const uint32_t* q_seqs;
     const uint32_t* kv_seqs;
-    int nseq, ntok, nkv, window, T, TI, tiles, kv_heads, prefix_blocks, lmax, sms;
+    int nseq, ntok, nkv, window, T, TI, tiles, mixed, kv_heads, prefix_blocks, lmax, sms;
     Header* head;
     int2 *rng, *segs;
     TileInfo* info;
@@ -128,122 +133,220 @@ struct PlanParams {
 __device__ __forceinline__ int warp_max_i(int v) { return __reduce_max_sync(0xffffffffu, v); }
 __device__ __forceinline__ int warp_min_i(int v) { return __reduce_min_sync(0xffffffffu, v); }
 
+// The own keys of a row that may see keys below `see` of the range [ks, ke).
+__device__ __forceinline__ int2 own_range(int see, int ks, int ke, int window) {
+    const int hi = max(ks, min(see, ke));
+    const int lo = window > 0 ? min(hi, max(ks, see - window)) : ks;
+    return make_int2(lo, hi);
+}
+
+// A sequence's rows [q0, q1) and keys [ks, ke), cut to the tensors; row q0 + i sees keys below see + i.
+struct Seq {
+    int q0, q1, ks, ke, see;
+    __device__ __forceinline__ Seq(const PlanParams& p, int s) {
+        const int64_t q = p.q_seqs[2 * s], n = p.q_seqs[2 * s + 1], k = p.kv_seqs[2 * s], m = p.kv_seqs[2 * s + 1];
+        q0 = int(min(q, int64_t(p.ntok)));
+        q1 = int(min(q + n, int64_t(p.ntok)));
+        ks = int(min(k, int64_t(p.nkv)));
+        ke = int(min(k + m, int64_t(p.nkv)));
+        // Rows and keys stay below 2^30, so a clamped value decides every row the same way.
+        see = int(max(int64_t(-(1 << 30)), min(k + m - n + 1, int64_t(1 << 30))));
+    }
+};
+
+// What the plan works on.  kShared: one CTA with everything in shared memory (ranges and segments of mixed
+// items only, at their slots), copied out at the end; else a cluster of CTAs on the workspace itself.
+template <bool kShared>
+struct PlanData {
+    TileInfo* info;
+    int2 *rng, *segs;
+    int TI;
+    // Item t's rows and segments; a shared mixed item's slot is kept in its `see`.
+    __device__ __forceinline__ int64_t at(int t) const { return int64_t(kShared ? info[t].see : t) * TI; }
+};
+
+// Segments, blocks and hulls of an item whose rows' ranges are in rng: its rows' own keys as disjoint
+// ascending segments, when the rows' ranges come in ascending order (lo never falls); else one segment
+// over all of them, the masks doing the rest.  By one warp.
+template <bool kShared>
+__device__ void plan_mixed(const PlanParams& p, const PlanData<kShared>& d, int t, int lane) {
+    const int2* rng = d.rng + d.at(t);
+    int2* seg = d.segs + d.at(t);
+    int lo_x[2] = {INT_MAX, INT_MAX}, hi_x[2] = {0, 0}, live = 0;
+    int end = -1, low = -1, nseg = 0;  // running maximum of hi and lo over the rows so far
+    bool sorted = true;
+    for (int i0 = 0; i0 < p.TI; i0 += 32) {
+        const int i = i0 + lane;
+        const int2 rg = i < p.TI && t * p.TI + i < p.ntok ? rng[i] : make_int2(0, -1);
+        const bool in = rg.y >= 0, some = rg.y > rg.x;
+        const int x = i >= p.T ? 1 : 0;
+#pragma unroll
+        for (int y = 0; y < 2; y++) {
+            lo_x[y] = min(lo_x[y], warp_min_i(some && x == y ? rg.x : INT_MAX));
+            hi_x[y] = max(hi_x[y], warp_max_i(some && x == y ? rg.y : 0));
+            if (__any_sync(0xffffffffu, in && x == y)) live |= 1 << y;
+        }
+        // Inclusive running maxima over the lanes, then those of the rows before each lane's.
+        int e = some ? rg.y : -1, l = some ? rg.x : -1;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int pe = __shfl_up_sync(0xffffffffu, e, o), pl = __shfl_up_sync(0xffffffffu, l, o);
+            if (lane >= o) {
+                e = max(e, pe);
+                l = max(l, pl);
+            }
+        }
+        int be = __shfl_up_sync(0xffffffffu, e, 1), bl = __shfl_up_sync(0xffffffffu, l, 1);
+        be = lane ? max(be, end) : end;
+        bl = lane ? max(bl, low) : low;
+        if (__any_sync(0xffffffffu, some && rg.x < bl)) sorted = false;
+        const bool fresh = some && rg.x > be;  // keys between be and lo are no row's
+        const unsigned fm = __ballot_sync(0xffffffffu, fresh);
+        if (fresh) {
+            const int at = nseg + __popc(fm & ((1u << lane) - 1));
+            seg[at].x = rg.x;
+            if (at > 0) seg[at - 1].y = be;
+        }
+        nseg += __popc(fm);
+        end = max(end, __shfl_sync(0xffffffffu, e, 31));
+        low = max(low, __shfl_sync(0xffffffffu, l, 31));
+    }
+    __syncwarp();
+    if (!sorted) {
+        nseg = 1;
+        if (lane == 0) seg[0] = make_int2(min(lo_x[0], lo_x[1]), max(hi_x[0], hi_x[1]));
+    } else if (nseg > 0 && lane == 0) {
+        seg[nseg - 1].y = end;
+    }
+    __syncwarp();
+    int nblk = 0;
+    for (int i = lane; i < nseg; i += 32) nblk += (seg[i].y - seg[i].x + kKeys - 1) / kKeys;
+    nblk = __reduce_add_sync(0xffffffffu, nblk) + (live ? p.prefix_blocks : 0);
+    const int slot = d.info[t].see;
+    __syncwarp();
+    if (lane == 0) d.info[t] = TileInfo{nblk, nseg, live ? 1 : 0, live, lo_x[0], hi_x[0], lo_x[1], hi_x[1], 0, slot, 0, 0};
+}
+
+template <bool kShared>
 __global__ void __launch_bounds__(1024) k_causal_plan(PlanParams p) {
+    extern __shared__ __align__(16) uint8_t plan_smem[];
     __shared__ int hist[kBuckets], warp_sum_s[32];
-    __shared__ int s_max, s_chunk;
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    pdl_wait();
-    pdl_launch();
-    if (tid == 0) {
-        p.head->err = 0;
-        s_max = 0;
+    __shared__ int s_max, s_chunk, s_slots;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int ctas = kShared ? 1 : int(gridDim.x), gtid = int(blockIdx.x) * 1024 + tid, gwarp = gtid >> 5, warps = ctas * 32;
+    const auto sync_all = [&]() {
+        if (ctas > 1) cluster_sync();
+        else __syncthreads();
+    };
+    PlanData<kShared> d{p.info, p.rng, p.segs, p.TI};
+    if (kShared) {
+        d.info = reinterpret_cast<TileInfo*>(plan_smem);
+        d.rng = reinterpret_cast<int2*>(d.info + p.tiles);
+        d.segs = d.rng + p.mixed * p.TI;
     }
     hist[tid] = 0;
-    // (lo, hi) per row; (0, -1) for rows of no sequence, which are never stored.
-    for (int r = tid; r < p.ntok; r += blockDim.x) p.rng[r] = make_int2(0, -1);
-    __syncthreads();
-    for (int s = warp; s < p.nseq; s += 32) {
-        const int64_t q0 = p.q_seqs[2 * s], n = p.q_seqs[2 * s + 1];
-        const int64_t k0 = p.kv_seqs[2 * s], m = p.kv_seqs[2 * s + 1];
-        // Ranges past the tensors are cut; a key range that starts outside holds no key.
-        const int64_t q1 = min(q0 + n, int64_t(p.ntok));
-        const int64_t ks = min(k0, int64_t(p.nkv)), ke = min(k0 + m, int64_t(p.nkv));
-        for (int64_t r = q0 + lane; r < q1; r += 32) {
-            const int64_t see = k0 + m - n + (r - q0) + 1;
-            const int64_t hi = max(ks, min(see, ke));
-            const int64_t lo = p.window > 0 ? min(hi, max(ks, see - p.window)) : ks;
-            p.rng[r] = make_int2(int(lo), int(hi));
+    if (tid == 0) s_max = s_slots = 0;
+    for (int t = gtid; kShared && t < p.tiles; t += 1024) d.info[t] = TileInfo{};  // no row of a sequence
+    pdl_wait();
+    pdl_launch();
+    if (gtid == 0) p.head->err = 0;
+    for (int t = gtid; !kShared && t < p.tiles; t += ctas * 1024) d.info[t] = TileInfo{};
+    sync_all();
+    // Items inside one sequence, one lane each; those a sequence begins or ends in are marked (live -1).
+    for (int s = gwarp; s < p.nseq; s += warps) {
+        const Seq q(p, s);
+        const int t1 = q.q1 / p.TI;
+        if (lane == 0 && q.q0 < q.q1) {
+            if (q.q0 % p.TI) d.info[q.q0 / p.TI].live = -1;
+            if (q.q1 % p.TI) d.info[q.q1 / p.TI].live = -1;
+        }
+        for (int t = (q.q0 + p.TI - 1) / p.TI + lane; t < t1; t += 32) {
+            const int see = q.see + (t * p.TI - q.q0);
+            const int2 a = own_range(see, q.ks, q.ke, p.window), b = own_range(see + p.T - 1, q.ks, q.ke, p.window);
+            const int2 c = own_range(see + p.T, q.ks, q.ke, p.window), e = own_range(see + p.TI - 1, q.ks, q.ke, p.window);
+            const bool two = p.TI > p.T;
+            const int lo = a.x, hi = two ? e.y : b.y;
+            TileInfo f{};
+            f.nseg = hi > lo ? 1 : 0;
+            f.nblk = p.prefix_blocks + (hi - lo + kKeys - 1) / kKeys;
+            f.pieces = 1;
+            f.live = two ? 3 : 1;
+            f.lo0 = a.x, f.hi0 = b.y;
+            f.lo1 = two ? c.x : INT_MAX, f.hi1 = two ? e.y : 0;
+            f.simple = 1;
+            f.see = see, f.ks = q.ks, f.ke = q.ke;
+            p.segs[int64_t(t) * p.TI] = make_int2(lo, hi);
+            d.info[t] = f;
         }
     }
-    __syncthreads();
-    // Per tile: its rows' own keys as disjoint ascending segments, when the rows' ranges come in
-    // ascending order (lo never falls); else one segment over all of them, the masks doing the rest.
-    for (int t = warp; t < p.tiles; t += 32) {
-        int2* seg = p.segs + int64_t(t) * p.TI;
-        int lo_x[2] = {INT_MAX, INT_MAX}, hi_x[2] = {0, 0}, live = 0;
-        int end = -1, low = -1, nseg = 0;  // running maximum of hi and lo over the rows so far
-        bool sorted = true;
-        for (int i0 = 0; i0 < p.TI; i0 += 32) {
-            const int i = i0 + lane, r = t * p.TI + i;
-            const int2 rg = i < p.TI && r < p.ntok ? p.rng[r] : make_int2(0, -1);
-            const bool in = rg.y >= 0, some = rg.y > rg.x;
-            const int x = i >= p.T ? 1 : 0;
-#pragma unroll
-            for (int y = 0; y < 2; y++) {
-                lo_x[y] = min(lo_x[y], warp_min_i(some && x == y ? rg.x : INT_MAX));
-                hi_x[y] = max(hi_x[y], warp_max_i(some && x == y ? rg.y : 0));
-                if (__any_sync(0xffffffffu, in && x == y)) live |= 1 << y;
-            }
-            // Inclusive running maxima over the lanes, then those of the rows before each lane's.
-            int e = some ? rg.y : -1, l = some ? rg.x : -1;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const int pe = __shfl_up_sync(0xffffffffu, e, o), pl = __shfl_up_sync(0xffffffffu, l, o);
-                if (lane >= o) {
-                    e = max(e, pe);
-                    l = max(l, pl);
-                }
-            }
-            int be = __shfl_up_sync(0xffffffffu, e, 1), bl = __shfl_up_sync(0xffffffffu, l, 1);
-            be = lane ? max(be, end) : end;
-            bl = lane ? max(bl, low) : low;
-            if (__any_sync(0xffffffffu, some && rg.x < bl)) sorted = false;
-            const bool fresh = some && rg.x > be;  // keys between be and lo are no row's
-            const unsigned fm = __ballot_sync(0xffffffffu, fresh);
-            if (fresh) {
-                const int at = nseg + __popc(fm & ((1u << lane) - 1));
-                seg[at].x = rg.x;
-                if (at > 0) seg[at - 1].y = be;
-            }
-            nseg += __popc(fm);
-            end = max(end, __shfl_sync(0xffffffffu, e, 31));
-            low = max(low, __shfl_sync(0xffffffffu, l, 31));
-        }
-        __syncwarp();
-        if (!sorted) {
-            nseg = 1;
-            if (lane == 0) seg[0] = make_int2(min(lo_x[0], lo_x[1]), max(hi_x[0], hi_x[1]));
-        } else if (nseg > 0 && lane == 0) {
-            seg[nseg - 1].y = end;
-        }
-        __syncwarp();
-        int nblk = 0;
-        for (int i = lane; i < nseg; i += 32) nblk += (seg[i].y - seg[i].x + kKeys - 1) / kKeys;
-        nblk = __reduce_add_sync(0xffffffffu, nblk) + (live ? p.prefix_blocks : 0);
-        if (lane == 0) {
-            p.info[t] = TileInfo{nblk, nseg, live ? 1 : 0, live, lo_x[0], hi_x[0], lo_x[1], hi_x[1]};
-            atomicMax(&s_max, nblk);
+    sync_all();
+    // The marked (mixed) items' rows: none of a sequence, then the sequences' first and last ones.
+    if (kShared) {
+        for (int t = tid; t < p.tiles; t += 1024)
+            if (d.info[t].live < 0) d.info[t].see = atomicAdd(&s_slots, 1);
+        for (int i = tid; i < p.mixed * p.TI; i += 1024) d.rng[i] = make_int2(0, -1);
+    } else {
+        for (int r = gtid; r < p.ntok; r += ctas * 1024)
+            if (d.info[r / p.TI].live < 0) d.rng[r] = make_int2(0, -1);
+    }
+    sync_all();
+    for (int s = gwarp; s < p.nseq; s += warps) {
+        const Seq q(p, s);
+        const int head_end = min(q.q1, (q.q0 + p.TI - 1) / p.TI * p.TI);
+        const auto fill = [&](int r0, int r1) {  // rows of one item
+            if (r0 >= r1) return;
+            const int t = r0 / p.TI;
+            if (d.info[t].live >= 0) return;  // another sequence claims the whole item
+            int2* rng = d.rng + d.at(t);
+            for (int r = r0 + lane; r < r1; r += 32) rng[r - t * p.TI] = own_range(q.see + (r - q.q0), q.ks, q.ke, p.window);
+        };
+        fill(q.q0, head_end);
+        fill(max(head_end, q.q1 / p.TI * p.TI), q.q1);
+    }
+    sync_all();
+    for (int t0 = gwarp; t0 < p.tiles; t0 += warps * 32) {  // each warp looks at 32 items, `warps` apart
+        const int mine = t0 + lane * warps;
+        unsigned todo = __ballot_sync(0xffffffffu, mine < p.tiles && d.info[mine].live < 0);
+        while (todo) {
+            const int b = __ffs(todo) - 1;
+            todo &= todo - 1;
+            plan_mixed<kShared>(p, d, t0 + b * warps, lane);
         }
     }
-    __syncthreads();
-    // Blocks per piece: the fewest for which the pieces of all tiles and KV heads still fit one round of
+    sync_all();
+    if (blockIdx.x != 0) return;
+    // Blocks per piece: the fewest for which the pieces of all items and KV heads still fit one round of
     // the SMs (a second, short round would cost as much as the first).
-    if (warp == 0) {
-        int lo = max(1, s_max);
-        if (p.lmax > 1) {
-            int hi = lo;  // fits: one piece per tile
-            lo = max(1, (s_max + p.lmax - 1) / p.lmax);
+    if (p.lmax > 1) {
+        int m = 0;
+        for (int t = tid; t < p.tiles; t += 1024) m = max(m, d.info[t].nblk);
+        m = warp_max_i(m);
+        if (lane == 0) atomicMax(&s_max, m);
+        __syncthreads();
+        if (warp == 0) {
+            // Fewer items than SMs here, so a lane holds up to a handful; `hi` fits, one piece per item.
+            int hi = max(1, s_max), lo = max(1, (s_max + p.lmax - 1) / p.lmax);
             while (lo < hi) {
                 const int mid = (lo + hi) >> 1;
                 int n = 0;
-                for (int t = lane; t < p.tiles; t += 32) n += max(p.info[t].live ? 1 : 0, (p.info[t].nblk + mid - 1) / mid);
+                for (int t = lane; t < p.tiles; t += 32) n += max(d.info[t].live ? 1 : 0, (d.info[t].nblk + mid - 1) / mid);
                 n = __reduce_add_sync(0xffffffffu, n);
                 if (int64_t(n) * p.kv_heads <= p.sms) hi = mid;
                 else lo = mid + 1;
             }
+            if (lane == 0) s_chunk = lo;
         }
-        if (lane == 0) s_chunk = lo;
+        __syncthreads();
     }
-    __syncthreads();
-    const int chunk = s_chunk;
+    const int chunk = p.lmax > 1 ? s_chunk : INT_MAX;
     // Costliest pieces first (a counting sort by blocks; the order within a bucket does not matter).
-    for (int t = tid; t < p.tiles; t += blockDim.x) {
-        TileInfo* f = p.info + t;
+    for (int t = tid; t < p.tiles; t += 1024) {
+        TileInfo* f = d.info + t;
+        const int nblk = f->nblk;
         if (!f->live) continue;
-        const int pieces = max(1, (f->nblk + chunk - 1) / chunk), sz = (f->nblk + pieces - 1) / pieces;
-        // The last piece may come out shorter, or empty and dropped.
-        const int used = sz ? (f->nblk + sz - 1) / sz : 1;
-        f->pieces = used;
+        const int pieces = max(1, nblk / chunk + (nblk % chunk ? 1 : 0)), sz = (nblk + pieces - 1) / pieces;
+        const int used = sz ? (nblk + sz - 1) / sz : 1;  // the last piece may come out empty, and is dropped
+        if (used > 1) f->pieces = used;
         atomicAdd(&hist[min(sz, kBuckets - 1)], used);
     }
     __syncthreads();
@@ -261,30 +364,52 @@ __global__ void __launch_bounds__(1024) k_causal_plan(PlanParams p) {
         int before = 0;
         for (int w = 0; w < warp; w++) before += warp_sum_s[w];
         hist[kBuckets - 1 - tid] = before + inc - v;
-        if (tid == blockDim.x - 1) p.head->nwork = before + inc;
+        if (tid == 1023) p.head->nwork = before + inc;
     }
     __syncthreads();
-    for (int t = tid; t < p.tiles; t += blockDim.x) {
-        const TileInfo f = p.info[t];
-        if (!f.live) continue;
-        const int sz = (f.nblk + f.pieces - 1) / f.pieces;
-        int at = atomicAdd(&hist[min(sz, kBuckets - 1)], f.pieces);
-        const int2* seg = p.segs + int64_t(t) * p.TI;
-        int s = 0, first = p.prefix_blocks;  // segment s starts at block `first`
-        for (int i = 0; i < f.pieces; i++, at++) {
-            const int b0 = i * sz, b1 = min(f.nblk, b0 + sz);
-            int pos = 0;
-            if (f.nseg > 0) {
-                while (s + 1 < f.nseg) {
-                    const int n = (seg[s].y - seg[s].x + kKeys - 1) / kKeys;
-                    if (b0 < first + n) break;
-                    first += n;
-                    s++;
+    for (int t = tid; t < p.tiles; t += 1024) {
+        const int4 f = *reinterpret_cast<const int4*>(d.info + t);  // nblk, nseg, pieces, live
+        if (!f.w || f.z > 1) continue;
+        const int at = atomicAdd(&hist[min(f.x, kBuckets - 1)], 1);
+        int pos = 0;
+        if (f.y > 0) pos = d.info[t].simple ? p.segs[int64_t(t) * p.TI].x : d.segs[d.at(t)].x;
+        p.work[at] = Work{t, 0, f.x, -1, 0, pos, f.y, f.w};
+    }
+    if (p.lmax > 1) {
+        for (int t = warp; t < p.tiles; t += 32) {  // a warp per cut item, a lane per piece
+            const int4 f = *reinterpret_cast<const int4*>(d.info + t);
+            if (!f.w || f.z <= 1) continue;
+            const int sz = (f.x + f.z - 1) / f.z;
+            int at = lane ? 0 : atomicAdd(&hist[min(sz, kBuckets - 1)], f.z);
+            at = __shfl_sync(0xffffffffu, at, 0);
+            const int2* seg = d.info[t].simple ? p.segs + int64_t(t) * p.TI : d.segs + d.at(t);
+            for (int i = lane; i < f.z; i += 32) {
+                const int b0 = i * sz, b1 = min(f.x, b0 + sz);
+                int s = 0, first = p.prefix_blocks, pos = 0;  // segment s starts at block `first`
+                if (f.y > 0) {
+                    while (s + 1 < f.y) {
+                        const int n = (seg[s].y - seg[s].x + kKeys - 1) / kKeys;
+                        if (b0 < first + n) break;
+                        first += n;
+                        s++;
+                    }
+                    pos = seg[s].x + max(0, b0 - first) * kKeys;
                 }
-                pos = seg[s].x + max(0, b0 - first) * kKeys;
+                p.work[at + i] = Work{t, b0, b1, i, s, pos, f.y, f.w};
             }
-            p.work[at] = Work{t, b0, b1, f.pieces > 1 ? i : -1, s, pos, f.nseg, f.live};
         }
+    }
+    if (kShared) {
+        for (int t = warp; t < p.tiles; t += 32) {
+            if (d.info[t].simple || !d.info[t].live) continue;
+            const int64_t from = d.at(t), to = int64_t(t) * p.TI;
+            for (int i = lane; i < p.TI; i += 32) {
+                if (t * p.TI + i < p.ntok) p.rng[to + i] = d.rng[from + i];
+                if (i < d.info[t].nseg) p.segs[to + i] = d.segs[from + i];
+            }
+        }
+        for (int i = tid; i < p.tiles * int(sizeof(TileInfo) / 16); i += 1024)
+            reinterpret_cast<int4*>(p.info)[i] = reinterpret_cast<const int4*>(d.info)[i];
     }
 }
 
@@ -309,7 +434,7 @@ struct TcParams {
     const void *q, *k, *v, *pk, *pv;
     void* out;
     int64_t q_stride, k_stride, v_stride, pk_stride, pv_stride, out_stride;
-    int heads, kv_heads, group, T, TI, ntok, prefix, prefix_blocks;
+    int heads, kv_heads, group, T, TI, ntok, window, prefix, prefix_blocks;
     float scale_log2e;
     Header* head;
     const int2 *rng, *segs;
@@ -701,7 +826,11 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1)
             const Piece s = load_piece(p, id);
             const int row = s.tile * p.TI + x * p.T + token;
             const bool query = r < live_rows && row < p.ntok;
-            const int2 rg = query ? p.rng[row] : make_int2(0, -1);
+            int2 rg = make_int2(0, -1);
+            if (query) {
+                const int4 f = reinterpret_cast<const int4*>(p.info + s.tile)[2];  // simple, see, ks, ke
+                rg = f.x ? own_range(f.y + (row - s.tile * p.TI), f.z, f.w, p.window) : p.rng[row];
+            }
             float m = -INFINITY, l = 0.f;
             int count = 0;
             for (Cursor c(p, s); c.b < s.b1; c.next(p, s)) {
@@ -853,43 +982,59 @@ struct MergeParams {
     const float2* ml;
 };
 
-// One warp per (row, head): out = sum_c 2^(m_c - m) O_c / sum_c 2^(m_c - m) l_c, m the largest m_c.
+// One CTA of 128 threads per (row, head): out = sum_c 2^(m_c - m) O_c / sum_c 2^(m_c - m) l_c, m the
+// largest m_c.  Thread c weighs piece c; the warps add every fourth piece each, joined in order.
 template <typename E, int D>
 __global__ void __launch_bounds__(128) k_causal_merge(MergeParams p) {
+    __shared__ float w[kMaxPieces], red_m[4], red_l[4], part[4][D];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     pdl_wait();
     pdl_launch();
-    const int64_t id = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 5);
-    const int lane = threadIdx.x & 31;
-    if (id >= int64_t(p.ntok) * p.heads) return;
-    const int row = int(id / p.heads);
-    const int n = p.info[row / p.TI].pieces;
-    if (n <= 1 || p.rng[row].y < 0) return;
-    const int64_t step = int64_t(p.ntok) * p.heads;
-    float2 a = lane < n ? p.ml[lane * step + id] : make_float2(-INFINITY, 0.f);
-    float2 b = lane + 32 < n ? p.ml[(lane + 32) * step + id] : make_float2(-INFINITY, 0.f);
-    const bool nan = __any_sync(0xffffffffu, isnan(a.x) || isnan(b.x));
-    const float m = warp_max(fmaxf(a.x, b.x));
-    float wa = a.x == -INFINITY ? 0.f : ex2_approx(a.x - m), wb = b.x == -INFINITY ? 0.f : ex2_approx(b.x - m);
-    const float l = warp_sum(wa * a.y + wb * b.y);
-    const float inv = nan ? NAN : l == 0.f ? 0.f : 1.0f / l;
-    float acc[D / 32];
+    const int row = int(blockIdx.x) / p.heads, head = int(blockIdx.x) - row * p.heads;
+    const TileInfo* f = p.info + row / p.TI;
+    const int n = f->pieces;
+    if (n <= 1 || !f->live || (!f->simple && p.rng[row].y < 0)) return;
+    const int64_t step = int64_t(p.ntok) * p.heads, id = int64_t(row) * p.heads + head;
+    const float2 ml = tid < n ? p.ml[tid * step + id] : make_float2(-INFINITY, 0.f);
+    const bool nan = __syncthreads_or(isnan(ml.x));
+    float m = warp_max(ml.x);
+    if (lane == 0) red_m[warp] = m;
+    __syncthreads();
+    m = fmaxf(fmaxf(red_m[0], red_m[1]), fmaxf(red_m[2], red_m[3]));
+    const float wt = ml.x == -INFINITY ? 0.f : ex2_approx(ml.x - m);  // 0: no visible key, and no row was left
+    if (tid < n) w[tid] = wt;
+    const float l = warp_sum(wt * ml.y);
+    if (lane == 0) red_l[warp] = l;
+    __syncthreads();
+    constexpr int P = D / 32;
+    float acc[P];
 #pragma unroll
-    for (int i = 0; i < D / 32; i++) acc[i] = 0.f;
-    for (int c = 0; c < n; c++) {
-        const float w = c < 32 ? __shfl_sync(0xffffffffu, wa, c) : __shfl_sync(0xffffffffu, wb, c - 32);
-        if (w == 0.f) continue;  // a piece without a visible key left no row
-        const float2* src = reinterpret_cast<const float2*>(p.o + (c * step + id) * D + lane * (D / 32));
+    for (int i = 0; i < P; i++) acc[i] = 0.f;
+#pragma unroll 4
+    for (int c = warp; c < n; c += 4) {
+        const float wc = w[c];
+        const float2* src = reinterpret_cast<const float2*>(p.o + (c * step + id) * D + lane * P);
 #pragma unroll
-        for (int i = 0; i < D / 64; i++) {
-            const float2 v = src[i];
-            acc[2 * i] = fmaf(w, v.x, acc[2 * i]);
-            acc[2 * i + 1] = fmaf(w, v.y, acc[2 * i + 1]);
+        for (int i = 0; i < P / 2; i++) {
+            const float2 v = wc != 0.f ? src[i] : make_float2(0.f, 0.f);
+            acc[2 * i] = fmaf(wc, v.x, acc[2 * i]);
+            acc[2 * i + 1] = fmaf(wc, v.y, acc[2 * i + 1]);
         }
     }
-    uint32_t* o = reinterpret_cast<uint32_t*>(static_cast<E*>(p.out) + row * p.out_stride + int64_t(id - int64_t(row) * p.heads) * D +
-                                              lane * (D / 32));
 #pragma unroll
-    for (int i = 0; i < D / 64; i++) o[i] = float_to_pair<E>(acc[2 * i] * inv, acc[2 * i + 1] * inv);
+    for (int i = 0; i < P; i++) part[warp][lane * P + i] = acc[i];
+    __syncthreads();
+    const float lt = (red_l[0] + red_l[1]) + (red_l[2] + red_l[3]);
+    const float inv = nan ? NAN : lt == 0.f ? 0.f : 1.0f / lt;
+    if (tid < D / 2) {
+        float v[2];
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            const int d = 2 * tid + i;
+            v[i] = ((part[0][d] + part[1][d]) + (part[2][d] + part[3][d])) * inv;
+        }
+        reinterpret_cast<uint32_t*>(static_cast<E*>(p.out) + row * p.out_stride + int64_t(head) * D)[tid] = float_to_pair<E>(v[0], v[1]);
+    }
 }
 
 // ------------------------------------------------------------------------------------ launch
@@ -913,14 +1058,14 @@ cudaError_t launch_t(const CausalLaunch& a, const Sizes& s, const Layout& l, cud
                          !encode_fp16_map(&mpv, pv, kw, uint64_t(a.prefix), 64, 32, uint64_t(a.pv_stride))))
         return cudaErrorInvalidValue;
     TcParams p{a.q, a.k, a.v, a.pk, a.pv, a.out, a.q_stride, a.k_stride, a.v_stride, a.pk_stride, a.pv_stride, a.out_stride,
-               a.heads, a.kv_heads, s.group, s.T, s.TI, a.ntok, a.prefix, (a.prefix + kKeys - 1) / kKeys, a.scale * kLog2e,
+               a.heads, a.kv_heads, s.group, s.T, s.TI, a.ntok, std::min(a.window, 1 << 30), a.prefix, (a.prefix + kKeys - 1) / kKeys, a.scale * kLog2e,
                l.head, l.rng, l.segs, l.info, l.work, l.o, l.ml};
     const int64_t most = s.lmax > 1 ? a.num_sms : int64_t(s.tiles) * a.kv_heads;
-    e = launch_pdl(k_causal_tc<E, D>, unsigned(std::min<int64_t>(a.num_sms, most)), C::kThreads, size_t(C::kSmem), stream, mq, mk, mv,
+    e = launch_pdl(k_causal_tc<E, D>, unsigned(std::min<int64_t>(a.num_sms, most)), C::kThreads, size_t(C::kSmem), stream, 1, mq, mk, mv,
                    mpk, mpv, p);
     if (e != cudaSuccess || s.lmax == 1) return e;
     MergeParams mp{a.out, a.out_stride, a.heads, a.ntok, s.TI, l.rng, l.info, l.o, l.ml};
-    return launch_pdl(k_causal_merge<E, D>, unsigned((int64_t(a.ntok) * a.heads + 3) / 4), 128, 0, stream, mp);
+    return launch_pdl(k_causal_merge<E, D>, unsigned(int64_t(a.ntok) * a.heads), 128, 0, stream, 1, mp);
 }
 
 template <typename E>
@@ -937,9 +1082,21 @@ size_t causal_workspace(const CausalLaunch& a) { return layout_of(a, sizes_of(a)
 cudaError_t launch_causal(const CausalLaunch& a, cudaStream_t stream) {
     const Sizes s = sizes_of(a);
     const Layout l = layout_of(a, s);
-    PlanParams pp{a.q_seqs, a.kv_seqs, a.nseq, a.ntok, a.nkv, a.window, s.T, s.TI, s.tiles, a.kv_heads,
+    const int window = std::min(a.window, 1 << 30);  // no range is longer
+    // Items that hold a sequence's first or last row, at most.
+    const int mixed = int(std::min<int64_t>(s.tiles, 2 * int64_t(a.nseq)));
+    PlanParams pp{a.q_seqs, a.kv_seqs, a.nseq, a.ntok, a.nkv, window, s.T, s.TI, s.tiles, mixed, a.kv_heads,
                   (a.prefix + kKeys - 1) / kKeys, s.lmax, a.num_sms, l.head, l.rng, l.segs, l.info, l.work};
-    const cudaError_t e = launch_pdl(k_causal_plan, 1, 1024, 0, stream, pp);
+    // Up to here the plan fits one CTA's shared memory (about 6000 rows in short sequences, 100,000 in long
+    // ones): no phase of it waits for global memory.  Beyond, a cluster of 8 works on the workspace.
+    const size_t smem = size_t(s.tiles) * sizeof(TileInfo) + size_t(mixed) * s.TI * 2 * sizeof(int2);
+    cudaError_t e;
+    if (smem <= kPlanSmem) {
+        e = cudaFuncSetAttribute(k_causal_plan<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(kPlanSmem));
+        if (e == cudaSuccess) e = launch_pdl(k_causal_plan<true>, 1, 1024, smem, stream, 1, pp);
+    } else {
+        e = launch_pdl(k_causal_plan<false>, 8, 1024, 0, stream, 8, pp);
+    }
     if (e != cudaSuccess) return e;
     return a.bf16 ? launch_e<__nv_bfloat16>(a, s, l, stream) : launch_e<__half>(a, s, l, stream);
 }

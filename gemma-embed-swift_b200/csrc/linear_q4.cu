@@ -322,7 +322,7 @@ cudaError_t launch_t(const Q4Launch& a, cudaStream_t stream) {
     const int stages = (a.k + kStageK - 1) / kStageK;
     p.S = std::max(1, std::min(std::min(kWarps / p.R, C::kMaxSplit), stages));
     p.Ks = (stages + p.S - 1) / p.S * kStageK;
-    return launch_pdl(k_linear_q4<T, NB, kMins>, unsigned(grid), kThreads, size_t(C::kSmem), stream, p);
+    return launch_pdl(k_linear_q4<T, NB, kMins>, unsigned(grid), kThreads, size_t(C::kSmem), stream, 1, p);
 }
 
 template <typename T, int NB>

@@ -12,10 +12,11 @@ namespace ge {
 // Launches with programmatic stream serialisation whatever the calling thread's policy: every kernel
 // of the operators waits for its predecessor (pdl_wait) before it touches memory.
 template <typename... KArgs, typename... Args>
-cudaError_t launch_pdl(void (*kern)(KArgs...), unsigned grid, unsigned block, size_t smem, cudaStream_t stream, Args&&... args) {
+cudaError_t launch_pdl(void (*kern)(KArgs...), unsigned grid, unsigned block, size_t smem, cudaStream_t stream, int cluster,
+                       Args&&... args) {
     const bool was = programmatic_launch();
     set_programmatic_launch(true);
-    const cudaError_t e = launch_kernel(kern, dim3(grid), dim3(block), smem, stream, 1, std::forward<Args>(args)...);
+    const cudaError_t e = launch_kernel(kern, dim3(grid), dim3(block), smem, stream, cluster, std::forward<Args>(args)...);
     set_programmatic_launch(was);
     return e;
 }

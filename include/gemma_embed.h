@@ -517,8 +517,8 @@ GE_API int ge_attention_workspace(int32_t device_ordinal, const ge_attention_sha
  * q[i] . k[j]) v[j] over the rows j <= i of its sequence (j > i - window under a window), head h
  * reading KV head h / (heads / kv_heads).  q and out are [ntok][heads][head_dim], k and v
  * [ntok][kv_heads][head_dim]; d_seqs holds nseq (start, length) pairs on the device.  Ranges are cut
- * at ntok, empty ones are allowed, ranges that share rows are not (their rows hold one or the
- * other); rows of `out` in no range are left as they were.  Scores, sums and maxima are fp32,
+ * at ntok and may be empty; query rows that two ranges share hold unspecified values.  Rows of `out` in
+ * no range are left as they were; `out` must not overlap the inputs.  Scores, sums and maxima are fp32,
  * probabilities are rounded to dtype before their product with v, the result once to dtype. */
 GE_API int ge_attention_causal(int32_t device_ordinal, const ge_attention_shape* shape, const void* d_q, const void* d_k,
                                const void* d_v, int32_t ntok, const uint32_t* d_seqs, int32_t nseq, void* d_out,

@@ -71,7 +71,7 @@ def test_causal_lengths(ge, torch, heads, kvh, dim, dtype, lens):
 
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("heads,kvh,dim", [(3, 1, 256), (8, 2, 128), (2, 2, 64)])
-@pytest.mark.parametrize("window", [1, 2, 63, 128, 200, 5000])
+@pytest.mark.parametrize("window", [1, 2, 63, 128, 200, 5000, 2**31 - 1])
 def test_causal_window(ge, torch, heads, kvh, dim, dtype, window):
     check_causal(ge, torch, [1, 130, 300, 77, 513], heads, kvh, dim, dtype, window=window)
 
@@ -506,3 +506,28 @@ def test_another_device_than_the_current_one(ge, torch):
         assert torch.cuda.current_device() == 0
     want, bound, _ = ref.attention(q, k, k, [(0, 9)], [(0, 9)], 0.125)
     ref.check(got, want, bound)
+
+
+@pytest.mark.parametrize("seqs", [[(40, 8)], [(0, 0)], [(100, 28), (100, 28)], [(0, 128), (5, 3), (60, 10)], [(64, 900)]])
+def test_rows_of_no_sequence_and_shared_rows(ge, torch, seqs):
+    """Most rows in no sequence, and ranges that share rows: no row outside every range is touched, rows of one
+    range alone are right (shared ones are unspecified)."""
+    q, k, v = (normal(torch, 31 + i, (1000, h, 64), "f16") for i, h in enumerate((2, 1, 1)))
+    out = torch.full_like(q, 7.0)
+    ge.attention_causal(q, k, v, dev(torch, seqs), out=out)
+    cover = torch.zeros(1000, dtype=torch.int32, device="cuda")
+    for s, n in seqs:
+        cover[s:s + n] += 1
+    assert (out[cover == 0] == 7.0).all()
+    if (cover < 2).all():
+        want, bound, touched = ref.attention(q, k, v, seqs, seqs, 0.125)
+        ref.check(out[touched], want[touched], bound[touched])
+
+
+def test_causal_more_sequences_than_the_plan_holds_in_one_cta(ge, torch):
+    """Thousands of short sequences (their plan is a cluster's), some of them empty, among long ones."""
+    lens = [int(n) for n in np.random.default_rng(6).integers(0, 12, 6000)]
+    lens[100] = 900
+    lens[4000] = 300
+    check_causal(ge, torch, lens, 4, 2, 64, "f16")
+    check_causal(ge, torch, lens, 2, 1, 256, "bf16", window=5)
