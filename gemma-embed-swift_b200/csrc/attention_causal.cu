@@ -52,7 +52,7 @@ constexpr float kGrow = 8.0f;  // log2 units a row's maximum may grow before it 
 constexpr int kKeys = 128;     // keys of a block
 constexpr int kMaxPieces = 128;
 constexpr int kBuckets = 1024;
-constexpr size_t kPlanSmem = 200 * 1024;
+constexpr int kMaxSms = 256;  // room for a cut call's items (fewer than SMs)
 
 // ------------------------------------------------------------------------------------ sizes
 constexpr int tiles_per_item(int hd) { return hd == 256 ? 1 : 2; }
@@ -84,9 +84,12 @@ struct alignas(16) TileInfo {
     // others' rows have theirs in rng.
     int simple, see, ks, ke;
 };
-struct Work {
-    int tile, b0, b1, piece;    // blocks [b0, b1) of the tile; piece -1: the whole tile, straight to the output
-    int seg, pos, nseg, live;   // where b0's own keys start
+// A piece of an item, all that the main kernel's roles need of it but further segments and mixed rows.
+struct alignas(16) Work {
+    int tile, b0, b1, piece;     // blocks [b0, b1) of the item; piece -1: the whole item, straight to the output
+    int seg, nseg, pos, end;     // where b0's own keys start, and that segment's end
+    int lo0, hi0, lo1, hi1;
+    int flags, see, ks, ke;      // flags: live, and 4 for simple
 };
 
 struct Layout {
@@ -123,7 +126,7 @@ Layout layout_of(const CausalLaunch& a, const Sizes& s) {
 struct PlanParams {
     const uint32_t* q_seqs;
     const uint32_t* kv_seqs;
-    int nseq, ntok, nkv, window, T, TI, tiles, mixed, kv_heads, prefix_blocks, lmax, sms;
+    int nseq, ntok, nkv, window, T, TI, tiles, kv_heads, prefix_blocks, lmax, sms;
     Header* head;
     int2 *rng, *segs;
     TileInfo* info;
@@ -143,8 +146,8 @@ __device__ __forceinline__ int2 own_range(int see, int ks, int ke, int window) {
 // A sequence's rows [q0, q1) and keys [ks, ke), cut to the tensors; row q0 + i sees keys below see + i.
 struct Seq {
     int q0, q1, ks, ke, see;
-    __device__ __forceinline__ Seq(const PlanParams& p, int s) {
-        const int64_t q = p.q_seqs[2 * s], n = p.q_seqs[2 * s + 1], k = p.kv_seqs[2 * s], m = p.kv_seqs[2 * s + 1];
+    __device__ __forceinline__ Seq(const PlanParams& p, const uint4& w) {
+        const int64_t q = w.x, n = w.y, k = w.z, m = w.w;
         q0 = int(min(q, int64_t(p.ntok)));
         q1 = int(min(q + n, int64_t(p.ntok)));
         ks = int(min(k, int64_t(p.nkv)));
@@ -154,37 +157,98 @@ struct Seq {
     }
 };
 
-// What the plan works on.  kShared: one CTA with everything in shared memory (ranges and segments of mixed
-// items only, at their slots), copied out at the end; else a cluster of CTAs on the workspace itself.
-template <bool kShared>
-struct PlanData {
-    TileInfo* info;
-    int2 *rng, *segs;
-    int TI;
-    // Item t's rows and segments; a shared mixed item's slot is kept in its `see`.
-    __device__ __forceinline__ int64_t at(int t) const { return int64_t(kShared ? info[t].see : t) * TI; }
-};
+// Sequence ranges in shared memory (those past kPlanSeqs are read from global memory).
+constexpr int kPlanSeqs = 4096, kMaxItemRows = 256;
+constexpr size_t plan_smem(int nseq) {
+    return size_t(nseq < kPlanSeqs ? nseq : kPlanSeqs) * sizeof(uint4) + 32 * 2 * kMaxItemRows * sizeof(int2);
+}
+__device__ __forceinline__ uint4 seq_words(const PlanParams& p, int s) {
+    return make_uint4(p.q_seqs[2 * s], p.q_seqs[2 * s + 1], p.kv_seqs[2 * s], p.kv_seqs[2 * s + 1]);
+}
+__device__ __forceinline__ uint4 shfl_words(const uint4& w, int src) {
+    return make_uint4(__shfl_sync(0xffffffffu, w.x, src), __shfl_sync(0xffffffffu, w.y, src), __shfl_sync(0xffffffffu, w.z, src),
+                      __shfl_sync(0xffffffffu, w.w, src));
+}
+// Rows a sequence has among [r0, r1), as offsets from r0: [x, y), empty unless x < y.
+__device__ __forceinline__ int2 rows_within(const uint4& w, int r0, int r1) {
+    const int64_t q0 = w.x, q1 = int64_t(w.x) + w.y;
+    return make_int2(int(min(max(q0, int64_t(r0)), int64_t(r1)) - r0), int(max(min(q1, int64_t(r1)), int64_t(r0)) - r0));
+}
 
-// Segments, blocks and hulls of an item whose rows' ranges are in rng: its rows' own keys as disjoint
-// ascending segments, when the rows' ranges come in ascending order (lo never falls); else one segment
-// over all of them, the masks doing the rest.  By one warp.
-template <bool kShared>
-__device__ void plan_mixed(const PlanParams& p, const PlanData<kShared>& d, int t, int lane) {
-    const int2* rng = d.rng + d.at(t);
-    int2* seg = d.segs + d.at(t);
-    int lo_x[2] = {INT_MAX, INT_MAX}, hi_x[2] = {0, 0}, live = 0;
-    int end = -1, low = -1, nseg = 0;  // running maximum of hi and lo over the rows so far
+// One item, by one warp: rng and seg are the warp's own shared memory.
+__device__ void plan_item(const PlanParams& p, const uint4* seqs, int2* rng, int2* seg, int t, int lane) {
+    const int r0 = t * p.TI, n = min(p.TI, p.ntok - r0);
+    TileInfo f{};
+    bool any = false;
+    for (int s0 = 0; s0 < p.nseq; s0 += 32) {
+        const int s = s0 + lane;
+        const uint4 w = s >= p.nseq ? make_uint4(0, 0, 0, 0) : s < kPlanSeqs ? seqs[s] : seq_words(p, s);
+        const int2 in = rows_within(w, r0, r0 + n);
+        any |= in.x < in.y;
+        const unsigned whole = __ballot_sync(0xffffffffu, in.x == 0 && in.y == n);
+        if (whole) {  // the item lies inside one sequence
+            const Seq q(p, shfl_words(w, __ffs(whole) - 1));
+            const int see = q.see + (r0 - q.q0), n0 = min(p.T, n);
+            const int2 a = own_range(see, q.ks, q.ke, p.window), b = own_range(see + n0 - 1, q.ks, q.ke, p.window);
+            const int2 e = own_range(see + n - 1, q.ks, q.ke, p.window);
+            f.live = n > n0 ? 3 : 1;
+            f.lo0 = a.x, f.hi0 = b.y;
+            f.lo1 = f.live == 3 ? own_range(see + n0, q.ks, q.ke, p.window).x : INT_MAX;
+            f.hi1 = f.live == 3 ? e.y : 0;
+            f.nseg = e.y > a.x ? 1 : 0;
+            f.nblk = p.prefix_blocks + (e.y - a.x + kKeys - 1) / kKeys;
+            f.simple = 1, f.see = see, f.ks = q.ks, f.ke = q.ke;
+            f.pieces = 1;
+            if (lane == 0) {
+                p.segs[int64_t(t) * p.TI] = make_int2(a.x, e.y);
+                p.info[t] = f;
+            }
+            return;
+        }
+    }
+    if (!__any_sync(0xffffffffu, any)) {
+        if (lane == 0) p.info[t] = f;  // live 0: no row of a sequence, no work
+        return;
+    }
+    for (int i = lane; i < p.TI; i += 32) rng[i] = make_int2(0, -1);
+    __syncwarp();
+    for (int s0 = 0; s0 < p.nseq; s0 += 32) {
+        const int s = s0 + lane;
+        const uint4 w = s >= p.nseq ? make_uint4(0, 0, 0, 0) : s < kPlanSeqs ? seqs[s] : seq_words(p, s);
+        const int2 in = rows_within(w, r0, r0 + n);
+        unsigned m = __ballot_sync(0xffffffffu, in.x < in.y);
+        if (__popc(m) > 4) {  // many short ones: a lane each
+            if (in.x < in.y) {
+                const Seq q(p, w);
+                for (int i = in.x; i < in.y; i++) rng[i] = own_range(q.see + (r0 + i - q.q0), q.ks, q.ke, p.window);
+            }
+        } else {
+            while (m) {
+                const int src = __ffs(m) - 1;
+                m &= m - 1;
+                const Seq q(p, shfl_words(w, src));
+                const int x = __shfl_sync(0xffffffffu, in.x, src), y = __shfl_sync(0xffffffffu, in.y, src);
+                for (int i = x + lane; i < y; i += 32) rng[i] = own_range(q.see + (r0 + i - q.q0), q.ks, q.ke, p.window);
+            }
+        }
+        __syncwarp();
+    }
+    // The rows' own keys as disjoint ascending segments, when the rows' ranges come in ascending order (lo
+    // never falls); else one segment over all of them, the masks doing the rest.
+    int lo_x[2] = {INT_MAX, INT_MAX}, hi_x[2] = {0, 0};
+    int end = -1, low = -1;  // running maximum of hi and lo over the rows so far
     bool sorted = true;
     for (int i0 = 0; i0 < p.TI; i0 += 32) {
         const int i = i0 + lane;
-        const int2 rg = i < p.TI && t * p.TI + i < p.ntok ? rng[i] : make_int2(0, -1);
+        const int2 rg = i < n ? rng[i] : make_int2(0, -1);
         const bool in = rg.y >= 0, some = rg.y > rg.x;
-        const int x = i >= p.T ? 1 : 0;
-#pragma unroll
-        for (int y = 0; y < 2; y++) {
-            lo_x[y] = min(lo_x[y], warp_min_i(some && x == y ? rg.x : INT_MAX));
-            hi_x[y] = max(hi_x[y], warp_max_i(some && x == y ? rg.y : 0));
-            if (__any_sync(0xffffffffu, in && x == y)) live |= 1 << y;
+        const bool x = i >= p.T;
+        if (__any_sync(0xffffffffu, in && !x)) f.live |= 1;
+        if (__any_sync(0xffffffffu, in && x)) f.live |= 2;
+        // Per lane, reduced once behind the loop.
+        if (some) {
+            lo_x[0] = min(lo_x[0], x ? INT_MAX : rg.x), hi_x[0] = max(hi_x[0], x ? 0 : rg.y);
+            lo_x[1] = min(lo_x[1], x ? rg.x : INT_MAX), hi_x[1] = max(hi_x[1], x ? rg.y : 0);
         }
         // Inclusive running maxima over the lanes, then those of the rows before each lane's.
         int e = some ? rg.y : -1, l = some ? rg.x : -1;
@@ -203,151 +267,109 @@ __device__ void plan_mixed(const PlanParams& p, const PlanData<kShared>& d, int 
         const bool fresh = some && rg.x > be;  // keys between be and lo are no row's
         const unsigned fm = __ballot_sync(0xffffffffu, fresh);
         if (fresh) {
-            const int at = nseg + __popc(fm & ((1u << lane) - 1));
+            const int at = f.nseg + __popc(fm & ((1u << lane) - 1));
             seg[at].x = rg.x;
             if (at > 0) seg[at - 1].y = be;
         }
-        nseg += __popc(fm);
+        f.nseg += __popc(fm);
         end = max(end, __shfl_sync(0xffffffffu, e, 31));
         low = max(low, __shfl_sync(0xffffffffu, l, 31));
     }
+    f.lo0 = warp_min_i(lo_x[0]), f.hi0 = warp_max_i(hi_x[0]);
+    f.lo1 = warp_min_i(lo_x[1]), f.hi1 = warp_max_i(hi_x[1]);
     __syncwarp();
     if (!sorted) {
-        nseg = 1;
-        if (lane == 0) seg[0] = make_int2(min(lo_x[0], lo_x[1]), max(hi_x[0], hi_x[1]));
-    } else if (nseg > 0 && lane == 0) {
-        seg[nseg - 1].y = end;
+        f.nseg = 1;
+        if (lane == 0) seg[0] = make_int2(min(f.lo0, f.lo1), max(f.hi0, f.hi1));
+    } else if (f.nseg > 0 && lane == 0) {
+        seg[f.nseg - 1].y = end;
     }
     __syncwarp();
     int nblk = 0;
-    for (int i = lane; i < nseg; i += 32) nblk += (seg[i].y - seg[i].x + kKeys - 1) / kKeys;
-    nblk = __reduce_add_sync(0xffffffffu, nblk) + (live ? p.prefix_blocks : 0);
-    const int slot = d.info[t].see;
+    for (int i = lane; i < f.nseg; i += 32) {
+        nblk += (seg[i].y - seg[i].x + kKeys - 1) / kKeys;
+        p.segs[int64_t(t) * p.TI + i] = seg[i];
+    }
+    for (int i = lane; i < n; i += 32) p.rng[r0 + i] = rng[i];
+    f.nblk = __reduce_add_sync(0xffffffffu, nblk) + p.prefix_blocks;
+    f.pieces = 1;
+    if (lane == 0) p.info[t] = f;
     __syncwarp();
-    if (lane == 0) d.info[t] = TileInfo{nblk, nseg, live ? 1 : 0, live, lo_x[0], hi_x[0], lo_x[1], hi_x[1], 0, slot, 0, 0};
 }
 
-template <bool kShared>
+// One cluster: the items by the warps of all its CTAs, then their pieces and order by the first CTA.
 __global__ void __launch_bounds__(1024) k_causal_plan(PlanParams p) {
-    extern __shared__ __align__(16) uint8_t plan_smem[];
-    __shared__ int hist[kBuckets], warp_sum_s[32];
-    __shared__ int s_max, s_chunk, s_slots;
+    extern __shared__ __align__(16) uint8_t plan_shared[];
+    __shared__ int hist[kBuckets], warp_sum_s[32], s_nblk[kMaxSms], s_chunk;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int ctas = kShared ? 1 : int(gridDim.x), gtid = int(blockIdx.x) * 1024 + tid, gwarp = gtid >> 5, warps = ctas * 32;
-    const auto sync_all = [&]() {
-        if (ctas > 1) cluster_sync();
-        else __syncthreads();
-    };
-    PlanData<kShared> d{p.info, p.rng, p.segs, p.TI};
-    if (kShared) {
-        d.info = reinterpret_cast<TileInfo*>(plan_smem);
-        d.rng = reinterpret_cast<int2*>(d.info + p.tiles);
-        d.segs = d.rng + p.mixed * p.TI;
-    }
+    const int ctas = int(gridDim.x);
+    uint4* seqs = reinterpret_cast<uint4*>(plan_shared);
+    int2* rng = reinterpret_cast<int2*>(seqs + min(p.nseq, kPlanSeqs)) + warp * 2 * kMaxItemRows;
     hist[tid] = 0;
-    if (tid == 0) s_max = s_slots = 0;
-    for (int t = gtid; kShared && t < p.tiles; t += 1024) d.info[t] = TileInfo{};  // no row of a sequence
     pdl_wait();
     pdl_launch();
-    if (gtid == 0) p.head->err = 0;
-    for (int t = gtid; !kShared && t < p.tiles; t += ctas * 1024) d.info[t] = TileInfo{};
-    sync_all();
-    // Items inside one sequence, one lane each; those a sequence begins or ends in are marked (live -1).
-    for (int s = gwarp; s < p.nseq; s += warps) {
-        const Seq q(p, s);
-        const int t1 = q.q1 / p.TI;
-        if (lane == 0 && q.q0 < q.q1) {
-            if (q.q0 % p.TI) d.info[q.q0 / p.TI].live = -1;
-            if (q.q1 % p.TI) d.info[q.q1 / p.TI].live = -1;
-        }
-        for (int t = (q.q0 + p.TI - 1) / p.TI + lane; t < t1; t += 32) {
-            const int see = q.see + (t * p.TI - q.q0);
-            const int2 a = own_range(see, q.ks, q.ke, p.window), b = own_range(see + p.T - 1, q.ks, q.ke, p.window);
-            const int2 c = own_range(see + p.T, q.ks, q.ke, p.window), e = own_range(see + p.TI - 1, q.ks, q.ke, p.window);
-            const bool two = p.TI > p.T;
-            const int lo = a.x, hi = two ? e.y : b.y;
-            TileInfo f{};
-            f.nseg = hi > lo ? 1 : 0;
-            f.nblk = p.prefix_blocks + (hi - lo + kKeys - 1) / kKeys;
-            f.pieces = 1;
-            f.live = two ? 3 : 1;
-            f.lo0 = a.x, f.hi0 = b.y;
-            f.lo1 = two ? c.x : INT_MAX, f.hi1 = two ? e.y : 0;
-            f.simple = 1;
-            f.see = see, f.ks = q.ks, f.ke = q.ke;
-            p.segs[int64_t(t) * p.TI] = make_int2(lo, hi);
-            d.info[t] = f;
-        }
-    }
-    sync_all();
-    // The marked (mixed) items' rows: none of a sequence, then the sequences' first and last ones.
-    if (kShared) {
-        for (int t = tid; t < p.tiles; t += 1024)
-            if (d.info[t].live < 0) d.info[t].see = atomicAdd(&s_slots, 1);
-        for (int i = tid; i < p.mixed * p.TI; i += 1024) d.rng[i] = make_int2(0, -1);
-    } else {
-        for (int r = gtid; r < p.ntok; r += ctas * 1024)
-            if (d.info[r / p.TI].live < 0) d.rng[r] = make_int2(0, -1);
-    }
-    sync_all();
-    for (int s = gwarp; s < p.nseq; s += warps) {
-        const Seq q(p, s);
-        const int head_end = min(q.q1, (q.q0 + p.TI - 1) / p.TI * p.TI);
-        const auto fill = [&](int r0, int r1) {  // rows of one item
-            if (r0 >= r1) return;
-            const int t = r0 / p.TI;
-            if (d.info[t].live >= 0) return;  // another sequence claims the whole item
-            int2* rng = d.rng + d.at(t);
-            for (int r = r0 + lane; r < r1; r += 32) rng[r - t * p.TI] = own_range(q.see + (r - q.q0), q.ks, q.ke, p.window);
-        };
-        fill(q.q0, head_end);
-        fill(max(head_end, q.q1 / p.TI * p.TI), q.q1);
-    }
-    sync_all();
-    for (int t0 = gwarp; t0 < p.tiles; t0 += warps * 32) {  // each warp looks at 32 items, `warps` apart
-        const int mine = t0 + lane * warps;
-        unsigned todo = __ballot_sync(0xffffffffu, mine < p.tiles && d.info[mine].live < 0);
-        while (todo) {
-            const int b = __ffs(todo) - 1;
-            todo &= todo - 1;
-            plan_mixed<kShared>(p, d, t0 + b * warps, lane);
-        }
-    }
-    sync_all();
+    for (int s = tid; s < min(p.nseq, kPlanSeqs); s += 1024) seqs[s] = seq_words(p, s);
+    if (blockIdx.x == 0 && tid == 0) p.head->err = 0;
+    __syncthreads();
+    for (int t = int(blockIdx.x) + warp * ctas; t < p.tiles; t += ctas * 32) plan_item(p, seqs, rng, rng + kMaxItemRows, t, lane);
+    if (ctas > 1) cluster_sync();
+    else __syncthreads();
     if (blockIdx.x != 0) return;
-    // Blocks per piece: the fewest for which the pieces of all items and KV heads still fit one round of
-    // the SMs (a second, short round would cost as much as the first).
+    int chunk = INT_MAX;
     if (p.lmax > 1) {
-        int m = 0;
-        for (int t = tid; t < p.tiles; t += 1024) m = max(m, d.info[t].nblk);
-        m = warp_max_i(m);
-        if (lane == 0) atomicMax(&s_max, m);
+        // Blocks per piece: the fewest for which the pieces of all items and KV heads still fit one round
+        // of the SMs (a second, short round would cost as much as the first).  There are fewer items
+        // than SMs; every warp tries a size.
+        if (tid < p.tiles) s_nblk[tid] = p.info[tid].nblk;
+        if (tid == 0) s_chunk = INT_MAX;
         __syncthreads();
-        if (warp == 0) {
-            // Fewer items than SMs here, so a lane holds up to a handful; `hi` fits, one piece per item.
-            int hi = max(1, s_max), lo = max(1, (s_max + p.lmax - 1) / p.lmax);
-            while (lo < hi) {
-                const int mid = (lo + hi) >> 1;
-                int n = 0;
-                for (int t = lane; t < p.tiles; t += 32) n += max(d.info[t].live ? 1 : 0, (d.info[t].nblk + mid - 1) / mid);
-                n = __reduce_add_sync(0xffffffffu, n);
-                if (int64_t(n) * p.kv_heads <= p.sms) hi = mid;
-                else lo = mid + 1;
-            }
-            if (lane == 0) s_chunk = lo;
+        int most = 1;
+        for (int t = lane; t < p.tiles; t += 32) most = max(most, s_nblk[t]);
+        most = warp_max_i(most);
+        for (int c0 = max(1, (most + p.lmax - 1) / p.lmax); chunk == INT_MAX; c0 += 32) {
+            const int c = min(c0 + warp, most);  // `most`, one piece per item, always fits
+            int n = 0;
+            for (int t = lane; t < p.tiles; t += 32) n += max(1, (s_nblk[t] + c - 1) / c);
+            n = __reduce_add_sync(0xffffffffu, n);
+            if (lane == 0 && (c == most || int64_t(n) * p.kv_heads <= p.sms)) atomicMin(&s_chunk, c);
+            __syncthreads();
+            chunk = s_chunk;
+            __syncthreads();
         }
-        __syncthreads();
     }
-    const int chunk = p.lmax > 1 ? s_chunk : INT_MAX;
-    // Costliest pieces first (a counting sort by blocks; the order within a bucket does not matter).
-    for (int t = tid; t < p.tiles; t += 1024) {
-        TileInfo* f = d.info + t;
-        const int nblk = f->nblk;
-        if (!f->live) continue;
-        const int pieces = max(1, nblk / chunk + (nblk % chunk ? 1 : 0)), sz = (nblk + pieces - 1) / pieces;
-        const int used = sz ? (nblk + sz - 1) / sz : 1;  // the last piece may come out empty, and is dropped
-        if (used > 1) f->pieces = used;
-        atomicAdd(&hist[min(sz, kBuckets - 1)], used);
+    // Costliest pieces first: a counting sort by blocks, the lanes of a bucket adding as one; the order
+    // within a bucket does not matter.
+    const auto pieces_of = [&](int nblk, int& sz) {
+        const int want = chunk == INT_MAX ? 1 : max(1, (nblk + chunk - 1) / chunk);
+        sz = (nblk + want - 1) / want;
+        return sz ? (nblk + sz - 1) / sz : 1;  // the last piece may come out empty, and is dropped
+    };
+    const auto add = [&](int bucket, int v) {  // adds v to the bucket; gives the sum before
+        const unsigned peers = __match_any_sync(0xffffffffu, bucket);
+        const int leader = __ffs(peers) - 1;
+        int sum = 0, before = 0;
+        if (p.lmax == 1) {  // v is 0 or 1
+            const unsigned ones = __ballot_sync(0xffffffffu, v) & peers;
+            sum = __popc(ones);
+            before = __popc(ones & ((1u << lane) - 1));
+        } else {
+            for (int l = 0; l < 32; l++) {
+                const int x = __shfl_sync(0xffffffffu, v, l);
+                if ((peers >> l) & 1) {
+                    if (l < lane) before += x;
+                    sum += x;
+                }
+            }
+        }
+        const int at = lane == leader ? atomicAdd(&hist[bucket], sum) : 0;
+        return __shfl_sync(0xffffffffu, at, leader) + before;
+    };
+    for (int t0 = warp * 32; t0 < p.tiles; t0 += 1024) {
+        const int t = t0 + lane;
+        const int4 f = t < p.tiles ? *reinterpret_cast<const int4*>(p.info + t) : make_int4(0, 0, 0, 0);  // nblk, nseg, pieces, live
+        int sz;
+        const int n = pieces_of(f.x, sz);
+        add(min(sz, kBuckets - 1), f.w ? n : 0);
     }
     __syncthreads();
     // Exclusive sums from the costliest bucket down: thread i holds bucket kBuckets - 1 - i.
@@ -361,55 +383,53 @@ __global__ void __launch_bounds__(1024) k_causal_plan(PlanParams p) {
         }
         if (lane == 31) warp_sum_s[warp] = inc;
         __syncthreads();
-        int before = 0;
-        for (int w = 0; w < warp; w++) before += warp_sum_s[w];
+        const int u = lane < warp ? warp_sum_s[lane] : 0;
+        const int before = __reduce_add_sync(0xffffffffu, u);
         hist[kBuckets - 1 - tid] = before + inc - v;
         if (tid == 1023) p.head->nwork = before + inc;
     }
     __syncthreads();
-    for (int t = tid; t < p.tiles; t += 1024) {
-        const int4 f = *reinterpret_cast<const int4*>(d.info + t);  // nblk, nseg, pieces, live
-        if (!f.w || f.z > 1) continue;
-        const int at = atomicAdd(&hist[min(f.x, kBuckets - 1)], 1);
-        int pos = 0;
-        if (f.y > 0) pos = d.info[t].simple ? p.segs[int64_t(t) * p.TI].x : d.segs[d.at(t)].x;
-        p.work[at] = Work{t, 0, f.x, -1, 0, pos, f.y, f.w};
+    for (int t0 = warp * 32; t0 < p.tiles; t0 += 1024) {
+        const int t = t0 + lane;
+        TileInfo f{};
+        if (t < p.tiles) f = p.info[t];
+        int sz;
+        const int n = pieces_of(f.nblk, sz);
+        const int at = add(min(sz, kBuckets - 1), f.live ? n : 0);
+        if (!f.live) continue;
+        if (n > 1) {
+            p.info[t].pieces = n;
+            s_nblk[t] = at;  // written below, by a warp
+            continue;
+        }
+        if (p.lmax > 1) s_nblk[t] = -1;
+        const int2 g = f.nseg > 0 ? p.segs[int64_t(t) * p.TI] : make_int2(0, 0);
+        p.work[at] = Work{t, 0, f.nblk, -1, 0, f.nseg, g.x, g.y, f.lo0, f.hi0, f.lo1, f.hi1, f.live | (f.simple << 2), f.see, f.ks, f.ke};
     }
-    if (p.lmax > 1) {
-        for (int t = warp; t < p.tiles; t += 32) {  // a warp per cut item, a lane per piece
-            const int4 f = *reinterpret_cast<const int4*>(d.info + t);
-            if (!f.w || f.z <= 1) continue;
-            const int sz = (f.x + f.z - 1) / f.z;
-            int at = lane ? 0 : atomicAdd(&hist[min(sz, kBuckets - 1)], f.z);
-            at = __shfl_sync(0xffffffffu, at, 0);
-            const int2* seg = d.info[t].simple ? p.segs + int64_t(t) * p.TI : d.segs + d.at(t);
-            for (int i = lane; i < f.z; i += 32) {
-                const int b0 = i * sz, b1 = min(f.x, b0 + sz);
-                int s = 0, first = p.prefix_blocks, pos = 0;  // segment s starts at block `first`
-                if (f.y > 0) {
-                    while (s + 1 < f.y) {
-                        const int n = (seg[s].y - seg[s].x + kKeys - 1) / kKeys;
-                        if (b0 < first + n) break;
-                        first += n;
-                        s++;
-                    }
-                    pos = seg[s].x + max(0, b0 - first) * kKeys;
+    if (p.lmax == 1) return;
+    __syncthreads();
+    for (int t = warp; t < p.tiles; t += 32) {  // cut items: a lane per piece
+        const int at = s_nblk[t];
+        const TileInfo f = p.info[t];
+        if (!f.live || at < 0) continue;
+        int sz;
+        const int n = pieces_of(f.nblk, sz);
+        const int2* seg = p.segs + int64_t(t) * p.TI;
+        for (int i = lane; i < n; i += 32) {
+            const int b0 = i * sz, b1 = min(f.nblk, b0 + sz);
+            int s = 0, first = p.prefix_blocks;  // segment s starts at block `first`
+            int2 g = make_int2(0, 0);
+            if (f.nseg > 0) {
+                g = seg[0];
+                for (; s + 1 < f.nseg; s++, g = seg[s]) {
+                    const int m = (g.y - g.x + kKeys - 1) / kKeys;
+                    if (b0 < first + m) break;
+                    first += m;
                 }
-                p.work[at + i] = Work{t, b0, b1, i, s, pos, f.y, f.w};
+                g.x += max(0, b0 - first) * kKeys;
             }
+            p.work[at + i] = Work{t, b0, b1, i, s, f.nseg, g.x, g.y, f.lo0, f.hi0, f.lo1, f.hi1, f.live | (f.simple << 2), f.see, f.ks, f.ke};
         }
-    }
-    if (kShared) {
-        for (int t = warp; t < p.tiles; t += 32) {
-            if (d.info[t].simple || !d.info[t].live) continue;
-            const int64_t from = d.at(t), to = int64_t(t) * p.TI;
-            for (int i = lane; i < p.TI; i += 32) {
-                if (t * p.TI + i < p.ntok) p.rng[to + i] = d.rng[from + i];
-                if (i < d.info[t].nseg) p.segs[to + i] = d.segs[from + i];
-            }
-        }
-        for (int i = tid; i < p.tiles * int(sizeof(TileInfo) / 16); i += 1024)
-            reinterpret_cast<int4*>(p.info)[i] = reinterpret_cast<const int4*>(d.info)[i];
     }
 }
 
@@ -438,7 +458,6 @@ struct TcParams {
     float scale_log2e;
     Header* head;
     const int2 *rng, *segs;
-    const TileInfo* info;
     const Work* work;
     float* o;
     float2* ml;
@@ -456,21 +475,22 @@ __device__ __forceinline__ bool elect_one() {
 
 // A piece of work as every role walks it.
 struct Piece {
-    int tile, kvh, b0, b1, piece, nseg, live;
+    int tile, kvh, b0, b1, piece, flags;
     int lo[2], hi[2];
-    int seg0, pos0;
+    int seg, nseg, pos, end;
+    int see, ks, ke;
     const int2* segs;
 };
 __device__ __forceinline__ Piece load_piece(const TcParams& p, int id) {
     const int w = id / p.kv_heads;
     const int4* src = reinterpret_cast<const int4*>(p.work + w);
-    const int4 a = src[0], b = src[1];
-    const int4 h = reinterpret_cast<const int4*>(p.info + a.x)[1];
+    const int4 a = src[0], b = src[1], c = src[2], d = src[3];
     Piece s;
     s.kvh = id - w * p.kv_heads;
     s.tile = a.x, s.b0 = a.y, s.b1 = a.z, s.piece = a.w;
-    s.seg0 = b.x, s.pos0 = b.y, s.nseg = b.z, s.live = b.w;
-    s.lo[0] = h.x, s.hi[0] = h.y, s.lo[1] = h.z, s.hi[1] = h.w;
+    s.seg = b.x, s.nseg = b.y, s.pos = b.z, s.end = b.w;
+    s.lo[0] = c.x, s.hi[0] = c.y, s.lo[1] = c.z, s.hi[1] = c.w;
+    s.flags = d.x, s.see = d.y, s.ks = d.z, s.ke = d.w;
     s.segs = p.segs + int64_t(a.x) * p.TI;
     return s;
 }
@@ -486,9 +506,9 @@ struct Cursor {
     }
     __device__ __forceinline__ Cursor(const TcParams& p, const Piece& s) {
         b = s.b0;
-        seg = s.seg0;
-        pos = s.pos0;
-        end = s.nseg > 0 ? s.segs[seg].y : 0;
+        seg = s.seg;
+        pos = s.pos;
+        end = s.end;
         set(p);
     }
     __device__ __forceinline__ void next(const TcParams& p, const Piece& s) {
@@ -505,7 +525,7 @@ struct Cursor {
     }
     // Whether tile x has a row that may see a key of the block.
     __device__ __forceinline__ bool active(const Piece& s, int x) const {
-        return prefix ? (s.live >> x) & 1 : (row < s.hi[x] && row + nv > s.lo[x]);
+        return prefix ? (s.flags >> x) & 1 : (row < s.hi[x] && row + nv > s.lo[x]);
     }
 };
 // Pieces are taken in turn, every second round backwards, so that the CTA with a round's costliest
@@ -827,10 +847,7 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1)
             const int row = s.tile * p.TI + x * p.T + token;
             const bool query = r < live_rows && row < p.ntok;
             int2 rg = make_int2(0, -1);
-            if (query) {
-                const int4 f = reinterpret_cast<const int4*>(p.info + s.tile)[2];  // simple, see, ks, ke
-                rg = f.x ? own_range(f.y + (row - s.tile * p.TI), f.z, f.w, p.window) : p.rng[row];
-            }
+            if (query) rg = s.flags & 4 ? own_range(s.see + (row - s.tile * p.TI), s.ks, s.ke, p.window) : p.rng[row];
             float m = -INFINITY, l = 0.f;
             int count = 0;
             for (Cursor c(p, s); c.b < s.b1; c.next(p, s)) {
@@ -1059,7 +1076,7 @@ cudaError_t launch_t(const CausalLaunch& a, const Sizes& s, const Layout& l, cud
         return cudaErrorInvalidValue;
     TcParams p{a.q, a.k, a.v, a.pk, a.pv, a.out, a.q_stride, a.k_stride, a.v_stride, a.pk_stride, a.pv_stride, a.out_stride,
                a.heads, a.kv_heads, s.group, s.T, s.TI, a.ntok, std::min(a.window, 1 << 30), a.prefix, (a.prefix + kKeys - 1) / kKeys, a.scale * kLog2e,
-               l.head, l.rng, l.segs, l.info, l.work, l.o, l.ml};
+               l.head, l.rng, l.segs, l.work, l.o, l.ml};
     const int64_t most = s.lmax > 1 ? a.num_sms : int64_t(s.tiles) * a.kv_heads;
     e = launch_pdl(k_causal_tc<E, D>, unsigned(std::min<int64_t>(a.num_sms, most)), C::kThreads, size_t(C::kSmem), stream, 1, mq, mk, mv,
                    mpk, mpv, p);
@@ -1083,20 +1100,12 @@ cudaError_t launch_causal(const CausalLaunch& a, cudaStream_t stream) {
     const Sizes s = sizes_of(a);
     const Layout l = layout_of(a, s);
     const int window = std::min(a.window, 1 << 30);  // no range is longer
-    // Items that hold a sequence's first or last row, at most.
-    const int mixed = int(std::min<int64_t>(s.tiles, 2 * int64_t(a.nseq)));
-    PlanParams pp{a.q_seqs, a.kv_seqs, a.nseq, a.ntok, a.nkv, window, s.T, s.TI, s.tiles, mixed, a.kv_heads,
+    PlanParams pp{a.q_seqs, a.kv_seqs, a.nseq, a.ntok, a.nkv, window, s.T, s.TI, s.tiles, a.kv_heads,
                   (a.prefix + kKeys - 1) / kKeys, s.lmax, a.num_sms, l.head, l.rng, l.segs, l.info, l.work};
-    // Up to here the plan fits one CTA's shared memory (about 6000 rows in short sequences, 100,000 in long
-    // ones): no phase of it waits for global memory.  Beyond, a cluster of 8 works on the workspace.
-    const size_t smem = size_t(s.tiles) * sizeof(TileInfo) + size_t(mixed) * s.TI * 2 * sizeof(int2);
-    cudaError_t e;
-    if (smem <= kPlanSmem) {
-        e = cudaFuncSetAttribute(k_causal_plan<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(kPlanSmem));
-        if (e == cudaSuccess) e = launch_pdl(k_causal_plan<true>, 1, 1024, smem, stream, 1, pp);
-    } else {
-        e = launch_pdl(k_causal_plan<false>, 8, 1024, 0, stream, 8, pp);
-    }
+    // A warp plans an item; up to 8 CTAs share them.
+    const int ctas = s.tiles <= 32 ? 1 : s.tiles <= 64 ? 2 : s.tiles <= 128 ? 4 : 8;
+    cudaError_t e = cudaFuncSetAttribute(k_causal_plan, cudaFuncAttributeMaxDynamicSharedMemorySize, int(plan_smem(kPlanSeqs)));
+    if (e == cudaSuccess) e = launch_pdl(k_causal_plan, unsigned(ctas), 1024, plan_smem(a.nseq), stream, ctas, pp);
     if (e != cudaSuccess) return e;
     return a.bf16 ? launch_e<__nv_bfloat16>(a, s, l, stream) : launch_e<__half>(a, s, l, stream);
 }
