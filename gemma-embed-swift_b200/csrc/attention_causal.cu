@@ -473,6 +473,29 @@ __device__ __forceinline__ bool elect_one() {
     return ok != 0;
 }
 
+// Two fp32 operations at a time.
+__device__ __forceinline__ uint64_t pack2(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ void unpack2(uint64_t v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+
 // A piece of work as every role walks it.
 struct Piece {
     int tile, kvh, b0, b1, piece, flags;
@@ -647,6 +670,8 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1)
     pdl_launch();
     const int total = p.head->nwork * p.kv_heads;
 
+    if (warp < 4) {
+    if constexpr (NT == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
     if (warp == 0 || warp == 2) {
         // ---------------------------------------------------------- TMA producers (Q and K; V)
         if (lane == 0) {
@@ -698,10 +723,12 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1)
         // ---------------------------------------------------------- MMA issuer (the whole warp walks along)
         const uint32_t id_s = idesc_of<E>(128, kKeys, 0);      // K-major Q and K
         const uint32_t id_o = idesc_of<E>(128, C::DS, 1);      // P from tensor memory, MN-major V
-        const uint32_t q_addr = smem_u32(smem), k_addr = smem_u32(smem + C::kOffK), v_addr = smem_u32(smem + C::kOffV);
+        // Descriptors of the tiles' starts; others lie (bytes / 16) further.
+        const uint64_t q_desc = sw128_desc(smem_u32(smem), 16, 1024), k_desc = sw128_desc(smem_u32(smem + C::kOffK), 16, 1024);
+        const uint64_t v_desc = sw128_desc(smem_u32(smem + C::kOffV), C::kChunk, 1024);
         bool ok = true;
         auto wait = [&](uint64_t* bar, uint32_t parity) {
-            ok = __all_sync(0xffffffffu, ok && mbar_wait(bar, parity, err));
+            if (!__all_sync(0xffffffffu, mbar_poll(bar, parity))) ok = __all_sync(0xffffffffu, mbar_wait(bar, parity, err));
             return ok;
         };
         int nq = 0, nk = 0, nv = 0;            // Q tiles, K stages and V stages used so far
@@ -720,100 +747,138 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1)
                 const bool more = c.b < s.b1;
                 int act = 0;
                 if (more)
-                    for (int x = 0; x < NT; x++) act |= c.active(s, x) ? 1 << x : 0;
-                // S of tile x (of head dim 256: into S buffer b)
-                auto scores = [&](int x, int b) {
-                    for (int h = 0; h < DH; h++) {
-                        const int st = (nk + h) % ST;
-                        if (!wait(&k_full[st], uint32_t(((nk + h) / ST) & 1))) return;
-                        tc_fence_after();
-                        if (elect_one()) {
-#pragma unroll
-                            for (int kk = 0; kk < C::DS / 16; kk++) {
-                                const uint64_t ad = sw128_desc(
-                                    q_addr + (x * C::QC + h * C::SC + (kk >> 2)) * C::kChunk + (kk & 3) * 32, 16, 1024);
-                                const uint64_t bd =
-                                    sw128_desc(k_addr + st * C::kStage + (kk >> 2) * C::kChunk + (kk & 3) * 32, 16, 1024);
-                                umma_f16(tmem + C::kTmemS + uint32_t(b * kKeys), ad, bd, id_s, (h | kk) != 0);
-                            }
-                            if (NT == 1) umma_commit(&k_empty[st]);
-                            if (h == DH - 1) umma_commit(&s_full[b]);
-                        }
-                        __syncwarp();
-                    }
-                };
-                // O of tile x += P of S buffer b times the block before's V
-                bool cleared = false;
-                auto values = [&](int x, int b, uint32_t parity) {
-                    if (!wait(&p_full[b], parity)) return;
-                    if (!((used >> x) & 1) && no[x] > 0 && !wait(&o_empty[x], uint32_t((no[x] - 1) & 1))) return;
-                    const int steps = (prev_nv + 15) / 16;
-                    for (int h = 0; h < DH; h++) {
-                        const int st = (nv + h) % ST;
-                        if (!wait(&v_full[st], uint32_t(((nv + h) / ST) & 1))) return;
-                        if (!cleared && (prev_nv & 15)) {
+                    for (int x = 0; x < NT; x++) act |= NT == 1 || c.active(s, x) ? 1 << x : 0;
+                if constexpr (NT == 2) {
+                    // This block's K and the block before's V first: once a tile's P has come, its PV and then its S
+                    // (over the P just read) go out together, and the other tile's softmax runs under them.
+                    const int ks = nk % ST, vs = nv % ST, steps = (prev_nv + 15) / 16;
+                    if (more && !wait(&k_full[ks], uint32_t((nk / ST) & 1))) break;
+                    if (prev_nv) {
+                        if (!wait(&v_full[vs], uint32_t((nv / ST) & 1))) break;
+                        if (prev_nv & 15) {
                             // Rows behind the block's last key, up to the product's step.
                             for (int i = lane; i < (steps * 16 - prev_nv) * C::SC * 8; i += 32) {
                                 const int rr = prev_nv + i / (C::SC * 8), ch = (i >> 3) % C::SC;
-                                *reinterpret_cast<uint4*>(smem + C::kOffV + st * C::kStage + ch * C::kChunk + rr * 128 +
-                                                          (i & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
+                                *reinterpret_cast<uint4*>(smem + C::kOffV + vs * C::kStage + ch * C::kChunk + rr * 128 + (i & 7) * 16) =
+                                    make_uint4(0u, 0u, 0u, 0u);
                             }
                             fence_proxy_async_smem();
                             __syncwarp();
                         }
-                        tc_fence_after();
-                        if (elect_one()) {
-                            for (int kk = 0; kk < steps; kk++) {
-                                const uint64_t bd = sw128_desc(v_addr + st * C::kStage + kk * 2048, C::kChunk, 1024);
-                                umma_f16_ta(tmem + uint32_t(x * D + h * C::DS), tmem + C::kTmemS + uint32_t(b * kKeys + kk * 8),
-                                            bd, id_o, ((used >> x) & 1) | (kk != 0));
-                            }
-                            if (NT == 1) {
-                                umma_commit(&v_empty[st]);
-                                if (h == DH - 1) umma_commit(pv_done);
-                            }
-                        }
-                        __syncwarp();
                     }
-                    if (NT == 2) cleared = true;
-                    if (!((used >> x) & 1)) no[x]++;
-                    used |= 1 << x;
-                };
-                if constexpr (NT == 2) {
-                    for (int x = 0; x < 2 && ok; x++) {
-                        if ((prev >> x) & 1) {
-                            values(x, x, uint32_t(np[x] & 1));
+                    const uint64_t kd = k_desc + uint32_t(__shfl_sync(0xffffffffu, ks, 0) * (C::kStage >> 4));
+                    const uint64_t vd = v_desc + uint32_t(__shfl_sync(0xffffffffu, vs, 0) * (C::kStage >> 4));
+#pragma unroll
+                    for (int x = 0; x < 2; x++) {
+                        const bool pv = (prev >> x) & 1, sc = (act >> x) & 1;
+                        const uint32_t begun = uint32_t(used >> x) & 1u;
+                        if (pv) {
+                            if (!begun && no[x] > 0 && !wait(&o_empty[x], uint32_t((no[x] - 1) & 1))) break;
+                            if (!wait(&p_full[x], uint32_t(np[x] & 1))) break;
                             np[x]++;
+                            if (!begun) no[x]++;
+                            used |= 1 << x;
                         }
-                        if (!more && ok && ((used >> x) & 1) && elect_one()) umma_commit(&o_full[x]);
+                        tc_fence_after();
+                        const uint32_t od = tmem + uint32_t(x * D), sd = tmem + C::kTmemS + uint32_t(x * kKeys);
+                        if (elect_one()) {
+                            if (pv) {
+                                if (steps == 8) {
+#pragma unroll
+                                    for (int kk = 0; kk < 8; kk++)
+                                        umma_f16_ta(od, sd + kk * 8, vd + uint32_t(kk * 128), id_o, kk ? 1u : begun);
+                                } else {
+#pragma unroll 1
+                                    for (int kk = 0; kk < steps; kk++)
+                                        umma_f16_ta(od, sd + kk * 8, vd + uint32_t(kk * 128), id_o, kk ? 1u : begun);
+                                }
+                            }
+                            if (sc) {
+#pragma unroll
+                                for (int kk = 0; kk < C::DS / 16; kk++)
+                                    umma_f16(sd, q_desc + uint32_t(((x * C::QC + (kk >> 2)) * C::kChunk + (kk & 3) * 32) >> 4),
+                                             kd + uint32_t(((kk >> 2) * C::kChunk + (kk & 3) * 32) >> 4), id_s, kk != 0);
+                                umma_commit(&s_full[x]);
+                            }
+                            if (!more && (pv || begun)) umma_commit(&o_full[x]);
+                            if (x == 1) {
+                                if (prev_nv) umma_commit(&v_empty[vs]);
+                                if (more) umma_commit(&k_empty[ks]);
+                            }
+                        }
                         __syncwarp();
-                        if (ok && ((act >> x) & 1)) scores(x, x);
                     }
-                    // A block no tile sees (between key ranges in falling order) is passed by once it has landed.
-                    if (ok && more && !act) wait(&k_full[nk % ST], uint32_t((nk / ST) & 1));
-                    if (ok && prev_nv && !prev) wait(&v_full[nv % ST], uint32_t((nv / ST) & 1));
                     if (!ok) break;
-                    if (elect_one()) {
-                        if (prev_nv) umma_commit(&v_empty[nv % ST]);
-                        if (more) umma_commit(&k_empty[nk % ST]);
-                    }
-                    __syncwarp();
                     if (prev_nv) nv++;
                     if (more) nk++;
                 } else {
                     if (more) {
-                        scores(0, ns[0] & 1);
+                        // S into the other of the two buffers, ahead of the block before's PV.
+                        const int b = ns[0] & 1;
+                        for (int h = 0; h < DH; h++) {
+                            const int st = (nk + h) % ST;
+                            if (!wait(&k_full[st], uint32_t(((nk + h) / ST) & 1))) break;
+                            tc_fence_after();
+                            const uint64_t kd = k_desc + uint32_t(__shfl_sync(0xffffffffu, st, 0) * (C::kStage >> 4));
+                            const uint32_t sd = tmem + C::kTmemS + uint32_t(__shfl_sync(0xffffffffu, b, 0) * kKeys);
+                            if (elect_one()) {
+#pragma unroll
+                                for (int kk = 0; kk < C::DS / 16; kk++)
+                                    umma_f16(sd, q_desc + uint32_t(((h * C::SC + (kk >> 2)) * C::kChunk + (kk & 3) * 32) >> 4),
+                                             kd + uint32_t(((kk >> 2) * C::kChunk + (kk & 3) * 32) >> 4), id_s, (h | kk) != 0);
+                                umma_commit(&k_empty[st]);
+                                if (h == DH - 1) umma_commit(&s_full[b]);
+                            }
+                            __syncwarp();
+                        }
+                        if (!ok) break;
                         ns[0]++;
                         nk += DH;
                     }
-                    if (ok && prev_nv) {
-                        values(0, np[0] & 1, uint32_t((np[0] >> 1) & 1));
+                    if (prev_nv) {
+                        const int b = np[0] & 1, steps = (prev_nv + 15) / 16;
+                        if (!used && no[0] > 0 && !wait(&o_empty[0], uint32_t((no[0] - 1) & 1))) break;
+                        for (int h = 0; h < DH; h++) {
+                            const int st = (nv + h) % ST;
+                            if (!wait(&v_full[st], uint32_t(((nv + h) / ST) & 1))) break;
+                            if (prev_nv & 15) {
+                                for (int i = lane; i < (steps * 16 - prev_nv) * C::SC * 8; i += 32) {
+                                    const int rr = prev_nv + i / (C::SC * 8), ch = (i >> 3) % C::SC;
+                                    *reinterpret_cast<uint4*>(smem + C::kOffV + st * C::kStage + ch * C::kChunk + rr * 128 + (i & 7) * 16) =
+                                        make_uint4(0u, 0u, 0u, 0u);
+                                }
+                                fence_proxy_async_smem();
+                                __syncwarp();
+                            }
+                            if (h == 0 && !wait(&p_full[b], uint32_t((np[0] >> 1) & 1))) break;
+                            tc_fence_after();
+                            const uint64_t vd = v_desc + uint32_t(__shfl_sync(0xffffffffu, st, 0) * (C::kStage >> 4));
+                            const uint32_t pd = tmem + C::kTmemS + uint32_t(__shfl_sync(0xffffffffu, b, 0) * kKeys), od = tmem + uint32_t(h * C::DS);
+                            const uint32_t begun = uint32_t(used);
+                            if (elect_one()) {
+                                if (steps == 8) {
+#pragma unroll
+                                    for (int kk = 0; kk < 8; kk++)
+                                        umma_f16_ta(od, pd + kk * 8, vd + uint32_t(kk * 128), id_o, kk ? 1u : begun);
+                                } else {
+#pragma unroll 1
+                                    for (int kk = 0; kk < steps; kk++)
+                                        umma_f16_ta(od, pd + kk * 8, vd + uint32_t(kk * 128), id_o, kk ? 1u : begun);
+                                }
+                                umma_commit(&v_empty[st]);
+                                if (h == DH - 1) {
+                                    umma_commit(pv_done);
+                                    if (!more) umma_commit(&o_full[0]);
+                                }
+                            }
+                            __syncwarp();
+                        }
+                        if (!ok) break;
                         np[0]++;
+                        if (!used) no[0]++;
+                        used = 1;
                         nv += DH;
                     }
-                    if (!ok) break;
-                    if (!more && elect_one()) umma_commit(&o_full[0]);
-                    __syncwarp();
                 }
                 if (!more) break;
                 prev = act;
@@ -830,99 +895,131 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1)
             drain(idle, 0);
         }
         __syncwarp();
-    } else if (warp >= 4) {
+    }
+    } else {
         // ---------------------------------------------------------- softmax and output, one thread per row
+        if constexpr (NT == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
         const int x = NT == 2 ? (warp - 4) >> 2 : 0;
         const int quad = warp & 3, r = quad * 32 + lane;
         const uint32_t lane_base = tmem + (uint32_t(quad * 32) << 16);
         const int token = r / p.group;
         bool ok = true;
+        // Every lane tests (the barrier is most often already there), then they agree.
         auto wait = [&](uint64_t* bar, uint32_t parity) {
-            ok = __all_sync(0xffffffffu, ok && mbar_wait(bar, parity, err));
+            if (!__all_sync(0xffffffffu, mbar_poll(bar, parity))) ok = __all_sync(0xffffffffu, mbar_wait(bar, parity, err));
             return ok;
         };
         int nb = 0, no = 0;  // blocks and items with an O so far
         for (int round = 0, id; ok && (id = piece_id(round)) < total; round++) {
             const Piece s = load_piece(p, id);
             const int row = s.tile * p.TI + x * p.T + token;
-            const bool query = r < live_rows && row < p.ntok;
             int2 rg = make_int2(0, -1);
-            if (query) rg = s.flags & 4 ? own_range(s.see + (row - s.tile * p.TI), s.ks, s.ke, p.window) : p.rng[row];
+            if (r < live_rows && row < p.ntok) rg = s.flags & 4 ? own_range(s.see + (row - s.tile * p.TI), s.ks, s.ke, p.window) : p.rng[row];
+            // Rows of no query take every score: never stored.
+            const bool in = rg.y >= 0;
+            const int row_lo = in ? rg.x : 0, row_hi = in ? rg.y : INT_MAX;
+            const int warp_lo = __reduce_max_sync(0xffffffffu, row_lo), warp_hi = __reduce_min_sync(0xffffffffu, row_hi);
+            const int tile_lo = x ? s.lo[1] : s.lo[0], tile_hi = x ? s.hi[1] : s.hi[0];
+            const bool tile_live = (s.flags >> x) & 1;
             float m = -INFINITY, l = 0.f;
-            int count = 0;
-            for (Cursor c(p, s); c.b < s.b1; c.next(p, s)) {
-                if (NT == 2 && !c.active(s, x)) continue;
-                const int b = NT == 2 ? x : nb & 1;
-                if (!wait(&s_full[b], uint32_t((NT == 2 ? nb : nb >> 1) & 1))) break;
-                nb++;
-                count++;
-                tc_fence_after();
-                const uint32_t scol = lane_base + C::kTmemS + uint32_t(b * kKeys);
-                uint32_t sr[128];
-#pragma unroll
-                for (int i = 0; i < 4; i++) tmem_ld32(scol + i * 32, *reinterpret_cast<uint32_t(*)[32]>(&sr[i * 32]));
-                tmem_wait_ld();
-                // The row's keys among the block's nv (a later segment's may start within 128 rows of this
-                // one's end).  Rows without a query take every score: finite, never stored.
-                const int lo = c.prefix || !query ? 0 : rg.x - c.row;
-                const int hi = !query ? kKeys : c.prefix ? c.nv : min(rg.y - c.row, c.nv);
-                if (__any_sync(0xffffffffu, lo > 0 || hi < kKeys)) {
-#pragma unroll
-                    for (int i = 0; i < 128; i++)
-                        if (i < lo || i >= hi) sr[i] = __float_as_uint(-INFINITY);
+            const int nb0 = nb;
+            // Runs of blocks: the prefix' and each segment's (of this piece), those the tile has rows for.
+            int b = s.b0, seg = s.seg, pos = s.pos, end = s.end;
+            while (ok && b < s.b1) {
+                const bool prefix = b < p.prefix_blocks;
+                int key = prefix ? b * kKeys : pos, lim = prefix ? p.prefix : end;
+                const int blocks = min(prefix ? p.prefix_blocks - b : (end - pos + kKeys - 1) / kKeys, s.b1 - b);
+                lim = min(lim, key + blocks * kKeys);
+                b += blocks;
+                if (!prefix && b < s.b1) {
+                    const int2 g = s.segs[++seg];
+                    pos = g.x, end = g.y;
                 }
-                float mp[8];
-#pragma unroll
-                for (int i = 0; i < 8; i++) mp[i] = __uint_as_float(sr[i]);
-#pragma unroll
-                for (int i = 8; i < 128; i++) mp[i & 7] = fmaxf(mp[i & 7], __uint_as_float(sr[i]));
-                const float mb = fmaxf(fmaxf(fmaxf(mp[0], mp[1]), fmaxf(mp[2], mp[3])),
-                                       fmaxf(fmaxf(mp[4], mp[5]), fmaxf(mp[6], mp[7]))) * p.scale_log2e;
-                const bool grow = mb > m + kGrow && m != -INFINITY;
-                if (__any_sync(0xffffffffu, grow)) {
-                    // O holds every product before this block's (of head dim 256: once the last has completed).
-                    if (NT == 1 && !wait(pv_done, uint32_t((nb - 2) & 1))) break;
+                // A block is active where the issuers' test says so: key < tile_hi and its end > tile_lo.
+                int stop = lim;
+                if (NT == 2) {
+                    if (prefix ? !tile_live : tile_lo >= lim) continue;
+                    if (!prefix) {
+                        if (tile_lo > key) key += (tile_lo - key) / kKeys * kKeys;
+                        stop = min(lim, tile_hi);
+                    }
+                }
+                // Blocks below `free` (and from warp_lo on) need no mask in this warp.
+                const int free = prefix ? lim : min(lim, warp_hi), from = prefix ? 0 : warp_lo;
+                for (; key < stop; key += kKeys, nb++) {
+                    const int buf = NT == 2 ? x : nb & 1;
+                    if (!wait(&s_full[buf], uint32_t((NT == 2 ? nb : nb >> 1) & 1))) break;
                     tc_fence_after();
-                    const float alpha = grow ? ex2_approx(m - mb) : 1.0f;
+                    const uint32_t scol = lane_base + C::kTmemS + uint32_t(buf * kKeys);
+                    uint32_t sr[kKeys];
+#pragma unroll
+                    for (int i = 0; i < kKeys / 32; i++) tmem_ld32(scol + i * 32, *reinterpret_cast<uint32_t(*)[32]>(&sr[i * 32]));
+                    tmem_wait_ld();
+                    if (key + kKeys > free || key < from) {
+                        // Keys of the row among the block's (a later segment's may start within a block's
+                        // length of this one's end).
+                        const int lo = prefix ? 0 : row_lo - key, hi = (in ? prefix ? lim : min(row_hi, lim) : INT_MAX) - key;
+#pragma unroll
+                        for (int i = 0; i < kKeys; i++)
+                            if (i < lo || i >= hi) sr[i] = __float_as_uint(-INFINITY);
+                    }
+                    float mp[4];  // four independent chains of three-way maxima
+#pragma unroll
+                    for (int i = 0; i < 4; i++) mp[i] = max3(__uint_as_float(sr[3 * i]), __uint_as_float(sr[3 * i + 1]), __uint_as_float(sr[3 * i + 2]));
+#pragma unroll
+                    for (int i = 12; i < kKeys; i += 2)
+                        mp[(i >> 1) & 3] = max3(mp[(i >> 1) & 3], __uint_as_float(sr[i]), __uint_as_float(sr[i + 1]));
+                    const float mb = fmaxf(max3(mp[0], mp[1], mp[2]), mp[3]) * p.scale_log2e;
+                    const bool grow = mb > m + kGrow;
+                    if (__any_sync(0xffffffffu, grow)) {
+                        // Also a row's first visible key: O and l are still 0 then (or not begun, in the item's first
+                        // block).
+                        const float alpha = m == -INFINITY || !grow ? 1.0f : ex2_approx(m - mb);
+                        if (__any_sync(0xffffffffu, alpha != 1.0f)) {
+                            // O is complete up to the block before: S came behind that PV (of head dim 256: ahead).
+                            if (NT == 1 && !wait(&pv_done[0], uint32_t((nb - 1) & 1))) break;
+                            tc_fence_after();
 #pragma unroll 1
-                    for (int i = 0; i < D / 32; i++) {
-                        uint32_t o[32];
-                        tmem_ld32(lane_base + uint32_t(x * D + i * 32), o);
-                        tmem_wait_ld();
+                            for (int i = 0; i < D / 32; i++) {
+                                uint32_t o[32];
+                                tmem_ld32(lane_base + uint32_t(x * D + i * 32), o);
+                                tmem_wait_ld();
 #pragma unroll
-                        for (int e = 0; e < 32; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
-                        tmem_st32(lane_base + uint32_t(x * D + i * 32), o);
+                                for (int e = 0; e < 32; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+                                tmem_st32(lane_base + uint32_t(x * D + i * 32), o);
+                            }
+                            l *= alpha;
+                        }
+                        if (grow) m = mb;
                     }
-                    if (grow) {
-                        l *= alpha;
-                        m = mb;
+                    const float mu = m == -INFINITY ? 0.f : -m;
+                    const uint64_t scale2 = pack2(p.scale_log2e, p.scale_log2e), mu2 = pack2(mu, mu);
+                    uint64_t ps[4] = {0, 0, 0, 0};
+#pragma unroll
+                    for (int h = 0; h < kKeys / 64; h++) {
+                        uint32_t pk[32];
+#pragma unroll
+                        for (int e = 0; e < 32; e++) {
+                            float p0, p1;
+                            unpack2(fma2(pack2(__uint_as_float(sr[h * 64 + 2 * e]), __uint_as_float(sr[h * 64 + 2 * e + 1])), scale2, mu2), p0, p1);
+                            p0 = ex2_approx(p0), p1 = ex2_approx(p1);
+                            ps[e & 3] = add2(ps[e & 3], pack2(p0, p1));
+                            pk[e] = float_to_pair<E>(p0, p1);
+                        }
+                        tmem_st32(scol + h * 32, pk);
                     }
+                    tmem_wait_st();
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&p_full[buf]);
+                    float l0, l1;
+                    unpack2(add2(add2(ps[0], ps[1]), add2(ps[2], ps[3])), l0, l1);
+                    l += l0 + l1;
                 }
-                if (m == -INFINITY) m = mb;  // the row's first visible key: O and l are still 0
-                const float mu = m == -INFINITY ? 0.f : m;
-                float ps[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int h = 0; h < 2; h++) {
-                    uint32_t pk[32];
-#pragma unroll
-                    for (int e = 0; e < 32; e++) {
-                        const float p0 = ex2_approx(fmaf(__uint_as_float(sr[h * 64 + 2 * e]), p.scale_log2e, -mu));
-                        const float p1 = ex2_approx(fmaf(__uint_as_float(sr[h * 64 + 2 * e + 1]), p.scale_log2e, -mu));
-                        ps[(2 * e) & 7] += p0;
-                        ps[(2 * e + 1) & 7] += p1;
-                        pk[e] = float_to_pair<E>(p0, p1);
-                    }
-                    tmem_st32(scol + h * 32, pk);
-                }
-                l += ((ps[0] + ps[1]) + (ps[2] + ps[3])) + ((ps[4] + ps[5]) + (ps[6] + ps[7]));
-                tmem_wait_st();
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&p_full[b]);
             }
+            const int count = nb - nb0;
             if (!ok) break;
             // ---- output
-            const bool in = rg.y >= 0;
             const int head = s.kvh * p.group + (r - token * p.group);
             const int64_t at = (int64_t(s.piece) * p.ntok + row) * p.heads + head;  // of a partial row
             const float inv = s.piece >= 0 ? 1.0f : l == 0.f ? 0.f : 1.0f / l;
