@@ -13,8 +13,10 @@
 // Stage of a warp: 16 rows x 256 weights (16 x 128 bytes, chunk c of row r at c ^ (r & 7), so that the
 // 32-bit reads of a fragment hit 32 banks).  The lane's word of a 32-weight group holds the group's
 // elements 8 c .. 8 c + 7; their nibbles come out as pairs (0, 4), (1, 5), (2, 6), (3, 7), which x is
-// stored to match: the products' k order is permuted the same on both sides.
-// x is staged 16 bytes at a time for all warps in two buffers of kXElems elements per 8 rows.
+// stored to match: the products' k order is permuted the same on both sides.  A stage's scales and minima
+// come along in its slot.
+// x is staged for all warps in two buffers of kXElems elements (all of it where it fits, so that the
+// warps never meet while they stream).
 #include <algorithm>
 
 #include "attention_rows.cuh"
@@ -26,21 +28,17 @@ namespace {
 
 constexpr int kWarps = 16, kThreads = kWarps * 32;
 constexpr int kStageK = 256;                   // weights of a row per stage
-constexpr int kStageBytes = 16 * kStageK / 2;  // 2 KB
-constexpr int kDepth = 4;
-constexpr int kXElems = 2048;                  // x elements of 8 rows per buffer
-
-template <int NB>
-struct Q4Cfg {
-    static constexpr int KC = kXElems / NB;           // k elements per row and buffer
-    static constexpr int kXRow = KC * 2 + 64;         // bytes; 64 over a multiple of 128: two rows, no conflict
-    static constexpr int kXBytes = 8 * NB * kXRow;
-    static constexpr int kSums = 8 * NB * (KC / 32);  // sums of x per row and 32 elements
-    static constexpr int kOffX = kWarps * kDepth * kStageBytes;
-    static constexpr int kOffSum = kOffX + 2 * kXBytes;
-    static constexpr int kSmem = kOffSum + 2 * kSums * 4;
-    static constexpr int kMaxSplit = KC / kStageK;
-};
+constexpr int kScaleRow = 16;                  // bytes of a row's scales (or mins) in a stage: up to 8 groups
+constexpr int kWeightBytes = 16 * kStageK / 2; // 2 KB
+constexpr int kStageBytes = kWeightBytes + 2 * 16 * kScaleRow;  // weights, scales, mins
+constexpr int kDepth = 3;
+constexpr int kXElems = 16384;                 // elements of x per buffer, all rows
+constexpr int kOffX = kWarps * kDepth * kStageBytes;
+constexpr int kXBytes = kXElems * 2 + kQ4MaxRows * 64;  // rows are 64 bytes over a multiple of 128 apart
+constexpr int kOffSum = kOffX + 2 * kXBytes;            // sums of x per 32 elements and row
+constexpr int kSumBytes = kXElems / 32 * 4;
+constexpr int kSmem = kOffSum + 2 * kSumBytes;
+static_assert(kSmem <= 227 * 1024, "shared memory");
 
 struct Q4Params {
     const void* x;
@@ -50,11 +48,16 @@ struct Q4Params {
     const __half *scales, *mins;
     void* out;
     int64_t out_stride;
-    int tiles, R, S, Ks;  // row tiles in all; tiles and k slices of a CTA at a time; k per slice
+    int tiles, R, S, Ks, kcs;  // row tiles in all; tiles and k slices of a CTA at a time; k per slice, and per x buffer
+    int fast_scales;           // scales (and mins) may be copied a stage's row at a time
 };
 
 __device__ __forceinline__ void cp16(uint32_t dst, const void* src, uint32_t bytes) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+template <int N>
+__device__ __forceinline__ void cp_small(uint32_t dst, const void* src) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst), "l"(src), "n"(N) : "memory");
 }
 __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
@@ -90,55 +93,65 @@ __device__ __forceinline__ void widen_bf16(uint32_t u, uint32_t (&t)[4]) {
     }
 }
 
-template <typename T>
+// d = a b (+ d), not volatile: the products of several groups may be interleaved.
+template <typename T, bool kFirst>
 __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    if constexpr (sizeof(T) == 2 && std::is_same<T, __half>::value)
-        asm volatile(
-            "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-            : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-    else
-        asm volatile(
-            "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-            : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    const float z = 0.f;
+    if constexpr (std::is_same<T, __half>::value) {
+        if constexpr (kFirst)
+            asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+                : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(z));
+        else
+            asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    } else {
+        if constexpr (kFirst)
+            asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+                : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(z));
+        else
+            asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    }
 }
 
 // NB: tiles of 8 rows of x.
 template <typename T, int NB, bool kMins>
 __global__ void __launch_bounds__(kThreads, 1) k_linear_q4(const __grid_constant__ Q4Params p) {
-    using C = Q4Cfg<NB>;
     extern __shared__ __align__(128) uint8_t smem[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int g = lane >> 2, c = lane & 3;
     const int rt = warp % p.R, sp = warp / p.R;
     const int t_begin = int(int64_t(blockIdx.x) * p.tiles / gridDim.x), t_end = int(int64_t(blockIdx.x + 1) * p.tiles / gridDim.x);
-    const int kcs = C::KC / p.S / kStageK * kStageK;  // k of a slice per buffer
-    const int chunk_stages = kcs / kStageK;
+    const int chunk_stages = p.kcs / kStageK;
     const int stages = (p.Ks + kStageK - 1) / kStageK, chunks = (stages + chunk_stages - 1) / chunk_stages;
     const int groups = p.k / p.group, gshift = p.group == 32 ? 5 : p.group == 64 ? 6 : 7;
+    const int x_row = p.S * p.kcs * 2 + 64;  // bytes between x's rows in a buffer
     uint8_t* ring = smem + warp * kDepth * kStageBytes;
     const uint32_t ring_addr = smem_u32(ring);
     pdl_wait();
     pdl_launch();
 
     // x of buffer `i` (elements [s Ks + i kcs, + kcs) of every slice s): up to four 16-byte units per thread.
-    constexpr int kUnits = 8 * NB * C::KC / 8 / kThreads;
-    const int units_row = p.S * kcs / 8;
+    constexpr int kUnits = kXElems / 8 / kThreads;
+    const int units_row = p.S * p.kcs / 8;
     uint4 xr[kUnits];
     auto load_x = [&](int i) {
 #pragma unroll
         for (int u = 0; u < kUnits; u++) {
             const int id = u * kThreads + threadIdx.x, r = id / units_row, e = (id - r * units_row) * 8;
-            const int s = e / kcs, off = i * kcs + (e - s * kcs), kk = s * p.Ks + off;
+            const int s = e / p.kcs, off = i * p.kcs + (e - s * p.kcs), kk = s * p.Ks + off;
             xr[u] = make_uint4(0u, 0u, 0u, 0u);
             if (r < p.rows && off < p.Ks && kk < p.k)
                 xr[u] = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.x) + r * p.x_stride + kk);
         }
     };
     auto store_x = [&](int i) {
-        uint8_t* buf = smem + C::kOffX + (i & 1) * C::kXBytes;
-        float* sums = reinterpret_cast<float*>(smem + C::kOffSum) + (i & 1) * C::kSums;
+        uint8_t* buf = smem + kOffX + (i & 1) * kXBytes;
+        float* sums = reinterpret_cast<float*>(smem + kOffSum + (i & 1) * kSumBytes);
 #pragma unroll
         for (int u = 0; u < kUnits; u++) {
             const int id = u * kThreads + threadIdx.x, r = id / units_row, e = (id - r * units_row) * 8;
@@ -153,7 +166,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_linear_q4(const __grid_constant
                 }
                 s += __shfl_xor_sync(0xffffffffu, s, 1);
                 s += __shfl_xor_sync(0xffffffffu, s, 2);
-                if (r < p.rows && (threadIdx.x & 3) == 0) sums[r * (C::KC / 32) + e / 32] = s;
+                if (r < p.rows && (threadIdx.x & 3) == 0) sums[(e / 32) * p.rows + r] = s;
             }
             if (r < p.rows) {
                 uint4 o;  // pairs (0, 4), (1, 5), (2, 6), (3, 7)
@@ -161,50 +174,55 @@ __global__ void __launch_bounds__(kThreads, 1) k_linear_q4(const __grid_constant
                 o.y = __byte_perm(v.x, v.z, 0x7632);
                 o.z = __byte_perm(v.y, v.w, 0x5410);
                 o.w = __byte_perm(v.y, v.w, 0x7632);
-                *reinterpret_cast<uint4*>(buf + r * C::kXRow + e * 2) = o;
+                *reinterpret_cast<uint4*>(buf + r * x_row + e * 2) = o;
             }
         }
     };
+    // Rows past the last repeat it: their products are not stored.
+    int xrow[NB], srow[NB][2];
+#pragma unroll
+    for (int b = 0; b < NB; b++) {
+        xrow[b] = min(b * 8 + g, p.rows - 1) * x_row + c * 16;
+        srow[b][0] = min(b * 8 + 2 * c, p.rows - 1);
+        srow[b][1] = min(b * 8 + 2 * c + 1, p.rows - 1);
+    }
 
     for (int base = t_begin; base < t_end; base += p.R) {
         const bool works = sp < p.S && base + rt < t_end;
         const int n0 = (base + rt) * 16, k0 = sp * p.Ks, k1 = min(p.k, k0 + p.Ks);
         const int mine = works ? max(0, (k1 - k0 + kStageK - 1) / kStageK) : 0;  // this warp's stages
-        // The four 16-byte chunks of a stage this lane copies: rows 4 i + lane / 8, chunk lane % 8.
-        auto copy = [&](int st) {
-            if (st < mine) {
-                const int kk = k0 + st * kStageK + (lane & 7) * 32;
-                const uint32_t bytes = kk < k1 ? 16u : 0u;  // zeros past the slice
+        // The four 16-byte chunks of a stage this lane copies: rows 4 i + lane / 8, chunk lane % 8 (swizzled, it
+        // differs by 4 between odd and even i).
+        const uint8_t* src[4];
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const int rr = i * 4 + (lane >> 3), n = min(n0 + rr, p.n - 1);
-                    cp16(ring_addr + uint32_t((st % kDepth) * kStageBytes + rr * 128 + (((lane & 7) ^ (rr & 7)) << 4)),
-                         p.values + int64_t(n) * (p.k >> 1) + (min(kk, p.k - 32) >> 1), bytes);
+        for (int i = 0; i < 4; i++)
+            src[i] = p.values + int64_t(min(n0 + i * 4 + (lane >> 3), p.n - 1)) * (p.k >> 1) + ((k0 + (lane & 7) * 32) >> 1);
+        const uint32_t dst = ring_addr + uint32_t((lane >> 3) * 128), c0 = uint32_t(((lane & 7) ^ (lane >> 3)) << 4), c1 = c0 ^ 64u;
+        // Scales by lanes 0-15, mins by lanes 16-31, a row each.
+        const __half* ssrc = (lane < 16 || !kMins ? p.scales : p.mins) + int64_t(min(n0 + (lane & 15), p.n - 1)) * groups + (k0 >> gshift);
+        auto copy = [&](int st, int at) {  // stage st into slot `at`
+            if (st < mine) {
+                const int kk = k0 + st * kStageK;
+                const bool in = kk + (lane & 7) * 32 < k1;  // zeros past the slice
+                const uint32_t slot = uint32_t(at * kStageBytes), to = dst + slot;
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                    cp16(to + uint32_t(i * 512) + (i & 1 ? c1 : c0), in ? src[i] + st * (kStageK / 2) : p.values, in ? 16u : 0u);
+                if (kMins || lane < 16) {
+                    const uint32_t sdst = ring_addr + slot + uint32_t(kWeightBytes + lane * kScaleRow);
+                    const __half* sp_ = ssrc + ((st * kStageK) >> gshift);
+                    if (p.fast_scales) {  // k is a multiple of the stage, so is every slice: whole rows
+                        if (gshift == 5) cp_small<16>(sdst, sp_);
+                        else if (gshift == 6) cp_small<8>(sdst, sp_);
+                        else cp_small<4>(sdst, sp_);
+                    } else {
+                        __half* out = reinterpret_cast<__half*>(ring + slot + kWeightBytes + lane * kScaleRow);
+                        for (int i = 0; i < (kStageK >> gshift); i++)
+                            out[i] = kk + (i << gshift) < k1 ? sp_[i] : __ushort_as_half(0);
+                    }
                 }
             }
             cp_commit();
-        };
-        // Scales (and mins) of rows g and g + 8, 32-weight groups 2 c and 2 c + 1 of a stage.
-        const int64_t ga = int64_t(min(n0 + g, p.n - 1)) * groups, gb = int64_t(min(n0 + g + 8, p.n - 1)) * groups;
-        struct Scales {
-            __half2 a, b, ma, mb;
-        };
-        auto load_scales = [&](int st) {
-            Scales s;
-            const __half2 zero = __half2half2(__ushort_as_half(0));
-            s.a = s.b = s.ma = s.mb = zero;
-            if (st >= mine) return s;
-            const int kk = k0 + st * kStageK + c * 64;
-            const int i0 = kk >> gshift, i1 = (kk + 32) >> gshift;
-            const bool in0 = kk < k1, in1 = kk + 32 < k1;
-            const __half z = __ushort_as_half(0);
-            s.a = __halves2half2(in0 ? p.scales[ga + i0] : z, in1 ? p.scales[ga + i1] : z);
-            s.b = __halves2half2(in0 ? p.scales[gb + i0] : z, in1 ? p.scales[gb + i1] : z);
-            if (kMins) {
-                s.ma = __halves2half2(in0 ? p.mins[ga + i0] : z, in1 ? p.mins[ga + i1] : z);
-                s.mb = __halves2half2(in0 ? p.mins[gb + i0] : z, in1 ? p.mins[gb + i1] : z);
-            }
-            return s;
         };
         float acc[NB][4];
 #pragma unroll
@@ -212,27 +230,29 @@ __global__ void __launch_bounds__(kThreads, 1) k_linear_q4(const __grid_constant
 #pragma unroll
             for (int i = 0; i < 4; i++) acc[b][i] = 0.f;
 
-        for (int st = 0; st < kDepth - 1; st++) copy(st);
-        Scales cur = load_scales(0), nxt = load_scales(1);
+        for (int st = 0; st < kDepth - 1; st++) copy(st, st);
+        int slot = 0;  // of the stage in turn
         load_x(0);
         store_x(0);
         __syncthreads();
         for (int ch = 0; ch < chunks; ch++) {
             if (ch + 1 < chunks) load_x(ch + 1);
-            const uint8_t* xb = smem + C::kOffX + (ch & 1) * C::kXBytes + g * C::kXRow + (sp * kcs + c * 8) * 2;
-            const float* sums = reinterpret_cast<const float*>(smem + C::kOffSum) + (ch & 1) * C::kSums + sp * kcs / 32;
+            const uint8_t* xb = smem + kOffX + (ch & 1) * kXBytes + sp * p.kcs * 2;
+            const float* sums = reinterpret_cast<const float*>(smem + kOffSum + (ch & 1) * kSumBytes) + sp * p.kcs / 32 * p.rows;
             for (int q = 0; q < chunk_stages; q++) {
                 const int st = ch * chunk_stages + q;
                 if (st >= mine) break;
-                const Scales later = load_scales(st + 2);
                 cp_wait<kDepth - 2>();
                 __syncwarp();
-                copy(st + kDepth - 1);
-                const uint8_t* w = ring + (st % kDepth) * kStageBytes + g * 128 + c * 4;
+                copy(st + kDepth - 1, slot == 0 ? kDepth - 1 : slot - 1);
+                const uint8_t* w = ring + slot * kStageBytes + g * 128 + c * 4;
+                const uint8_t* scr = ring + slot * kStageBytes + kWeightBytes + g * kScaleRow;
+                slot = slot == kDepth - 1 ? 0 : slot + 1;
+                const int swz = g << 4;
 #pragma unroll
                 for (int j = 0; j < kStageK / 32; j++) {
-                    const uint32_t ua = *reinterpret_cast<const uint32_t*>(w + ((j ^ g) << 4));
-                    const uint32_t ub = *reinterpret_cast<const uint32_t*>(w + 1024 + ((j ^ g) << 4));
+                    const uint32_t ua = *reinterpret_cast<const uint32_t*>(w + ((j << 4) ^ swz));
+                    const uint32_t ub = *reinterpret_cast<const uint32_t*>(w + 1024 + ((j << 4) ^ swz));
                     uint32_t ta[4], tb[4];
                     if constexpr (std::is_same<T, __half>::value) {
                         widen_f16<!kMins>(ua, ta);
@@ -241,30 +261,24 @@ __global__ void __launch_bounds__(kThreads, 1) k_linear_q4(const __grid_constant
                         widen_bf16<!kMins>(ua, ta);
                         widen_bf16<!kMins>(ub, tb);
                     }
-                    const int src = (lane & 28) | (j >> 1);
-                    auto pick = [&](const __half2& h) {
-                        const __half2 v = __shfl_sync(0xffffffffu, h, src);
-                        return (j & 1) ? __high2float(v) : __low2float(v);
-                    };
-                    const float sa = pick(cur.a), sb = pick(cur.b);
-                    const float ma = kMins ? pick(cur.ma) : 0.f, mb = kMins ? pick(cur.mb) : 0.f;
+                    const __half* sj = reinterpret_cast<const __half*>(scr) + ((j * 32) >> gshift);
+                    const float sa = __half2float(sj[0]), sb = __half2float(sj[8 * kScaleRow / 2]);
+                    const float ma = kMins ? __half2float(sj[16 * kScaleRow / 2]) : 0.f;
+                    const float mb = kMins ? __half2float(sj[24 * kScaleRow / 2]) : 0.f;
                     const uint32_t a0[4] = {ta[0], tb[0], ta[1], tb[1]}, a1[4] = {ta[2], tb[2], ta[3], tb[3]};
 #pragma unroll
                     for (int b = 0; b < NB; b++) {
-                        uint4 xv = make_uint4(0u, 0u, 0u, 0u);
-                        if (b * 8 + g < p.rows)
-                            xv = *reinterpret_cast<const uint4*>(xb + b * 8 * C::kXRow + (q * kStageK + j * 32) * 2);
-                        float d[4] = {0.f, 0.f, 0.f, 0.f};
-                        mma16816<T>(d, a0, xv.x, xv.y);
-                        mma16816<T>(d, a1, xv.z, xv.w);
+                        const uint4 xv = *reinterpret_cast<const uint4*>(xb + xrow[b] + (q * kStageK + j * 32) * 2);
+                        float d[4];
+                        mma16816<T, true>(d, a0, xv.x, xv.y);
+                        mma16816<T, false>(d, a1, xv.z, xv.w);
                         acc[b][0] = fmaf(sa, d[0], acc[b][0]);
                         acc[b][1] = fmaf(sa, d[1], acc[b][1]);
                         acc[b][2] = fmaf(sb, d[2], acc[b][2]);
                         acc[b][3] = fmaf(sb, d[3], acc[b][3]);
                         if (kMins) {
-                            const int r0 = b * 8 + 2 * c, at = q * (kStageK / 32) + j;
-                            const float x0 = r0 < p.rows ? sums[r0 * (C::KC / 32) + at] : 0.f;
-                            const float x1 = r0 + 1 < p.rows ? sums[(r0 + 1) * (C::KC / 32) + at] : 0.f;
+                            const float* xs = sums + (q * (kStageK / 32) + j) * p.rows;
+                            const float x0 = xs[srow[b][0]], x1 = xs[srow[b][1]];
                             acc[b][0] = fmaf(ma, x0, acc[b][0]);
                             acc[b][1] = fmaf(ma, x1, acc[b][1]);
                             acc[b][2] = fmaf(mb, x0, acc[b][2]);
@@ -272,8 +286,6 @@ __global__ void __launch_bounds__(kThreads, 1) k_linear_q4(const __grid_constant
                         }
                     }
                 }
-                cur = nxt;
-                nxt = later;
             }
             if (ch + 1 < chunks) store_x(ch + 1);
             __syncthreads();
@@ -312,17 +324,19 @@ __global__ void __launch_bounds__(kThreads, 1) k_linear_q4(const __grid_constant
 
 template <typename T, int NB, bool kMins>
 cudaError_t launch_t(const Q4Launch& a, cudaStream_t stream) {
-    using C = Q4Cfg<NB>;
-    cudaError_t e = cudaFuncSetAttribute(k_linear_q4<T, NB, kMins>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
+    cudaError_t e = cudaFuncSetAttribute(k_linear_q4<T, NB, kMins>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
     if (e != cudaSuccess) return e;
-    Q4Params p{a.x, a.x_stride, a.rows, a.n, a.k, a.group, a.values, a.scales, a.mins, a.out, a.out_stride, 0, 0, 0, 0};
+    Q4Params p{a.x, a.x_stride, a.rows, a.n, a.k, a.group, a.values, a.scales, a.mins, a.out, a.out_stride, 0, 0, 0, 0, 0, 0};
     p.tiles = (a.n + 15) / 16;
     const int grid = std::min(p.tiles, a.num_sms);
     p.R = std::min(kWarps, (p.tiles + grid - 1) / grid);
-    const int stages = (a.k + kStageK - 1) / kStageK;
-    p.S = std::max(1, std::min(std::min(kWarps / p.R, C::kMaxSplit), stages));
+    const int stages = (a.k + kStageK - 1) / kStageK, per_buffer = kXElems / a.rows / kStageK;  // stages of all rows in a buffer
+    p.S = std::max(1, std::min(std::min(kWarps / p.R, per_buffer), stages));
     p.Ks = (stages + p.S - 1) / p.S * kStageK;
-    return launch_pdl(k_linear_q4<T, NB, kMins>, unsigned(grid), kThreads, size_t(C::kSmem), stream, 1, p);
+    p.kcs = std::min(per_buffer / p.S * kStageK, p.Ks);
+    const uintptr_t at = reinterpret_cast<uintptr_t>(a.scales) | reinterpret_cast<uintptr_t>(a.mins);
+    p.fast_scales = a.k % kStageK == 0 && at % 16 == 0;
+    return launch_pdl(k_linear_q4<T, NB, kMins>, unsigned(grid), kThreads, size_t(kSmem), stream, 1, p);
 }
 
 template <typename T, int NB>
