@@ -49,7 +49,7 @@ struct Q4Params {
     void* out;
     int64_t out_stride;
     int tiles, R, S, Ks, kcs;  // row tiles in all; tiles and k slices of a CTA at a time; k per slice, and per x buffer
-    int fast_scales;           // scales (and mins) may be copied a stage's row at a time
+    int whole;                 // 1: k is a multiple of the stage; 2: and the scales are aligned to 16 bytes
 };
 
 __device__ __forceinline__ void cp16(uint32_t dst, const void* src, uint32_t bytes) {
@@ -68,6 +68,12 @@ __device__ __forceinline__ void cp_wait() {
 // Eight 4-bit values as four exact pairs (0, 4), (1, 5), (2, 6), (3, 7), less 8 each where `kSigned`.
 // fp16: 1024 + q has q as its low bits (and 1024 + 16 q the bits four places up, brought back by an
 // exact multiply-add); bf16 holds 128 + q alike.
+// (a & mask) | bits in one instruction.
+__device__ __forceinline__ uint32_t and_or(uint32_t a, uint32_t mask, uint32_t bits) {
+    uint32_t r;
+    asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(r) : "r"(a), "r"(mask), "r"(bits));
+    return r;
+}
 template <bool kSigned>
 __device__ __forceinline__ void widen_f16(uint32_t u, uint32_t (&t)[4]) {
     const __half2 off = __float2half2_rn(kSigned ? -1032.f : -1024.f);
@@ -75,7 +81,7 @@ __device__ __forceinline__ void widen_f16(uint32_t u, uint32_t (&t)[4]) {
 #pragma unroll
     for (int i = 0; i < 2; i++) {
         const uint32_t v = i ? u >> 8 : u;
-        const uint32_t a = (v & 0x000f000fu) | 0x64006400u, b = (v & 0x00f000f0u) | 0x64006400u;
+        const uint32_t a = and_or(v, 0x000f000fu, 0x64006400u), b = and_or(v, 0x00f000f0u, 0x64006400u);
         const __half2 ha = __hadd2(*reinterpret_cast<const __half2*>(&a), off);
         const __half2 hb = __hfma2(*reinterpret_cast<const __half2*>(&b), sixteenth, off16);
         t[2 * i] = *reinterpret_cast<const uint32_t*>(&ha);
@@ -87,7 +93,7 @@ __device__ __forceinline__ void widen_bf16(uint32_t u, uint32_t (&t)[4]) {
     const __nv_bfloat162 off = __float2bfloat162_rn(kSigned ? -136.f : -128.f);
 #pragma unroll
     for (int i = 0; i < 4; i++) {
-        const uint32_t a = ((u >> (4 * i)) & 0x000f000fu) | 0x43004300u;
+        const uint32_t a = and_or(u >> (4 * i), 0x000f000fu, 0x43004300u);
         const __nv_bfloat162 h = __hadd2(*reinterpret_cast<const __nv_bfloat162*>(&a), off);
         t[i] = *reinterpret_cast<const uint32_t*>(&h);
     }
@@ -192,7 +198,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_linear_q4(const __grid_constant
         const int n0 = (base + rt) * 16, k0 = sp * p.Ks, k1 = min(p.k, k0 + p.Ks);
         const int mine = works ? max(0, (k1 - k0 + kStageK - 1) / kStageK) : 0;  // this warp's stages
         // The four 16-byte chunks of a stage this lane copies: rows 4 i + lane / 8, chunk lane % 8 (swizzled, it
-        // differs by 4 between odd and even i).
+        // differs by 4 between odd and even i); the pointers move on by a stage with every copy.
         const uint8_t* src[4];
 #pragma unroll
         for (int i = 0; i < 4; i++)
@@ -200,27 +206,31 @@ __global__ void __launch_bounds__(kThreads, 1) k_linear_q4(const __grid_constant
         const uint32_t dst = ring_addr + uint32_t((lane >> 3) * 128), c0 = uint32_t(((lane & 7) ^ (lane >> 3)) << 4), c1 = c0 ^ 64u;
         // Scales by lanes 0-15, mins by lanes 16-31, a row each.
         const __half* ssrc = (lane < 16 || !kMins ? p.scales : p.mins) + int64_t(min(n0 + (lane & 15), p.n - 1)) * groups + (k0 >> gshift);
-        auto copy = [&](int st, int at) {  // stage st into slot `at`
+        const uint32_t sdst = ring_addr + uint32_t(kWeightBytes + lane * kScaleRow);
+        auto copy = [&](int st, int at) {  // stage st, the next in turn, into the slot at byte `at` of the ring
             if (st < mine) {
-                const int kk = k0 + st * kStageK;
-                const bool in = kk + (lane & 7) * 32 < k1;  // zeros past the slice
-                const uint32_t slot = uint32_t(at * kStageBytes), to = dst + slot;
+                if (p.whole) {  // k is a multiple of the stage: no chunk lies past its slice
 #pragma unroll
-                for (int i = 0; i < 4; i++)
-                    cp16(to + uint32_t(i * 512) + (i & 1 ? c1 : c0), in ? src[i] + st * (kStageK / 2) : p.values, in ? 16u : 0u);
+                    for (int i = 0; i < 4; i++) cp16(dst + uint32_t(at + i * 512) + (i & 1 ? c1 : c0), src[i], 16u);
+                } else {
+                    const bool in = k0 + st * kStageK + (lane & 7) * 32 < k1;  // zeros past the slice
+#pragma unroll
+                    for (int i = 0; i < 4; i++) cp16(dst + uint32_t(at + i * 512) + (i & 1 ? c1 : c0), in ? src[i] : p.values, in ? 16u : 0u);
+                }
                 if (kMins || lane < 16) {
-                    const uint32_t sdst = ring_addr + slot + uint32_t(kWeightBytes + lane * kScaleRow);
-                    const __half* sp_ = ssrc + ((st * kStageK) >> gshift);
-                    if (p.fast_scales) {  // k is a multiple of the stage, so is every slice: whole rows
-                        if (gshift == 5) cp_small<16>(sdst, sp_);
-                        else if (gshift == 6) cp_small<8>(sdst, sp_);
-                        else cp_small<4>(sdst, sp_);
+                    if (p.whole == 2) {  // and the scales' rows are aligned: a row of the stage's at once
+                        if (gshift == 5) cp_small<16>(sdst + uint32_t(at), ssrc);
+                        else if (gshift == 6) cp_small<8>(sdst + uint32_t(at), ssrc);
+                        else cp_small<4>(sdst + uint32_t(at), ssrc);
                     } else {
-                        __half* out = reinterpret_cast<__half*>(ring + slot + kWeightBytes + lane * kScaleRow);
+                        __half* out = reinterpret_cast<__half*>(ring + at + kWeightBytes + lane * kScaleRow);
                         for (int i = 0; i < (kStageK >> gshift); i++)
-                            out[i] = kk + (i << gshift) < k1 ? sp_[i] : __ushort_as_half(0);
+                            out[i] = k0 + st * kStageK + (i << gshift) < k1 ? ssrc[i] : __ushort_as_half(0);
                     }
                 }
+#pragma unroll
+                for (int i = 0; i < 4; i++) src[i] += kStageK / 2;
+                ssrc += kStageK >> gshift;
             }
             cp_commit();
         };
@@ -230,8 +240,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_linear_q4(const __grid_constant
 #pragma unroll
             for (int i = 0; i < 4; i++) acc[b][i] = 0.f;
 
-        for (int st = 0; st < kDepth - 1; st++) copy(st, st);
-        int slot = 0;  // of the stage in turn
+        for (int st = 0; st < kDepth - 1; st++) copy(st, st * kStageBytes);
+        int slot = 0;  // of the stage in turn, in bytes
         load_x(0);
         store_x(0);
         __syncthreads();
@@ -244,15 +254,40 @@ __global__ void __launch_bounds__(kThreads, 1) k_linear_q4(const __grid_constant
                 if (st >= mine) break;
                 cp_wait<kDepth - 2>();
                 __syncwarp();
-                copy(st + kDepth - 1, slot == 0 ? kDepth - 1 : slot - 1);
-                const uint8_t* w = ring + slot * kStageBytes + g * 128 + c * 4;
-                const uint8_t* scr = ring + slot * kStageBytes + kWeightBytes + g * kScaleRow;
-                slot = slot == kDepth - 1 ? 0 : slot + 1;
-                const int swz = g << 4;
+                copy(st + kDepth - 1, slot == 0 ? (kDepth - 1) * kStageBytes : slot - kStageBytes);
+                // Group j's words lie at w ^ 16 j (row g, chunk j ^ g) and 1 KB on (row g + 8).
+                const int w = warp * kDepth * kStageBytes + slot + g * 128 + (g << 4) + c * 4;
+                const uint8_t* scr = ring + slot + kWeightBytes + g * kScaleRow;
+                slot = slot == (kDepth - 1) * kStageBytes ? 0 : slot + kStageBytes;
+                // A row's scales of the stage's eight 32-weight groups, two to a word.
+                const auto scales = [&](int off, uint32_t (&v)[4]) {
+                    const uint4 u = *reinterpret_cast<const uint4*>(scr + off);
+                    if (gshift == 5) {
+                        v[0] = u.x, v[1] = u.y, v[2] = u.z, v[3] = u.w;
+                    } else if (gshift == 6) {
+                        v[0] = __byte_perm(u.x, 0, 0x1010), v[1] = __byte_perm(u.x, 0, 0x3232);
+                        v[2] = __byte_perm(u.y, 0, 0x1010), v[3] = __byte_perm(u.y, 0, 0x3232);
+                    } else {
+                        v[0] = v[1] = __byte_perm(u.x, 0, 0x1010);
+                        v[2] = v[3] = __byte_perm(u.x, 0, 0x3232);
+                    }
+                };
+                const auto pick = [](const uint32_t (&v)[4], int j) {
+                    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&v[j >> 1]));
+                    return j & 1 ? f.y : f.x;
+                };
+                uint32_t sav[4], sbv[4], mav[4], mbv[4];
+                scales(0, sav);
+                scales(8 * kScaleRow, sbv);
+                if (kMins) {
+                    scales(16 * kScaleRow, mav);
+                    scales(24 * kScaleRow, mbv);
+                }
+                const uint8_t* const xq = xb + q * kStageK * 2;
 #pragma unroll
                 for (int j = 0; j < kStageK / 32; j++) {
-                    const uint32_t ua = *reinterpret_cast<const uint32_t*>(w + ((j << 4) ^ swz));
-                    const uint32_t ub = *reinterpret_cast<const uint32_t*>(w + 1024 + ((j << 4) ^ swz));
+                    const uint32_t ua = *reinterpret_cast<const uint32_t*>(smem + (w ^ (j << 4)));
+                    const uint32_t ub = *reinterpret_cast<const uint32_t*>(smem + (w ^ (j << 4)) + 1024);
                     uint32_t ta[4], tb[4];
                     if constexpr (std::is_same<T, __half>::value) {
                         widen_f16<!kMins>(ua, ta);
@@ -261,14 +296,12 @@ __global__ void __launch_bounds__(kThreads, 1) k_linear_q4(const __grid_constant
                         widen_bf16<!kMins>(ua, ta);
                         widen_bf16<!kMins>(ub, tb);
                     }
-                    const __half* sj = reinterpret_cast<const __half*>(scr) + ((j * 32) >> gshift);
-                    const float sa = __half2float(sj[0]), sb = __half2float(sj[8 * kScaleRow / 2]);
-                    const float ma = kMins ? __half2float(sj[16 * kScaleRow / 2]) : 0.f;
-                    const float mb = kMins ? __half2float(sj[24 * kScaleRow / 2]) : 0.f;
+                    const float sa = pick(sav, j), sb = pick(sbv, j);
+                    const float ma = kMins ? pick(mav, j) : 0.f, mb = kMins ? pick(mbv, j) : 0.f;
                     const uint32_t a0[4] = {ta[0], tb[0], ta[1], tb[1]}, a1[4] = {ta[2], tb[2], ta[3], tb[3]};
 #pragma unroll
                     for (int b = 0; b < NB; b++) {
-                        const uint4 xv = *reinterpret_cast<const uint4*>(xb + xrow[b] + (q * kStageK + j * 32) * 2);
+                        const uint4 xv = *reinterpret_cast<const uint4*>(xq + xrow[b] + j * 64);
                         float d[4];
                         mma16816<T, true>(d, a0, xv.x, xv.y);
                         mma16816<T, false>(d, a1, xv.z, xv.w);
@@ -335,7 +368,7 @@ cudaError_t launch_t(const Q4Launch& a, cudaStream_t stream) {
     p.Ks = (stages + p.S - 1) / p.S * kStageK;
     p.kcs = std::min(per_buffer / p.S * kStageK, p.Ks);
     const uintptr_t at = reinterpret_cast<uintptr_t>(a.scales) | reinterpret_cast<uintptr_t>(a.mins);
-    p.fast_scales = a.k % kStageK == 0 && at % 16 == 0;
+    p.whole = a.k % kStageK ? 0 : at % 16 ? 1 : 2;
     return launch_pdl(k_linear_q4<T, NB, kMins>, unsigned(grid), kThreads, size_t(kSmem), stream, 1, p);
 }
 
