@@ -68,7 +68,8 @@ Sizes sizes_of(const CausalLaunch& a) {
     s.tiles = (a.ntok + s.TI - 1) / s.TI;
     // Pieces a tile may be cut into: enough for two rounds of the SMs, one where the tiles fill them.
     const int64_t units = std::max<int64_t>(int64_t(s.tiles) * a.kv_heads, 1);
-    s.lmax = units >= a.num_sms ? 1 : int(std::min<int64_t>(kMaxPieces, (2 * a.num_sms + units - 1) / units));
+    // Calls over few keys are not cut: a merge costs more than the blocks it would spread.
+    s.lmax = units >= a.num_sms || int64_t(a.prefix) + a.nkv <= 4 * kKeys ? 1 : int(std::min<int64_t>(kMaxPieces, (2 * a.num_sms + units - 1) / units));
     return s;
 }
 
@@ -180,6 +181,7 @@ __device__ void plan_item(const PlanParams& p, const uint4* seqs, int2* rng, int
     const int r0 = t * p.TI, n = min(p.TI, p.ntok - r0);
     TileInfo f{};
     bool any = false;
+#pragma unroll 1
     for (int s0 = 0; s0 < p.nseq; s0 += 32) {
         const int s = s0 + lane;
         const uint4 w = s >= p.nseq ? make_uint4(0, 0, 0, 0) : s < kPlanSeqs ? seqs[s] : seq_words(p, s);
@@ -210,8 +212,10 @@ __device__ void plan_item(const PlanParams& p, const uint4* seqs, int2* rng, int
         if (lane == 0) p.info[t] = f;  // live 0: no row of a sequence, no work
         return;
     }
+#pragma unroll 1
     for (int i = lane; i < p.TI; i += 32) rng[i] = make_int2(0, -1);
     __syncwarp();
+#pragma unroll 1
     for (int s0 = 0; s0 < p.nseq; s0 += 32) {
         const int s = s0 + lane;
         const uint4 w = s >= p.nseq ? make_uint4(0, 0, 0, 0) : s < kPlanSeqs ? seqs[s] : seq_words(p, s);
@@ -220,14 +224,17 @@ __device__ void plan_item(const PlanParams& p, const uint4* seqs, int2* rng, int
         if (__popc(m) > 4) {  // many short ones: a lane each
             if (in.x < in.y) {
                 const Seq q(p, w);
+#pragma unroll 1
                 for (int i = in.x; i < in.y; i++) rng[i] = own_range(q.see + (r0 + i - q.q0), q.ks, q.ke, p.window);
             }
         } else {
+#pragma unroll 1
             while (m) {
                 const int src = __ffs(m) - 1;
                 m &= m - 1;
                 const Seq q(p, shfl_words(w, src));
                 const int x = __shfl_sync(0xffffffffu, in.x, src), y = __shfl_sync(0xffffffffu, in.y, src);
+#pragma unroll 1
                 for (int i = x + lane; i < y; i += 32) rng[i] = own_range(q.see + (r0 + i - q.q0), q.ks, q.ke, p.window);
             }
         }
@@ -238,6 +245,7 @@ __device__ void plan_item(const PlanParams& p, const uint4* seqs, int2* rng, int
     int lo_x[2] = {INT_MAX, INT_MAX}, hi_x[2] = {0, 0};
     int end = -1, low = -1;  // running maximum of hi and lo over the rows so far
     bool sorted = true;
+#pragma unroll 1
     for (int i0 = 0; i0 < p.TI; i0 += 32) {
         const int i = i0 + lane;
         const int2 rg = i < n ? rng[i] : make_int2(0, -1);
@@ -286,10 +294,12 @@ __device__ void plan_item(const PlanParams& p, const uint4* seqs, int2* rng, int
     }
     __syncwarp();
     int nblk = 0;
+#pragma unroll 1
     for (int i = lane; i < f.nseg; i += 32) {
         nblk += (seg[i].y - seg[i].x + kKeys - 1) / kKeys;
         p.segs[int64_t(t) * p.TI + i] = seg[i];
     }
+#pragma unroll 1
     for (int i = lane; i < n; i += 32) p.rng[r0 + i] = rng[i];
     f.nblk = __reduce_add_sync(0xffffffffu, nblk) + p.prefix_blocks;
     f.pieces = 1;
@@ -308,9 +318,11 @@ __global__ void __launch_bounds__(1024) k_causal_plan(PlanParams p) {
     hist[tid] = 0;
     pdl_wait();
     pdl_launch();
+#pragma unroll 1
     for (int s = tid; s < min(p.nseq, kPlanSeqs); s += 1024) seqs[s] = seq_words(p, s);
     if (blockIdx.x == 0 && tid == 0) p.head->err = 0;
     __syncthreads();
+#pragma unroll 1
     for (int t = int(blockIdx.x) + warp * ctas; t < p.tiles; t += ctas * 32) plan_item(p, seqs, rng, rng + kMaxItemRows, t, lane);
     if (ctas > 1) cluster_sync();
     else __syncthreads();
@@ -324,11 +336,14 @@ __global__ void __launch_bounds__(1024) k_causal_plan(PlanParams p) {
         if (tid == 0) s_chunk = INT_MAX;
         __syncthreads();
         int most = 1;
+#pragma unroll 1
         for (int t = lane; t < p.tiles; t += 32) most = max(most, s_nblk[t]);
         most = warp_max_i(most);
+#pragma unroll 1
         for (int c0 = max(1, (most + p.lmax - 1) / p.lmax); chunk == INT_MAX; c0 += 32) {
             const int c = min(c0 + warp, most);  // `most`, one piece per item, always fits
             int n = 0;
+#pragma unroll 1
             for (int t = lane; t < p.tiles; t += 32) n += max(1, (s_nblk[t] + c - 1) / c);
             n = __reduce_add_sync(0xffffffffu, n);
             if (lane == 0 && (c == most || int64_t(n) * p.kv_heads <= p.sms)) atomicMin(&s_chunk, c);
@@ -353,6 +368,7 @@ __global__ void __launch_bounds__(1024) k_causal_plan(PlanParams p) {
             sum = __popc(ones);
             before = __popc(ones & ((1u << lane) - 1));
         } else {
+#pragma unroll 1
             for (int l = 0; l < 32; l++) {
                 const int x = __shfl_sync(0xffffffffu, v, l);
                 if ((peers >> l) & 1) {
@@ -364,6 +380,7 @@ __global__ void __launch_bounds__(1024) k_causal_plan(PlanParams p) {
         const int at = lane == leader ? atomicAdd(&hist[bucket], sum) : 0;
         return __shfl_sync(0xffffffffu, at, leader) + before;
     };
+#pragma unroll 1
     for (int t0 = warp * 32; t0 < p.tiles; t0 += 1024) {
         const int t = t0 + lane;
         const int4 f = t < p.tiles ? *reinterpret_cast<const int4*>(p.info + t) : make_int4(0, 0, 0, 0);  // nblk, nseg, pieces, live
@@ -389,6 +406,7 @@ __global__ void __launch_bounds__(1024) k_causal_plan(PlanParams p) {
         if (tid == 1023) p.head->nwork = before + inc;
     }
     __syncthreads();
+#pragma unroll 1
     for (int t0 = warp * 32; t0 < p.tiles; t0 += 1024) {
         const int t = t0 + lane;
         TileInfo f{};
@@ -408,6 +426,7 @@ __global__ void __launch_bounds__(1024) k_causal_plan(PlanParams p) {
     }
     if (p.lmax == 1) return;
     __syncthreads();
+#pragma unroll 1
     for (int t = warp; t < p.tiles; t += 32) {  // cut items: a lane per piece
         const int at = s_nblk[t];
         const TileInfo f = p.info[t];
@@ -415,12 +434,14 @@ __global__ void __launch_bounds__(1024) k_causal_plan(PlanParams p) {
         int sz;
         const int n = pieces_of(f.nblk, sz);
         const int2* seg = p.segs + int64_t(t) * p.TI;
+#pragma unroll 1
         for (int i = lane; i < n; i += 32) {
             const int b0 = i * sz, b1 = min(f.nblk, b0 + sz);
             int s = 0, first = p.prefix_blocks;  // segment s starts at block `first`
             int2 g = make_int2(0, 0);
             if (f.nseg > 0) {
                 g = seg[0];
+#pragma unroll 1
                 for (; s + 1 < f.nseg; s++, g = seg[s]) {
                     const int m = (g.y - g.x + kKeys - 1) / kKeys;
                     if (b0 < first + m) break;
@@ -455,6 +476,7 @@ struct TcParams {
     void* out;
     int64_t q_stride, k_stride, v_stride, pk_stride, pv_stride, out_stride;
     int heads, kv_heads, group, T, TI, ntok, window, prefix, prefix_blocks;
+    uint32_t kv_magic;  // ceil(2^32 / kv_heads)
     float scale_log2e;
     Header* head;
     const int2 *rng, *segs;
@@ -473,6 +495,16 @@ __device__ __forceinline__ bool elect_one() {
     return ok != 0;
 }
 
+// A word with its n lowest bits set (0 below 0, all above 32).
+__device__ __forceinline__ uint32_t low_bits(int n) { return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1u; }
+// The waits' slow parts out of line: the kernel's roles hold dozens of waits, and at an item's turn code that
+// has left the instruction cache costs more than the work.
+__device__ __forceinline__ bool wait_slow(uint64_t* bar, uint32_t parity, int* err) { return mbar_wait(bar, parity, err); }
+__device__ __forceinline__ bool wait_asleep(uint64_t* bar, uint32_t parity, int* err) { return mbar_wait_sleep(bar, parity, err, 32); }
+// The whole warp: every lane tests (the barrier is most often already there), then they agree.
+__device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t parity, int* err) {
+    return __all_sync(0xffffffffu, mbar_poll(bar, parity)) || __all_sync(0xffffffffu, wait_slow(bar, parity, err));
+}
 // Two fp32 operations at a time.
 __device__ __forceinline__ uint64_t pack2(float a, float b) {
     uint64_t r;
@@ -504,18 +536,40 @@ struct Piece {
     int see, ks, ke;
     const int2* segs;
 };
-__device__ __forceinline__ Piece load_piece(const TcParams& p, int id) {
-    const int w = id / p.kv_heads;
-    const int4* src = reinterpret_cast<const int4*>(p.work + w);
-    const int4 a = src[0], b = src[1], c = src[2], d = src[3];
+// A piece's words, asked for one piece ahead so that their way from memory is under the work before.
+struct RawPiece {
+    int4 a, b, c, d;
+    int id;
+};
+// The piece of work item `id` (one per KV head): id / kv_heads, by a multiplication that is at most one off.
+__device__ __forceinline__ int piece_index(const TcParams& p, int id) {
+    if (p.kv_heads == 1) return id;
+    const int q = int(__umulhi(uint32_t(id), p.kv_magic));
+    return q * p.kv_heads > id ? q - 1 : q;
+}
+__device__ __forceinline__ RawPiece fetch_piece(const TcParams& p, int id, int total) {
+    RawPiece r;
+    r.id = id;
+    r.a = r.b = r.c = r.d = make_int4(0, 0, 0, 0);
+    if (id < total) {
+        const int4* src = reinterpret_cast<const int4*>(p.work + piece_index(p, id));
+        r.a = src[0], r.b = src[1], r.c = src[2], r.d = src[3];
+    }
+    return r;
+}
+__device__ __forceinline__ Piece piece_of(const TcParams& p, const RawPiece& r) {
     Piece s;
-    s.kvh = id - w * p.kv_heads;
-    s.tile = a.x, s.b0 = a.y, s.b1 = a.z, s.piece = a.w;
-    s.seg = b.x, s.nseg = b.y, s.pos = b.z, s.end = b.w;
-    s.lo[0] = c.x, s.hi[0] = c.y, s.lo[1] = c.z, s.hi[1] = c.w;
-    s.flags = d.x, s.see = d.y, s.ks = d.z, s.ke = d.w;
-    s.segs = p.segs + int64_t(a.x) * p.TI;
+    s.kvh = r.id - piece_index(p, r.id) * p.kv_heads;
+    s.tile = r.a.x, s.b0 = r.a.y, s.b1 = r.a.z, s.piece = r.a.w;
+    s.seg = r.b.x, s.nseg = r.b.y, s.pos = r.b.z, s.end = r.b.w;
+    s.lo[0] = r.c.x, s.hi[0] = r.c.y, s.lo[1] = r.c.z, s.hi[1] = r.c.w;
+    s.flags = r.d.x, s.see = r.d.y, s.ks = r.d.z, s.ke = r.d.w;
+    s.segs = p.segs + int64_t(r.a.x) * p.TI;
     return s;
+}
+// For the warps short of registers: the next piece's words into the L1 cache.
+__device__ __forceinline__ void prefetch_piece(const TcParams& p, int id, int total) {
+    if (id < total) asm volatile("prefetch.global.L1 [%0];" ::"l"(p.work + piece_index(p, id)));
 }
 // Walks a piece's key blocks: prefix blocks, then blocks of the own-key segments.
 struct Cursor {
@@ -683,12 +737,15 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1)
             bool ok = true;
             int issued = 0, issued_q = 0;
             for (int round = 0, id; ok && (id = piece_id(round)) < total; round++) {
-                const Piece s = load_piece(p, id);
+                const Piece s = piece_of(p, fetch_piece(p, id, total));
+                prefetch_piece(p, piece_id(round + 1), total);
                 if (s.b0 >= s.b1) continue;
                 if (keys) {
-                    if (!mbar_wait_sleep(q_empty, uint32_t(issued_q & 1) ^ 1u, err, 32)) break;
+                    if (!wait_asleep(q_empty, uint32_t(issued_q & 1) ^ 1u, err)) break;
                     mbar_expect_tx(q_full, uint32_t(NT * C::QC * 128 * live_rows));
+#pragma unroll 1
                     for (int x = 0; x < NT; x++)
+#pragma unroll 1
                         for (int c = 0; c < C::QC; c++)
                             tma_load_3d(smem + (x * C::QC + c) * C::kChunk, &mapQ, q_full, c * 64, s.kvh * p.group,
                                         s.tile * p.TI + x * p.T);
@@ -699,12 +756,14 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1)
                     const CUtensorMap* map = c.prefix ? shared : own;
                     for (int h = 0; h < DH; h++) {
                         const int st = issued % ST;
-                        if (!mbar_wait_sleep(&empty[st], uint32_t((issued / ST) & 1) ^ 1u, err, 32)) {
+                        if (!wait_asleep(&empty[st], uint32_t((issued / ST) & 1) ^ 1u, err)) {
                             ok = false;
                             break;
                         }
                         mbar_expect_tx(&full[st], uint32_t(boxes * C::SC * 4096));
+#pragma unroll 1
                         for (int ch = 0; ch < C::SC; ch++)
+#pragma unroll 1
                             for (int b = 0; b < boxes; b++)
                                 tma_load_2d(ring + st * C::kStage + ch * C::kChunk + b * 4096, map, &full[st],
                                             s.kvh * D + h * C::DS + ch * 64, c.row + b * 32);
@@ -714,6 +773,7 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1)
             }
             // Every issued load lands before the CTA exits, also after an error.
             if (issued_q > 0) drain(q_full, uint32_t((issued_q - 1) & 1));
+#pragma unroll 1
             for (int st = 0; st < ST; st++) {
                 const int n = issued / ST + (st < issued % ST ? 1 : 0);
                 if (n > 0) drain(&full[st], uint32_t((n - 1) & 1));
@@ -728,14 +788,15 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1)
         const uint64_t v_desc = sw128_desc(smem_u32(smem + C::kOffV), C::kChunk, 1024);
         bool ok = true;
         auto wait = [&](uint64_t* bar, uint32_t parity) {
-            if (!__all_sync(0xffffffffu, mbar_poll(bar, parity))) ok = __all_sync(0xffffffffu, mbar_wait(bar, parity, err));
+            ok = wait_warp(bar, parity, err);
             return ok;
         };
         int nq = 0, nk = 0, nv = 0;            // Q tiles, K stages and V stages used so far
         int ns[2] = {0, 0}, np[2] = {0, 0};    // S and PV products per S buffer (NT 2) or in all (NT 1, [0])
         int no[2] = {0, 0};                    // items with an O, per tile
         for (int round = 0, id; ok && (id = piece_id(round)) < total; round++) {
-            const Piece s = load_piece(p, id);
+            const Piece s = piece_of(p, fetch_piece(p, id, total));
+            prefetch_piece(p, piece_id(round + 1), total);
             if (s.b0 >= s.b1) continue;
             if (!wait(q_full, uint32_t(nq & 1))) break;
             nq++;
@@ -757,6 +818,7 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1)
                         if (!wait(&v_full[vs], uint32_t((nv / ST) & 1))) break;
                         if (prev_nv & 15) {
                             // Rows behind the block's last key, up to the product's step.
+#pragma unroll 1
                             for (int i = lane; i < (steps * 16 - prev_nv) * C::SC * 8; i += 32) {
                                 const int rr = prev_nv + i / (C::SC * 8), ch = (i >> 3) % C::SC;
                                 *reinterpret_cast<uint4*>(smem + C::kOffV + vs * C::kStage + ch * C::kChunk + rr * 128 + (i & 7) * 16) =
@@ -842,7 +904,8 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1)
                             const int st = (nv + h) % ST;
                             if (!wait(&v_full[st], uint32_t(((nv + h) / ST) & 1))) break;
                             if (prev_nv & 15) {
-                                for (int i = lane; i < (steps * 16 - prev_nv) * C::SC * 8; i += 32) {
+    #pragma unroll 1
+                            for (int i = lane; i < (steps * 16 - prev_nv) * C::SC * 8; i += 32) {
                                     const int rr = prev_nv + i / (C::SC * 8), ch = (i >> 3) % C::SC;
                                     *reinterpret_cast<uint4*>(smem + C::kOffV + st * C::kStage + ch * C::kChunk + rr * 128 + (i & 7) * 16) =
                                         make_uint4(0u, 0u, 0u, 0u);
@@ -904,17 +967,26 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1)
         const uint32_t lane_base = tmem + (uint32_t(quad * 32) << 16);
         const int token = r / p.group;
         bool ok = true;
-        // Every lane tests (the barrier is most often already there), then they agree.
         auto wait = [&](uint64_t* bar, uint32_t parity) {
-            if (!__all_sync(0xffffffffu, mbar_poll(bar, parity))) ok = __all_sync(0xffffffffu, mbar_wait(bar, parity, err));
+            ok = __all_sync(0xffffffffu, mbar_poll(bar, parity)) || __all_sync(0xffffffffu, mbar_wait(bar, parity, err));
             return ok;
         };
         int nb = 0, no = 0;  // blocks and items with an O so far
-        for (int round = 0, id; ok && (id = piece_id(round)) < total; round++) {
-            const Piece s = load_piece(p, id);
-            const int row = s.tile * p.TI + x * p.T + token;
-            int2 rg = make_int2(0, -1);
-            if (r < live_rows && row < p.ntok) rg = s.flags & 4 ? own_range(s.see + (row - s.tile * p.TI), s.ks, s.ke, p.window) : p.rng[row];
+        int round = 0;
+        RawPiece next = fetch_piece(p, piece_id(0), total);
+        // The row of the piece in `next`, and its range where the plan wrote it.
+        const auto row_of = [&]() { return next.a.x * p.TI + x * p.T + token; };
+        const auto range_of = [&]() {
+            const bool stored = next.id < total && r < live_rows && row_of() < p.ntok && !(next.d.x & 4);
+            return stored ? p.rng[row_of()] : make_int2(0, -1);
+        };
+        int2 range = range_of();
+        while (ok && next.id < total) {
+            const Piece s = piece_of(p, next);
+            const int row = row_of();
+            int2 rg = range;
+            if ((s.flags & 4) && r < live_rows && row < p.ntok) rg = own_range(s.see + (row - s.tile * p.TI), s.ks, s.ke, p.window);
+            next = fetch_piece(p, piece_id(++round), total);
             // Rows of no query take every score: never stored.
             const bool in = rg.y >= 0;
             const int row_lo = in ? rg.x : 0, row_hi = in ? rg.y : INT_MAX;
@@ -960,8 +1032,12 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1)
                         // length of this one's end).
                         const int lo = prefix ? 0 : row_lo - key, hi = (in ? prefix ? lim : min(row_hi, lim) : INT_MAX) - key;
 #pragma unroll
-                        for (int i = 0; i < kKeys; i++)
-                            if (i < lo || i >= hi) sr[i] = __float_as_uint(-INFINITY);
+                        for (int w = 0; w < kKeys / 32; w++) {  // bit i: key 32 w + i is the row's
+                            const uint32_t bits = low_bits(hi - 32 * w) & ~low_bits(lo - 32 * w);
+#pragma unroll
+                            for (int i = 0; i < 32; i++)
+                                if (!(bits & (1u << i))) sr[32 * w + i] = __float_as_uint(-INFINITY);
+                        }
                     }
                     float mp[4];  // four independent chains of three-way maxima
 #pragma unroll
@@ -1020,6 +1096,7 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1)
             const int count = nb - nb0;
             if (!ok) break;
             // ---- output
+            range = range_of();  // of the next piece
             const int head = s.kvh * p.group + (r - token * p.group);
             const int64_t at = (int64_t(s.piece) * p.ntok + row) * p.heads + head;  // of a partial row
             const float inv = s.piece >= 0 ? 1.0f : l == 0.f ? 0.f : 1.0f / l;
@@ -1089,32 +1166,39 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1)
 struct MergeParams {
     void* out;
     int64_t out_stride;
-    int heads, ntok, TI;
+    int heads, ntok, TI, lmax;
     const int2* rng;
     const TileInfo* info;
     const float* o;
     const float2* ml;
 };
 
-// One CTA of 128 threads per (row, head): out = sum_c 2^(m_c - m) O_c / sum_c 2^(m_c - m) l_c, m the
-// largest m_c.  Thread c weighs piece c; the warps add every fourth piece each, joined in order.
+// One CTA of 256 threads per (row, head): out = sum_c 2^(m_c - m) O_c / sum_c 2^(m_c - m) l_c, m the
+// largest m_c.  Thread c weighs piece c; the warps add every eighth piece each, joined in order.  The
+// loads that say whether and how many pieces there are go out together with the pieces' maxima.
 template <typename E, int D>
-__global__ void __launch_bounds__(128) k_causal_merge(MergeParams p) {
-    __shared__ float w[kMaxPieces], red_m[4], red_l[4], part[4][D];
+__global__ void __launch_bounds__(256) k_causal_merge(MergeParams p) {
+    __shared__ float w[kMaxPieces], red_m[8], red_l[8], part[8][D];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     pdl_wait();
     pdl_launch();
     const int row = int(blockIdx.x) / p.heads, head = int(blockIdx.x) - row * p.heads;
-    const TileInfo* f = p.info + row / p.TI;
-    const int n = f->pieces;
-    if (n <= 1 || !f->live || (!f->simple && p.rng[row].y < 0)) return;
     const int64_t step = int64_t(p.ntok) * p.heads, id = int64_t(row) * p.heads + head;
-    const float2 ml = tid < n ? p.ml[tid * step + id] : make_float2(-INFINITY, 0.f);
+    const TileInfo* f = p.info + row / p.TI;
+    const int4 info = *reinterpret_cast<const int4*>(f);  // nblk, nseg, pieces, live
+    const int simple = f->simple;
+    const int2 rng = p.rng[row];
+    float2 ml = tid < p.lmax ? p.ml[tid * step + id] : make_float2(-INFINITY, 0.f);
+    const int n = info.z;
+    if (n <= 1 || !info.w || (!simple && rng.y < 0)) return;
+    if (tid >= n) ml = make_float2(-INFINITY, 0.f);
     const bool nan = __syncthreads_or(isnan(ml.x));
     float m = warp_max(ml.x);
     if (lane == 0) red_m[warp] = m;
     __syncthreads();
-    m = fmaxf(fmaxf(red_m[0], red_m[1]), fmaxf(red_m[2], red_m[3]));
+    m = red_m[0];
+#pragma unroll
+    for (int i = 1; i < 8; i++) m = fmaxf(m, red_m[i]);
     const float wt = ml.x == -INFINITY ? 0.f : ex2_approx(ml.x - m);  // 0: no visible key, and no row was left
     if (tid < n) w[tid] = wt;
     const float l = warp_sum(wt * ml.y);
@@ -1125,7 +1209,7 @@ __global__ void __launch_bounds__(128) k_causal_merge(MergeParams p) {
 #pragma unroll
     for (int i = 0; i < P; i++) acc[i] = 0.f;
 #pragma unroll 4
-    for (int c = warp; c < n; c += 4) {
+    for (int c = warp; c < n; c += 8) {
         const float wc = w[c];
         const float2* src = reinterpret_cast<const float2*>(p.o + (c * step + id) * D + lane * P);
 #pragma unroll
@@ -1138,16 +1222,17 @@ __global__ void __launch_bounds__(128) k_causal_merge(MergeParams p) {
 #pragma unroll
     for (int i = 0; i < P; i++) part[warp][lane * P + i] = acc[i];
     __syncthreads();
-    const float lt = (red_l[0] + red_l[1]) + (red_l[2] + red_l[3]);
-    const float inv = nan ? NAN : lt == 0.f ? 0.f : 1.0f / lt;
     if (tid < D / 2) {
-        float v[2];
+        float lt = 0.f, v[2] = {0.f, 0.f};
 #pragma unroll
-        for (int i = 0; i < 2; i++) {
-            const int d = 2 * tid + i;
-            v[i] = ((part[0][d] + part[1][d]) + (part[2][d] + part[3][d])) * inv;
+        for (int i = 0; i < 8; i++) {
+            lt += red_l[i];
+            v[0] += part[i][2 * tid];
+            v[1] += part[i][2 * tid + 1];
         }
-        reinterpret_cast<uint32_t*>(static_cast<E*>(p.out) + row * p.out_stride + int64_t(head) * D)[tid] = float_to_pair<E>(v[0], v[1]);
+        const float inv = nan ? NAN : lt == 0.f ? 0.f : 1.0f / lt;
+        reinterpret_cast<uint32_t*>(static_cast<E*>(p.out) + row * p.out_stride + int64_t(head) * D)[tid] =
+            float_to_pair<E>(v[0] * inv, v[1] * inv);
     }
 }
 
@@ -1155,8 +1240,8 @@ __global__ void __launch_bounds__(128) k_causal_merge(MergeParams p) {
 template <typename E, int D>
 cudaError_t launch_t(const CausalLaunch& a, const Sizes& s, const Layout& l, cudaStream_t stream) {
     using C = Cfg<D>;
-    // Per device the kernel needs its shared-memory limit raised; the call is cheap and may run during a capture.
-    cudaError_t e = cudaFuncSetAttribute(k_causal_tc<E, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
+    static std::atomic<uint64_t> devices{0};
+    cudaError_t e = allow_smem(k_causal_tc<E, D>, C::kSmem, devices);
     if (e != cudaSuccess) return e;
     const __half *q = static_cast<const __half*>(a.q), *k = static_cast<const __half*>(a.k), *v = static_cast<const __half*>(a.v);
     const __half *pk = static_cast<const __half*>(a.pk), *pv = static_cast<const __half*>(a.pv);
@@ -1172,14 +1257,14 @@ cudaError_t launch_t(const CausalLaunch& a, const Sizes& s, const Layout& l, cud
                          !encode_fp16_map(&mpv, pv, kw, uint64_t(a.prefix), 64, 32, uint64_t(a.pv_stride))))
         return cudaErrorInvalidValue;
     TcParams p{a.q, a.k, a.v, a.pk, a.pv, a.out, a.q_stride, a.k_stride, a.v_stride, a.pk_stride, a.pv_stride, a.out_stride,
-               a.heads, a.kv_heads, s.group, s.T, s.TI, a.ntok, std::min(a.window, 1 << 30), a.prefix, (a.prefix + kKeys - 1) / kKeys, a.scale * kLog2e,
+               a.heads, a.kv_heads, s.group, s.T, s.TI, a.ntok, std::min(a.window, 1 << 30), a.prefix, (a.prefix + kKeys - 1) / kKeys, uint32_t(((uint64_t(1) << 32) + a.kv_heads - 1) / a.kv_heads), a.scale * kLog2e,
                l.head, l.rng, l.segs, l.work, l.o, l.ml};
     const int64_t most = s.lmax > 1 ? a.num_sms : int64_t(s.tiles) * a.kv_heads;
     e = launch_pdl(k_causal_tc<E, D>, unsigned(std::min<int64_t>(a.num_sms, most)), C::kThreads, size_t(C::kSmem), stream, 1, mq, mk, mv,
                    mpk, mpv, p);
     if (e != cudaSuccess || s.lmax == 1) return e;
-    MergeParams mp{a.out, a.out_stride, a.heads, a.ntok, s.TI, l.rng, l.info, l.o, l.ml};
-    return launch_pdl(k_causal_merge<E, D>, unsigned(int64_t(a.ntok) * a.heads), 128, 0, stream, 1, mp);
+    MergeParams mp{a.out, a.out_stride, a.heads, a.ntok, s.TI, s.lmax, l.rng, l.info, l.o, l.ml};
+    return launch_pdl(k_causal_merge<E, D>, unsigned(int64_t(a.ntok) * a.heads), 256, 0, stream, 1, mp);
 }
 
 template <typename E>
@@ -1201,7 +1286,8 @@ cudaError_t launch_causal(const CausalLaunch& a, cudaStream_t stream) {
                   (a.prefix + kKeys - 1) / kKeys, s.lmax, a.num_sms, l.head, l.rng, l.segs, l.info, l.work};
     // A warp plans an item; up to 8 CTAs share them.
     const int ctas = s.tiles <= 32 ? 1 : s.tiles <= 64 ? 2 : s.tiles <= 128 ? 4 : 8;
-    cudaError_t e = cudaFuncSetAttribute(k_causal_plan, cudaFuncAttributeMaxDynamicSharedMemorySize, int(plan_smem(kPlanSeqs)));
+    static std::atomic<uint64_t> devices{0};
+    cudaError_t e = allow_smem(k_causal_plan, int(plan_smem(kPlanSeqs)), devices);
     if (e == cudaSuccess) e = launch_pdl(k_causal_plan, unsigned(ctas), 1024, plan_smem(a.nseq), stream, ctas, pp);
     if (e != cudaSuccess) return e;
     return a.bf16 ? launch_e<__nv_bfloat16>(a, s, l, stream) : launch_e<__half>(a, s, l, stream);

@@ -8,8 +8,8 @@
 // but for a few rows).  Every 32 weights the integer sums are scaled in fp32: acc += scale * sum, plus
 // min * (sum of x) with minima, so no weight is ever rounded.
 //
-// One CTA per SM, 16 warps.  A warp owns 16 output columns n (a row tile) and, where the CTA's tiles
-// leave warps over, one of S slices of k; the slices' sums are joined in shared memory in order.
+// One CTA per SM, 16 warps.  A warp owns 16 output columns n (a row tile) or, where the CTA has fewer
+// tiles than warps, a part of k of one; the parts' sums are joined in shared memory in order.
 // Stage of a warp: 16 rows x 256 weights (16 x 128 bytes, chunk c of row r at c ^ (r & 7), so that the
 // 32-bit reads of a fragment hit 32 banks).  The lane's word of a 32-weight group holds the group's
 // elements 8 c .. 8 c + 7; their nibbles come out as pairs (0, 4), (1, 5), (2, 6), (3, 7), which x is
@@ -35,8 +35,8 @@ constexpr int kDepth = 3;
 constexpr int kXElems = 16384;                 // elements of x per buffer, all rows
 constexpr int kOffX = kWarps * kDepth * kStageBytes;
 constexpr int kXBytes = kXElems * 2 + kQ4MaxRows * 64;  // rows are 64 bytes over a multiple of 128 apart
-constexpr int kOffSum = kOffX + 2 * kXBytes;            // sums of x per 32 elements and row
-constexpr int kSumBytes = kXElems / 32 * 4;
+constexpr int kOffSum = kOffX + 2 * kXBytes;            // sums of x per 32 elements and row, 8 NB rows apart
+constexpr int kSumBytes = 4096;
 constexpr int kSmem = kOffSum + 2 * kSumBytes;
 static_assert(kSmem <= 227 * 1024, "shared memory");
 
@@ -48,7 +48,7 @@ struct Q4Params {
     const __half *scales, *mins;
     void* out;
     int64_t out_stride;
-    int tiles, R, S, Ks, kcs;  // row tiles in all; tiles and k slices of a CTA at a time; k per slice, and per x buffer
+    int tiles, R, kc;          // row tiles in all; tiles of a CTA at a time; k per x buffer
     int whole;                 // 1: k is a multiple of the stage; 2: and the scales are aligned to 16 bytes
 };
 
@@ -130,29 +130,41 @@ __global__ void __launch_bounds__(kThreads, 1) k_linear_q4(const __grid_constant
     extern __shared__ __align__(128) uint8_t smem[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int g = lane >> 2, c = lane & 3;
-    const int rt = warp % p.R, sp = warp / p.R;
+    // Warp w takes part w / R of tile w % R; the first tiles have a part more where 16 is no multiple of R.
+    const int rt = warp % p.R, part = warp / p.R, parts = kWarps / p.R + (rt < kWarps % p.R ? 1 : 0);
     const int t_begin = int(int64_t(blockIdx.x) * p.tiles / gridDim.x), t_end = int(int64_t(blockIdx.x + 1) * p.tiles / gridDim.x);
-    const int chunk_stages = p.kcs / kStageK;
-    const int stages = (p.Ks + kStageK - 1) / kStageK, chunks = (stages + chunk_stages - 1) / chunk_stages;
+    // k runs in chunks of an x buffer, a chunk's stages are shared out over the parts.
+    const int stages = (p.k + kStageK - 1) / kStageK, chunk_stages = p.kc / kStageK, chunks = (stages + chunk_stages - 1) / chunk_stages;
+    const auto part_of = [&](int ch, int& from, int& to) {
+        const int lo = ch * chunk_stages, n = min(stages - lo, chunk_stages);
+        from = lo + n * part / parts;
+        to = lo + n * (part + 1) / parts;
+    };
     const int groups = p.k / p.group, gshift = p.group == 32 ? 5 : p.group == 64 ? 6 : 7;
-    const int x_row = p.S * p.kcs * 2 + 64;  // bytes between x's rows in a buffer
+    const int x_row = p.kc * 2 + 64;  // bytes between x's rows in a buffer
     uint8_t* ring = smem + warp * kDepth * kStageBytes;
     const uint32_t ring_addr = smem_u32(ring);
     pdl_wait();
     pdl_launch();
 
-    // x of buffer `i` (elements [s Ks + i kcs, + kcs) of every slice s): up to four 16-byte units per thread.
+    // x of chunk `i`: up to four 16-byte units per thread.
     constexpr int kUnits = kXElems / 8 / kThreads;
-    const int units_row = p.S * p.kcs / 8;
+    const int units_row = p.kc / 8;
     uint4 xr[kUnits];
+    int ur[kUnits], ue[kUnits];  // each unit's row and element
+#pragma unroll
+    for (int u = 0; u < kUnits; u++) {
+        const int id = u * kThreads + threadIdx.x;
+        ur[u] = id / units_row;
+        ue[u] = (id - ur[u] * units_row) * 8;
+    }
     auto load_x = [&](int i) {
 #pragma unroll
         for (int u = 0; u < kUnits; u++) {
-            const int id = u * kThreads + threadIdx.x, r = id / units_row, e = (id - r * units_row) * 8;
-            const int s = e / p.kcs, off = i * p.kcs + (e - s * p.kcs), kk = s * p.Ks + off;
+            const int kk = i * p.kc + ue[u];
             xr[u] = make_uint4(0u, 0u, 0u, 0u);
-            if (r < p.rows && off < p.Ks && kk < p.k)
-                xr[u] = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.x) + r * p.x_stride + kk);
+            if (ur[u] < p.rows && kk < p.k)
+                xr[u] = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.x) + ur[u] * p.x_stride + kk);
         }
     };
     auto store_x = [&](int i) {
@@ -160,7 +172,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_linear_q4(const __grid_constant
         float* sums = reinterpret_cast<float*>(smem + kOffSum + (i & 1) * kSumBytes);
 #pragma unroll
         for (int u = 0; u < kUnits; u++) {
-            const int id = u * kThreads + threadIdx.x, r = id / units_row, e = (id - r * units_row) * 8;
+            const int r = ur[u], e = ue[u];
             const uint4 v = xr[u];
             if (kMins) {
                 float s = 0.f;
@@ -172,7 +184,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_linear_q4(const __grid_constant
                 }
                 s += __shfl_xor_sync(0xffffffffu, s, 1);
                 s += __shfl_xor_sync(0xffffffffu, s, 2);
-                if (r < p.rows && (threadIdx.x & 3) == 0) sums[(e / 32) * p.rows + r] = s;
+                if (r < p.rows && (threadIdx.x & 3) == 0) sums[(e / 32) * 8 * NB + r] = s;
             }
             if (r < p.rows) {
                 uint4 o;  // pairs (0, 4), (1, 5), (2, 6), (3, 7)
@@ -185,52 +197,55 @@ __global__ void __launch_bounds__(kThreads, 1) k_linear_q4(const __grid_constant
         }
     };
     // Rows past the last repeat it: their products are not stored.
-    int xrow[NB], srow[NB][2];
+    int xrow[NB];
 #pragma unroll
-    for (int b = 0; b < NB; b++) {
-        xrow[b] = min(b * 8 + g, p.rows - 1) * x_row + c * 16;
-        srow[b][0] = min(b * 8 + 2 * c, p.rows - 1);
-        srow[b][1] = min(b * 8 + 2 * c + 1, p.rows - 1);
-    }
+    for (int b = 0; b < NB; b++) xrow[b] = min(b * 8 + g, p.rows - 1) * x_row + c * 16;
 
     for (int base = t_begin; base < t_end; base += p.R) {
-        const bool works = sp < p.S && base + rt < t_end;
-        const int n0 = (base + rt) * 16, k0 = sp * p.Ks, k1 = min(p.k, k0 + p.Ks);
-        const int mine = works ? max(0, (k1 - k0 + kStageK - 1) / kStageK) : 0;  // this warp's stages
+        const bool works = base + rt < t_end;
+        const int n0 = (base + rt) * 16;
+        // The stages copied so far: the next one, the end of its chunk's part and the chunk.
+        int cs = 0, ce = 0, cch = -1;
+        const auto settle = [&]() {  // past empty parts; cch == chunks: nothing is left
+            while (cs >= ce && ++cch < chunks) part_of(cch, cs, ce);
+        };
+        if (works) settle();
+        else cch = chunks;
         // The four 16-byte chunks of a stage this lane copies: rows 4 i + lane / 8, chunk lane % 8 (swizzled, it
         // differs by 4 between odd and even i); the pointers move on by a stage with every copy.
         const uint8_t* src[4];
 #pragma unroll
         for (int i = 0; i < 4; i++)
-            src[i] = p.values + int64_t(min(n0 + i * 4 + (lane >> 3), p.n - 1)) * (p.k >> 1) + ((k0 + (lane & 7) * 32) >> 1);
+            src[i] = p.values + int64_t(min(n0 + i * 4 + (lane >> 3), p.n - 1)) * (p.k >> 1) + (lane & 7) * 16;
         const uint32_t dst = ring_addr + uint32_t((lane >> 3) * 128), c0 = uint32_t(((lane & 7) ^ (lane >> 3)) << 4), c1 = c0 ^ 64u;
         // Scales by lanes 0-15, mins by lanes 16-31, a row each.
-        const __half* ssrc = (lane < 16 || !kMins ? p.scales : p.mins) + int64_t(min(n0 + (lane & 15), p.n - 1)) * groups + (k0 >> gshift);
+        const __half* ssrc = (lane < 16 || !kMins ? p.scales : p.mins) + int64_t(min(n0 + (lane & 15), p.n - 1)) * groups;
         const uint32_t sdst = ring_addr + uint32_t(kWeightBytes + lane * kScaleRow);
-        auto copy = [&](int st, int at) {  // stage st, the next in turn, into the slot at byte `at` of the ring
-            if (st < mine) {
-                if (p.whole) {  // k is a multiple of the stage: no chunk lies past its slice
+        auto copy = [&](int at) {  // the next stage in turn, into the slot at byte `at` of the ring
+            if (cch < chunks) {
+                const int off = cs * (kStageK / 2);
+                if (p.whole) {  // k is a multiple of the stage
 #pragma unroll
-                    for (int i = 0; i < 4; i++) cp16(dst + uint32_t(at + i * 512) + (i & 1 ? c1 : c0), src[i], 16u);
+                    for (int i = 0; i < 4; i++) cp16(dst + uint32_t(at + i * 512) + (i & 1 ? c1 : c0), src[i] + off, 16u);
                 } else {
-                    const bool in = k0 + st * kStageK + (lane & 7) * 32 < k1;  // zeros past the slice
+                    const bool in = cs * kStageK + (lane & 7) * 32 < p.k;  // zeros past k
 #pragma unroll
-                    for (int i = 0; i < 4; i++) cp16(dst + uint32_t(at + i * 512) + (i & 1 ? c1 : c0), in ? src[i] : p.values, in ? 16u : 0u);
+                    for (int i = 0; i < 4; i++) cp16(dst + uint32_t(at + i * 512) + (i & 1 ? c1 : c0), in ? src[i] + off : p.values, in ? 16u : 0u);
                 }
                 if (kMins || lane < 16) {
+                    const __half* from = ssrc + ((cs * kStageK) >> gshift);
                     if (p.whole == 2) {  // and the scales' rows are aligned: a row of the stage's at once
-                        if (gshift == 5) cp_small<16>(sdst + uint32_t(at), ssrc);
-                        else if (gshift == 6) cp_small<8>(sdst + uint32_t(at), ssrc);
-                        else cp_small<4>(sdst + uint32_t(at), ssrc);
+                        if (gshift == 5) cp_small<16>(sdst + uint32_t(at), from);
+                        else if (gshift == 6) cp_small<8>(sdst + uint32_t(at), from);
+                        else cp_small<4>(sdst + uint32_t(at), from);
                     } else {
                         __half* out = reinterpret_cast<__half*>(ring + at + kWeightBytes + lane * kScaleRow);
                         for (int i = 0; i < (kStageK >> gshift); i++)
-                            out[i] = k0 + st * kStageK + (i << gshift) < k1 ? ssrc[i] : __ushort_as_half(0);
+                            out[i] = cs * kStageK + (i << gshift) < p.k ? from[i] : __ushort_as_half(0);
                     }
                 }
-#pragma unroll
-                for (int i = 0; i < 4; i++) src[i] += kStageK / 2;
-                ssrc += kStageK >> gshift;
+                cs++;
+                settle();
             }
             cp_commit();
         };
@@ -240,21 +255,22 @@ __global__ void __launch_bounds__(kThreads, 1) k_linear_q4(const __grid_constant
 #pragma unroll
             for (int i = 0; i < 4; i++) acc[b][i] = 0.f;
 
-        for (int st = 0; st < kDepth - 1; st++) copy(st, st * kStageBytes);
+        for (int i = 0; i < kDepth - 1; i++) copy(i * kStageBytes);
         int slot = 0;  // of the stage in turn, in bytes
         load_x(0);
         store_x(0);
         __syncthreads();
         for (int ch = 0; ch < chunks; ch++) {
             if (ch + 1 < chunks) load_x(ch + 1);
-            const uint8_t* xb = smem + kOffX + (ch & 1) * kXBytes + sp * p.kcs * 2;
-            const float* sums = reinterpret_cast<const float*>(smem + kOffSum + (ch & 1) * kSumBytes) + sp * p.kcs / 32 * p.rows;
-            for (int q = 0; q < chunk_stages; q++) {
-                const int st = ch * chunk_stages + q;
-                if (st >= mine) break;
+            const uint8_t* xb = smem + kOffX + (ch & 1) * kXBytes;
+            const float* sums = reinterpret_cast<const float*>(smem + kOffSum + (ch & 1) * kSumBytes) + 2 * c;
+            int from = 0, to = 0;
+            if (works) part_of(ch, from, to);
+            for (int st = from; st < to; st++) {
+                const int q = st - ch * chunk_stages;
                 cp_wait<kDepth - 2>();
                 __syncwarp();
-                copy(st + kDepth - 1, slot == 0 ? (kDepth - 1) * kStageBytes : slot - kStageBytes);
+                copy(slot == 0 ? (kDepth - 1) * kStageBytes : slot - kStageBytes);
                 // Group j's words lie at w ^ 16 j (row g, chunk j ^ g) and 1 KB on (row g + 8).
                 const int w = warp * kDepth * kStageBytes + slot + g * 128 + (g << 4) + c * 4;
                 const uint8_t* scr = ring + slot + kWeightBytes + g * kScaleRow;
@@ -310,12 +326,12 @@ __global__ void __launch_bounds__(kThreads, 1) k_linear_q4(const __grid_constant
                         acc[b][2] = fmaf(sb, d[2], acc[b][2]);
                         acc[b][3] = fmaf(sb, d[3], acc[b][3]);
                         if (kMins) {
-                            const float* xs = sums + (q * (kStageK / 32) + j) * p.rows;
-                            const float x0 = xs[srow[b][0]], x1 = xs[srow[b][1]];
-                            acc[b][0] = fmaf(ma, x0, acc[b][0]);
-                            acc[b][1] = fmaf(ma, x1, acc[b][1]);
-                            acc[b][2] = fmaf(mb, x0, acc[b][2]);
-                            acc[b][3] = fmaf(mb, x1, acc[b][3]);
+                            // Sums of rows 8 b + 2 c and the next (what lies there past the last row is not stored).
+                            const float2 xs = *reinterpret_cast<const float2*>(sums + (q * (kStageK / 32) + j) * 8 * NB + b * 8);
+                            acc[b][0] = fmaf(ma, xs.x, acc[b][0]);
+                            acc[b][1] = fmaf(ma, xs.y, acc[b][1]);
+                            acc[b][2] = fmaf(mb, xs.x, acc[b][2]);
+                            acc[b][3] = fmaf(mb, xs.y, acc[b][3]);
                         }
                     }
                 }
@@ -325,23 +341,22 @@ __global__ void __launch_bounds__(kThreads, 1) k_linear_q4(const __grid_constant
         }
         cp_wait<0>();
         __syncwarp();
-        // Sums of the k slices, in order, through the ring (every stage has been read).
+        // Sums of the parts, in order, through the ring (every stage has been read).
         float4* red = reinterpret_cast<float4*>(smem);
-        if (p.S > 1) {
-            __syncthreads();
-            if (works && sp > 0)
+        if (p.R < kWarps) {
+            if (works && part > 0)
 #pragma unroll
                 for (int b = 0; b < NB; b++) red[(warp * NB + b) * 32 + lane] = make_float4(acc[b][0], acc[b][1], acc[b][2], acc[b][3]);
             __syncthreads();
-            if (works && sp == 0)
-                for (int s = 1; s < p.S; s++)
+            if (works && part == 0)
+                for (int i = 1; i < parts; i++)
 #pragma unroll
                     for (int b = 0; b < NB; b++) {
-                        const float4 v = red[((s * p.R + rt) * NB + b) * 32 + lane];
+                        const float4 v = red[((i * p.R + rt) * NB + b) * 32 + lane];
                         acc[b][0] += v.x, acc[b][1] += v.y, acc[b][2] += v.z, acc[b][3] += v.w;
                     }
         }
-        if (works && sp == 0) {
+        if (works && part == 0) {
             T* out = static_cast<T*>(p.out);
 #pragma unroll
             for (int b = 0; b < NB; b++)
@@ -357,16 +372,17 @@ __global__ void __launch_bounds__(kThreads, 1) k_linear_q4(const __grid_constant
 
 template <typename T, int NB, bool kMins>
 cudaError_t launch_t(const Q4Launch& a, cudaStream_t stream) {
-    cudaError_t e = cudaFuncSetAttribute(k_linear_q4<T, NB, kMins>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+    static std::atomic<uint64_t> devices{0};
+    cudaError_t e = allow_smem(k_linear_q4<T, NB, kMins>, kSmem, devices);
     if (e != cudaSuccess) return e;
-    Q4Params p{a.x, a.x_stride, a.rows, a.n, a.k, a.group, a.values, a.scales, a.mins, a.out, a.out_stride, 0, 0, 0, 0, 0, 0};
+    Q4Params p{a.x, a.x_stride, a.rows, a.n, a.k, a.group, a.values, a.scales, a.mins, a.out, a.out_stride, 0, 0, 0, 0};
     p.tiles = (a.n + 15) / 16;
     const int grid = std::min(p.tiles, a.num_sms);
     p.R = std::min(kWarps, (p.tiles + grid - 1) / grid);
-    const int stages = (a.k + kStageK - 1) / kStageK, per_buffer = kXElems / a.rows / kStageK;  // stages of all rows in a buffer
-    p.S = std::max(1, std::min(std::min(kWarps / p.R, per_buffer), stages));
-    p.Ks = (stages + p.S - 1) / p.S * kStageK;
-    p.kcs = std::min(per_buffer / p.S * kStageK, p.Ks);
+    const int stages = (a.k + kStageK - 1) / kStageK;
+    int per_buffer = kXElems / a.rows / kStageK;  // stages of all rows in an x buffer
+    if (kMins) per_buffer = std::min(per_buffer, kSumBytes / (4 * 8 * NB * kStageK / 32));
+    p.kc = std::min(per_buffer, stages) * kStageK;
     const uintptr_t at = reinterpret_cast<uintptr_t>(a.scales) | reinterpret_cast<uintptr_t>(a.mins);
     p.whole = a.k % kStageK ? 0 : at % 16 ? 1 : 2;
     return launch_pdl(k_linear_q4<T, NB, kMins>, unsigned(grid), kThreads, size_t(kSmem), stream, 1, p);

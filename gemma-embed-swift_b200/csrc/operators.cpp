@@ -17,14 +17,14 @@ namespace {
 int fail(int code, const std::string& msg) { return ge::set_thread_error(code, msg); }
 int invalid(const std::string& msg) { return fail(GE_ERR_INVALID_OPTIONS, "invalid options: " + msg); }
 
-// Puts the calling thread's current device back on every return path.
+// Puts the calling thread's current device back on every return path, where it was changed.
 struct DeviceGuard {
-    int saved = -1;
+    int saved = -1, used = -1;
     DeviceGuard() {
         if (cudaGetDevice(&saved) != cudaSuccess) saved = -1;
     }
     ~DeviceGuard() {
-        if (saved >= 0) cudaSetDevice(saved);
+        if (saved >= 0 && used >= 0 && used != saved) cudaSetDevice(saved);
     }
 };
 
@@ -33,14 +33,15 @@ std::mutex g_mu;
 int g_sms[kMaxDevices] = {};  // per device: its SM count, once it is known to be an sm_100 device
 
 // Makes `device` current and returns its SM count; 0 with the status in *rc when it cannot be used.
-int use_device(int device, int* rc) {
+int use_device(DeviceGuard& keep, int device, int* rc) {
     const auto failed = [&](cudaError_t e) {
         *rc = fail(GE_ERR_NO_DEVICE, std::string("cannot use CUDA device: ") + cudaGetErrorString(e));
         return 0;
     };
     if (device < 0 || device >= kMaxDevices) return failed(cudaErrorInvalidDevice);
-    cudaError_t e = cudaSetDevice(device);
+    cudaError_t e = device == keep.saved ? cudaSuccess : cudaSetDevice(device);
     if (e != cudaSuccess) return failed(e);
+    keep.used = device;
     std::lock_guard<std::mutex> g(g_mu);
     if (g_sms[device]) return g_sms[device];
     int major = 0, sms = 0;
@@ -119,7 +120,7 @@ int run_attention(int device, const ge_attention_shape* s, ge::CausalLaunch& a, 
     if (!a.q_seqs || !a.kv_seqs || (reinterpret_cast<uintptr_t>(a.q_seqs) & 3) || (reinterpret_cast<uintptr_t>(a.kv_seqs) & 3))
         return invalid("sequence ranges are NULL or not 4-byte aligned");
     DeviceGuard keep;
-    a.num_sms = use_device(device, &rc);
+    a.num_sms = use_device(keep, device, &rc);
     if (!a.num_sms) return rc;
     const size_t need = ge::causal_workspace(a);
     if (!a.workspace || workspace_bytes < 0 || size_t(workspace_bytes) < need ||
@@ -142,8 +143,9 @@ int ge_attention_workspace(int32_t device_ordinal, const ge_attention_shape* sha
     ge::CausalLaunch a;
     fill_shape(a, shape);
     a.ntok = ntok;
+    a.nkv = kMaxRows;  // however many keys the call has
     a.prefix = prefix_len;
-    a.num_sms = use_device(device_ordinal, &rc);
+    a.num_sms = use_device(keep, device_ordinal, &rc);
     if (!a.num_sms) return rc;
     *bytes = int64_t(ge::causal_workspace(a));
     return GE_OK;
@@ -224,7 +226,7 @@ int ge_linear_q4(int32_t device_ordinal, int32_t dtype, const void* d_x, int64_t
     DeviceGuard keep;
     int rc = GE_OK;
     ge::Q4Launch a;
-    a.num_sms = use_device(device_ordinal, &rc);
+    a.num_sms = use_device(keep, device_ordinal, &rc);
     if (!a.num_sms) return rc;
     a.bf16 = dtype == GE_BF16;
     a.x = d_x;

@@ -5,9 +5,22 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "kernels.hpp"
 
 namespace ge {
+
+// Raises `kern`'s dynamic shared-memory limit, once per device and kernel (legal during a capture).
+template <typename K>
+cudaError_t allow_smem(K* kern, int bytes, std::atomic<uint64_t>& devices) {
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess || (dev < 64 && (devices.load(std::memory_order_acquire) >> dev) & 1)) return e;
+    e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == cudaSuccess && dev < 64) devices.fetch_or(uint64_t(1) << dev, std::memory_order_release);
+    return e;
+}
 
 // Launches with programmatic stream serialisation whatever the calling thread's policy: every kernel
 // of the operators waits for its predecessor (pdl_wait) before it touches memory.

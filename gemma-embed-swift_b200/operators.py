@@ -46,7 +46,9 @@ def _call(rc: int):
 @functools.cache
 def _torch():
     import torch
-    return torch, {torch.float16: 0, torch.bfloat16: 1}
+    # The current stream's handle without building a torch.cuda.Stream (a microsecond of every call).
+    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda d: torch.cuda.current_stream(d).cuda_stream)
+    return torch, {torch.float16: 0, torch.bfloat16: 1}, raw
 
 
 def _dtype(t) -> int:
@@ -92,9 +94,9 @@ def _ranges(name: str, t, device: int) -> int:
 
 def _stream(stream, device: int):
     """The stream's handle, and a context in which torch allocates on it (None: already so)."""
-    torch = _torch()[0]
+    torch, _, raw = _torch()
     if stream is None:
-        return torch.cuda.current_stream(device).cuda_stream, None
+        return raw(device), None
     if hasattr(stream, "cuda_stream"):
         if stream.device.index != device:
             raise _invalid(f"the stream is on {stream.device}, not on cuda:{device}")
@@ -144,7 +146,7 @@ def _attention(q, k, v, prefix_k, prefix_v, q_seqs, kv_seqs, scale, window, out,
     nbytes = _workspace_bytes(device, code, heads, kv_heads, dim, scale, window, ntok, prefix)
     with on or _HERE:
         if out is None:
-            out = torch.empty((ntok, heads, dim), dtype=dtype, device=q.device)
+            out = q.new_empty((ntok, heads, dim))
             out_stride = heads * dim
         else:
             rows, _, out_stride = _heads("out", out, device, dtype, heads, dim)
@@ -270,7 +272,7 @@ def linear_q4(x, weight: Q4Weight, out=None, stream=None):
     out_stride = n
     if out is None:
         with on or _HERE:
-            out = torch.empty((rows, n), dtype=x.dtype, device=x.device)
+            out = x.new_empty((rows, n))
     else:
         _on_device("out", out, device)
         if out.dtype != x.dtype or out.shape != (rows, n) or (n > 1 and out.stride(1) != 1):
