@@ -159,7 +159,7 @@ struct Seq {
 };
 
 // Sequence ranges in shared memory (those past kPlanSeqs are read from global memory).
-constexpr int kPlanSeqs = 4096, kMaxItemRows = 256;
+constexpr int kPlanSeqs = 4096, kMaxItemRows = 256, kPlanItems = 64;  // items planned by one CTA
 constexpr size_t plan_smem(int nseq) {
     return size_t(nseq < kPlanSeqs ? nseq : kPlanSeqs) * sizeof(uint4) + 32 * 2 * kMaxItemRows * sizeof(int2);
 }
@@ -176,8 +176,9 @@ __device__ __forceinline__ int2 rows_within(const uint4& w, int r0, int r1) {
     return make_int2(int(min(max(q0, int64_t(r0)), int64_t(r1)) - r0), int(max(min(q1, int64_t(r1)), int64_t(r0)) - r0));
 }
 
-// One item, by one warp: rng and seg are the warp's own shared memory.
-__device__ void plan_item(const PlanParams& p, const uint4* seqs, int2* rng, int2* seg, int t, int lane) {
+// One item, by one warp: rng and seg are the warp's own shared memory.  Its segments and (mixed) rows go to the
+// workspace.
+__device__ TileInfo plan_item(const PlanParams& p, const uint4* seqs, int2* rng, int2* seg, int t, int lane) {
     const int r0 = t * p.TI, n = min(p.TI, p.ntok - r0);
     TileInfo f{};
     bool any = false;
@@ -201,17 +202,11 @@ __device__ void plan_item(const PlanParams& p, const uint4* seqs, int2* rng, int
             f.nblk = p.prefix_blocks + (e.y - a.x + kKeys - 1) / kKeys;
             f.simple = 1, f.see = see, f.ks = q.ks, f.ke = q.ke;
             f.pieces = 1;
-            if (lane == 0) {
-                p.segs[int64_t(t) * p.TI] = make_int2(a.x, e.y);
-                p.info[t] = f;
-            }
-            return;
+            if (lane == 0) p.segs[int64_t(t) * p.TI] = make_int2(a.x, e.y);
+            return f;
         }
     }
-    if (!__any_sync(0xffffffffu, any)) {
-        if (lane == 0) p.info[t] = f;  // live 0: no row of a sequence, no work
-        return;
-    }
+    if (!__any_sync(0xffffffffu, any)) return f;  // live 0: no row of a sequence, no work
 #pragma unroll 1
     for (int i = lane; i < p.TI; i += 32) rng[i] = make_int2(0, -1);
     __syncwarp();
@@ -303,38 +298,91 @@ __device__ void plan_item(const PlanParams& p, const uint4* seqs, int2* rng, int
     for (int i = lane; i < n; i += 32) p.rng[r0 + i] = rng[i];
     f.nblk = __reduce_add_sync(0xffffffffu, nblk) + p.prefix_blocks;
     f.pieces = 1;
-    if (lane == 0) p.info[t] = f;
     __syncwarp();
+    return f;
 }
 
 // One cluster: the items by the warps of all its CTAs, then their pieces and order by the first CTA.
 __global__ void __launch_bounds__(1024) k_causal_plan(PlanParams p) {
     extern __shared__ __align__(16) uint8_t plan_shared[];
-    __shared__ int hist[kBuckets], warp_sum_s[32], s_nblk[kMaxSms], s_chunk;
+    __shared__ int hist[kBuckets], warp_sum_s[32], s_nblk[kMaxSms], s_at[kMaxSms], s_chunk;
+    __shared__ TileInfo s_info[kPlanItems];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int ctas = int(gridDim.x);
     uint4* seqs = reinterpret_cast<uint4*>(plan_shared);
     int2* rng = reinterpret_cast<int2*>(seqs + min(p.nseq, kPlanSeqs)) + warp * 2 * kMaxItemRows;
     hist[tid] = 0;
+    if (tid == 0) s_chunk = INT_MAX;
     pdl_wait();
     pdl_launch();
 #pragma unroll 1
     for (int s = tid; s < min(p.nseq, kPlanSeqs); s += 1024) seqs[s] = seq_words(p, s);
     if (blockIdx.x == 0 && tid == 0) p.head->err = 0;
     __syncthreads();
+    // A single CTA keeps the items' infos at hand; a cluster's come back through global memory.
+    const TileInfo* info = ctas == 1 ? s_info : p.info;
 #pragma unroll 1
-    for (int t = int(blockIdx.x) + warp * ctas; t < p.tiles; t += ctas * 32) plan_item(p, seqs, rng, rng + kMaxItemRows, t, lane);
+    for (int t = int(blockIdx.x) + warp * ctas; t < p.tiles; t += ctas * 32) {
+        const TileInfo f = plan_item(p, seqs, rng, rng + kMaxItemRows, t, lane);
+        if (lane == 0) {
+            p.info[t] = f;
+            if (ctas == 1) s_info[t] = f;
+        }
+    }
     if (ctas > 1) cluster_sync();
     else __syncthreads();
     if (blockIdx.x != 0) return;
-    int chunk = INT_MAX;
-    if (p.lmax > 1) {
-        // Blocks per piece: the fewest for which the pieces of all items and KV heads still fit one round
-        // of the SMs (a second, short round would cost as much as the first).  There are fewer items
-        // than SMs; every warp tries a size.
-        if (tid < p.tiles) s_nblk[tid] = p.info[tid].nblk;
-        if (tid == 0) s_chunk = INT_MAX;
+    const auto whole = [&](int t, const TileInfo& f) {
+        const int2 g = f.nseg > 0 ? p.segs[int64_t(t) * p.TI] : make_int2(0, 0);
+        return Work{t, 0, f.nblk, -1, 0, f.nseg, g.x, g.y, f.lo0, f.hi0, f.lo1, f.hi1, f.live | (f.simple << 2), f.see, f.ks, f.ke};
+    };
+    if (int64_t(p.tiles) * p.kv_heads > p.sms) {
+        // Several rounds of the SMs: whole items, costliest first, by a counting sort over their blocks; the order
+        // within a bucket does not matter.  The lanes of a bucket add as one.
+        const auto add = [&](int bucket, bool one) {  // counts into the bucket; gives the count before
+            const unsigned peers = __match_any_sync(0xffffffffu, bucket), ones = __ballot_sync(0xffffffffu, one) & peers;
+            const int leader = __ffs(peers) - 1, at = lane == leader ? atomicAdd(&hist[bucket], __popc(ones)) : 0;
+            return __shfl_sync(0xffffffffu, at, leader) + __popc(ones & ((1u << lane) - 1));
+        };
+#pragma unroll 1
+        for (int t0 = warp * 32; t0 < p.tiles; t0 += 1024) {
+            const int t = t0 + lane;
+            const int4 f = t < p.tiles ? *reinterpret_cast<const int4*>(info + t) : make_int4(0, 0, 0, 0);  // nblk, nseg, pieces, live
+            add(min(f.x, kBuckets - 1), f.w != 0);
+        }
         __syncthreads();
+        // Exclusive sums from the costliest bucket down: thread i holds bucket kBuckets - 1 - i.
+        const int v = hist[kBuckets - 1 - tid];
+        int inc = v;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int u = __shfl_up_sync(0xffffffffu, inc, o);
+            if (lane >= o) inc += u;
+        }
+        if (lane == 31) warp_sum_s[warp] = inc;
+        __syncthreads();
+        const int u = lane < warp ? warp_sum_s[lane] : 0;
+        const int before = __reduce_add_sync(0xffffffffu, u);
+        hist[kBuckets - 1 - tid] = before + inc - v;
+        if (tid == 1023) p.head->nwork = before + inc;
+        __syncthreads();
+#pragma unroll 1
+        for (int t0 = warp * 32; t0 < p.tiles; t0 += 1024) {
+            const int t = t0 + lane;
+            TileInfo f{};
+            if (t < p.tiles) f = info[t];
+            const int at = add(min(f.nblk, kBuckets - 1), f.live != 0);
+            if (f.live) p.work[at] = whole(t, f);
+        }
+        return;
+    }
+    // One round of the SMs (fewer items than SMs): items in order, cut into pieces where that is allowed.
+    int chunk = INT_MAX;
+    if (tid < p.tiles) s_nblk[tid] = info[tid].nblk;
+    __syncthreads();
+    if (p.lmax > 1) {
+        // Blocks per piece: the fewest for which the pieces of all items and KV heads still fit one round (a
+        // second, short round would cost as much as the first).  Every warp tries a size.
         int most = 1;
 #pragma unroll 1
         for (int t = lane; t < p.tiles; t += 32) most = max(most, s_nblk[t]);
@@ -352,87 +400,40 @@ __global__ void __launch_bounds__(1024) k_causal_plan(PlanParams p) {
             __syncthreads();
         }
     }
-    // Costliest pieces first: a counting sort by blocks, the lanes of a bucket adding as one; the order
-    // within a bucket does not matter.
     const auto pieces_of = [&](int nblk, int& sz) {
         const int want = chunk == INT_MAX ? 1 : max(1, (nblk + chunk - 1) / chunk);
         sz = (nblk + want - 1) / want;
         return sz ? (nblk + sz - 1) / sz : 1;  // the last piece may come out empty, and is dropped
     };
-    const auto add = [&](int bucket, int v) {  // adds v to the bucket; gives the sum before
-        const unsigned peers = __match_any_sync(0xffffffffu, bucket);
-        const int leader = __ffs(peers) - 1;
-        int sum = 0, before = 0;
-        if (p.lmax == 1) {  // v is 0 or 1
-            const unsigned ones = __ballot_sync(0xffffffffu, v) & peers;
-            sum = __popc(ones);
-            before = __popc(ones & ((1u << lane) - 1));
-        } else {
+    if (warp == 0) {  // where each item's pieces start in the list
+        int base = 0;
 #pragma unroll 1
-            for (int l = 0; l < 32; l++) {
-                const int x = __shfl_sync(0xffffffffu, v, l);
-                if ((peers >> l) & 1) {
-                    if (l < lane) before += x;
-                    sum += x;
-                }
-            }
-        }
-        const int at = lane == leader ? atomicAdd(&hist[bucket], sum) : 0;
-        return __shfl_sync(0xffffffffu, at, leader) + before;
-    };
-#pragma unroll 1
-    for (int t0 = warp * 32; t0 < p.tiles; t0 += 1024) {
-        const int t = t0 + lane;
-        const int4 f = t < p.tiles ? *reinterpret_cast<const int4*>(p.info + t) : make_int4(0, 0, 0, 0);  // nblk, nseg, pieces, live
-        int sz;
-        const int n = pieces_of(f.x, sz);
-        add(min(sz, kBuckets - 1), f.w ? n : 0);
-    }
-    __syncthreads();
-    // Exclusive sums from the costliest bucket down: thread i holds bucket kBuckets - 1 - i.
-    {
-        const int v = hist[kBuckets - 1 - tid];
-        int inc = v;
+        for (int t0 = 0; t0 < p.tiles; t0 += 32) {
+            const int t = t0 + lane;
+            int sz, n = t < p.tiles && info[t].live ? pieces_of(s_nblk[t], sz) : 0, inc = n;
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int u = __shfl_up_sync(0xffffffffu, inc, o);
-            if (lane >= o) inc += u;
+            for (int o = 1; o < 32; o <<= 1) {
+                const int w = __shfl_up_sync(0xffffffffu, inc, o);
+                if (lane >= o) inc += w;
+            }
+            if (t < p.tiles) s_at[t] = base + inc - n;
+            base += __shfl_sync(0xffffffffu, inc, 31);
         }
-        if (lane == 31) warp_sum_s[warp] = inc;
-        __syncthreads();
-        const int u = lane < warp ? warp_sum_s[lane] : 0;
-        const int before = __reduce_add_sync(0xffffffffu, u);
-        hist[kBuckets - 1 - tid] = before + inc - v;
-        if (tid == 1023) p.head->nwork = before + inc;
+        if (lane == 0) p.head->nwork = base;
     }
     __syncthreads();
 #pragma unroll 1
-    for (int t0 = warp * 32; t0 < p.tiles; t0 += 1024) {
-        const int t = t0 + lane;
-        TileInfo f{};
-        if (t < p.tiles) f = p.info[t];
+    for (int t = warp; t < p.tiles; t += 32) {  // a lane per piece
+        const TileInfo f = info[t];
+        if (!f.live) continue;
+        const int at = s_at[t];
         int sz;
         const int n = pieces_of(f.nblk, sz);
-        const int at = add(min(sz, kBuckets - 1), f.live ? n : 0);
-        if (!f.live) continue;
-        if (n > 1) {
-            p.info[t].pieces = n;
-            s_nblk[t] = at;  // written below, by a warp
+        if (n == 1) {
+            if (lane == 0) p.work[at] = whole(t, f);
             continue;
         }
-        if (p.lmax > 1) s_nblk[t] = -1;
-        const int2 g = f.nseg > 0 ? p.segs[int64_t(t) * p.TI] : make_int2(0, 0);
-        p.work[at] = Work{t, 0, f.nblk, -1, 0, f.nseg, g.x, g.y, f.lo0, f.hi0, f.lo1, f.hi1, f.live | (f.simple << 2), f.see, f.ks, f.ke};
-    }
-    if (p.lmax == 1) return;
-    __syncthreads();
-#pragma unroll 1
-    for (int t = warp; t < p.tiles; t += 32) {  // cut items: a lane per piece
-        const int at = s_nblk[t];
-        const TileInfo f = p.info[t];
-        if (!f.live || at < 0) continue;
-        int sz;
-        const int n = pieces_of(f.nblk, sz);
+        if (lane == 0) p.info[t].pieces = n;
         const int2* seg = p.segs + int64_t(t) * p.TI;
 #pragma unroll 1
         for (int i = lane; i < n; i += 32) {
@@ -1285,7 +1286,7 @@ cudaError_t launch_causal(const CausalLaunch& a, cudaStream_t stream) {
     PlanParams pp{a.q_seqs, a.kv_seqs, a.nseq, a.ntok, a.nkv, window, s.T, s.TI, s.tiles, a.kv_heads,
                   (a.prefix + kKeys - 1) / kKeys, s.lmax, a.num_sms, l.head, l.rng, l.segs, l.info, l.work};
     // A warp plans an item; up to 8 CTAs share them.
-    const int ctas = s.tiles <= 32 ? 1 : s.tiles <= 64 ? 2 : s.tiles <= 128 ? 4 : 8;
+    const int ctas = s.tiles <= kPlanItems ? 1 : s.tiles <= 128 ? 4 : 8;
     static std::atomic<uint64_t> devices{0};
     cudaError_t e = allow_smem(k_causal_plan, int(plan_smem(kPlanSeqs)), devices);
     if (e == cudaSuccess) e = launch_pdl(k_causal_plan, unsigned(ctas), 1024, plan_smem(a.nseq), stream, ctas, pp);
