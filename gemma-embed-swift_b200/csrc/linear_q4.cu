@@ -35,7 +35,7 @@ constexpr int kDepth = 3;
 constexpr int kXElems = 16384;                 // elements of x per buffer, all rows
 constexpr int kOffX = kWarps * kDepth * kStageBytes;
 constexpr int kXBytes = kXElems * 2 + kQ4MaxRows * 64;  // rows are 64 bytes over a multiple of 128 apart
-constexpr int kOffSum = kOffX + 2 * kXBytes;            // sums of x per 32 elements and row, 8 NB rows apart
+constexpr int kOffSum = kOffX + 2 * kXBytes;            // sums of x per group and row, 8 NB rows apart
 constexpr int kSumBytes = 4096;
 constexpr int kSmem = kOffSum + 2 * kSumBytes;
 static_assert(kSmem <= 227 * 1024, "shared memory");
@@ -124,8 +124,8 @@ __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], 
     }
 }
 
-// NB: tiles of 8 rows of x.
-template <typename T, int NB, bool kMins>
+// NB: tiles of 8 rows of x; kPer: 32-weight units of a group, summed by the products before they are scaled.
+template <typename T, int NB, bool kMins, int kPer>
 __global__ void __launch_bounds__(kThreads, 1) k_linear_q4(const __grid_constant__ Q4Params p) {
     extern __shared__ __align__(128) uint8_t smem[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -140,7 +140,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_linear_q4(const __grid_constant
         from = lo + n * part / parts;
         to = lo + n * (part + 1) / parts;
     };
-    const int groups = p.k / p.group, gshift = p.group == 32 ? 5 : p.group == 64 ? 6 : 7;
+    constexpr int gshift = kPer == 1 ? 5 : kPer == 2 ? 6 : 7;
+    const int groups = p.k >> gshift;
     const int x_row = p.kc * 2 + 64;  // bytes between x's rows in a buffer
     uint8_t* ring = smem + warp * kDepth * kStageBytes;
     const uint32_t ring_addr = smem_u32(ring);
@@ -151,20 +152,18 @@ __global__ void __launch_bounds__(kThreads, 1) k_linear_q4(const __grid_constant
     constexpr int kUnits = kXElems / 8 / kThreads;
     const int units_row = p.kc / 8;
     uint4 xr[kUnits];
-    int ur[kUnits], ue[kUnits];  // each unit's row and element
+    int unit[kUnits];  // each unit's row (high half) and first element (low half)
 #pragma unroll
     for (int u = 0; u < kUnits; u++) {
-        const int id = u * kThreads + threadIdx.x;
-        ur[u] = id / units_row;
-        ue[u] = (id - ur[u] * units_row) * 8;
+        const int id = u * kThreads + threadIdx.x, r = id / units_row;
+        unit[u] = r << 16 | (id - r * units_row) * 8;
     }
     auto load_x = [&](int i) {
 #pragma unroll
         for (int u = 0; u < kUnits; u++) {
-            const int kk = i * p.kc + ue[u];
+            const int r = unit[u] >> 16, kk = i * p.kc + (unit[u] & 0xffff);
             xr[u] = make_uint4(0u, 0u, 0u, 0u);
-            if (ur[u] < p.rows && kk < p.k)
-                xr[u] = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.x) + ur[u] * p.x_stride + kk);
+            if (r < p.rows && kk < p.k) xr[u] = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.x) + r * p.x_stride + kk);
         }
     };
     auto store_x = [&](int i) {
@@ -172,7 +171,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_linear_q4(const __grid_constant
         float* sums = reinterpret_cast<float*>(smem + kOffSum + (i & 1) * kSumBytes);
 #pragma unroll
         for (int u = 0; u < kUnits; u++) {
-            const int r = ur[u], e = ue[u];
+            const int r = unit[u] >> 16, e = unit[u] & 0xffff;
             const uint4 v = xr[u];
             if (kMins) {
                 float s = 0.f;
@@ -182,9 +181,9 @@ __global__ void __launch_bounds__(kThreads, 1) k_linear_q4(const __grid_constant
                     const float2 f = pair_to_float<T>(w[j]);
                     s += f.x + f.y;
                 }
-                s += __shfl_xor_sync(0xffffffffu, s, 1);
-                s += __shfl_xor_sync(0xffffffffu, s, 2);
-                if (r < p.rows && (threadIdx.x & 3) == 0) sums[(e / 32) * 8 * NB + r] = s;
+#pragma unroll
+                for (int o = 1; o < 4 * kPer; o <<= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+                if (r < p.rows && (threadIdx.x & (4 * kPer - 1)) == 0) sums[(e >> gshift) * 8 * NB + r] = s;
             }
             if (r < p.rows) {
                 uint4 o;  // pairs (0, 4), (1, 5), (2, 6), (3, 7)
@@ -235,9 +234,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_linear_q4(const __grid_constant
                 if (kMins || lane < 16) {
                     const __half* from = ssrc + ((cs * kStageK) >> gshift);
                     if (p.whole == 2) {  // and the scales' rows are aligned: a row of the stage's at once
-                        if (gshift == 5) cp_small<16>(sdst + uint32_t(at), from);
-                        else if (gshift == 6) cp_small<8>(sdst + uint32_t(at), from);
-                        else cp_small<4>(sdst + uint32_t(at), from);
+                        cp_small<16 / kPer>(sdst + uint32_t(at), from);
                     } else {
                         __half* out = reinterpret_cast<__half*>(ring + at + kWeightBytes + lane * kScaleRow);
                         for (int i = 0; i < (kStageK >> gshift); i++)
@@ -275,18 +272,10 @@ __global__ void __launch_bounds__(kThreads, 1) k_linear_q4(const __grid_constant
                 const int w = warp * kDepth * kStageBytes + slot + g * 128 + (g << 4) + c * 4;
                 const uint8_t* scr = ring + slot + kWeightBytes + g * kScaleRow;
                 slot = slot == (kDepth - 1) * kStageBytes ? 0 : slot + kStageBytes;
-                // A row's scales of the stage's eight 32-weight groups, two to a word.
+                // A row's scales of the stage's 8 / kPer groups, two to a word.
                 const auto scales = [&](int off, uint32_t (&v)[4]) {
                     const uint4 u = *reinterpret_cast<const uint4*>(scr + off);
-                    if (gshift == 5) {
-                        v[0] = u.x, v[1] = u.y, v[2] = u.z, v[3] = u.w;
-                    } else if (gshift == 6) {
-                        v[0] = __byte_perm(u.x, 0, 0x1010), v[1] = __byte_perm(u.x, 0, 0x3232);
-                        v[2] = __byte_perm(u.y, 0, 0x1010), v[3] = __byte_perm(u.y, 0, 0x3232);
-                    } else {
-                        v[0] = v[1] = __byte_perm(u.x, 0, 0x1010);
-                        v[2] = v[3] = __byte_perm(u.x, 0, 0x3232);
-                    }
+                    v[0] = u.x, v[1] = u.y, v[2] = u.z, v[3] = u.w;
                 };
                 const auto pick = [](const uint32_t (&v)[4], int j) {
                     const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&v[j >> 1]));
@@ -301,33 +290,41 @@ __global__ void __launch_bounds__(kThreads, 1) k_linear_q4(const __grid_constant
                 }
                 const uint8_t* const xq = xb + q * kStageK * 2;
 #pragma unroll
-                for (int j = 0; j < kStageK / 32; j++) {
-                    const uint32_t ua = *reinterpret_cast<const uint32_t*>(smem + (w ^ (j << 4)));
-                    const uint32_t ub = *reinterpret_cast<const uint32_t*>(smem + (w ^ (j << 4)) + 1024);
-                    uint32_t ta[4], tb[4];
-                    if constexpr (std::is_same<T, __half>::value) {
-                        widen_f16<!kMins>(ua, ta);
-                        widen_f16<!kMins>(ub, tb);
-                    } else {
-                        widen_bf16<!kMins>(ua, ta);
-                        widen_bf16<!kMins>(ub, tb);
+                for (int j = 0; j < kStageK / 32 / kPer; j++) {
+                    float d[NB][4];
+#pragma unroll
+                    for (int u = 0; u < kPer; u++) {
+                        const int at = (j * kPer + u) << 4;
+                        const uint32_t ua = *reinterpret_cast<const uint32_t*>(smem + (w ^ at));
+                        const uint32_t ub = *reinterpret_cast<const uint32_t*>(smem + (w ^ at) + 1024);
+                        uint32_t ta[4], tb[4];
+                        if constexpr (std::is_same<T, __half>::value) {
+                            widen_f16<!kMins>(ua, ta);
+                            widen_f16<!kMins>(ub, tb);
+                        } else {
+                            widen_bf16<!kMins>(ua, ta);
+                            widen_bf16<!kMins>(ub, tb);
+                        }
+                        const uint32_t a0[4] = {ta[0], tb[0], ta[1], tb[1]}, a1[4] = {ta[2], tb[2], ta[3], tb[3]};
+#pragma unroll
+                        for (int b = 0; b < NB; b++) {
+                            const uint4 xv = *reinterpret_cast<const uint4*>(xq + xrow[b] + (j * kPer + u) * 64);
+                            if (u == 0) mma16816<T, true>(d[b], a0, xv.x, xv.y);
+                            else mma16816<T, false>(d[b], a0, xv.x, xv.y);
+                            mma16816<T, false>(d[b], a1, xv.z, xv.w);
+                        }
                     }
                     const float sa = pick(sav, j), sb = pick(sbv, j);
                     const float ma = kMins ? pick(mav, j) : 0.f, mb = kMins ? pick(mbv, j) : 0.f;
-                    const uint32_t a0[4] = {ta[0], tb[0], ta[1], tb[1]}, a1[4] = {ta[2], tb[2], ta[3], tb[3]};
 #pragma unroll
                     for (int b = 0; b < NB; b++) {
-                        const uint4 xv = *reinterpret_cast<const uint4*>(xq + xrow[b] + j * 64);
-                        float d[4];
-                        mma16816<T, true>(d, a0, xv.x, xv.y);
-                        mma16816<T, false>(d, a1, xv.z, xv.w);
-                        acc[b][0] = fmaf(sa, d[0], acc[b][0]);
-                        acc[b][1] = fmaf(sa, d[1], acc[b][1]);
-                        acc[b][2] = fmaf(sb, d[2], acc[b][2]);
-                        acc[b][3] = fmaf(sb, d[3], acc[b][3]);
+                        acc[b][0] = fmaf(sa, d[b][0], acc[b][0]);
+                        acc[b][1] = fmaf(sa, d[b][1], acc[b][1]);
+                        acc[b][2] = fmaf(sb, d[b][2], acc[b][2]);
+                        acc[b][3] = fmaf(sb, d[b][3], acc[b][3]);
                         if (kMins) {
                             // Sums of rows 8 b + 2 c and the next (what lies there past the last row is not stored).
-                            const float2 xs = *reinterpret_cast<const float2*>(sums + (q * (kStageK / 32) + j) * 8 * NB + b * 8);
+                            const float2 xs = *reinterpret_cast<const float2*>(sums + (q * (kStageK / 32 / kPer) + j) * 8 * NB + b * 8);
                             acc[b][0] = fmaf(ma, xs.x, acc[b][0]);
                             acc[b][1] = fmaf(ma, xs.y, acc[b][1]);
                             acc[b][2] = fmaf(mb, xs.x, acc[b][2]);
@@ -370,10 +367,10 @@ __global__ void __launch_bounds__(kThreads, 1) k_linear_q4(const __grid_constant
     }
 }
 
-template <typename T, int NB, bool kMins>
+template <typename T, int NB, bool kMins, int kPer>
 cudaError_t launch_t(const Q4Launch& a, cudaStream_t stream) {
     static std::atomic<uint64_t> devices{0};
-    cudaError_t e = allow_smem(k_linear_q4<T, NB, kMins>, kSmem, devices);
+    cudaError_t e = allow_smem(k_linear_q4<T, NB, kMins, kPer>, kSmem, devices);
     if (e != cudaSuccess) return e;
     Q4Params p{a.x, a.x_stride, a.rows, a.n, a.k, a.group, a.values, a.scales, a.mins, a.out, a.out_stride, 0, 0, 0, 0};
     p.tiles = (a.n + 15) / 16;
@@ -381,16 +378,23 @@ cudaError_t launch_t(const Q4Launch& a, cudaStream_t stream) {
     p.R = std::min(kWarps, (p.tiles + grid - 1) / grid);
     const int stages = (a.k + kStageK - 1) / kStageK;
     int per_buffer = kXElems / a.rows / kStageK;  // stages of all rows in an x buffer
-    if (kMins) per_buffer = std::min(per_buffer, kSumBytes / (4 * 8 * NB * kStageK / 32));
+    if (kMins) per_buffer = std::min(per_buffer, kSumBytes / (4 * 8 * NB * (kStageK / 32 / kPer)));
     p.kc = std::min(per_buffer, stages) * kStageK;
     const uintptr_t at = reinterpret_cast<uintptr_t>(a.scales) | reinterpret_cast<uintptr_t>(a.mins);
     p.whole = a.k % kStageK ? 0 : at % 16 ? 1 : 2;
-    return launch_pdl(k_linear_q4<T, NB, kMins>, unsigned(grid), kThreads, size_t(kSmem), stream, 1, p);
+    return launch_pdl(k_linear_q4<T, NB, kMins, kPer>, unsigned(grid), kThreads, size_t(kSmem), stream, 1, p);
+}
+
+template <typename T, int NB, bool kMins>
+cudaError_t launch_g(const Q4Launch& a, cudaStream_t stream) {
+    if (a.group == 32) return launch_t<T, NB, kMins, 1>(a, stream);
+    if (a.group == 64) return launch_t<T, NB, kMins, 2>(a, stream);
+    return launch_t<T, NB, kMins, 4>(a, stream);
 }
 
 template <typename T, int NB>
 cudaError_t launch_m(const Q4Launch& a, cudaStream_t stream) {
-    return a.mins ? launch_t<T, NB, true>(a, stream) : launch_t<T, NB, false>(a, stream);
+    return a.mins ? launch_g<T, NB, true>(a, stream) : launch_g<T, NB, false>(a, stream);
 }
 
 template <typename T>
