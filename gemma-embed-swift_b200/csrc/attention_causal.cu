@@ -50,6 +50,12 @@ namespace {
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kGrow = 8.0f;  // log2 units a row's maximum may grow before it is moved
 constexpr int kKeys = 128;     // keys of a block
+// Probabilities are held times 2^kRaise: fp16's smallest numbers then stand for probabilities of 2^-31, not 2^-24,
+// so that many small ones beside a large one keep their sum (P stays within 2^(kGrow + 7), below fp16's largest).
+template <typename E>
+constexpr float kRaise = 0.f;
+template <>
+constexpr float kRaise<__half> = 7.f;
 constexpr int kMaxPieces = 128;
 constexpr int kBuckets = 1024;
 constexpr int kMaxSms = 256;  // room for a cut call's items (fewer than SMs)
@@ -176,6 +182,70 @@ __device__ __forceinline__ int2 rows_within(const uint4& w, int r0, int r1) {
     return make_int2(int(min(max(q0, int64_t(r0)), int64_t(r1)) - r0), int(max(min(q1, int64_t(r1)), int64_t(r0)) - r0));
 }
 
+// The disjoint ascending segments of n ranges whose lo never falls (empty ones aside), into seg, which may be
+// the ranges' own memory; false where a lo falls.
+__device__ bool find_segments(const PlanParams& p, const int2* ranges, int2* seg, int n, int lane, int& nseg) {
+    int end = -1, low = -1;  // running maximum of hi and lo over the ranges so far
+    nseg = 0;
+#pragma unroll 1
+    for (int i0 = 0; i0 < n; i0 += 32) {
+        const int i = i0 + lane;
+        const int2 rg = i < n ? ranges[i] : make_int2(0, -1);
+        const bool some = rg.y > rg.x;
+        // Inclusive running maxima over the lanes, then those of the ranges before each lane's.
+        int e = some ? rg.y : -1, l = some ? rg.x : -1;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int pe = __shfl_up_sync(0xffffffffu, e, o), pl = __shfl_up_sync(0xffffffffu, l, o);
+            if (lane >= o) {
+                e = max(e, pe);
+                l = max(l, pl);
+            }
+        }
+        int be = __shfl_up_sync(0xffffffffu, e, 1), bl = __shfl_up_sync(0xffffffffu, l, 1);
+        be = lane ? max(be, end) : end;
+        bl = lane ? max(bl, low) : low;
+        if (__any_sync(0xffffffffu, some && rg.x < bl)) return false;
+        const bool fresh = some && rg.x > be;  // keys between be and lo are no row's
+        const unsigned fm = __ballot_sync(0xffffffffu, fresh);
+        if (fresh) {
+            const int at = nseg + __popc(fm & ((1u << lane) - 1));
+            seg[at].x = rg.x;
+            if (at > 0) seg[at - 1].y = be;
+        }
+        nseg += __popc(fm);
+        end = max(end, __shfl_sync(0xffffffffu, e, 31));
+        low = max(low, __shfl_sync(0xffffffffu, l, 31));
+        __syncwarp();
+    }
+    if (nseg > 0 && lane == 0) seg[nseg - 1].y = end;
+    __syncwarp();
+    return true;
+}
+
+// The n ranges of rng in ascending order of lo, empty ones last, into the kMaxItemRows places of seg (a bitonic
+// sort by the warp).
+__device__ void sort_ranges(const int2* rng, int2* seg, int n, int lane) {
+#pragma unroll 1
+    for (int i = lane; i < kMaxItemRows; i += 32) {
+        const int2 rg = i < n ? rng[i] : make_int2(0, -1);
+        seg[i] = rg.y > rg.x ? rg : make_int2(INT_MAX, INT_MAX);
+    }
+    __syncwarp();
+#pragma unroll 1
+    for (int size = 2; size <= kMaxItemRows; size *= 2)
+#pragma unroll 1
+        for (int step = size / 2; step > 0; step /= 2) {
+#pragma unroll 1
+            for (int t = lane; t < kMaxItemRows / 2; t += 32) {
+                const int i = 2 * t - (t & (step - 1)), j = i + step;
+                const int2 a = seg[i], b = seg[j];
+                if ((a.x > b.x) == ((i & size) == 0)) seg[i] = b, seg[j] = a;
+            }
+            __syncwarp();
+        }
+}
+
 // One item, by one warp: rng and seg are the warp's own shared memory.  Its segments and (mixed) rows go to the
 // workspace.
 __device__ TileInfo plan_item(const PlanParams& p, const uint4* seqs, int2* rng, int2* seg, int t, int lane) {
@@ -235,59 +305,28 @@ __device__ TileInfo plan_item(const PlanParams& p, const uint4* seqs, int2* rng,
         }
         __syncwarp();
     }
-    // The rows' own keys as disjoint ascending segments, when the rows' ranges come in ascending order (lo
-    // never falls); else one segment over all of them, the masks doing the rest.
+    // Tiles with rows, and the hulls of their keys.
     int lo_x[2] = {INT_MAX, INT_MAX}, hi_x[2] = {0, 0};
-    int end = -1, low = -1;  // running maximum of hi and lo over the rows so far
-    bool sorted = true;
 #pragma unroll 1
     for (int i0 = 0; i0 < p.TI; i0 += 32) {
         const int i = i0 + lane;
         const int2 rg = i < n ? rng[i] : make_int2(0, -1);
-        const bool in = rg.y >= 0, some = rg.y > rg.x;
-        const bool x = i >= p.T;
+        const bool in = rg.y >= 0, x = i >= p.T;
         if (__any_sync(0xffffffffu, in && !x)) f.live |= 1;
         if (__any_sync(0xffffffffu, in && x)) f.live |= 2;
-        // Per lane, reduced once behind the loop.
-        if (some) {
+        if (rg.y > rg.x) {  // per lane, reduced once behind the loop
             lo_x[0] = min(lo_x[0], x ? INT_MAX : rg.x), hi_x[0] = max(hi_x[0], x ? 0 : rg.y);
             lo_x[1] = min(lo_x[1], x ? rg.x : INT_MAX), hi_x[1] = max(hi_x[1], x ? rg.y : 0);
         }
-        // Inclusive running maxima over the lanes, then those of the rows before each lane's.
-        int e = some ? rg.y : -1, l = some ? rg.x : -1;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int pe = __shfl_up_sync(0xffffffffu, e, o), pl = __shfl_up_sync(0xffffffffu, l, o);
-            if (lane >= o) {
-                e = max(e, pe);
-                l = max(l, pl);
-            }
-        }
-        int be = __shfl_up_sync(0xffffffffu, e, 1), bl = __shfl_up_sync(0xffffffffu, l, 1);
-        be = lane ? max(be, end) : end;
-        bl = lane ? max(bl, low) : low;
-        if (__any_sync(0xffffffffu, some && rg.x < bl)) sorted = false;
-        const bool fresh = some && rg.x > be;  // keys between be and lo are no row's
-        const unsigned fm = __ballot_sync(0xffffffffu, fresh);
-        if (fresh) {
-            const int at = f.nseg + __popc(fm & ((1u << lane) - 1));
-            seg[at].x = rg.x;
-            if (at > 0) seg[at - 1].y = be;
-        }
-        f.nseg += __popc(fm);
-        end = max(end, __shfl_sync(0xffffffffu, e, 31));
-        low = max(low, __shfl_sync(0xffffffffu, l, 31));
+    }
+    // The rows' own keys as disjoint ascending segments, by one pass over the ranges in ascending order (lo
+    // never falls): as the rows have them, or, where a row's lo falls, sorted into seg first.
+    if (!find_segments(p, rng, seg, n, lane, f.nseg)) {
+        sort_ranges(rng, seg, n, lane);
+        find_segments(p, seg, seg, kMaxItemRows, lane, f.nseg);
     }
     f.lo0 = warp_min_i(lo_x[0]), f.hi0 = warp_max_i(hi_x[0]);
     f.lo1 = warp_min_i(lo_x[1]), f.hi1 = warp_max_i(hi_x[1]);
-    __syncwarp();
-    if (!sorted) {
-        f.nseg = 1;
-        if (lane == 0) seg[0] = make_int2(min(f.lo0, f.lo1), max(f.hi0, f.hi1));
-    } else if (f.nseg > 0 && lane == 0) {
-        seg[f.nseg - 1].y = end;
-    }
-    __syncwarp();
     int nblk = 0;
 #pragma unroll 1
     for (int i = lane; i < f.nseg; i += 32) {
@@ -479,6 +518,7 @@ struct TcParams {
     int heads, kv_heads, group, T, TI, ntok, window, prefix, prefix_blocks;
     uint32_t kv_magic;  // ceil(2^32 / kv_heads)
     float scale_log2e;
+    uint64_t wait_ns;
     Header* head;
     const int2 *rng, *segs;
     const Work* work;
@@ -498,13 +538,30 @@ __device__ __forceinline__ bool elect_one() {
 
 // A word with its n lowest bits set (0 below 0, all above 32).
 __device__ __forceinline__ uint32_t low_bits(int n) { return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1u; }
-// The waits' slow parts out of line: the kernel's roles hold dozens of waits, and at an item's turn code that
-// has left the instruction cache costs more than the work.
-__device__ __forceinline__ bool wait_slow(uint64_t* bar, uint32_t parity, int* err) { return mbar_wait(bar, parity, err); }
-__device__ __forceinline__ bool wait_asleep(uint64_t* bar, uint32_t parity, int* err) { return mbar_wait_sleep(bar, parity, err, 32); }
+// Waits give up after `limit` nanoseconds, or once another thread has: kWaitLimitNs and what a warp may take to
+// recompute its rows from the definition meanwhile (wait_limit).
+template <bool kSleep>
+__device__ __forceinline__ bool wait_slow(uint64_t* bar, uint32_t parity, int* err, uint64_t limit) {
+    if (mbar_test(bar, parity)) return true;
+    const uint64_t t0 = globaltimer();
+    for (uint32_t spin = 1;; spin++) {
+        if (kSleep) __nanosleep(32);
+        if (mbar_test(bar, parity)) return true;
+        if ((spin & (kSleep ? 15 : 63)) == 0) {
+            if (*reinterpret_cast<volatile int*>(err) != 0) return false;
+            if (globaltimer() - t0 > limit) {
+                atomicCAS(err, 0, kErrTimeout);
+                return false;
+            }
+        }
+    }
+}
+// A warp recomputes 32 rows over all keys at most, at about 0.25 us for a key of a row (8 heads of 128 wide, 8192
+// rows that all see an infinite value: 69 ms, 0.13 ms without it); 1 us is allowed.
+constexpr uint64_t wait_limit(int64_t keys) { return kWaitLimitNs + uint64_t(keys) * 32 * 1000; }
 // The whole warp: every lane tests (the barrier is most often already there), then they agree.
-__device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t parity, int* err) {
-    return __all_sync(0xffffffffu, mbar_poll(bar, parity)) || __all_sync(0xffffffffu, wait_slow(bar, parity, err));
+__device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t parity, int* err, uint64_t limit) {
+    return __all_sync(0xffffffffu, mbar_poll(bar, parity)) || __all_sync(0xffffffffu, wait_slow<false>(bar, parity, err, limit));
 }
 // Two fp32 operations at a time.
 __device__ __forceinline__ uint64_t pack2(float a, float b) {
@@ -742,7 +799,7 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1)
                 prefetch_piece(p, piece_id(round + 1), total);
                 if (s.b0 >= s.b1) continue;
                 if (keys) {
-                    if (!wait_asleep(q_empty, uint32_t(issued_q & 1) ^ 1u, err)) break;
+                    if (!wait_slow<true>(q_empty, uint32_t(issued_q & 1) ^ 1u, err, p.wait_ns)) break;
                     mbar_expect_tx(q_full, uint32_t(NT * C::QC * 128 * live_rows));
 #pragma unroll 1
                     for (int x = 0; x < NT; x++)
@@ -757,7 +814,7 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1)
                     const CUtensorMap* map = c.prefix ? shared : own;
                     for (int h = 0; h < DH; h++) {
                         const int st = issued % ST;
-                        if (!wait_asleep(&empty[st], uint32_t((issued / ST) & 1) ^ 1u, err)) {
+                        if (!wait_slow<true>(&empty[st], uint32_t((issued / ST) & 1) ^ 1u, err, p.wait_ns)) {
                             ok = false;
                             break;
                         }
@@ -789,7 +846,7 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1)
         const uint64_t v_desc = sw128_desc(smem_u32(smem + C::kOffV), C::kChunk, 1024);
         bool ok = true;
         auto wait = [&](uint64_t* bar, uint32_t parity) {
-            ok = wait_warp(bar, parity, err);
+            ok = wait_warp(bar, parity, err, p.wait_ns);
             return ok;
         };
         int nq = 0, nk = 0, nv = 0;            // Q tiles, K stages and V stages used so far
@@ -905,8 +962,8 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1)
                             const int st = (nv + h) % ST;
                             if (!wait(&v_full[st], uint32_t(((nv + h) / ST) & 1))) break;
                             if (prev_nv & 15) {
-    #pragma unroll 1
-                            for (int i = lane; i < (steps * 16 - prev_nv) * C::SC * 8; i += 32) {
+#pragma unroll 1
+                                for (int i = lane; i < (steps * 16 - prev_nv) * C::SC * 8; i += 32) {
                                     const int rr = prev_nv + i / (C::SC * 8), ch = (i >> 3) % C::SC;
                                     *reinterpret_cast<uint4*>(smem + C::kOffV + st * C::kStage + ch * C::kChunk + rr * 128 + (i & 7) * 16) =
                                         make_uint4(0u, 0u, 0u, 0u);
@@ -969,7 +1026,7 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1)
         const int token = r / p.group;
         bool ok = true;
         auto wait = [&](uint64_t* bar, uint32_t parity) {
-            ok = __all_sync(0xffffffffu, mbar_poll(bar, parity)) || __all_sync(0xffffffffu, mbar_wait(bar, parity, err));
+            ok = wait_warp(bar, parity, err, p.wait_ns);
             return ok;
         };
         int nb = 0, no = 0;  // blocks and items with an O so far
@@ -1069,7 +1126,7 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1)
                         }
                         if (grow) m = mb;
                     }
-                    const float mu = m == -INFINITY ? 0.f : -m;
+                    const float mu = m == -INFINITY ? 0.f : kRaise<E> - m;
                     const uint64_t scale2 = pack2(p.scale_log2e, p.scale_log2e), mu2 = pack2(mu, mu);
                     uint64_t ps[4] = {0, 0, 0, 0};
 #pragma unroll
@@ -1101,7 +1158,7 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1)
             const int head = s.kvh * p.group + (r - token * p.group);
             const int64_t at = (int64_t(s.piece) * p.ntok + row) * p.heads + head;  // of a partial row
             const float inv = s.piece >= 0 ? 1.0f : l == 0.f ? 0.f : 1.0f / l;
-            if (in && s.piece >= 0) p.ml[at] = make_float2(m, l);
+            if (in && s.piece >= 0) p.ml[at] = make_float2(m - kRaise<E>, l);
             bool bad = false;
             if (count) {
                 if (!wait(&o_full[x], uint32_t(no & 1))) break;
@@ -1193,7 +1250,7 @@ __global__ void __launch_bounds__(256) k_causal_merge(MergeParams p) {
     const int n = info.z;
     if (n <= 1 || !info.w || (!simple && rng.y < 0)) return;
     if (tid >= n) ml = make_float2(-INFINITY, 0.f);
-    const bool nan = __syncthreads_or(isnan(ml.x));
+    const bool nan = __syncthreads_or(isnan(ml.y));  // of a piece: its row is NaN whatever its weight
     float m = warp_max(ml.x);
     if (lane == 0) red_m[warp] = m;
     __syncthreads();
@@ -1259,6 +1316,7 @@ cudaError_t launch_t(const CausalLaunch& a, const Sizes& s, const Layout& l, cud
         return cudaErrorInvalidValue;
     TcParams p{a.q, a.k, a.v, a.pk, a.pv, a.out, a.q_stride, a.k_stride, a.v_stride, a.pk_stride, a.pv_stride, a.out_stride,
                a.heads, a.kv_heads, s.group, s.T, s.TI, a.ntok, std::min(a.window, 1 << 30), a.prefix, (a.prefix + kKeys - 1) / kKeys, uint32_t(((uint64_t(1) << 32) + a.kv_heads - 1) / a.kv_heads), a.scale * kLog2e,
+               wait_limit(int64_t(a.prefix) + a.nkv),
                l.head, l.rng, l.segs, l.work, l.o, l.ml};
     const int64_t most = s.lmax > 1 ? a.num_sms : int64_t(s.tiles) * a.kv_heads;
     e = launch_pdl(k_causal_tc<E, D>, unsigned(std::min<int64_t>(a.num_sms, most)), C::kThreads, size_t(C::kSmem), stream, 1, mq, mk, mv,

@@ -1,7 +1,7 @@
 // attention_rows.cuh -- one attention row of ge_attention_causal / ge_attention_prefix by one warp,
 // straight from the definition: lane l holds dims [l * D / 32, (l + 1) * D / 32) of the row, and the
 // running maximum m (log2 units), sum l and unnormalised output of a softmax are kept in fp32
-// over one key at a time.  It reads the visible keys and values only, so nothing a masked place
+// over its keys.  It reads the visible keys and values only, so nothing a masked place
 // holds can reach the row.
 #pragma once
 
@@ -62,27 +62,57 @@ __device__ __forceinline__ void row_begin(RowState<D>& s, const T* q, int lane) 
     s.l = 0.f;
 }
 
-// Adds keys [0, n) at k, v (rows `k_stride`, `v_stride` elements apart).
+// Adds keys [0, n) at k, v (rows `k_stride`, `v_stride` elements apart), eight at a time: their loads and
+// sums are independent, so a key costs a fraction of a trip to memory.
 template <typename T, int D>
 __device__ void row_keys(RowState<D>& s, const T* k, const T* v, int64_t k_stride, int64_t v_stride, int n,
                          float scale_log2e, int lane) {
-    for (int j = 0; j < n; j++) {
-        float x[D / 32];
-        row_load<T, D>(k + int64_t(j) * k_stride, lane, x);
-        float d = 0.f;
+    constexpr int B = 8, W = D / 64;  // keys at a time; a lane's words of a row
+    for (int j = 0; j < n; j += B) {
+        const int count = min(B, n - j);
+        uint32_t kw[B][W], vw[B][W];
 #pragma unroll
-        for (int i = 0; i < D / 32; i++) d = fmaf(s.q[i], x[i], d);
-        d = warp_sum(d) * scale_log2e;
-        const float m = fmaxf(s.m, d);
+        for (int b = 0; b < B; b++) {
+            const int64_t at = j + min(b, count - 1);
+            const uint32_t* kp = reinterpret_cast<const uint32_t*>(k + at * k_stride + lane * (D / 32));
+            const uint32_t* vp = reinterpret_cast<const uint32_t*>(v + at * v_stride + lane * (D / 32));
+#pragma unroll
+            for (int i = 0; i < W; i++) kw[b][i] = kp[i], vw[b][i] = vp[i];
+        }
+        float d[B], m = s.m;
+#pragma unroll
+        for (int b = 0; b < B; b++) {
+            d[b] = 0.f;
+#pragma unroll
+            for (int i = 0; i < W; i++) {
+                const float2 x = pair_to_float<T>(kw[b][i]);
+                d[b] = fmaf(s.q[2 * i + 1], x.y, fmaf(s.q[2 * i], x.x, d[b]));
+            }
+        }
+#pragma unroll
+        for (int b = 0; b < B; b++) {
+            d[b] = warp_sum(d[b]) * scale_log2e;
+            m = fmaxf(m, d[b]);
+        }
         const float alpha = s.m == m ? 1.0f : ex2_approx(s.m - m);
-        // A score of -inf under a finite maximum weighs 0; with no finite score yet it counts
-        // nothing either (m stays -inf).
-        const float p = m == -INFINITY ? 0.f : ex2_approx(d - m);
-        row_load<T, D>(v + int64_t(j) * v_stride, lane, x);
-        s.l = fmaf(s.l, alpha, p);
+        s.m = m;
+        s.l *= alpha;
 #pragma unroll
-        for (int i = 0; i < D / 32; i++) s.o[i] = fmaf(s.o[i], alpha, p * x[i]);
-        s.m = isnan(d) ? d : m;
+        for (int i = 0; i < D / 32; i++) s.o[i] *= alpha;
+#pragma unroll
+        for (int b = 0; b < B; b++) {
+            if (b >= count) break;
+            // A score of -inf under a finite maximum weighs 0; with no finite score yet it counts nothing either
+            // (m stays -inf).  A NaN score, which the maximum passes over, makes the sum NaN.
+            const float p = m == -INFINITY && !isnan(d[b]) ? 0.f : ex2_approx(d[b] - m);
+            s.l += p;
+#pragma unroll
+            for (int i = 0; i < W; i++) {
+                const float2 x = pair_to_float<T>(vw[b][i]);
+                s.o[2 * i] = fmaf(p, x.x, s.o[2 * i]);
+                s.o[2 * i + 1] = fmaf(p, x.y, s.o[2 * i + 1]);
+            }
+        }
     }
 }
 

@@ -4,7 +4,10 @@ behind a shared prefix, and products of a few rows with 4-bit weights.
 They need no model and keep nothing between calls (the entry points are ge_attention_causal,
 ge_attention_prefix and ge_linear_q4 of include/gemma_embed.h).  Every call enqueues its work on
 `stream` -- a torch stream, a raw cudaStream_t, or None for torch's current stream of the
-tensors' device -- and returns without synchronising; it may be captured into a CUDA graph.
+tensors' device -- and returns without synchronising; it may be captured into a CUDA graph.  A stream
+other than the current one has to be behind the work that fills the inputs; their memory is not reused
+before the call's work there has ended.  There is no backward pass: inputs that require a gradient are
+refused while gradients are recorded.
 
     out = attention_causal(q, k, v, seqs)               # q [T, H, D], k and v [T, KV, D]
     last = attention_prefix(q, k, v, q_seqs, kv_seqs, prefix_k, prefix_v)
@@ -68,11 +71,17 @@ def _on_device(name: str, t, device: Optional[int] = None) -> int:
     return d
 
 
+def _no_gradient(name: str, t):
+    if t.requires_grad and _torch()[0].is_grad_enabled():
+        raise _invalid(f"{name} requires a gradient, and the operator has no backward pass (call it under torch.no_grad())")
+
+
 def _heads(name: str, t, device: int, dtype, heads: Optional[int], dim: int):
     """Checks a [rows, heads, dim] tensor; gives its rows, heads and the elements between its rows."""
     _on_device(name, t, device)
     if t.dtype != dtype:
         raise _invalid(f"{name} is {t.dtype}, not {dtype}")
+    _no_gradient(name, t)
     shape = t.shape
     if len(shape) != 3 or shape[2] != dim or (heads is not None and shape[1] != heads):
         want = f"[rows, {heads if heads is not None else 'heads'}, {dim}]"
@@ -93,17 +102,34 @@ def _ranges(name: str, t, device: int) -> int:
 
 
 def _stream(stream, device: int):
-    """The stream's handle, and a context in which torch allocates on it (None: already so)."""
+    """The stream's handle, and the stream itself where it is not the current one."""
     torch, _, raw = _torch()
     if stream is None:
         return raw(device), None
     if hasattr(stream, "cuda_stream"):
         if stream.device.index != device:
             raise _invalid(f"the stream is on {stream.device}, not on cuda:{device}")
-        return stream.cuda_stream, torch.cuda.stream(stream)
-    handle = int(stream)
-    s = torch.cuda.ExternalStream(handle, device=device) if handle else torch.cuda.default_stream(device)
-    return handle, torch.cuda.stream(s)
+        handle, s = stream.cuda_stream, stream
+    else:
+        handle, s = int(stream), None
+    if handle == raw(device):
+        return handle, None
+    if s is None:
+        s = torch.cuda.ExternalStream(handle, device=device) if handle else torch.cuda.default_stream(device)
+    return handle, s
+
+
+def _on(s):
+    """A context in which torch allocates on stream `s` (None: already so)."""
+    return _HERE if s is None else _torch()[0].cuda.stream(s)
+
+
+def _in_use(s, *tensors):
+    """Keeps the tensors' memory from reuse until what stream `s` has been given has run."""
+    if s is not None:
+        for t in tensors:
+            if t is not None:
+                t.record_stream(s)
 
 
 @functools.lru_cache(maxsize=1024)
@@ -142,9 +168,9 @@ def _attention(q, k, v, prefix_k, prefix_v, q_seqs, kv_seqs, scale, window, out,
             raise _invalid(f"q_seqs names {nseq} sequences, kv_seqs {kv_seqs.shape[0]}")
     scale = 1.0 / math.sqrt(dim) if scale is None else float(scale)
     window = int(window)
-    handle, on = _stream(stream, device)
+    handle, side = _stream(stream, device)
     nbytes = _workspace_bytes(device, code, heads, kv_heads, dim, scale, window, ntok, prefix)
-    with on or _HERE:
+    with _on(side):
         if out is None:
             out = q.new_empty((ntok, heads, dim))
             out_stride = heads * dim
@@ -164,6 +190,7 @@ def _attention(q, k, v, prefix_k, prefix_v, q_seqs, kv_seqs, scale, window, out,
                                    prefix_v.data_ptr(), prefix, q_seqs.data_ptr(), kv_seqs.data_ptr(), nseq, out.data_ptr(),
                                    ws.data_ptr(), nbytes, handle)
     _call(rc)
+    _in_use(side, q, k, v, prefix_k, prefix_v, q_seqs, kv_seqs, out)
     return out
 
 
@@ -191,7 +218,7 @@ def attention_prefix(q, k, v, q_seqs, kv_seqs, prefix_k, prefix_v, scale: Option
     return _attention(q, k, v, prefix_k, prefix_v, q_seqs, kv_seqs, scale, 0, out, stream)
 
 
-@dataclass
+@dataclass(frozen=True)
 class Q4Weight:
     """A linear layer's 4-bit weights: values [n, k / 2] uint8 (element 2 i in the low half of byte i),
     scales and optionally mins [n, k / group] float16.  w = scale (q - 8), with mins scale q + min."""
@@ -268,10 +295,11 @@ def linear_q4(x, weight: Q4Weight, out=None, stream=None):
     x_stride, step = x.stride()
     if step != 1:
         raise _invalid("x's columns must lie side by side")
-    handle, on = _stream(stream, device)
+    _no_gradient("x", x)
+    handle, side = _stream(stream, device)
     out_stride = n
     if out is None:
-        with on or _HERE:
+        with _on(side):
             out = x.new_empty((rows, n))
     else:
         _on_device("out", out, device)
@@ -282,4 +310,5 @@ def linear_q4(x, weight: Q4Weight, out=None, stream=None):
     _call(_lib.lib().ge_linear_q4(device, dtype, x.data_ptr(), x_stride if rows > 1 else k, rows, k, values.data_ptr(),
                                   weight.scales.data_ptr(), None if mins is None else mins.data_ptr(), weight.group, n,
                                   out.data_ptr(), out_stride, handle))
+    _in_use(side, x, values, weight.scales, mins, out)
     return out

@@ -509,7 +509,9 @@ typedef struct ge_attention_shape {
 /* Bytes of device workspace the attention calls below need for `ntok` query rows behind a prefix of
  * `prefix_len` rows (0 for ge_attention_causal).  The workspace must be 256-byte aligned; what it
  * holds is free again once the call's work has completed, and calls that may overlap on the GPU
- * (other streams, captured graphs replayed at the same time) need one each. */
+ * (other streams, captured graphs replayed at the same time) need one each.  Its first 32-bit word is 0
+ * after a call's work, or GE_ERR_TIMEOUT where a wait inside the kernel ran out (2 s and more, which no
+ * argument can bring about); `out` is then not to be used. */
 GE_API int ge_attention_workspace(int32_t device_ordinal, const ge_attention_shape* shape, int32_t ntok,
                                   int32_t prefix_len, int64_t* bytes);
 
@@ -519,7 +521,9 @@ GE_API int ge_attention_workspace(int32_t device_ordinal, const ge_attention_sha
  * [ntok][kv_heads][head_dim]; d_seqs holds nseq (start, length) pairs on the device.  Ranges are cut
  * at ntok and may be empty; query rows that two ranges share hold unspecified values.  Rows of `out` in
  * no range are left as they were; `out` must not overlap the inputs.  Scores, sums and maxima are fp32,
- * probabilities are rounded to dtype before their product with v, the result once to dtype. */
+ * probabilities are rounded to dtype before their product with v, the result once to dtype.  What masked
+ * places hold never reaches a row; infinite or NaN values among the keys near a row cost time, since such
+ * rows are computed again one by one. */
 GE_API int ge_attention_causal(int32_t device_ordinal, const ge_attention_shape* shape, const void* d_q, const void* d_k,
                                const void* d_v, int32_t ntok, const uint32_t* d_seqs, int32_t nseq, void* d_out,
                                void* workspace, int64_t workspace_bytes, void* stream);
@@ -529,7 +533,7 @@ GE_API int ge_attention_causal(int32_t device_ordinal, const ge_attention_shape*
  * Sequence s has the query rows d_q_seqs[s] = (start, n) of q (ntok rows) and the key rows
  * d_kv_seqs[s] = (start, m) of k and v (nkv rows); the queries stand at the end, so query i sees the
  * own keys j <= m - n + i (none where that is negative).  n = 1 is the step of a single token.
- * Key ranges may be shared, in any order (fastest in the order of the queries).  A row that sees no
+ * Key ranges may be shared, in any order.  A row that sees no
  * key at all gives zeros.  Otherwise as ge_attention_causal; a window is refused. */
 GE_API int ge_attention_prefix(int32_t device_ordinal, const ge_attention_shape* shape, const void* d_q, int32_t ntok,
                                const void* d_k, const void* d_v, int32_t nkv, const void* d_prefix_k,

@@ -531,3 +531,110 @@ def test_causal_more_sequences_than_the_plan_holds_in_one_cta(ge, torch):
     lens[4000] = 300
     check_causal(ge, torch, lens, 4, 2, 64, "f16")
     check_causal(ge, torch, lens, 2, 1, 256, "bf16", window=5)
+
+
+@pytest.mark.parametrize("heads,kvh,dim", [(8, 2, 128), (3, 1, 256), (2, 2, 64)])
+def test_prefix_scattered_slots(ge, torch, heads, kvh, dim):
+    """A few sequences in a cache of many slots, in no order: the keys between them are no row's."""
+    rng = np.random.default_rng(12)
+    slot, slots, used = 640, 64, 23
+    klens = [int(x) for x in rng.integers(0, 200, used)]
+    qlens = [int(x) for x in rng.integers(0, 4, used)]
+    kr = [(int(s) * slot, n) for s, n in zip(rng.permutation(slots)[:used], klens)]
+    qr = ranges(qlens)
+    q = normal(torch, 1, (sum(qlens), heads, dim), "bf16")
+    k, v = (torch.full((slots * slot, kvh, dim), float("nan"), dtype=q.dtype, device="cuda") for _ in range(2))
+    for i, (s, n) in enumerate(kr):
+        k[s:s + n], v[s:s + n] = normal(torch, 100 + i, (n, kvh, dim), "bf16"), normal(torch, 200 + i, (n, kvh, dim), "bf16")
+    pk, pv = normal(torch, 4, (77, kvh, dim), "bf16"), normal(torch, 5, (77, kvh, dim), "bf16")
+    got = ge.attention_prefix(q, k, v, dev(torch, qr), dev(torch, kr), pk, pv)
+    want, bound, _ = ref.attention(q, k, v, qr, kr, 1 / math.sqrt(dim), prefix_k=pk, prefix_v=pv)
+    ref.check(got, want, bound)
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_small_probabilities_keep_their_sum(ge, torch, dim):
+    """One key far above all the others, whose value is 0: fp16 outputs are the sum of hundreds of
+    probabilities of 2^-24.6, held to 2^-24 in steps of 2^-31."""
+    n = 512
+    q, k, v = (torch.zeros((n, 1, dim), dtype=torch.float16, device="cuda") for _ in range(3))
+    q[:, :, 0] = 1.0
+    k[1:, :, 0] = -17.05
+    v[1:] = 16.0
+    got = ge.attention_causal(q, k, v, dev(torch, [(0, n)]), scale=1.0).double()
+    want, _, _ = ref.attention(q, k, v, [(0, n)], [(0, n)], 1.0)
+    # Half a step of a probability below fp16's normal range, 2^-25 / 2^7, relative to 2^-24.6; exponentials and
+    # sums (2^-18); the result's own half step, relative and below the normal range.
+    bound = want * (2.0 ** -(25 + 7 - 24.6) + 2.0 ** -18 + 2.0 ** -11) + 2.0 ** -25
+    ref.check(got, want, bound)
+
+
+@pytest.mark.parametrize("heads,kvh,dim", [(4, 1, 128), (2, 2, 64), (3, 1, 256)])
+def test_an_infinite_value_every_row_sees(ge, torch, heads, kvh, dim):
+    """Every row is recomputed; its other columns are as without it."""
+    n = 3000
+    q, k, v = (normal(torch, 40 + i, (n, h, dim), "f16") for i, h in enumerate((heads, kvh, kvh)))
+    v[0, :, 3] = float("inf")
+    got = ge.attention_causal(q, k, v, dev(torch, [(0, n)]))
+    want, bound, _ = ref.attention(q, k, v, [(0, n)], [(0, n)], 1 / math.sqrt(dim))
+    assert not torch.isfinite(got[:, :, 3]).any()
+    keep = [i for i in range(dim) if i != 3]
+    ref.check(got[..., keep], want[..., keep], bound[..., keep])
+
+
+def test_inputs_dropped_while_another_stream_reads_them(ge, torch):
+    """Memory of inputs that were dropped after the call is not given out again before its work is done."""
+    q, k, v = (normal(torch, 50 + i, (700, h, 128), "bf16") for i, h in enumerate((8, 2, 2)))
+    s = dev(torch, [(0, 700)])
+    w = q4(torch, ge, 600, 512, 32, False)
+    x = normal(torch, 9, (4, 512), "f16")
+    want, y = ge.attention_causal(q, k, v, s), ge.linear_q4(x, w)
+    side = torch.cuda.Stream()
+    a, b, c, d, e = q.clone(), k.clone(), v.clone(), s.clone(), x.clone()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(100_000_000)
+    got = ge.attention_causal(a, b, c, d, stream=side)
+    z = ge.linear_q4(e, w, stream=side)
+    del a, b, c, d, e
+    junk = [torch.full_like(t, 7) for t in (q, k, v, s, x) for _ in range(3)]
+    torch.cuda.synchronize()
+    assert torch.equal(got, want) and torch.equal(z, y)
+    del junk
+
+
+def test_inputs_that_require_a_gradient_are_refused(ge, torch):
+    q, k, s = normal(torch, 1, (8, 4, 64), "f16"), normal(torch, 2, (8, 2, 64), "f16"), dev(torch, [(0, 8)])
+    w = q4(torch, ge, 8, 64, 32, False)
+    want = ge.attention_causal(q, k, k, s)
+    x = q.flatten(1)[:, :64].contiguous()
+    y = ge.linear_q4(x, w)
+    q.requires_grad_()
+    x.requires_grad_()
+    for call in (lambda: ge.attention_causal(q, k, k, s), lambda: ge.attention_prefix(q, k, k, s, s, k, k), lambda: ge.linear_q4(x, w)):
+        with pytest.raises(ge.GemmaEmbedError) as e:
+            call()
+        assert e.value.case == "invalidOptions"
+    with torch.no_grad():
+        assert torch.equal(ge.attention_causal(q, k, k, s), want) and torch.equal(ge.linear_q4(x, w), y)
+
+
+@pytest.mark.parametrize("mins", [False, True])
+@pytest.mark.parametrize("rows", [3, 20])
+def test_linear_q4_wide(ge, torch, rows, mins):
+    """More output columns than the SMs hold at once."""
+    w = q4(torch, ge, 41003, 320, 32, mins)
+    x = normal(torch, 11, (rows, 320), "bf16")
+    want, bound = ref.linear_q4(x, w.values, w.scales, w.mins)
+    ref.check(ge.linear_q4(x, w), want, bound)
+
+
+@pytest.mark.parametrize("group", [32, 64, 128])
+def test_linear_q4_scales_off_16_bytes(ge, torch, group):
+    n, k = 301, 1024
+    w = q4(torch, ge, n, k, group, True)
+    off = lambda t: torch.cat([t.new_zeros(1), t.flatten()])[1:].view(t.shape)
+    x = normal(torch, 12, (6, k), "f16")
+    want = ge.linear_q4(x, w)
+    assert torch.equal(ge.linear_q4(x, ge.Q4Weight(w.values, off(w.scales), w.mins)), want)
+    assert torch.equal(ge.linear_q4(x, ge.Q4Weight(w.values, w.scales, off(w.mins))), want)
