@@ -518,7 +518,7 @@ struct TcParams {
     int heads, kv_heads, group, T, TI, ntok, window, prefix, prefix_blocks;
     uint32_t kv_magic;  // ceil(2^32 / kv_heads)
     float scale_log2e;
-    uint64_t wait_ns;
+    int64_t wait_cycles;
     Header* head;
     const int2 *rng, *segs;
     const Work* work;
@@ -538,31 +538,37 @@ __device__ __forceinline__ bool elect_one() {
 
 // A word with its n lowest bits set (0 below 0, all above 32).
 __device__ __forceinline__ uint32_t low_bits(int n) { return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1u; }
-// Waits give up after `limit` nanoseconds, or once another thread has: kWaitLimitNs and what a warp may take to
-// recompute its rows from the definition meanwhile (wait_limit).
+// Waits for the phase of parity `parity`, at most `limit` cycles: then the error is recorded and every role comes
+// to its end, each within its own next wait.  Little code: the roles hold dozens of waits, and at an item's turn
+// code that has left the instruction cache costs more than the work.
 template <bool kSleep>
-__device__ __forceinline__ bool wait_slow(uint64_t* bar, uint32_t parity, int* err, uint64_t limit) {
+__device__ __forceinline__ bool wait_on(uint64_t* bar, uint32_t parity, int* err, int64_t limit) {
     if (mbar_test(bar, parity)) return true;
-    const uint64_t t0 = globaltimer();
-    for (uint32_t spin = 1;; spin++) {
+    const int64_t t0 = clock64();
+    while (!mbar_test(bar, parity)) {
         if (kSleep) __nanosleep(32);
-        if (mbar_test(bar, parity)) return true;
-        if ((spin & (kSleep ? 15 : 63)) == 0) {
-            if (*reinterpret_cast<volatile int*>(err) != 0) return false;
-            if (globaltimer() - t0 > limit) {
-                atomicCAS(err, 0, kErrTimeout);
-                return false;
-            }
+        if (clock64() - t0 > limit) {
+            *err = kErrTimeout;
+            return false;
         }
     }
+    return true;
 }
-// A warp recomputes 32 rows over all keys at most, at about 0.25 us for a key of a row (8 heads of 128 wide, 8192
-// rows that all see an infinite value: 69 ms, 0.13 ms without it); 1 us is allowed.
-constexpr uint64_t wait_limit(int64_t keys) { return kWaitLimitNs + uint64_t(keys) * 32 * 1000; }
-// The whole warp: every lane tests (the barrier is most often already there), then they agree.
-__device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t parity, int* err, uint64_t limit) {
-    return __all_sync(0xffffffffu, mbar_poll(bar, parity)) || __all_sync(0xffffffffu, wait_slow<false>(bar, parity, err, limit));
+// The same by a whole warp, whose lanes agree.
+__device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t parity, int* err, int64_t limit) {
+    if (__all_sync(0xffffffffu, mbar_poll(bar, parity))) return true;
+    const int64_t t0 = clock64();
+    while (!__all_sync(0xffffffffu, mbar_test(bar, parity)))
+        if (__any_sync(0xffffffffu, clock64() - t0 > limit)) {
+            *err = kErrTimeout;
+            return false;
+        }
+    return true;
 }
+// kWaitLimitNs at 2 GHz, and more over many keys: a warp recomputes 32 rows over all of them at most, at about 0.25 us
+// for a key of a row (8 heads of 128 wide, 8192 rows that all see an infinite value: 69 ms, 0.13 ms without it); 1 us
+// is allowed.
+constexpr int64_t wait_limit(int64_t keys) { return 2 * (int64_t(kWaitLimitNs) + keys * 32 * 1000); }
 // Two fp32 operations at a time.
 __device__ __forceinline__ uint64_t pack2(float a, float b) {
     uint64_t r;
@@ -687,10 +693,12 @@ __host__ __device__ constexpr uint32_t idesc_of<__nv_bfloat16>(int M, int N, int
     return idesc_f16(M, N, 0, b_mn) | (1u << 7) | (1u << 10);  // A and B: bf16
 }
 
-// One row of a piece from the definition, by a whole warp; stored like the epilogue does.
+// One row of piece `id` from the definition, by a whole warp; stored like the epilogue does.  It reads the
+// piece again: one handed over would live in memory for all of the callers' work.
 template <typename E, int D>
-__device__ __noinline__ void exact_row(const TcParams& p, const Piece& s, int row, int head, int2 rg) {
+__device__ __forceinline__ void exact_row(const TcParams& p, int id, int row, int head, int2 rg) {
     const int lane = threadIdx.x & 31;
+    const Piece s = piece_of(p, fetch_piece(p, id, id + 1));
     RowState<D> st;
     row_begin<E, D>(st, static_cast<const E*>(p.q) + row * p.q_stride + int64_t(head) * D, lane);
     const int64_t col = int64_t(s.kvh) * D;
@@ -799,7 +807,7 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1)
                 prefetch_piece(p, piece_id(round + 1), total);
                 if (s.b0 >= s.b1) continue;
                 if (keys) {
-                    if (!wait_slow<true>(q_empty, uint32_t(issued_q & 1) ^ 1u, err, p.wait_ns)) break;
+                    if (!wait_on<true>(q_empty, uint32_t(issued_q & 1) ^ 1u, err, p.wait_cycles)) break;
                     mbar_expect_tx(q_full, uint32_t(NT * C::QC * 128 * live_rows));
 #pragma unroll 1
                     for (int x = 0; x < NT; x++)
@@ -814,7 +822,7 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1)
                     const CUtensorMap* map = c.prefix ? shared : own;
                     for (int h = 0; h < DH; h++) {
                         const int st = issued % ST;
-                        if (!wait_slow<true>(&empty[st], uint32_t((issued / ST) & 1) ^ 1u, err, p.wait_ns)) {
+                        if (!wait_on<true>(&empty[st], uint32_t((issued / ST) & 1) ^ 1u, err, p.wait_cycles)) {
                             ok = false;
                             break;
                         }
@@ -846,7 +854,7 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1)
         const uint64_t v_desc = sw128_desc(smem_u32(smem + C::kOffV), C::kChunk, 1024);
         bool ok = true;
         auto wait = [&](uint64_t* bar, uint32_t parity) {
-            ok = wait_warp(bar, parity, err, p.wait_ns);
+            ok = wait_warp(bar, parity, err, p.wait_cycles);
             return ok;
         };
         int nq = 0, nk = 0, nv = 0;            // Q tiles, K stages and V stages used so far
@@ -1026,7 +1034,7 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1)
         const int token = r / p.group;
         bool ok = true;
         auto wait = [&](uint64_t* bar, uint32_t parity) {
-            ok = wait_warp(bar, parity, err, p.wait_ns);
+            ok = wait_warp(bar, parity, err, p.wait_cycles);
             return ok;
         };
         int nb = 0, no = 0;  // blocks and items with an O so far
@@ -1041,7 +1049,7 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1)
         int2 range = range_of();
         while (ok && next.id < total) {
             const Piece s = piece_of(p, next);
-            const int row = row_of();
+            const int id = next.id, row = row_of();
             int2 rg = range;
             if ((s.flags & 4) && r < live_rows && row < p.ntok) rg = own_range(s.see + (row - s.tile * p.TI), s.ks, s.ke, p.window);
             next = fetch_piece(p, piece_id(++round), total);
@@ -1207,7 +1215,7 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1)
                 const int src = __ffs(redo) - 1;
                 redo &= redo - 1;
                 const int2 g = make_int2(__shfl_sync(0xffffffffu, rg.x, src), __shfl_sync(0xffffffffu, rg.y, src));
-                exact_row<E, D>(p, s, __shfl_sync(0xffffffffu, row, src), __shfl_sync(0xffffffffu, head, src), g);
+                exact_row<E, D>(p, id, __shfl_sync(0xffffffffu, row, src), __shfl_sync(0xffffffffu, head, src), g);
             }
         }
     }
