@@ -516,6 +516,7 @@ struct TcParams {
     void* out;
     int64_t q_stride, k_stride, v_stride, pk_stride, pv_stride, out_stride;
     int heads, kv_heads, group, T, TI, ntok, window, prefix, prefix_blocks;
+    bool out_wide;      // rows of out start on 32-byte boundaries
     uint32_t kv_magic;  // ceil(2^32 / kv_heads)
     float scale_log2e;
     int64_t wait_cycles;
@@ -569,6 +570,12 @@ __device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t parity, int* e
 // for a key of a row (8 heads of 128 wide, 8192 rows that all see an infinite value: 69 ms, 0.13 ms without it); 1 us
 // is allowed.
 constexpr int64_t wait_limit(int64_t keys) { return 2 * (int64_t(kWaitLimitNs) + keys * 32 * 1000); }
+// 32 bytes at once, to a 32-byte boundary: a store touches a line for every lane's row, so half as many go out.
+__device__ __forceinline__ void store32(void* p, const uint32_t (&w)[8]) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]),
+                 "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+                 : "memory");
+}
 // Two fp32 operations at a time.
 __device__ __forceinline__ uint64_t pack2(float a, float b) {
     uint64_t r;
@@ -1193,19 +1200,24 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1)
                 for (int e = 0; e < 32; e++) z = fmaf(__uint_as_float(o[e]), 0.f, z);
                 bad |= z != 0.f;  // NaN: a value is infinite or NaN
                 if (in && s.piece < 0) {
-                    uint4* dst = reinterpret_cast<uint4*>(static_cast<E*>(p.out) + row * p.out_stride + int64_t(head) * D + i * 32);
+                    uint32_t* dst = reinterpret_cast<uint32_t*>(static_cast<E*>(p.out) + row * p.out_stride + int64_t(head) * D + i * 32);
 #pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        uint32_t w[4];
+                    for (int e = 0; e < 2; e++) {
+                        uint32_t w[8];
 #pragma unroll
-                        for (int f = 0; f < 4; f++)
-                            w[f] = float_to_pair<E>(__uint_as_float(o[8 * e + 2 * f]) * inv, __uint_as_float(o[8 * e + 2 * f + 1]) * inv);
-                        dst[e] = make_uint4(w[0], w[1], w[2], w[3]);
+                        for (int f = 0; f < 8; f++)
+                            w[f] = float_to_pair<E>(__uint_as_float(o[16 * e + 2 * f]) * inv, __uint_as_float(o[16 * e + 2 * f + 1]) * inv);
+                        if (p.out_wide) {
+                            store32(dst + 8 * e, w);
+                        } else {
+                            *reinterpret_cast<uint4*>(dst + 8 * e) = make_uint4(w[0], w[1], w[2], w[3]);
+                            *reinterpret_cast<uint4*>(dst + 8 * e + 4) = make_uint4(w[4], w[5], w[6], w[7]);
+                        }
                     }
                 } else if (in) {
-                    uint4* dst = reinterpret_cast<uint4*>(p.o + at * D + i * 32);
+                    float* dst = p.o + at * D + i * 32;
 #pragma unroll
-                    for (int e = 0; e < 8; e++) dst[e] = make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+                    for (int e = 0; e < 4; e++) store32(dst + 8 * e, *reinterpret_cast<const uint32_t(*)[8]>(&o[8 * e]));
                 }
                 __syncwarp();
             }
@@ -1323,7 +1335,9 @@ cudaError_t launch_t(const CausalLaunch& a, const Sizes& s, const Layout& l, cud
                          !encode_fp16_map(&mpv, pv, kw, uint64_t(a.prefix), 64, 32, uint64_t(a.pv_stride))))
         return cudaErrorInvalidValue;
     TcParams p{a.q, a.k, a.v, a.pk, a.pv, a.out, a.q_stride, a.k_stride, a.v_stride, a.pk_stride, a.pv_stride, a.out_stride,
-               a.heads, a.kv_heads, s.group, s.T, s.TI, a.ntok, std::min(a.window, 1 << 30), a.prefix, (a.prefix + kKeys - 1) / kKeys, uint32_t(((uint64_t(1) << 32) + a.kv_heads - 1) / a.kv_heads), a.scale * kLog2e,
+               a.heads, a.kv_heads, s.group, s.T, s.TI, a.ntok, std::min(a.window, 1 << 30), a.prefix, (a.prefix + kKeys - 1) / kKeys,
+               reinterpret_cast<uintptr_t>(a.out) % 32 == 0 && a.out_stride % 16 == 0,
+               uint32_t(((uint64_t(1) << 32) + a.kv_heads - 1) / a.kv_heads), a.scale * kLog2e,
                wait_limit(int64_t(a.prefix) + a.nkv),
                l.head, l.rng, l.segs, l.work, l.o, l.ml};
     const int64_t most = s.lmax > 1 ? a.num_sms : int64_t(s.tiles) * a.kv_heads;

@@ -638,3 +638,16 @@ def test_linear_q4_scales_off_16_bytes(ge, torch, group):
     want = ge.linear_q4(x, w)
     assert torch.equal(ge.linear_q4(x, ge.Q4Weight(w.values, off(w.scales), w.mins)), want)
     assert torch.equal(ge.linear_q4(x, ge.Q4Weight(w.values, w.scales, off(w.mins))), want)
+
+
+@pytest.mark.parametrize("offset,extra", [(8, 0), (0, 8), (16, 16)])
+def test_outputs_in_wider_rows(ge, torch, offset, extra):
+    """Rows of `out` on 16- and on 32-byte boundaries, beside columns that stay as they are."""
+    heads, kvh, dim, n = 4, 2, 64, 150
+    q, k, v = (normal(torch, 60 + i, (n, h, dim), "f16") for i, h in enumerate((heads, kvh, kvh)))
+    wide = torch.full((n, heads * dim + 32 + extra), 7.0, dtype=q.dtype, device="cuda")
+    out = wide[:, offset:offset + heads * dim].unflatten(1, (heads, dim))
+    ge.attention_causal(q, k, v, dev(torch, [(0, n)]), out=out)
+    want, bound, _ = ref.attention(q, k, v, [(0, n)], [(0, n)], 0.125)
+    ref.check(out, want, bound)
+    assert (wide[:, :offset] == 7.0).all() and (wide[:, offset + heads * dim:] == 7.0).all()
