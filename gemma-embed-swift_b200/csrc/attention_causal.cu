@@ -505,8 +505,12 @@ struct Cfg {
     static constexpr int kChunk = 128 * 128;
     static constexpr int kStage = SC * kChunk;
     static constexpr int kQ = NT * QC * kChunk;
-    static constexpr int kOffK = kQ, kOffV = kOffK + ST * kStage, kOffBar = kOffV + ST * kStage;
+    static constexpr int kOffK = kQ, kOffV = kOffK + ST * kStage, kOffOut = kOffV + ST * kStage;
+    static constexpr bool kBoxes = D == 128;             // outputs leave as boxes where they can
+    static constexpr int kOutBuf = 32 * 64;              // 32 columns of a warp's rows on their way out, two per warp
+    static constexpr int kOffBar = kOffOut + (kBoxes ? NT * 4 * 2 * kOutBuf : 0);
     static constexpr int kSmem = kOffBar + 512 + 1024;
+    static_assert(kSmem <= 227 * 1024, "shared memory");
     static constexpr int kThreads = 128 + 128 * NT;
     static constexpr uint32_t kTmemS = 256;              // O in [0, 256), S and P in [256, 512)
 };
@@ -517,6 +521,7 @@ struct TcParams {
     int64_t q_stride, k_stride, v_stride, pk_stride, pv_stride, out_stride;
     int heads, kv_heads, group, T, TI, ntok, window, prefix, prefix_blocks;
     bool out_wide;      // rows of out start on 32-byte boundaries
+    bool out_boxes;     // a warp's 32 rows of a tile are a box of out
     uint32_t kv_magic;  // ceil(2^32 / kv_heads)
     float scale_log2e;
     int64_t wait_cycles;
@@ -736,7 +741,8 @@ template <typename E, int D>
 __global__ void __launch_bounds__(Cfg<D>::kThreads, 1)
     k_causal_tc(const __grid_constant__ CUtensorMap mapQ, const __grid_constant__ CUtensorMap mapK,
                 const __grid_constant__ CUtensorMap mapV, const __grid_constant__ CUtensorMap mapPK,
-                const __grid_constant__ CUtensorMap mapPV, const __grid_constant__ TcParams p) {
+                const __grid_constant__ CUtensorMap mapPV, const __grid_constant__ CUtensorMap mapO,
+                const __grid_constant__ TcParams p) {
     using C = Cfg<D>;
     constexpr int NT = C::NT, ST = C::ST, DH = C::DH;
     extern __shared__ uint8_t smem_raw[];
@@ -1175,6 +1181,10 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1)
             const float inv = s.piece >= 0 ? 1.0f : l == 0.f ? 0.f : 1.0f / l;
             if (in && s.piece >= 0) p.ml[at] = make_float2(m - kRaise<E>, l);
             bool bad = false;
+            // Whole rows of head dim 128 leave as boxes through shared memory, where all of the warp's belong to a sequence:
+            // the threads do not wait for the stores (64 texts of 300 tokens, 32 heads: 129 us, by stores 140).  Head dim
+            // 64 gains nothing (88 us both ways), 256 loses with its four warps (148 us for 141).
+            const bool box = C::kBoxes && p.out_boxes && s.piece < 0 && __all_sync(0xffffffffu, in || row >= p.ntok);
             if (count) {
                 if (!wait(&o_full[x], uint32_t(no & 1))) break;
                 no++;
@@ -1199,7 +1209,25 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1)
 #pragma unroll
                 for (int e = 0; e < 32; e++) z = fmaf(__uint_as_float(o[e]), 0.f, z);
                 bad |= z != 0.f;  // NaN: a value is infinite or NaN
-                if (in && s.piece < 0) {
+                if (box) {
+                    uint8_t* buf = smem + C::kOffOut + ((warp - 4) * 2 + (i & 1)) * C::kOutBuf;
+                    if (lane == 0) bulk_wait_read<1>();  // the copy before the last has left the buffer
+                    __syncwarp();
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        uint32_t w[4];
+#pragma unroll
+                        for (int f = 0; f < 4; f++)
+                            w[f] = float_to_pair<E>(__uint_as_float(o[8 * e + 2 * f]) * inv, __uint_as_float(o[8 * e + 2 * f + 1]) * inv);
+                        *reinterpret_cast<uint4*>(buf + lane * 64 + ((e ^ ((lane >> 1) & 3)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+                    }
+                    fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane == 0 && row < p.ntok) {
+                        tma_store_3d(&mapO, buf, i * 32, head, row);
+                        bulk_commit();
+                    }
+                } else if (in && s.piece < 0) {
                     uint32_t* dst = reinterpret_cast<uint32_t*>(static_cast<E*>(p.out) + row * p.out_stride + int64_t(head) * D + i * 32);
 #pragma unroll
                     for (int e = 0; e < 2; e++) {
@@ -1226,12 +1254,15 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1)
             while (redo) {
                 const int src = __ffs(redo) - 1;
                 redo &= redo - 1;
+                if (C::kBoxes) bulk_wait_all();  // lane 0's copies of the rows are behind
+                __syncwarp();
                 const int2 g = make_int2(__shfl_sync(0xffffffffu, rg.x, src), __shfl_sync(0xffffffffu, rg.y, src));
                 exact_row<E, D>(p, id, __shfl_sync(0xffffffffu, row, src), __shfl_sync(0xffffffffu, head, src), g);
             }
         }
     }
 
+    if (C::kBoxes && warp >= 4 && lane == 0) bulk_wait_all();
     tc_fence_before();
     __syncthreads();
     if (warp == 3) {
@@ -1334,15 +1365,22 @@ cudaError_t launch_t(const CausalLaunch& a, const Sizes& s, const Layout& l, cud
     if (a.prefix > 0 && (!encode_fp16_map(&mpk, pk, kw, uint64_t(a.prefix), 64, 32, uint64_t(a.pk_stride)) ||
                          !encode_fp16_map(&mpv, pv, kw, uint64_t(a.prefix), 64, 32, uint64_t(a.pv_stride))))
         return cudaErrorInvalidValue;
+    // A warp's rows of a tile: all heads of some tokens, or some heads of one.
+    const bool boxes = C::kBoxes && (s.group & (s.group - 1)) == 0;
+    CUtensorMap mo = mq;
+    const uint32_t box_heads = uint32_t(std::min(s.group, 32));
+    if (boxes && !encode_fp16_map_3d(&mo, static_cast<const __half*>(a.out), D, uint64_t(a.heads), uint64_t(a.ntok), 32, box_heads,
+                                     32 / box_heads, uint64_t(a.out_stride), CU_TENSOR_MAP_SWIZZLE_64B))
+        return cudaErrorInvalidValue;
     TcParams p{a.q, a.k, a.v, a.pk, a.pv, a.out, a.q_stride, a.k_stride, a.v_stride, a.pk_stride, a.pv_stride, a.out_stride,
                a.heads, a.kv_heads, s.group, s.T, s.TI, a.ntok, std::min(a.window, 1 << 30), a.prefix, (a.prefix + kKeys - 1) / kKeys,
-               reinterpret_cast<uintptr_t>(a.out) % 32 == 0 && a.out_stride % 16 == 0,
+               reinterpret_cast<uintptr_t>(a.out) % 32 == 0 && a.out_stride % 16 == 0, boxes,
                uint32_t(((uint64_t(1) << 32) + a.kv_heads - 1) / a.kv_heads), a.scale * kLog2e,
                wait_limit(int64_t(a.prefix) + a.nkv),
                l.head, l.rng, l.segs, l.work, l.o, l.ml};
     const int64_t most = s.lmax > 1 ? a.num_sms : int64_t(s.tiles) * a.kv_heads;
     e = launch_pdl(k_causal_tc<E, D>, unsigned(std::min<int64_t>(a.num_sms, most)), C::kThreads, size_t(C::kSmem), stream, 1, mq, mk, mv,
-                   mpk, mpv, p);
+                   mpk, mpv, mo, p);
     if (e != cudaSuccess || s.lmax == 1) return e;
     MergeParams mp{a.out, a.out_stride, a.heads, a.ntok, s.TI, s.lmax, l.rng, l.info, l.o, l.ml};
     return launch_pdl(k_causal_merge<E, D>, unsigned(int64_t(a.ntok) * a.heads), 256, 0, stream, 1, mp);

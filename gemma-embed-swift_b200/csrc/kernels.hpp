@@ -358,9 +358,9 @@ bool encode_attention_maps(AttnMaps& m, const __half* q, const __half* k, const 
 bool encode_fp16_map(CUtensorMap* map, const void* ptr, uint64_t inner, uint64_t outer, uint32_t box_inner,
                      uint32_t box_outer, uint64_t row_stride = 0);
 // The same over a [d2][d1][d0] array with boxes b0 x b1 x b2; d2 steps are stride2 elements
-// apart (0: d0 * d1).
+// apart (0: d0 * d1).  The swizzle spans a box row of 64 elements, or 32 with CU_TENSOR_MAP_SWIZZLE_64B.
 bool encode_fp16_map_3d(CUtensorMap* map, const void* ptr, uint64_t d0, uint64_t d1, uint64_t d2, uint32_t b0,
-                        uint32_t b1, uint32_t b2, uint64_t stride2 = 0);
+                        uint32_t b1, uint32_t b2, uint64_t stride2 = 0, CUtensorMapSwizzle swizzle = CU_TENSOR_MAP_SWIZZLE_128B);
 
 struct AttnLaunch {
     const __half* q;  // [rows][heads * hd]
