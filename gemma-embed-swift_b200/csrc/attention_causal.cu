@@ -11,11 +11,15 @@
 // the prefix' tiles serve the rows of many sequences at once.
 //
 // Three kernels, each waiting for the one before (programmatic dependent launch):
-//   k_causal_plan   one CTA: (lo, hi) per row, per tile the disjoint key segments its rows see, and the
-//                   list of work pieces, costliest first.  When the tiles of all KV heads do not fill
-//                   the GPU, a tile's key blocks are cut into pieces that do.
+//   k_causal_plan   (lo, hi) per row where a tile mixes sequences, per item (below) the disjoint key segments its
+//                   rows see, and the list of work pieces.  A warp plans an item; one CTA up to 64 items, which
+//                   hand their results on through shared memory, else a cluster of 4 or 8.  Items that fill the
+//                   SMs more than once go costliest first (a counting sort); fewer are cut into pieces of their key
+//                   blocks that fill the SMs once, unless there are few keys.  Bound by latency: 6 us for 8
+//                   queries, 18 us for 64 documents, of which the kernel after it hides its own set-up.
 //   k_causal_tc     persistent, one CTA per SM: walks the pieces in turn (below)
-//   k_causal_merge  only where tiles were cut: joins the pieces' partial rows by their maxima and sums
+//   k_causal_merge  only where tiles may be cut: joins the pieces' partial rows by their maxima and sums, a CTA per
+//                   row and head; bound by latency (8 to 11 us with its launch, cold).
 // The result of a row depends only on its own ranges and, through the pieces, on the call's sizes:
 // which CTA takes a piece changes nothing.
 //
@@ -37,7 +41,16 @@
 // segment never meets the product.  Keys masked for some rows of a tile only (later tokens, other
 // sequences) do meet it, with P = 0: where their values are infinite or NaN, 0 x V leaves NaN in rows that
 // must not see it, and the epilogue recomputes rows with non-finite outputs from the definition
-// (attention_rows.cuh), key by key.
+// (attention_rows.cuh), which reads a row's own keys only.
+//
+// What bounds it: on long sequences the softmax beside the products (of a tile's block, about 1350 cycles for a warp
+// that has the scheduler to itself, for 1090 of the tensor core); on texts of a few hundred tokens the turn from one
+// item to the next (Q's load, the first softmax and the epilogue have nothing beside them).  Measured:
+//   2 x 4096 tokens, 32 heads of 128 on 8      0.239 ms, 1150 TFLOP/s
+//   4 x 4096 tokens, 4 heads of 256 on 2       0.119 ms, 1155 TFLOP/s
+//   2 x 8192 tokens, 12 heads of 64            0.285 ms,  722 TFLOP/s (a 64 wide S costs half the product, the
+//                                              same softmax)
+//   64 x 300 tokens, 32 heads of 128 on 8      0.129 ms,  367 TFLOP/s; 394 MB of tensors, 3.0 TB/s
 #include <algorithm>
 
 #include "attention_rows.cuh"
@@ -72,9 +85,10 @@ Sizes sizes_of(const CausalLaunch& a) {
     s.T = 128 / s.group;
     s.TI = s.T * tiles_per_item(a.hd);
     s.tiles = (a.ntok + s.TI - 1) / s.TI;
-    // Pieces a tile may be cut into: enough for two rounds of the SMs, one where the tiles fill them.
+    // Pieces an item may be cut into: enough to fill the SMs twice (the plan fills them once), one where the items
+    // do so already.
     const int64_t units = std::max<int64_t>(int64_t(s.tiles) * a.kv_heads, 1);
-    // Calls over few keys are not cut: a merge costs more than the blocks it would spread.
+    // Calls over few keys are not cut: a block costs about 2 us, the merge's launch and run 8.
     s.lmax = units >= a.num_sms || int64_t(a.prefix) + a.nkv <= 4 * kKeys ? 1 : int(std::min<int64_t>(kMaxPieces, (2 * a.num_sms + units - 1) / units));
     return s;
 }
@@ -804,240 +818,240 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1)
     const int total = p.head->nwork * p.kv_heads;
 
     if (warp < 4) {
-    if constexpr (NT == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
-    if (warp == 0 || warp == 2) {
-        // ---------------------------------------------------------- TMA producers (Q and K; V)
-        if (lane == 0) {
-            const bool keys = warp == 0;
-            uint64_t *full = keys ? k_full : v_full, *empty = keys ? k_empty : v_empty;
-            uint8_t* ring = smem + (keys ? C::kOffK : C::kOffV);
-            const CUtensorMap* own = keys ? &mapK : &mapV;
-            const CUtensorMap* shared = keys ? &mapPK : &mapPV;
+        if constexpr (NT == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
+        if (warp == 0 || warp == 2) {
+            // ---------------------------------------------------------- TMA producers (Q and K; V)
+            if (lane == 0) {
+                const bool keys = warp == 0;
+                uint64_t *full = keys ? k_full : v_full, *empty = keys ? k_empty : v_empty;
+                uint8_t* ring = smem + (keys ? C::kOffK : C::kOffV);
+                const CUtensorMap* own = keys ? &mapK : &mapV;
+                const CUtensorMap* shared = keys ? &mapPK : &mapPV;
+                bool ok = true;
+                int issued = 0, issued_q = 0;
+                for (int round = 0, id; ok && (id = piece_id(round)) < total; round++) {
+                    const Piece s = piece_of(p, fetch_piece(p, id, total));
+                    prefetch_piece(p, piece_id(round + 1), total);
+                    if (s.b0 >= s.b1) continue;
+                    if (keys) {
+                        if (!wait_on<true>(q_empty, uint32_t(issued_q & 1) ^ 1u, err, p.wait_cycles)) break;
+                        mbar_expect_tx(q_full, uint32_t(NT * C::QC * 128 * live_rows));
+#pragma unroll 1
+                        for (int x = 0; x < NT; x++)
+#pragma unroll 1
+                            for (int c = 0; c < C::QC; c++)
+                                tma_load_3d(smem + (x * C::QC + c) * C::kChunk, &mapQ, q_full, c * 64, s.kvh * p.group,
+                                            s.tile * p.TI + x * p.T);
+                        issued_q++;
+                    }
+                    for (Cursor c(p, s); ok && c.b < s.b1; c.next(p, s)) {
+                        const int boxes = (c.nv + 31) / 32;
+                        const CUtensorMap* map = c.prefix ? shared : own;
+                        for (int h = 0; h < DH; h++) {
+                            const int st = issued % ST;
+                            if (!wait_on<true>(&empty[st], uint32_t((issued / ST) & 1) ^ 1u, err, p.wait_cycles)) {
+                                ok = false;
+                                break;
+                            }
+                            mbar_expect_tx(&full[st], uint32_t(boxes * C::SC * 4096));
+#pragma unroll 1
+                            for (int ch = 0; ch < C::SC; ch++)
+#pragma unroll 1
+                                for (int b = 0; b < boxes; b++)
+                                    tma_load_2d(ring + st * C::kStage + ch * C::kChunk + b * 4096, map, &full[st],
+                                                s.kvh * D + h * C::DS + ch * 64, c.row + b * 32);
+                            issued++;
+                        }
+                    }
+                }
+                // Every issued load lands before the CTA exits, also after an error.
+                if (issued_q > 0) drain(q_full, uint32_t((issued_q - 1) & 1));
+#pragma unroll 1
+                for (int st = 0; st < ST; st++) {
+                    const int n = issued / ST + (st < issued % ST ? 1 : 0);
+                    if (n > 0) drain(&full[st], uint32_t((n - 1) & 1));
+                }
+            }
+        } else if (warp == 1) {
+            // ---------------------------------------------------------- MMA issuer (the whole warp walks along)
+            const uint32_t id_s = idesc_of<E>(128, kKeys, 0);      // K-major Q and K
+            const uint32_t id_o = idesc_of<E>(128, C::DS, 1);      // P from tensor memory, MN-major V
+            // Descriptors of the tiles' starts; others lie (bytes / 16) further.
+            const uint64_t q_desc = sw128_desc(smem_u32(smem), 16, 1024), k_desc = sw128_desc(smem_u32(smem + C::kOffK), 16, 1024);
+            const uint64_t v_desc = sw128_desc(smem_u32(smem + C::kOffV), C::kChunk, 1024);
             bool ok = true;
-            int issued = 0, issued_q = 0;
+            auto wait = [&](uint64_t* bar, uint32_t parity) {
+                ok = wait_warp(bar, parity, err, p.wait_cycles);
+                return ok;
+            };
+            int nq = 0, nk = 0, nv = 0;            // Q tiles, K stages and V stages used so far
+            int ns[2] = {0, 0}, np[2] = {0, 0};    // S and PV products per S buffer (NT 2) or in all (NT 1, [0])
+            int no[2] = {0, 0};                    // items with an O, per tile
             for (int round = 0, id; ok && (id = piece_id(round)) < total; round++) {
                 const Piece s = piece_of(p, fetch_piece(p, id, total));
                 prefetch_piece(p, piece_id(round + 1), total);
                 if (s.b0 >= s.b1) continue;
-                if (keys) {
-                    if (!wait_on<true>(q_empty, uint32_t(issued_q & 1) ^ 1u, err, p.wait_cycles)) break;
-                    mbar_expect_tx(q_full, uint32_t(NT * C::QC * 128 * live_rows));
-#pragma unroll 1
-                    for (int x = 0; x < NT; x++)
-#pragma unroll 1
-                        for (int c = 0; c < C::QC; c++)
-                            tma_load_3d(smem + (x * C::QC + c) * C::kChunk, &mapQ, q_full, c * 64, s.kvh * p.group,
-                                        s.tile * p.TI + x * p.T);
-                    issued_q++;
-                }
-                for (Cursor c(p, s); ok && c.b < s.b1; c.next(p, s)) {
-                    const int boxes = (c.nv + 31) / 32;
-                    const CUtensorMap* map = c.prefix ? shared : own;
-                    for (int h = 0; h < DH; h++) {
-                        const int st = issued % ST;
-                        if (!wait_on<true>(&empty[st], uint32_t((issued / ST) & 1) ^ 1u, err, p.wait_cycles)) {
-                            ok = false;
-                            break;
-                        }
-                        mbar_expect_tx(&full[st], uint32_t(boxes * C::SC * 4096));
-#pragma unroll 1
-                        for (int ch = 0; ch < C::SC; ch++)
-#pragma unroll 1
-                            for (int b = 0; b < boxes; b++)
-                                tma_load_2d(ring + st * C::kStage + ch * C::kChunk + b * 4096, map, &full[st],
-                                            s.kvh * D + h * C::DS + ch * 64, c.row + b * 32);
-                        issued++;
-                    }
-                }
-            }
-            // Every issued load lands before the CTA exits, also after an error.
-            if (issued_q > 0) drain(q_full, uint32_t((issued_q - 1) & 1));
-#pragma unroll 1
-            for (int st = 0; st < ST; st++) {
-                const int n = issued / ST + (st < issued % ST ? 1 : 0);
-                if (n > 0) drain(&full[st], uint32_t((n - 1) & 1));
-            }
-        }
-    } else if (warp == 1) {
-        // ---------------------------------------------------------- MMA issuer (the whole warp walks along)
-        const uint32_t id_s = idesc_of<E>(128, kKeys, 0);      // K-major Q and K
-        const uint32_t id_o = idesc_of<E>(128, C::DS, 1);      // P from tensor memory, MN-major V
-        // Descriptors of the tiles' starts; others lie (bytes / 16) further.
-        const uint64_t q_desc = sw128_desc(smem_u32(smem), 16, 1024), k_desc = sw128_desc(smem_u32(smem + C::kOffK), 16, 1024);
-        const uint64_t v_desc = sw128_desc(smem_u32(smem + C::kOffV), C::kChunk, 1024);
-        bool ok = true;
-        auto wait = [&](uint64_t* bar, uint32_t parity) {
-            ok = wait_warp(bar, parity, err, p.wait_cycles);
-            return ok;
-        };
-        int nq = 0, nk = 0, nv = 0;            // Q tiles, K stages and V stages used so far
-        int ns[2] = {0, 0}, np[2] = {0, 0};    // S and PV products per S buffer (NT 2) or in all (NT 1, [0])
-        int no[2] = {0, 0};                    // items with an O, per tile
-        for (int round = 0, id; ok && (id = piece_id(round)) < total; round++) {
-            const Piece s = piece_of(p, fetch_piece(p, id, total));
-            prefetch_piece(p, piece_id(round + 1), total);
-            if (s.b0 >= s.b1) continue;
-            if (!wait(q_full, uint32_t(nq & 1))) break;
-            nq++;
-            tc_fence_after();
-            Cursor c(p, s);
-            int prev = 0, prev_nv = 0;  // the block before: the tiles it is active for, its keys
-            int used = 0;               // tiles with an O in this item
-            for (;;) {
-                const bool more = c.b < s.b1;
-                int act = 0;
-                if (more)
-                    for (int x = 0; x < NT; x++) act |= NT == 1 || c.active(s, x) ? 1 << x : 0;
-                if constexpr (NT == 2) {
-                    // This block's K and the block before's V first: once a tile's P has come, its PV and then its S
-                    // (over the P just read) go out together, and the other tile's softmax runs under them.
-                    const int ks = nk % ST, vs = nv % ST, steps = (prev_nv + 15) / 16;
-                    if (more && !wait(&k_full[ks], uint32_t((nk / ST) & 1))) break;
-                    if (prev_nv) {
-                        if (!wait(&v_full[vs], uint32_t((nv / ST) & 1))) break;
-                        if (prev_nv & 15) {
-                            // Rows behind the block's last key, up to the product's step.
-#pragma unroll 1
-                            for (int i = lane; i < (steps * 16 - prev_nv) * C::SC * 8; i += 32) {
-                                const int rr = prev_nv + i / (C::SC * 8), ch = (i >> 3) % C::SC;
-                                *reinterpret_cast<uint4*>(smem + C::kOffV + vs * C::kStage + ch * C::kChunk + rr * 128 + (i & 7) * 16) =
-                                    make_uint4(0u, 0u, 0u, 0u);
-                            }
-                            fence_proxy_async_smem();
-                            __syncwarp();
-                        }
-                    }
-                    const uint64_t kd = k_desc + uint32_t(__shfl_sync(0xffffffffu, ks, 0) * (C::kStage >> 4));
-                    const uint64_t vd = v_desc + uint32_t(__shfl_sync(0xffffffffu, vs, 0) * (C::kStage >> 4));
-#pragma unroll
-                    for (int x = 0; x < 2; x++) {
-                        const bool pv = (prev >> x) & 1, sc = (act >> x) & 1;
-                        const uint32_t begun = uint32_t(used >> x) & 1u;
-                        if (pv) {
-                            if (!begun && no[x] > 0 && !wait(&o_empty[x], uint32_t((no[x] - 1) & 1))) break;
-                            if (!wait(&p_full[x], uint32_t(np[x] & 1))) break;
-                            np[x]++;
-                            if (!begun) no[x]++;
-                            used |= 1 << x;
-                        }
-                        tc_fence_after();
-                        const uint32_t od = tmem + uint32_t(x * D), sd = tmem + C::kTmemS + uint32_t(x * kKeys);
-                        if (elect_one()) {
-                            if (pv) {
-                                if (steps == 8) {
-#pragma unroll
-                                    for (int kk = 0; kk < 8; kk++)
-                                        umma_f16_ta(od, sd + kk * 8, vd + uint32_t(kk * 128), id_o, kk ? 1u : begun);
-                                } else {
-#pragma unroll 1
-                                    for (int kk = 0; kk < steps; kk++)
-                                        umma_f16_ta(od, sd + kk * 8, vd + uint32_t(kk * 128), id_o, kk ? 1u : begun);
-                                }
-                            }
-                            if (sc) {
-#pragma unroll
-                                for (int kk = 0; kk < C::DS / 16; kk++)
-                                    umma_f16(sd, q_desc + uint32_t(((x * C::QC + (kk >> 2)) * C::kChunk + (kk & 3) * 32) >> 4),
-                                             kd + uint32_t(((kk >> 2) * C::kChunk + (kk & 3) * 32) >> 4), id_s, kk != 0);
-                                umma_commit(&s_full[x]);
-                            }
-                            if (!more && (pv || begun)) umma_commit(&o_full[x]);
-                            if (x == 1) {
-                                if (prev_nv) umma_commit(&v_empty[vs]);
-                                if (more) umma_commit(&k_empty[ks]);
-                            }
-                        }
-                        __syncwarp();
-                    }
-                    if (!ok) break;
-                    if (prev_nv) nv++;
-                    if (more) nk++;
-                } else {
-                    if (more) {
-                        // S into the other of the two buffers, ahead of the block before's PV.
-                        const int b = ns[0] & 1;
-                        for (int h = 0; h < DH; h++) {
-                            const int st = (nk + h) % ST;
-                            if (!wait(&k_full[st], uint32_t(((nk + h) / ST) & 1))) break;
-                            tc_fence_after();
-                            const uint64_t kd = k_desc + uint32_t(__shfl_sync(0xffffffffu, st, 0) * (C::kStage >> 4));
-                            const uint32_t sd = tmem + C::kTmemS + uint32_t(__shfl_sync(0xffffffffu, b, 0) * kKeys);
-                            if (elect_one()) {
-#pragma unroll
-                                for (int kk = 0; kk < C::DS / 16; kk++)
-                                    umma_f16(sd, q_desc + uint32_t(((h * C::SC + (kk >> 2)) * C::kChunk + (kk & 3) * 32) >> 4),
-                                             kd + uint32_t(((kk >> 2) * C::kChunk + (kk & 3) * 32) >> 4), id_s, (h | kk) != 0);
-                                umma_commit(&k_empty[st]);
-                                if (h == DH - 1) umma_commit(&s_full[b]);
-                            }
-                            __syncwarp();
-                        }
-                        if (!ok) break;
-                        ns[0]++;
-                        nk += DH;
-                    }
-                    if (prev_nv) {
-                        const int b = np[0] & 1, steps = (prev_nv + 15) / 16;
-                        if (!used && no[0] > 0 && !wait(&o_empty[0], uint32_t((no[0] - 1) & 1))) break;
-                        for (int h = 0; h < DH; h++) {
-                            const int st = (nv + h) % ST;
-                            if (!wait(&v_full[st], uint32_t(((nv + h) / ST) & 1))) break;
+                if (!wait(q_full, uint32_t(nq & 1))) break;
+                nq++;
+                tc_fence_after();
+                Cursor c(p, s);
+                int prev = 0, prev_nv = 0;  // the block before: the tiles it is active for, its keys
+                int used = 0;               // tiles with an O in this item
+                for (;;) {
+                    const bool more = c.b < s.b1;
+                    int act = 0;
+                    if (more)
+                        for (int x = 0; x < NT; x++) act |= NT == 1 || c.active(s, x) ? 1 << x : 0;
+                    if constexpr (NT == 2) {
+                        // This block's K and the block before's V first: once a tile's P has come, its PV and then its S
+                        // (over the P just read) go out together, and the other tile's softmax runs under them.
+                        const int ks = nk % ST, vs = nv % ST, steps = (prev_nv + 15) / 16;
+                        if (more && !wait(&k_full[ks], uint32_t((nk / ST) & 1))) break;
+                        if (prev_nv) {
+                            if (!wait(&v_full[vs], uint32_t((nv / ST) & 1))) break;
                             if (prev_nv & 15) {
+                                // Rows behind the block's last key, up to the product's step.
 #pragma unroll 1
                                 for (int i = lane; i < (steps * 16 - prev_nv) * C::SC * 8; i += 32) {
                                     const int rr = prev_nv + i / (C::SC * 8), ch = (i >> 3) % C::SC;
-                                    *reinterpret_cast<uint4*>(smem + C::kOffV + st * C::kStage + ch * C::kChunk + rr * 128 + (i & 7) * 16) =
+                                    *reinterpret_cast<uint4*>(smem + C::kOffV + vs * C::kStage + ch * C::kChunk + rr * 128 + (i & 7) * 16) =
                                         make_uint4(0u, 0u, 0u, 0u);
                                 }
                                 fence_proxy_async_smem();
                                 __syncwarp();
                             }
-                            if (h == 0 && !wait(&p_full[b], uint32_t((np[0] >> 1) & 1))) break;
-                            tc_fence_after();
-                            const uint64_t vd = v_desc + uint32_t(__shfl_sync(0xffffffffu, st, 0) * (C::kStage >> 4));
-                            const uint32_t pd = tmem + C::kTmemS + uint32_t(__shfl_sync(0xffffffffu, b, 0) * kKeys), od = tmem + uint32_t(h * C::DS);
-                            const uint32_t begun = uint32_t(used);
-                            if (elect_one()) {
-                                if (steps == 8) {
+                        }
+                        const uint64_t kd = k_desc + uint32_t(__shfl_sync(0xffffffffu, ks, 0) * (C::kStage >> 4));
+                        const uint64_t vd = v_desc + uint32_t(__shfl_sync(0xffffffffu, vs, 0) * (C::kStage >> 4));
 #pragma unroll
-                                    for (int kk = 0; kk < 8; kk++)
-                                        umma_f16_ta(od, pd + kk * 8, vd + uint32_t(kk * 128), id_o, kk ? 1u : begun);
-                                } else {
+                        for (int x = 0; x < 2; x++) {
+                            const bool pv = (prev >> x) & 1, sc = (act >> x) & 1;
+                            const uint32_t begun = uint32_t(used >> x) & 1u;
+                            if (pv) {
+                                if (!begun && no[x] > 0 && !wait(&o_empty[x], uint32_t((no[x] - 1) & 1))) break;
+                                if (!wait(&p_full[x], uint32_t(np[x] & 1))) break;
+                                np[x]++;
+                                if (!begun) no[x]++;
+                                used |= 1 << x;
+                            }
+                            tc_fence_after();
+                            const uint32_t od = tmem + uint32_t(x * D), sd = tmem + C::kTmemS + uint32_t(x * kKeys);
+                            if (elect_one()) {
+                                if (pv) {
+                                    if (steps == 8) {
+#pragma unroll
+                                        for (int kk = 0; kk < 8; kk++)
+                                            umma_f16_ta(od, sd + kk * 8, vd + uint32_t(kk * 128), id_o, kk ? 1u : begun);
+                                    } else {
 #pragma unroll 1
-                                    for (int kk = 0; kk < steps; kk++)
-                                        umma_f16_ta(od, pd + kk * 8, vd + uint32_t(kk * 128), id_o, kk ? 1u : begun);
+                                        for (int kk = 0; kk < steps; kk++)
+                                            umma_f16_ta(od, sd + kk * 8, vd + uint32_t(kk * 128), id_o, kk ? 1u : begun);
+                                    }
                                 }
-                                umma_commit(&v_empty[st]);
-                                if (h == DH - 1) {
-                                    umma_commit(pv_done);
-                                    if (!more) umma_commit(&o_full[0]);
+                                if (sc) {
+#pragma unroll
+                                    for (int kk = 0; kk < C::DS / 16; kk++)
+                                        umma_f16(sd, q_desc + uint32_t(((x * C::QC + (kk >> 2)) * C::kChunk + (kk & 3) * 32) >> 4),
+                                                 kd + uint32_t(((kk >> 2) * C::kChunk + (kk & 3) * 32) >> 4), id_s, kk != 0);
+                                    umma_commit(&s_full[x]);
+                                }
+                                if (!more && (pv || begun)) umma_commit(&o_full[x]);
+                                if (x == 1) {
+                                    if (prev_nv) umma_commit(&v_empty[vs]);
+                                    if (more) umma_commit(&k_empty[ks]);
                                 }
                             }
                             __syncwarp();
                         }
                         if (!ok) break;
-                        np[0]++;
-                        if (!used) no[0]++;
-                        used = 1;
-                        nv += DH;
+                        if (prev_nv) nv++;
+                        if (more) nk++;
+                    } else {
+                        if (more) {
+                            // S into the other of the two buffers, ahead of the block before's PV.
+                            const int b = ns[0] & 1;
+                            for (int h = 0; h < DH; h++) {
+                                const int st = (nk + h) % ST;
+                                if (!wait(&k_full[st], uint32_t(((nk + h) / ST) & 1))) break;
+                                tc_fence_after();
+                                const uint64_t kd = k_desc + uint32_t(__shfl_sync(0xffffffffu, st, 0) * (C::kStage >> 4));
+                                const uint32_t sd = tmem + C::kTmemS + uint32_t(__shfl_sync(0xffffffffu, b, 0) * kKeys);
+                                if (elect_one()) {
+#pragma unroll
+                                    for (int kk = 0; kk < C::DS / 16; kk++)
+                                        umma_f16(sd, q_desc + uint32_t(((h * C::SC + (kk >> 2)) * C::kChunk + (kk & 3) * 32) >> 4),
+                                                 kd + uint32_t(((kk >> 2) * C::kChunk + (kk & 3) * 32) >> 4), id_s, (h | kk) != 0);
+                                    umma_commit(&k_empty[st]);
+                                    if (h == DH - 1) umma_commit(&s_full[b]);
+                                }
+                                __syncwarp();
+                            }
+                            if (!ok) break;
+                            ns[0]++;
+                            nk += DH;
+                        }
+                        if (prev_nv) {
+                            const int b = np[0] & 1, steps = (prev_nv + 15) / 16;
+                            if (!used && no[0] > 0 && !wait(&o_empty[0], uint32_t((no[0] - 1) & 1))) break;
+                            for (int h = 0; h < DH; h++) {
+                                const int st = (nv + h) % ST;
+                                if (!wait(&v_full[st], uint32_t(((nv + h) / ST) & 1))) break;
+                                if (prev_nv & 15) {
+#pragma unroll 1
+                                    for (int i = lane; i < (steps * 16 - prev_nv) * C::SC * 8; i += 32) {
+                                        const int rr = prev_nv + i / (C::SC * 8), ch = (i >> 3) % C::SC;
+                                        *reinterpret_cast<uint4*>(smem + C::kOffV + st * C::kStage + ch * C::kChunk + rr * 128 + (i & 7) * 16) =
+                                            make_uint4(0u, 0u, 0u, 0u);
+                                    }
+                                    fence_proxy_async_smem();
+                                    __syncwarp();
+                                }
+                                if (h == 0 && !wait(&p_full[b], uint32_t((np[0] >> 1) & 1))) break;
+                                tc_fence_after();
+                                const uint64_t vd = v_desc + uint32_t(__shfl_sync(0xffffffffu, st, 0) * (C::kStage >> 4));
+                                const uint32_t pd = tmem + C::kTmemS + uint32_t(__shfl_sync(0xffffffffu, b, 0) * kKeys), od = tmem + uint32_t(h * C::DS);
+                                const uint32_t begun = uint32_t(used);
+                                if (elect_one()) {
+                                    if (steps == 8) {
+#pragma unroll
+                                        for (int kk = 0; kk < 8; kk++)
+                                            umma_f16_ta(od, pd + kk * 8, vd + uint32_t(kk * 128), id_o, kk ? 1u : begun);
+                                    } else {
+#pragma unroll 1
+                                        for (int kk = 0; kk < steps; kk++)
+                                            umma_f16_ta(od, pd + kk * 8, vd + uint32_t(kk * 128), id_o, kk ? 1u : begun);
+                                    }
+                                    umma_commit(&v_empty[st]);
+                                    if (h == DH - 1) {
+                                        umma_commit(pv_done);
+                                        if (!more) umma_commit(&o_full[0]);
+                                    }
+                                }
+                                __syncwarp();
+                            }
+                            if (!ok) break;
+                            np[0]++;
+                            if (!used) no[0]++;
+                            used = 1;
+                            nv += DH;
+                        }
                     }
+                    if (!more) break;
+                    prev = act;
+                    prev_nv = c.nv;
+                    c.next(p, s);
+                    // Every S of the item has read Q.
+                    if (c.b >= s.b1 && elect_one()) umma_commit(q_empty);
+                    __syncwarp();
                 }
-                if (!more) break;
-                prev = act;
-                prev_nv = c.nv;
-                c.next(p, s);
-                // Every S of the item has read Q.
-                if (c.b >= s.b1 && elect_one()) umma_commit(q_empty);
-                __syncwarp();
             }
+            // The products in flight end before the CTA gives its memory back.
+            if (elect_one()) {
+                umma_commit(idle);
+                drain(idle, 0);
+            }
+            __syncwarp();
         }
-        // The products in flight end before the CTA gives its memory back.
-        if (elect_one()) {
-            umma_commit(idle);
-            drain(idle, 0);
-        }
-        __syncwarp();
-    }
     } else {
         // ---------------------------------------------------------- softmax and output, one thread per row
         if constexpr (NT == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");

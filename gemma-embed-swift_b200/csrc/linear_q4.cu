@@ -5,7 +5,7 @@
 // its own per warp, no barrier in the way) and are widened on the fly to 16-bit integers, which are
 // exact, for the warp's 16 x 8 x 16 tensor products with fp32 sums (a warp's product costs fewer
 // issue slots than one multiply-add per weight and row, and a 128-row tcgen05 tile would be empty
-// but for a few rows).  Every 32 weights the integer sums are scaled in fp32: acc += scale * sum, plus
+// but for a few rows).  Every group's integer sums are scaled in fp32: acc += scale * sum, plus
 // min * (sum of x) with minima, so no weight is ever rounded.
 //
 // One CTA per SM, 16 warps.  A warp owns 16 output columns n (a row tile) or, where the CTA has fewer
@@ -17,6 +17,17 @@
 // come along in its slot.
 // x is staged for all warps in two buffers of kXElems elements (all of it where it fits, so that the
 // warps never meet while they stream).
+//
+// What bounds it now: neither memory (2 to 3.5 of 6.6 TB/s) nor one pipe (12 rows: 44 % of the issue slots, 48 % of
+// shared memory's, 23 % of the tensor products'), but a warp's dependent steps from a stage's arrival through widening,
+// products and scaling, at four warps to a scheduler; for many rows also the chunks of x, whose ends the warps wait for
+// together, and that 9 to 15 tiles leave some of 16 warps half idle.  A CTA takes as many of its tiles at once as it
+// has warps: fewer, with parts of k on more warps, were slower (16384 x 8192, 1 row: 7 tiles at once 21.4 us, 4 + 3
+// 24.7, one by one 34.5; 28671 x 8192, 12 rows: 13 at once 64, 7 + 6 67, 5 + 5 + 3 76).  Measured, weights from memory:
+//   16384 x 8192, groups of 32, 1 row, fp16              21.4 us, 3.5 TB/s
+//   28671 x 8192, groups of 128 with mins, 12 rows, bf16   64 us, 2.0 TB/s
+//   41003 x 4096, groups of 32, 4 rows, fp16               33 us, 2.9 TB/s
+//    2304 x 768, groups of 32, 1 row, fp16                3.0 us (a launch and one trip to memory)
 #include <algorithm>
 
 #include "attention_rows.cuh"
@@ -65,15 +76,15 @@ __device__ __forceinline__ void cp_wait() {
     asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
-// Eight 4-bit values as four exact pairs (0, 4), (1, 5), (2, 6), (3, 7), less 8 each where `kSigned`.
-// fp16: 1024 + q has q as its low bits (and 1024 + 16 q the bits four places up, brought back by an
-// exact multiply-add); bf16 holds 128 + q alike.
 // (a & mask) | bits in one instruction.
 __device__ __forceinline__ uint32_t and_or(uint32_t a, uint32_t mask, uint32_t bits) {
     uint32_t r;
     asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(r) : "r"(a), "r"(mask), "r"(bits));
     return r;
 }
+// Eight 4-bit values as four exact pairs (0, 4), (1, 5), (2, 6), (3, 7), less 8 each where `kSigned`.
+// fp16: 1024 + q has q as its low bits (and 1024 + 16 q the bits four places up, brought back by an
+// exact multiply-add); bf16 holds 128 + q alike.
 template <bool kSigned>
 __device__ __forceinline__ void widen_f16(uint32_t u, uint32_t (&t)[4]) {
     const __half2 off = __float2half2_rn(kSigned ? -1032.f : -1024.f);
