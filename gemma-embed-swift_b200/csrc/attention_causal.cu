@@ -104,6 +104,7 @@ struct alignas(16) TileInfo {
     // Items inside one sequence (simple): row i sees [ks, ke) up to key see + i, as own_range has it; the
     // others' rows have theirs in rng.
     int simple, see, ks, ke;
+    int pos, end, spare[2];        // the first own-key segment
 };
 // A piece of an item, all that the main kernel's roles need of it but further segments and mixed rows.
 struct alignas(16) Work {
@@ -167,33 +168,43 @@ __device__ __forceinline__ int2 own_range(int see, int ks, int ke, int window) {
 // A sequence's rows [q0, q1) and keys [ks, ke), cut to the tensors; row q0 + i sees keys below see + i.
 struct Seq {
     int q0, q1, ks, ke, see;
-    __device__ __forceinline__ Seq(const PlanParams& p, const uint4& w) {
-        const int64_t q = w.x, n = w.y, k = w.z, m = w.w;
-        q0 = int(min(q, int64_t(p.ntok)));
-        q1 = int(min(q + n, int64_t(p.ntok)));
-        ks = int(min(k, int64_t(p.nkv)));
-        ke = int(min(k + m, int64_t(p.nkv)));
-        // Rows and keys stay below 2^30, so a clamped value decides every row the same way.
-        see = int(max(int64_t(-(1 << 30)), min(k + m - n + 1, int64_t(1 << 30))));
-    }
 };
+__device__ __forceinline__ Seq seq_of(const PlanParams& p, int s) {
+    const int64_t q = p.q_seqs[2 * s], n = p.q_seqs[2 * s + 1], k = p.kv_seqs[2 * s], m = p.kv_seqs[2 * s + 1];
+    Seq r;
+    r.q0 = int(min(q, int64_t(p.ntok)));
+    r.q1 = int(min(q + n, int64_t(p.ntok)));
+    r.ks = int(min(k, int64_t(p.nkv)));
+    r.ke = int(min(k + m, int64_t(p.nkv)));
+    // Rows and keys stay below 2^30, so a clamped value decides every row the same way.
+    r.see = int(max(int64_t(-(1 << 30)), min(k + m - n + 1, int64_t(1 << 30))));
+    return r;
+}
 
-// Sequence ranges in shared memory (those past kPlanSeqs are read from global memory).
+// Sequences in shared memory (those past kPlanSeqs are read from global memory every time).
 constexpr int kPlanSeqs = 4096, kMaxItemRows = 256, kPlanItems = 64;  // items planned by one CTA
+struct Seqs {
+    int4* range;  // q0, q1, ks, ke
+    int* see;
+};
 constexpr size_t plan_smem(int nseq) {
-    return size_t(nseq < kPlanSeqs ? nseq : kPlanSeqs) * sizeof(uint4) + 32 * 2 * kMaxItemRows * sizeof(int2);
+    return size_t(((nseq < kPlanSeqs ? nseq : kPlanSeqs) + 3) / 4 * 4) * (sizeof(int4) + sizeof(int)) + 32 * 2 * kMaxItemRows * sizeof(int2);
 }
-__device__ __forceinline__ uint4 seq_words(const PlanParams& p, int s) {
-    return make_uint4(p.q_seqs[2 * s], p.q_seqs[2 * s + 1], p.kv_seqs[2 * s], p.kv_seqs[2 * s + 1]);
+__device__ __forceinline__ Seq seq_at(const PlanParams& p, const Seqs& seqs, int s) {
+    if (s >= kPlanSeqs) return seq_of(p, s);
+    const int4 r = seqs.range[s];
+    return Seq{r.x, r.y, r.z, r.w, seqs.see[s]};
 }
-__device__ __forceinline__ uint4 shfl_words(const uint4& w, int src) {
-    return make_uint4(__shfl_sync(0xffffffffu, w.x, src), __shfl_sync(0xffffffffu, w.y, src), __shfl_sync(0xffffffffu, w.z, src),
-                      __shfl_sync(0xffffffffu, w.w, src));
-}
-// Rows a sequence has among [r0, r1), as offsets from r0: [x, y), empty unless x < y.
-__device__ __forceinline__ int2 rows_within(const uint4& w, int r0, int r1) {
-    const int64_t q0 = w.x, q1 = int64_t(w.x) + w.y;
-    return make_int2(int(min(max(q0, int64_t(r0)), int64_t(r1)) - r0), int(max(min(q1, int64_t(r1)), int64_t(r0)) - r0));
+// Rows sequence s has among [r0, r1), as offsets from r0: [x, y), empty unless x < y.
+__device__ __forceinline__ int2 rows_within(const PlanParams& p, const Seqs& seqs, int s, int r0, int r1) {
+    int2 q = make_int2(0, 0);
+    if (s < kPlanSeqs) {
+        if (s < p.nseq) q = *reinterpret_cast<const int2*>(&seqs.range[s]);
+    } else if (s < p.nseq) {
+        const Seq r = seq_of(p, s);
+        q = make_int2(r.q0, r.q1);
+    }
+    return make_int2(max(q.x, r0) - r0, min(q.y, r1) - r0);
 }
 
 // The disjoint ascending segments of n ranges whose lo never falls (empty ones aside), into seg, which may be
@@ -262,19 +273,17 @@ __device__ void sort_ranges(const int2* rng, int2* seg, int n, int lane) {
 
 // One item, by one warp: rng and seg are the warp's own shared memory.  Its segments and (mixed) rows go to the
 // workspace.
-__device__ TileInfo plan_item(const PlanParams& p, const uint4* seqs, int2* rng, int2* seg, int t, int lane) {
+__device__ TileInfo plan_item(const PlanParams& p, const Seqs& seqs, int2* rng, int2* seg, int t, int lane) {
     const int r0 = t * p.TI, n = min(p.TI, p.ntok - r0);
     TileInfo f{};
     bool any = false;
 #pragma unroll 1
     for (int s0 = 0; s0 < p.nseq; s0 += 32) {
-        const int s = s0 + lane;
-        const uint4 w = s >= p.nseq ? make_uint4(0, 0, 0, 0) : s < kPlanSeqs ? seqs[s] : seq_words(p, s);
-        const int2 in = rows_within(w, r0, r0 + n);
+        const int2 in = rows_within(p, seqs, s0 + lane, r0, r0 + n);
         any |= in.x < in.y;
         const unsigned whole = __ballot_sync(0xffffffffu, in.x == 0 && in.y == n);
         if (whole) {  // the item lies inside one sequence
-            const Seq q(p, shfl_words(w, __ffs(whole) - 1));
+            const Seq q = seq_at(p, seqs, s0 + __ffs(whole) - 1);
             const int see = q.see + (r0 - q.q0), n0 = min(p.T, n);
             const int2 a = own_range(see, q.ks, q.ke, p.window), b = own_range(see + n0 - 1, q.ks, q.ke, p.window);
             const int2 e = own_range(see + n - 1, q.ks, q.ke, p.window);
@@ -286,7 +295,7 @@ __device__ TileInfo plan_item(const PlanParams& p, const uint4* seqs, int2* rng,
             f.nblk = p.prefix_blocks + (e.y - a.x + kKeys - 1) / kKeys;
             f.simple = 1, f.see = see, f.ks = q.ks, f.ke = q.ke;
             f.pieces = 1;
-            if (lane == 0) p.segs[int64_t(t) * p.TI] = make_int2(a.x, e.y);
+            f.pos = a.x, f.end = e.y;
             return f;
         }
     }
@@ -296,13 +305,11 @@ __device__ TileInfo plan_item(const PlanParams& p, const uint4* seqs, int2* rng,
     __syncwarp();
 #pragma unroll 1
     for (int s0 = 0; s0 < p.nseq; s0 += 32) {
-        const int s = s0 + lane;
-        const uint4 w = s >= p.nseq ? make_uint4(0, 0, 0, 0) : s < kPlanSeqs ? seqs[s] : seq_words(p, s);
-        const int2 in = rows_within(w, r0, r0 + n);
+        const int2 in = rows_within(p, seqs, s0 + lane, r0, r0 + n);
         unsigned m = __ballot_sync(0xffffffffu, in.x < in.y);
         if (__popc(m) > 4) {  // many short ones: a lane each
             if (in.x < in.y) {
-                const Seq q(p, w);
+                const Seq q = seq_at(p, seqs, s0 + lane);
 #pragma unroll 1
                 for (int i = in.x; i < in.y; i++) rng[i] = own_range(q.see + (r0 + i - q.q0), q.ks, q.ke, p.window);
             }
@@ -311,7 +318,7 @@ __device__ TileInfo plan_item(const PlanParams& p, const uint4* seqs, int2* rng,
             while (m) {
                 const int src = __ffs(m) - 1;
                 m &= m - 1;
-                const Seq q(p, shfl_words(w, src));
+                const Seq q = seq_at(p, seqs, s0 + src);
                 const int x = __shfl_sync(0xffffffffu, in.x, src), y = __shfl_sync(0xffffffffu, in.y, src);
 #pragma unroll 1
                 for (int i = x + lane; i < y; i += 32) rng[i] = own_range(q.see + (r0 + i - q.q0), q.ks, q.ke, p.window);
@@ -349,6 +356,7 @@ __device__ TileInfo plan_item(const PlanParams& p, const uint4* seqs, int2* rng,
     }
 #pragma unroll 1
     for (int i = lane; i < n; i += 32) p.rng[r0 + i] = rng[i];
+    if (f.nseg > 0) f.pos = seg[0].x, f.end = seg[0].y;
     f.nblk = __reduce_add_sync(0xffffffffu, nblk) + p.prefix_blocks;
     f.pieces = 1;
     __syncwarp();
@@ -362,14 +370,19 @@ __global__ void __launch_bounds__(1024) k_causal_plan(PlanParams p) {
     __shared__ TileInfo s_info[kPlanItems];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int ctas = int(gridDim.x);
-    uint4* seqs = reinterpret_cast<uint4*>(plan_shared);
-    int2* rng = reinterpret_cast<int2*>(seqs + min(p.nseq, kPlanSeqs)) + warp * 2 * kMaxItemRows;
+    const int kept = min(p.nseq, kPlanSeqs), room = (kept + 3) / 4 * 4;
+    const Seqs seqs{reinterpret_cast<int4*>(plan_shared), reinterpret_cast<int*>(plan_shared + size_t(room) * sizeof(int4))};
+    int2* rng = reinterpret_cast<int2*>(seqs.see + room) + warp * 2 * kMaxItemRows;
     hist[tid] = 0;
     if (tid == 0) s_chunk = INT_MAX;
     pdl_wait();
     pdl_launch();
 #pragma unroll 1
-    for (int s = tid; s < min(p.nseq, kPlanSeqs); s += 1024) seqs[s] = seq_words(p, s);
+    for (int s = tid; s < kept; s += 1024) {
+        const Seq r = seq_of(p, s);
+        seqs.range[s] = make_int4(r.q0, r.q1, r.ks, r.ke);
+        seqs.see[s] = r.see;
+    }
     if (blockIdx.x == 0 && tid == 0) p.head->err = 0;
     __syncthreads();
     // A single CTA keeps the items' infos at hand; a cluster's come back through global memory.
@@ -386,8 +399,7 @@ __global__ void __launch_bounds__(1024) k_causal_plan(PlanParams p) {
     else __syncthreads();
     if (blockIdx.x != 0) return;
     const auto whole = [&](int t, const TileInfo& f) {
-        const int2 g = f.nseg > 0 ? p.segs[int64_t(t) * p.TI] : make_int2(0, 0);
-        return Work{t, 0, f.nblk, -1, 0, f.nseg, g.x, g.y, f.lo0, f.hi0, f.lo1, f.hi1, f.live | (f.simple << 2), f.see, f.ks, f.ke};
+        return Work{t, 0, f.nblk, -1, 0, f.nseg, f.pos, f.end, f.lo0, f.hi0, f.lo1, f.hi1, f.live | (f.simple << 2), f.see, f.ks, f.ke};
     };
     if (int64_t(p.tiles) * p.kv_heads > p.sms) {
         // Several rounds of the SMs: whole items, costliest first, by a counting sort over their blocks; the order
@@ -494,7 +506,7 @@ __global__ void __launch_bounds__(1024) k_causal_plan(PlanParams p) {
             int s = 0, first = p.prefix_blocks;  // segment s starts at block `first`
             int2 g = make_int2(0, 0);
             if (f.nseg > 0) {
-                g = seg[0];
+                g = make_int2(f.pos, f.end);
 #pragma unroll 1
                 for (; s + 1 < f.nseg; s++, g = seg[s]) {
                     const int m = (g.y - g.x + kKeys - 1) / kKeys;
