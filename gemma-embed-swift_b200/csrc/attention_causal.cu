@@ -15,8 +15,10 @@
 //                   rows see, and the list of work pieces.  A warp plans an item; one CTA up to 64 items, which
 //                   hand their results on through shared memory, else a cluster of 4 or 8.  Items that fill the
 //                   SMs more than once go costliest first (a counting sort); fewer are cut into pieces of their key
-//                   blocks that fill the SMs once, unless there are few keys.  Bound by latency: 6 us for 8
-//                   queries, 18 us for 64 documents, of which the kernel after it hides its own set-up.
+//                   blocks that fill the SMs once, unless there are few keys.  Bound by latency: 5 us for 8
+//                   queries, 10 us for 64 documents (300 items), 17 us for 50,000 tokens of one KV head of 256
+//                   (1240 items); sorting by all CTAs of the cluster won 2 us
+//                   at 1100 items and lost 1 at 300.
 //   k_causal_tc     persistent, one CTA per SM: walks the pieces in turn (below)
 //   k_causal_merge  only where tiles may be cut: joins the pieces' partial rows by their maxima and sums, a CTA per
 //                   row and head; bound by latency (8 to 11 us with its launch, cold).
