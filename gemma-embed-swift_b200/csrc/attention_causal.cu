@@ -17,11 +17,10 @@
 //                   SMs more than once go costliest first (a counting sort); fewer are cut into pieces of their key
 //                   blocks that fill the SMs once, unless there are few keys.  Bound by latency: 5 us for 8
 //                   queries, 10 us for 64 documents (300 items), 17 us for 50,000 tokens of one KV head of 256
-//                   (1240 items); sorting by all CTAs of the cluster won 2 us
-//                   at 1100 items and lost 1 at 300.
+//                   (1240 items); sorting by all CTAs of the cluster won 2 us at 1100 items and lost 1 at 300.
 //   k_causal_tc     persistent, one CTA per SM: walks the pieces in turn (below)
 //   k_causal_merge  only where tiles may be cut: joins the pieces' partial rows by their maxima and sums, a CTA per
-//                   row and head; bound by latency (8 to 11 us with its launch, cold).
+//                   row and head; bound by latency (5 to 7 us).
 // The result of a row depends only on its own ranges and, through the pieces, on the call's sizes:
 // which CTA takes a piece changes nothing.
 //
@@ -33,7 +32,7 @@
 // S_1(j), so that one tile's softmax runs under the other tile's products; head dim 256 has two S
 // buffers instead and runs S(j) ahead of PV(j - 1).  The running maximum of a row is moved (and its O
 // rescaled) only when it grows by more than 2^8; until then every term of the row shares the old one, so
-// the result is exact and P stays within 2^8.  P in 16 bits is the operand the product takes; sums are
+// the result is exact and P stays within 2^8 (2^15 as fp16 holds it, kRaise).  P in 16 bits is the operand the product takes; sums are
 // taken over the unrounded fp32 values.
 //   warp 0   TMA producer of Q and K      warp 1   MMA issuer
 //   warp 2   TMA producer of V            warp 3   owns tensor memory
@@ -90,7 +89,7 @@ Sizes sizes_of(const CausalLaunch& a) {
     // Pieces an item may be cut into: enough to fill the SMs twice (the plan fills them once), one where the items
     // do so already.
     const int64_t units = std::max<int64_t>(int64_t(s.tiles) * a.kv_heads, 1);
-    // Calls over few keys are not cut: a block costs about 2 us, the merge's launch and run 8.
+    // Calls over few keys are not cut: a block costs about 2 us, the merge's launch and run 6.
     s.lmax = units >= a.num_sms || int64_t(a.prefix) + a.nkv <= 4 * kKeys ? 1 : int(std::min<int64_t>(kMaxPieces, (2 * a.num_sms + units - 1) / units));
     return s;
 }
@@ -1310,12 +1309,13 @@ struct MergeParams {
     const float2* ml;
 };
 
-// One CTA of 256 threads per (row, head): out = sum_c 2^(m_c - m) O_c / sum_c 2^(m_c - m) l_c, m the
-// largest m_c.  Thread c weighs piece c; the warps add every eighth piece each, joined in order.  The
+// One CTA of W warps per (row, head): out = sum_c 2^(m_c - m) O_c / sum_c 2^(m_c - m) l_c, m the
+// largest m_c.  Thread c weighs piece c; the warps add every W-th piece each, joined in order.  The
 // loads that say whether and how many pieces there are go out together with the pieces' maxima.
-template <typename E, int D>
-__global__ void __launch_bounds__(256) k_causal_merge(MergeParams p) {
-    __shared__ float w[kMaxPieces], red_m[8], red_l[8], part[8][D];
+template <typename E, int D, int W>
+__global__ void __launch_bounds__(32 * W) k_causal_merge(MergeParams p) {
+    static_assert(32 * W >= kMaxPieces && 32 * W >= D / 2, "a thread per piece and per pair of columns");
+    __shared__ float w[kMaxPieces], red_m[W], red_l[W], part[W][D];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     pdl_wait();
     pdl_launch();
@@ -1335,7 +1335,7 @@ __global__ void __launch_bounds__(256) k_causal_merge(MergeParams p) {
     __syncthreads();
     m = red_m[0];
 #pragma unroll
-    for (int i = 1; i < 8; i++) m = fmaxf(m, red_m[i]);
+    for (int i = 1; i < W; i++) m = fmaxf(m, red_m[i]);
     const float wt = ml.x == -INFINITY ? 0.f : ex2_approx(ml.x - m);  // 0: no visible key, and no row was left
     if (tid < n) w[tid] = wt;
     const float l = warp_sum(wt * ml.y);
@@ -1346,7 +1346,7 @@ __global__ void __launch_bounds__(256) k_causal_merge(MergeParams p) {
 #pragma unroll
     for (int i = 0; i < P; i++) acc[i] = 0.f;
 #pragma unroll 4
-    for (int c = warp; c < n; c += 8) {
+    for (int c = warp; c < n; c += W) {
         const float wc = w[c];
         const float2* src = reinterpret_cast<const float2*>(p.o + (c * step + id) * D + lane * P);
 #pragma unroll
@@ -1362,7 +1362,7 @@ __global__ void __launch_bounds__(256) k_causal_merge(MergeParams p) {
     if (tid < D / 2) {
         float lt = 0.f, v[2] = {0.f, 0.f};
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
+        for (int i = 0; i < W; i++) {
             lt += red_l[i];
             v[0] += part[i][2 * tid];
             v[1] += part[i][2 * tid + 1];
@@ -1411,7 +1411,11 @@ cudaError_t launch_t(const CausalLaunch& a, const Sizes& s, const Layout& l, cud
                    mpk, mpv, mo, p);
     if (e != cudaSuccess || s.lmax == 1) return e;
     MergeParams mp{a.out, a.out_stride, a.heads, a.ntok, s.TI, s.lmax, l.rng, l.info, l.o, l.ml};
-    return launch_pdl(k_causal_merge<E, D>, unsigned(int64_t(a.ntok) * a.heads), 256, 0, stream, 1, mp);
+    // Eight warps a row where all rows are resident at once, else four, so that twice as many are (64 rows of 32
+    // heads, 18 pieces: 6.7 us with four, 8.8 with eight; 2 rows of 3 heads, 128 pieces: 7.7 and 4.9).
+    const int64_t rows = int64_t(a.ntok) * a.heads;
+    if (rows > 8 * a.num_sms) return launch_pdl(k_causal_merge<E, D, 4>, unsigned(rows), 128, 0, stream, 1, mp);
+    return launch_pdl(k_causal_merge<E, D, 8>, unsigned(rows), 256, 0, stream, 1, mp);
 }
 
 template <typename E>

@@ -237,6 +237,7 @@ class Q4Weight:
             _on_device(name, t, device)
             if t.dtype != torch.float16 or t.dim() != 2 or t.shape[0] != self.n or not t.is_contiguous():
                 raise _invalid(f"{name} must be a contiguous [{self.n}, k / group] float16 tensor")
+            _no_gradient(name, t)
         if self.mins is not None and self.mins.shape != self.scales.shape:
             raise _invalid(f"mins must have the shape of scales, {list(self.scales.shape)}")
         groups = self.scales.shape[1]
@@ -303,6 +304,7 @@ def linear_q4(x, weight: Q4Weight, out=None, stream=None):
             out = x.new_empty((rows, n))
     else:
         _on_device("out", out, device)
+        _no_gradient("out", out)
         if out.dtype != x.dtype or out.shape != (rows, n) or (n > 1 and out.stride(1) != 1):
             raise _invalid(f"out must be a [{rows}, {n}] {x.dtype} tensor with its columns side by side")
         if rows > 1:

@@ -651,3 +651,24 @@ def test_outputs_in_wider_rows(ge, torch, offset, extra):
     want, bound, _ = ref.attention(q, k, v, [(0, n)], [(0, n)], 0.125)
     ref.check(out, want, bound)
     assert (wide[:, :offset] == 7.0).all() and (wide[:, offset + heads * dim:] == 7.0).all()
+
+
+@pytest.mark.parametrize("heads,kvh", [(1, 1), (16, 1), (32, 1), (64, 1), (128, 1), (64, 2), (12, 2)])
+@pytest.mark.parametrize("gap", [0, 3])
+def test_causal_128_wide_outputs(ge, torch, heads, kvh, gap):
+    """Every way a warp's rows may lie in `out`: tokens with all their heads, parts of a token's heads, rows of
+    no sequence among them, a last tile that ends inside."""
+    check_causal(ge, torch, [40, 1, 130, 7], heads, kvh, 128, "bf16", gap=gap)
+
+
+def test_outputs_and_scales_that_require_a_gradient_are_refused(ge, torch):
+    w = q4(torch, ge, 8, 64, 32, True)
+    x = normal(torch, 1, (2, 64), "f16")
+    q, k, s = normal(torch, 1, (8, 4, 64), "f16"), normal(torch, 2, (8, 2, 64), "f16"), dev(torch, [(0, 8)])
+    grad = lambda t: t.detach().clone().requires_grad_()
+    for call in (lambda: ge.linear_q4(x, w, out=grad(normal(torch, 2, (2, 8), "f16"))),
+                 lambda: ge.Q4Weight(w.values, grad(w.scales), w.mins), lambda: ge.Q4Weight(w.values, w.scales, grad(w.mins)),
+                 lambda: ge.attention_causal(q, k, k, s, out=grad(q))):
+        with pytest.raises(ge.GemmaEmbedError) as e:
+            call()
+        assert e.value.case == "invalidOptions"
