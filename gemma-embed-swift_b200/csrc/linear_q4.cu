@@ -21,9 +21,10 @@
 // What bounds it now: neither memory (2 to 3.5 of 6.6 TB/s) nor one pipe (12 rows: 44 % of the issue slots, 48 % of
 // shared memory's, 23 % of the tensor products'), but a warp's dependent steps from a stage's arrival through widening,
 // products and scaling, at four warps to a scheduler; for many rows also the chunks of x, whose ends the warps wait for
-// together, and that 9 to 15 tiles leave some of 16 warps half idle.  A CTA takes as many of its tiles at once as it
-// has warps: fewer, with parts of k on more warps, were slower (16384 x 8192, 1 row: 7 tiles at once 21.4 us, 4 + 3
-// 24.7, one by one 34.5; 28671 x 8192, 12 rows: 13 at once 64, 7 + 6 67, 5 + 5 + 3 76).  Measured, weights from memory:
+// together.  A CTA takes as many of its tiles at once as it has warps: fewer, with parts of k on more warps, were slower
+// (16384 x 8192, 1 row: 7 tiles at once 21.4 us, 4 + 3 24.7, one by one 34.5; 28671 x 8192, 12 rows: 13 at once 64,
+// 7 + 6 67, 5 + 5 + 3 76), and sharing a chunk's stages of all tiles out evenly, up to two tiles a warp, won nothing
+// either (23.3 and 67).  Measured, weights from memory:
 //   16384 x 8192, groups of 32, 1 row, fp16              21.4 us, 3.5 TB/s
 //   28671 x 8192, groups of 128 with mins, 12 rows, bf16   64 us, 2.0 TB/s
 //   41003 x 4096, groups of 32, 4 rows, fp16               33 us, 2.9 TB/s
@@ -45,7 +46,8 @@ constexpr int kStageBytes = kWeightBytes + 2 * 16 * kScaleRow;  // weights, scal
 constexpr int kDepth = 3;
 constexpr int kXElems = 16384;                 // elements of x per buffer, all rows
 constexpr int kOffX = kWarps * kDepth * kStageBytes;
-constexpr int kXBytes = kXElems * 2 + kQ4MaxRows * 64;  // rows are 64 bytes over a multiple of 128 apart
+constexpr int kRows = 32;                      // of a launch
+constexpr int kXBytes = kXElems * 2 + kRows * 64;  // rows are 64 bytes over a multiple of 128 apart
 constexpr int kOffSum = kOffX + 2 * kXBytes;            // sums of x per group and row, 8 NB rows apart
 constexpr int kSumBytes = 4096;
 constexpr int kSmem = kOffSum + 2 * kSumBytes;
@@ -412,8 +414,18 @@ template <typename T>
 cudaError_t launch_e(const Q4Launch& a, cudaStream_t stream) {
     if (a.rows <= 8) return launch_m<T, 1>(a, stream);
     if (a.rows <= 16) return launch_m<T, 2>(a, stream);
-    if (a.rows <= 32) return launch_m<T, 4>(a, stream);
-    return launch_m<T, 8>(a, stream);
+    if (a.rows <= kRows) return launch_m<T, 4>(a, stream);
+    // More rows in two halves, each over all weights (the second from the L2 cache where they fit): sums of 64 rows
+    // spill, and their x leaves room for one stage at a time, which only one part of k works on (16384 x 4096, groups of
+    // 64 with mins, bf16, 64 rows: 115 us at once, 72 in halves; 33 rows of groups of 32: 78 and 45).
+    Q4Launch half = a;
+    half.rows = (a.rows + 1) / 2;
+    cudaError_t e = launch_e<T>(half, stream);
+    if (e != cudaSuccess) return e;
+    half.x = static_cast<const T*>(a.x) + half.rows * a.x_stride;
+    half.out = static_cast<T*>(a.out) + half.rows * a.out_stride;
+    half.rows = a.rows - half.rows;
+    return launch_e<T>(half, stream);
 }
 
 }  // namespace
