@@ -6,7 +6,8 @@
 // exact, for the warp's 16 x 8 x 16 tensor products with fp32 sums (a warp's product costs fewer
 // issue slots than one multiply-add per weight and row, and a 128-row tcgen05 tile would be empty
 // but for a few rows).  Every group's integer sums are scaled in fp32: acc += scale * sum, plus
-// min * (sum of x) with minima, so no weight is ever rounded.
+// min * (sum of x) with minima, so no weight is ever rounded; results that are not finite are summed again from the
+// definition (from_definition).
 //
 // One CTA per SM, 16 warps.  A warp owns 16 output columns n (a row tile) or, where the CTA has fewer
 // tiles than warps, a part of k of one; the parts' sums are joined in shared memory in order.
@@ -134,6 +135,55 @@ __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], 
             asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    }
+}
+
+// The sum of a warp's results that are not finite, again from the definition, in 64 bits: an infinite x times a
+// weight's two parts may be inf - inf, and the integer sums of bf16 values above 1e35 may pass fp32 where the scaled ones
+// do not.  Bit 4 b + i of `bad` is the lane's acc[b][i].  What is finite needs none of this: it had finite terms only.
+// Out of line, since next to no call takes it.  One infinity in one row of 12 of 28671 x 8192: 0.38 ms, without it 0.06;
+// in each of 64 rows of 16384 x 4096 6.3 and 0.07.  Rows full of NaN (padding never written) end at their first
+// elements: 64 of them 0.62 ms.
+template <typename T, int NB, bool kMins, int kPer>
+__device__ __noinline__ void from_definition(const Q4Params& p, int n0, uint32_t bad) {
+    constexpr int gshift = kPer == 1 ? 5 : kPer == 2 ? 6 : 7;
+    const int lane = threadIdx.x & 31;
+#pragma unroll 1
+    for (int bit = 0; bit < 4 * NB; bit++) {
+        unsigned lanes = __ballot_sync(0xffffffffu, (bad >> bit) & 1u);
+#pragma unroll 1
+        while (lanes) {
+            const int of = __ffs(lanes) - 1;
+            lanes &= lanes - 1;
+            const int n = n0 + (of >> 2) + ((bit >> 1) & 1) * 8, r = (bit >> 2) * 8 + 2 * (of & 3) + (bit & 1);
+            const T* x = static_cast<const T*>(p.x) + r * p.x_stride;
+            const uint8_t* values = p.values + int64_t(n) * (p.k >> 1);
+            const int64_t row = int64_t(n) * (p.k >> gshift);
+            double sum = 0.0;
+#pragma unroll 1
+            for (int e0 = 0; e0 < p.k; e0 += 256) {
+                const int e = e0 + lane * 8;
+                if (e < p.k) {
+                    const uint32_t q = *reinterpret_cast<const uint32_t*>(values + (e >> 1));
+                    const uint4 xv = *reinterpret_cast<const uint4*>(x + e);
+                    const uint32_t xw[4] = {xv.x, xv.y, xv.z, xv.w};
+                    const double scale = double(__half2float(p.scales[row + (e >> gshift)]));
+                    const double low = kMins ? double(__half2float(p.mins[row + (e >> gshift)])) : 0.0;
+#pragma unroll
+                    for (int j = 0; j < 8; j++) {
+                        const float2 f = pair_to_float<T>(xw[j >> 1]);
+                        const int v = int((q >> (4 * j)) & 15u);
+                        // The weight is exact: 4 bits times 11, 40 places apart from the minimum at most.
+                        const double w = kMins ? fma(scale, double(v), low) : scale * double(v - 8);
+                        sum = fma(double(j & 1 ? f.y : f.x), w, sum);
+                    }
+                }
+                if (__any_sync(0xffffffffu, isnan(sum))) break;  // so is the result: a row full of NaN ends here
+            }
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+            if (lane == of) static_cast<T*>(p.out)[r * p.out_stride + n] = T(sum);
+        }
     }
 }
 
@@ -368,13 +418,18 @@ __global__ void __launch_bounds__(kThreads, 1) k_linear_q4(const __grid_constant
         }
         if (works && part == 0) {
             T* out = static_cast<T*>(p.out);
+            uint32_t bad = 0;  // results that are not finite
 #pragma unroll
             for (int b = 0; b < NB; b++)
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
                     const int n = n0 + g + (i >> 1) * 8, r = b * 8 + 2 * c + (i & 1);
-                    if (n < p.n && r < p.rows) out[r * p.out_stride + n] = T(acc[b][i]);
+                    if (n < p.n && r < p.rows) {
+                        out[r * p.out_stride + n] = T(acc[b][i]);
+                        if (!isfinite(acc[b][i])) bad |= 1u << (4 * b + i);
+                    }
                 }
+            if (__any_sync(0xffffffffu, bad != 0)) from_definition<T, NB, kMins, kPer>(p, n0, bad);
         }
         __syncthreads();  // the next tiles' copies and x reuse the memory read above
     }

@@ -1,0 +1,116 @@
+"""The operators on device tensors at the edges of what their calls allow, on a B200: infinities and sums past
+the types, and what a caller relies on around a call."""
+import math
+
+import numpy as np
+import pytest
+
+import operator_reference as ref
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def torch(cuda_device):
+    import torch
+    return torch
+
+
+def dt(torch, name):
+    return {"f16": torch.float16, "bf16": torch.bfloat16}[name]
+
+
+def normal(torch, seed, shape, dtype, scale=1.0):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    return (torch.randn(shape, generator=g, device="cuda") * scale).to(dt(torch, dtype))
+
+
+def dev(torch, r):
+    return torch.tensor(r, dtype=torch.int32, device="cuda").reshape(-1, 2)
+
+
+# ---------------------------------------------------------------------------- 4-bit products
+def q4(torch, ge, n, k, group, mins, seed=1, step=0.02):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    values = torch.randint(0, 256, (n, k // 2), generator=g, device="cuda", dtype=torch.uint8)
+    scales = (torch.rand((n, k // group), generator=g, device="cuda") * step + step / 20).half()
+    lows = (torch.randn((n, k // group), generator=g, device="cuda") * 2.5 * step).half() if mins else None
+    return ge.Q4Weight(values, scales, lows)
+
+
+def dense(torch, w):
+    """The weights in float64, which holds them exactly."""
+    q = torch.stack([w.values & 15, w.values >> 4], -1).flatten(1).double()
+    s = w.scales.double().repeat_interleave(w.group, 1)
+    return (q - 8) * s if w.mins is None else q * s + w.mins.double().repeat_interleave(w.group, 1)
+
+
+def by_terms(torch, x, w):
+    """x w^T from the definition, each sum over its terms as they are: infinities and NaN as IEEE has them."""
+    return torch.stack([(row.double()[None] * dense(torch, w)).sum(1) for row in x])
+
+
+def check_same(torch, got, want, bound):
+    """Finite where `want` is and within bound, else the same infinity or NaN."""
+    want_t = want.to(got.dtype).double()  # what passes the type's largest number is its infinity
+    finite = torch.isfinite(want_t)
+    assert torch.equal(torch.isnan(got), torch.isnan(want_t))
+    inf = torch.isinf(want_t)
+    assert torch.equal(got[inf].double(), want_t[inf])
+    assert torch.isfinite(got[finite]).all()
+    assert ((got.double() - want).abs()[finite] <= bound[finite]).all()
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("mins", [False, True])
+@pytest.mark.parametrize("group,k,n,rows", [(32, 96, 5, 1), (64, 512, 300, 5), (128, 1152, 37, 12), (32, 4096, 2500, 20), (64, 320, 130, 40)])
+def test_linear_q4_infinite_inputs(ge, torch, dtype, mins, group, k, n, rows):
+    """Rows with an infinity give what the definition gives -- an infinity of the weight's sign, NaN where the
+    weight is 0 -- and leave the other rows alone bit for bit."""
+    w = q4(torch, ge, n, k, group, mins)
+    x = normal(torch, 3, (rows, k), dtype)
+    clean = ge.linear_q4(x, w)
+    hit = sorted({0, rows // 2, rows - 1})
+    for i, r in enumerate(hit):
+        x[r, (k - 1, 7, k // 2)[i]] = (math.inf, -math.inf, math.inf)[i]
+    got = ge.linear_q4(x, w)
+    check_same(torch, got[hit], by_terms(torch, x[hit], w), torch.zeros((len(hit), n), device="cuda"))
+    rest = [r for r in range(rows) if r not in hit]
+    assert torch.equal(got[rest], clean[rest])
+
+
+@pytest.mark.parametrize("mins", [False, True])
+def test_linear_q4_two_infinities_and_nan(ge, torch, mins):
+    w = q4(torch, ge, 77, 256, 32, mins)
+    x = normal(torch, 4, (3, 256), "f16")
+    x[0, 3], x[0, 200] = math.inf, -math.inf
+    x[1, 9] = math.nan
+    check_same(torch, ge.linear_q4(x, w), by_terms(torch, x, w), ref.linear_q4(x.nan_to_num(0, 0, 0), w.values, w.scales, w.mins)[1])
+
+
+@pytest.mark.parametrize("mins", [False, True])
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("rows,n,k", [(1, 33, 128), (12, 300, 640), (40, 50, 2048)])
+def test_linear_q4_sums_past_32_bits(ge, torch, mins, group, rows, n, k):
+    """bf16 values near the type's largest: sums of x times the 4-bit integers pass fp32, the scaled ones do not."""
+    w = q4(torch, ge, n, k, group, mins, step=1e-4)
+    x = (torch.sign(normal(torch, 5, (rows, k), "bf16").float()) * 2e38).bfloat16()
+    x[0] = 2e38
+    want = by_terms(torch, x, w)
+    bound = ref.linear_q4(x, w.values, w.scales, w.mins)[1]
+    check_same(torch, ge.linear_q4(x, w), want, bound)
+
+
+def test_linear_q4_infinite_scales(ge, torch):
+    """A scale or minimum of infinity meets every weight of its group."""
+    w = q4(torch, ge, 20, 256, 32, True)
+    w.scales[3, 2] = math.inf
+    w.mins[5, 0] = -math.inf
+    w.scales[7, 7] = math.nan
+    x = normal(torch, 6, (2, 256), "f16")
+    keep = [i for i in range(20) if i not in (3, 5, 7)]
+    got = ge.linear_q4(x, w)
+    want = by_terms(torch, x, w)
+    bound = ref.linear_q4(x, w.values, w.scales.nan_to_num(0, 0, 0), w.mins.nan_to_num(0, 0, 0))[1]
+    check_same(torch, got, want, bound)
+    assert torch.isfinite(got[:, keep]).all()
