@@ -732,6 +732,10 @@ __host__ __device__ constexpr uint32_t idesc_of<__nv_bfloat16>(int M, int N, int
     return idesc_f16(M, N, 0, b_mn) | (1u << 7) | (1u << 10);  // A and B: bf16
 }
 
+// 1 / l for a row's sum l.  A finite score leaves a sum of 2^-8 and more, so l = 0 is a row that sees no key, whose
+// result is 0, or keys whose scores are all -infinity, a softmax of 0 / 0.
+__device__ __forceinline__ float inverse_sum(float l, bool sees) { return l != 0.f ? 1.0f / l : sees ? NAN : 0.f; }
+
 // One row of piece `id` from the definition, by a whole warp; stored like the epilogue does.  It reads the
 // piece again: one handed over would live in memory for all of the callers' work.
 template <typename E, int D>
@@ -751,7 +755,7 @@ __device__ __forceinline__ void exact_row(const TcParams& p, int id, int row, in
                        p.scale_log2e, lane);
     }
     if (s.piece < 0) {
-        const float inv = st.l == 0.f ? 0.f : 1.0f / st.l;
+        const float inv = inverse_sum(st.l, p.prefix > 0 || rg.y > rg.x);
         uint32_t* o = reinterpret_cast<uint32_t*>(static_cast<E*>(p.out) + row * p.out_stride + int64_t(head) * D + lane * (D / 32));
 #pragma unroll
         for (int i = 0; i < D / 64; i++) o[i] = float_to_pair<E>(st.o[2 * i] * inv, st.o[2 * i + 1] * inv);
@@ -1205,7 +1209,7 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1)
             range = range_of();  // of the next piece
             const int head = s.kvh * p.group + (r - token * p.group);
             const int64_t at = (int64_t(s.piece) * p.ntok + row) * p.heads + head;  // of a partial row
-            const float inv = s.piece >= 0 ? 1.0f : l == 0.f ? 0.f : 1.0f / l;
+            const float inv = s.piece >= 0 ? 1.0f : inverse_sum(l, p.prefix > 0 || rg.y > rg.x);
             if (in && s.piece >= 0) p.ml[at] = make_float2(m - kRaise<E>, l);
             bool bad = false;
             // Whole rows of head dim 128 leave as boxes through shared memory, where all of the warp's belong to a sequence:
@@ -1302,7 +1306,7 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1)
 struct MergeParams {
     void* out;
     int64_t out_stride;
-    int heads, ntok, TI, lmax;
+    int heads, ntok, TI, lmax, prefix, window;
     const int2* rng;
     const TileInfo* info;
     const float* o;
@@ -1367,7 +1371,12 @@ __global__ void __launch_bounds__(32 * W) k_causal_merge(MergeParams p) {
             v[0] += part[i][2 * tid];
             v[1] += part[i][2 * tid + 1];
         }
-        const float inv = nan ? NAN : lt == 0.f ? 0.f : 1.0f / lt;
+        bool sees = p.prefix > 0;
+        if (lt == 0.f && !sees) {
+            const int2 own = simple ? own_range(f->see + (row - row / p.TI * p.TI), f->ks, f->ke, p.window) : rng;
+            sees = own.y > own.x;
+        }
+        const float inv = nan ? NAN : inverse_sum(lt, sees);
         reinterpret_cast<uint32_t*>(static_cast<E*>(p.out) + row * p.out_stride + int64_t(head) * D)[tid] =
             float_to_pair<E>(v[0] * inv, v[1] * inv);
     }
@@ -1410,7 +1419,7 @@ cudaError_t launch_t(const CausalLaunch& a, const Sizes& s, const Layout& l, cud
     e = launch_pdl(k_causal_tc<E, D>, unsigned(std::min<int64_t>(a.num_sms, most)), C::kThreads, size_t(C::kSmem), stream, 1, mq, mk, mv,
                    mpk, mpv, mo, p);
     if (e != cudaSuccess || s.lmax == 1) return e;
-    MergeParams mp{a.out, a.out_stride, a.heads, a.ntok, s.TI, s.lmax, l.rng, l.info, l.o, l.ml};
+    MergeParams mp{a.out, a.out_stride, a.heads, a.ntok, s.TI, s.lmax, a.prefix, p.window, l.rng, l.info, l.o, l.ml};
     // Eight warps a row where all rows are resident at once, else four, so that twice as many are (64 rows of 32
     // heads, 18 pieces: 6.7 us with four, 8.8 with eight; 2 rows of 3 heads, 128 pieces: 7.7 and 4.9).
     const int64_t rows = int64_t(a.ntok) * a.heads;

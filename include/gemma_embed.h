@@ -534,7 +534,8 @@ GE_API int ge_attention_causal(int32_t device_ordinal, const ge_attention_shape*
  * d_kv_seqs[s] = (start, m) of k and v (nkv rows); the queries stand at the end, so query i sees the
  * own keys j <= m - n + i (none where that is negative).  n = 1 is the step of a single token.
  * Key ranges may be shared, in any order.  A row that sees no
- * key at all gives zeros.  Otherwise as ge_attention_causal; a window is refused. */
+ * key at all gives zeros; one whose keys all score -infinity gives NaN (0 / 0), in either call.  Otherwise as
+ * ge_attention_causal; a window is refused. */
 GE_API int ge_attention_prefix(int32_t device_ordinal, const ge_attention_shape* shape, const void* d_q, int32_t ntok,
                                const void* d_k, const void* d_v, int32_t nkv, const void* d_prefix_k,
                                const void* d_prefix_v, int32_t prefix_len, const uint32_t* d_q_seqs,

@@ -114,3 +114,58 @@ def test_linear_q4_infinite_scales(ge, torch):
     bound = ref.linear_q4(x, w.values, w.scales.nan_to_num(0, 0, 0), w.mins.nan_to_num(0, 0, 0))[1]
     check_same(torch, got, want, bound)
     assert torch.isfinite(got[:, keep]).all()
+
+
+# ---------------------------------------------------------------------------- attention
+@pytest.mark.parametrize("heads,kvh,dim", [(4, 1, 128), (2, 2, 64), (3, 1, 256), (6, 2, 128)])
+def test_scores_of_minus_infinity_alone(ge, torch, heads, kvh, dim):
+    """A row all of whose keys score -infinity is 0 / 0; with one finite score it is that key's value, and a row
+    that sees no key stays 0."""
+    n, dead = 300, 170
+    q, k, v = (normal(torch, 70 + i, (n, h, dim), "f16") for i, h in enumerate((heads, kvh, kvh)))
+    q[..., 0] = 1.0
+    k[:dead, :, 0] = -math.inf
+    k[dead + 1:, :, 0] = -math.inf
+    got = ge.attention_causal(q, k, v, dev(torch, [(0, n)]))
+    assert torch.isnan(got[:dead]).all()
+    assert torch.equal(got[dead:], v[dead].repeat_interleave(heads // kvh, 0)[None].expand(n - dead, -1, -1))
+    # Short sequences, whose rows share a tile.
+    r = [(0, 40), (dead - 20, 21), (200, 9)]
+    out = ge.attention_causal(q, k, v, dev(torch, r), out=torch.full_like(q, 7.0))
+    assert torch.isnan(out[:40]).all() and torch.isnan(out[dead - 20:dead]).all() and torch.isnan(out[200:209]).all()
+    assert torch.equal(out[dead], v[dead].repeat_interleave(heads // kvh, 0))
+    assert (out[40:dead - 20] == 7.0).all() and (out[dead + 1:200] == 7.0).all() and (out[209:] == 7.0).all()
+
+
+@pytest.mark.parametrize("heads,kvh,dim", [(4, 1, 128), (2, 2, 64), (3, 1, 256)])
+@pytest.mark.parametrize("plen,own", [(2000, 700), (2000, 0), (0, 900), (5, 3)])
+def test_scores_of_minus_infinity_alone_across_pieces(ge, torch, heads, kvh, dim, plen, own):
+    """The same where the keys are split: single tokens behind a prefix, one of them without keys of its own."""
+    q, k, v = (normal(torch, 80 + i, (r, h, dim), "f16") for i, (r, h) in enumerate(((3, heads), (own, kvh), (own, kvh))))
+    pk, pv = normal(torch, 84, (plen, kvh, dim), "f16"), normal(torch, 85, (plen, kvh, dim), "f16")
+    q[..., 0] = 1.0
+    k[..., 0] = pk[..., 0] = -math.inf
+    qr, kr = [(0, 1), (1, 1), (2, 1)], [(0, own), (0, own // 2), (0, 0)]
+    call = lambda: ge.attention_prefix(q, k, v, dev(torch, qr), dev(torch, kr), pk, pv)
+    got = call()
+    sees = [plen + m > 0 for _, m in kr]
+    for i, s in enumerate(sees):
+        assert torch.isnan(got[i]).all() if s else (got[i] == 0).all()
+    if plen:
+        pk[plen // 3, :, 0] = 0.0
+        assert torch.equal(call(), pv[plen // 3].repeat_interleave(heads // kvh, 0)[None].expand(3, -1, -1))
+
+
+@pytest.mark.parametrize("window", [0, 700])
+@pytest.mark.parametrize("heads,kvh,dim", [(1, 1, 128), (3, 1, 256), (1, 1, 64)])
+def test_scores_of_minus_infinity_alone_in_a_cut_prompt(ge, torch, heads, kvh, dim, window):
+    """One long prompt, whose few items are cut along the keys."""
+    n = 2500
+    q, k, v = (normal(torch, 90 + i, (n, h, dim), "bf16") for i, h in enumerate((heads, kvh, kvh)))
+    q[..., 0] = 1.0
+    k[..., 0] = -math.inf
+    k[1000, :, 0] = 0.0
+    got = ge.attention_causal(q, k, v, dev(torch, [(0, n)]), window=window)
+    end = 1000 + window if window else n
+    assert torch.isnan(got[:1000]).all() and torch.isnan(got[end:]).all()
+    assert torch.equal(got[1000:end], v[1000].repeat_interleave(heads // kvh, 0)[None].expand(end - 1000, -1, -1))
