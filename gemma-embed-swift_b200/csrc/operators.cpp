@@ -72,7 +72,9 @@ int check_shape(const ge_attention_shape* s, bool prefix) {
     if (s->heads < 1 || s->kv_heads < 1 || s->heads > 65535 || s->heads % s->kv_heads)
         return invalid("heads must be a multiple of kv_heads, both from 1 to 65535");
     if (s->heads / s->kv_heads > 128) return invalid("at most 128 heads may share a KV head");
-    if (!(s->scale > 0.0f) || !std::isfinite(s->scale)) return invalid("scale must be positive and finite");
+    // The kernels take scores times scale log2 e, which has to be finite itself (0 times it is the score of a zero query).
+    if (!(s->scale > 0.0f) || !std::isfinite(s->scale * 1.4426950408889634f))
+        return invalid("scale must be positive, and finite times log2 e");
     if (s->window < 0) return invalid("window must not be negative");
     if (prefix && s->window > 0) return invalid("a window does not go with a shared prefix");
     return GE_OK;

@@ -500,7 +500,7 @@ typedef struct ge_attention_shape {
     int32_t heads;     /* query heads, a multiple of kv_heads (at most 128 times) */
     int32_t kv_heads;
     int32_t head_dim;  /* 64, 128 or 256 */
-    float scale;       /* of q . k, positive and finite */
+    float scale;       /* of q . k, positive; scale * log2(e) finite */
     int32_t window;    /* ge_attention_causal: keys a query sees, itself included; 0: all before it */
     /* Elements between rows, multiples of 8; every tensor starts on a 16-byte boundary. */
     int64_t q_stride, k_stride, v_stride, prefix_k_stride, prefix_v_stride, out_stride;

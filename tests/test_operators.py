@@ -159,3 +159,11 @@ def test_python_wrappers_refuse_host_tensors(ge):
     with pytest.raises(ge.GemmaEmbedError) as e:
         ge.Q4Weight.from_blocks(b"\0" * 17, "Q4_0", 1, 32)
     assert e.value.case == "invalidOptions"
+
+
+@pytest.mark.parametrize("scale", [2.4e38, 3.4e38])
+def test_attention_refuses_scales_past_the_kernels_units(lib, scale):
+    """A finite scale whose product with log2 e is not: a zero query's scores would be 0 x infinity."""
+    for call in (causal, prefix):
+        rc, msg = call(lib, shape(lib, scale=scale))
+        assert rc == 9 and "scale" in msg
