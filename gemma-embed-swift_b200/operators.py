@@ -29,6 +29,9 @@ from . import _lib
 __all__ = ["attention_causal", "attention_prefix", "linear_q4", "Q4Weight"]
 
 _HERE = contextlib.nullcontext()
+# What the entry points take, checked here where a larger number would reach them as its lowest 32 bits.
+MAX_ROWS, MAX_HEADS, MAX_SEQUENCES, MAX_WINDOW = 1 << 30, 65535, (1 << 31) - 1, (1 << 31) - 1
+Q4_MAX_ROWS, Q4_MAX_N, Q4_MAX_K = 64, 1 << 30, 65536
 Q4_TYPES = {"Q4_0": 2, "Q4_1": 3}  # GGUF tensor type ids (ge_q4_type)
 
 
@@ -87,6 +90,8 @@ def _heads(name: str, t, device: int, dtype, heads: Optional[int], dim: int):
         want = f"[rows, {heads if heads is not None else 'heads'}, {dim}]"
         raise _invalid(f"{name} must be {want}, got {list(shape)}")
     rows, n, _ = shape
+    if rows > MAX_ROWS or n > MAX_HEADS:
+        raise _invalid(f"{name} must have at most 2^30 rows and {MAX_HEADS} heads, got {list(shape)}")
     s0, s1, s2 = t.stride()
     if (dim > 1 and s2 != 1) or (n > 1 and s1 != dim):
         raise _invalid(f"{name}'s heads must lie side by side in a row (strides {t.stride()})")
@@ -98,6 +103,8 @@ def _ranges(name: str, t, device: int) -> int:
     _on_device(name, t, device)
     if t.dtype not in (torch.int32, torch.uint32) or t.dim() != 2 or t.shape[1] != 2 or not t.is_contiguous():
         raise _invalid(f"{name} must be a contiguous [sequences, 2] int32 tensor of (start, length)")
+    if t.shape[0] > MAX_SEQUENCES:
+        raise _invalid(f"{name} names {t.shape[0]} sequences, past 2^31 - 1")
     return t.shape[0]
 
 
@@ -167,7 +174,9 @@ def _attention(q, k, v, prefix_k, prefix_v, q_seqs, kv_seqs, scale, window, out,
         if _ranges("kv_seqs", kv_seqs, device) != nseq:
             raise _invalid(f"q_seqs names {nseq} sequences, kv_seqs {kv_seqs.shape[0]}")
     scale = 1.0 / math.sqrt(dim) if scale is None else float(scale)
-    window = int(window)
+    window = min(int(window), MAX_WINDOW)  # no range is longer
+    if window < 0:
+        raise _invalid("window must not be negative")
     handle, side = _stream(stream, device)
     nbytes = _workspace_bytes(device, code, heads, kv_heads, dim, scale, window, ntok, prefix)
     with _on(side):
@@ -293,6 +302,8 @@ def linear_q4(x, weight: Q4Weight, out=None, stream=None):
     if len(shape) != 2 or shape[1] != k:
         raise _invalid(f"x must be [rows, {k}], got {list(shape)}")
     rows = shape[0]
+    if rows > Q4_MAX_ROWS or n > Q4_MAX_N or k > Q4_MAX_K:
+        raise _invalid(f"linear_q4 takes up to {Q4_MAX_ROWS} rows, n up to 2^30 and k up to {Q4_MAX_K}; got {rows} rows, n {n}, k {k}")
     x_stride, step = x.stride()
     if step != 1:
         raise _invalid("x's columns must lie side by side")

@@ -167,3 +167,74 @@ def test_attention_refuses_scales_past_the_kernels_units(lib, scale):
     for call in (causal, prefix):
         rc, msg = call(lib, shape(lib, scale=scale))
         assert rc == 9 and "scale" in msg
+
+
+class Recorder:
+    """In place of the library: notes the calls, and answers that all is well."""
+
+    def __init__(self):
+        self.calls = []
+
+    def __getattr__(self, name):
+        def call(*a):
+            self.calls.append((name, a))
+            return 0
+        return call
+
+
+@pytest.fixture()
+def hostside(ge, monkeypatch):
+    """The wrappers up to the library's call, with tensors of any device taken for CUDA tensors."""
+    ops = importlib.import_module("gemma-embed-swift_b200.operators")
+    rec = Recorder()
+    monkeypatch.setattr(ops, "_on_device", lambda name, t, device=None: 0)
+    monkeypatch.setattr(ops, "_stream", lambda stream, device: (0, None))
+    monkeypatch.setattr(ops, "_workspace_bytes", lambda *a: 256)
+    monkeypatch.setattr(ops._lib, "lib", lambda: rec)
+    return ops, rec
+
+
+def meta(*shape, dtype="float16"):
+    """A tensor of any size without memory."""
+    import torch
+    return torch.empty(shape, dtype=getattr(torch, dtype), device="meta")
+
+
+@pytest.mark.parametrize("window,handed", [(0, 0), (5, 5), (2**31 - 1, 2**31 - 1), (2**31, 2**31 - 1), (2**32, 2**31 - 1),
+                                           (2**32 + 1, 2**31 - 1), (2**70, 2**31 - 1), (-1, None), (-2**32, None), (-2**32 + 7, None)])
+def test_windows_past_32_bits(hostside, ge, window, handed):
+    """A window longer than any range is no window; nothing wraps to a small one."""
+    import torch
+    ops, rec = hostside
+    q, s = torch.zeros(4, 2, 64, dtype=torch.float16), torch.zeros(1, 2, dtype=torch.int32)
+    if handed is None:
+        with pytest.raises(ge.GemmaEmbedError) as e:
+            ops.attention_causal(q, q, q, s, window=window)
+        assert e.value.case == "invalidOptions" and not rec.calls
+    else:
+        ops.attention_causal(q, q, q, s, window=window)
+        (name, a), = rec.calls
+        assert name == "ge_attention_causal" and a[1].window == handed
+
+
+def test_counts_past_32_bits_are_refused(hostside, ge):
+    """Row, head and sequence counts and weight sizes whose lowest 32 bits would pass for others."""
+    ops, rec = hostside
+    big = 1 << 32
+    q, k, s = meta(8, 4, 64), meta(8, 2, 64), meta(1, 2, dtype="int32")
+    w = lambda n, k: ops.Q4Weight(meta(n, k // 2, dtype="uint8"), meta(n, k // 32))
+    bad = [lambda: ops.attention_causal(meta(big + 8, 4, 64), meta(big + 8, 2, 64), meta(big + 8, 2, 64), s),
+           lambda: ops.attention_causal(meta(0, big + 4, 64), meta(0, 2, 64), meta(0, 2, 64), s),
+           lambda: ops.attention_causal(q, k, k, meta(big, 2, dtype="int32")),
+           lambda: ops.attention_causal(q, k, k, meta(big + 1, 2, dtype="int32")),
+           lambda: ops.attention_prefix(q, meta(big, 2, 64), meta(big, 2, 64), s, s, k, k),
+           lambda: ops.attention_prefix(q, k, k, s, s, meta(big, 2, 64), meta(big, 2, 64)),
+           lambda: ops.linear_q4(meta(big, 64), w(8, 64)),
+           lambda: ops.linear_q4(meta(1, 64).expand(big + 2, 64), w(8, 64)),
+           lambda: ops.linear_q4(meta(65, 64), w(8, 64)),
+           lambda: ops.linear_q4(meta(2, 64), w(big + 8, 64)),
+           lambda: ops.linear_q4(meta(2, big + 64), w(8, big + 64))]
+    for i, call in enumerate(bad):
+        with pytest.raises(ge.GemmaEmbedError) as e:
+            call()
+        assert e.value.case == "invalidOptions" and not rec.calls, i
