@@ -6,8 +6,8 @@ ge_attention_prefix and ge_linear_q4 of include/gemma_embed.h).  Every call enqu
 `stream` -- a torch stream, a raw cudaStream_t, or None for torch's current stream of the
 tensors' device -- and returns without synchronising; it may be captured into a CUDA graph.  A stream
 other than the current one has to be behind the work that fills the inputs; their memory is not reused
-before the call's work there has ended.  There is no backward pass: inputs that require a gradient are
-refused while gradients are recorded.
+before the call's work there has ended.  There is no derivative: inputs that require a gradient are
+refused while gradients are recorded, dual tensors of forward-mode differentiation always.
 
     out = attention_causal(q, k, v, seqs)               # q [T, H, D], k and v [T, KV, D]
     last = attention_prefix(q, k, v, q_seqs, kv_seqs, prefix_k, prefix_v)
@@ -57,6 +57,12 @@ def _torch():
     return torch, {torch.float16: 0, torch.bfloat16: 1}, raw
 
 
+@functools.cache
+def _forward_ad():
+    from torch.autograd import forward_ad
+    return forward_ad
+
+
 def _dtype(t) -> int:
     code = _torch()[1].get(t.dtype)
     if code is None:
@@ -77,6 +83,10 @@ def _on_device(name: str, t, device: Optional[int] = None) -> int:
 def _no_gradient(name: str, t):
     if t.requires_grad and _torch()[0].is_grad_enabled():
         raise _invalid(f"{name} requires a gradient, and the operator has no backward pass (call it under torch.no_grad())")
+    # Inside a forward-mode level (a dual tensor's tangent is not seen from outside).
+    forward = _forward_ad()
+    if forward._current_level >= 0 and forward.unpack_dual(t).tangent is not None:
+        raise _invalid(f"{name} carries a forward-mode tangent, and the operator has no derivative")
 
 
 def _heads(name: str, t, device: int, dtype, heads: Optional[int], dim: int):

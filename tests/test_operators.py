@@ -187,7 +187,7 @@ def hostside(ge, monkeypatch):
     """The wrappers up to the library's call, with tensors of any device taken for CUDA tensors."""
     ops = importlib.import_module("gemma-embed-swift_b200.operators")
     rec = Recorder()
-    monkeypatch.setattr(ops, "_on_device", lambda name, t, device=None: 0)
+    monkeypatch.setattr(ops, "_on_device", lambda name, t, device=None: t.get_device())
     monkeypatch.setattr(ops, "_stream", lambda stream, device: (0, None))
     monkeypatch.setattr(ops, "_workspace_bytes", lambda *a: 256)
     monkeypatch.setattr(ops._lib, "lib", lambda: rec)
@@ -238,3 +238,29 @@ def test_counts_past_32_bits_are_refused(hostside, ge):
         with pytest.raises(ge.GemmaEmbedError) as e:
             call()
         assert e.value.case == "invalidOptions" and not rec.calls, i
+
+
+def test_dual_tensors_are_refused(hostside, ge):
+    """Forward-mode differentiation: a tangent would be dropped without a word."""
+    import torch
+    import torch.autograd.forward_ad as forward
+    ops, rec = hostside
+    q, k, s = torch.zeros(4, 2, 64).half(), torch.zeros(4, 1, 64).half(), torch.zeros(1, 2, dtype=torch.int32)
+    x, o = torch.zeros(2, 64).half(), torch.zeros(2, 8).half()
+    w = ops.Q4Weight(torch.zeros(8, 32, dtype=torch.uint8), torch.zeros(8, 2).half())
+    with forward.dual_level():
+        d = lambda t: forward.make_dual(t, torch.ones_like(t))
+        bad = [lambda: ops.attention_causal(d(q), k, k, s), lambda: ops.attention_causal(q, d(k), k, s),
+               lambda: ops.attention_causal(q, k, d(k), s), lambda: ops.attention_causal(q, k, k, s, out=d(q)),
+               lambda: ops.attention_prefix(q, k, k, s, s, d(k), k), lambda: ops.attention_prefix(q, k, k, s, s, k, d(k)),
+               lambda: ops.linear_q4(d(x), w), lambda: ops.linear_q4(x, w, out=d(o)),
+               lambda: ops.Q4Weight(w.values, d(w.scales)), lambda: ops.Q4Weight(w.values, w.scales, d(w.scales))]
+        for i, call in enumerate(bad):
+            for context in (torch.enable_grad, torch.no_grad):
+                with context(), pytest.raises(ge.GemmaEmbedError) as e:
+                    call()
+                assert e.value.case == "invalidOptions" and "tangent" in str(e.value), i
+        assert not rec.calls
+        ops.attention_causal(q, k, k, s)  # others pass inside a level too
+        ops.linear_q4(x, w)
+    assert [name for name, _ in rec.calls] == ["ge_attention_causal", "ge_linear_q4"]
