@@ -318,6 +318,10 @@ def linear_q4(x, weight: Q4Weight, out=None, stream=None):
     if step != 1:
         raise _invalid("x's columns must lie side by side")
     _no_gradient("x", x)
+    if weight.scales.requires_grad or (mins is not None and mins.requires_grad):  # since the weight was made
+        for name, t in (("scales", weight.scales), ("mins", mins)):
+            if t is not None:
+                _no_gradient(name, t)
     handle, side = _stream(stream, device)
     out_stride = n
     if out is None:

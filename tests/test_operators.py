@@ -264,3 +264,23 @@ def test_dual_tensors_are_refused(hostside, ge):
         ops.attention_causal(q, k, k, s)  # others pass inside a level too
         ops.linear_q4(x, w)
     assert [name for name, _ in rec.calls] == ["ge_attention_causal", "ge_linear_q4"]
+
+
+def test_scales_that_require_a_gradient_by_the_call_are_refused(hostside, ge):
+    """A weight made while no gradients are recorded, or whose scales came to require one afterwards."""
+    import torch
+    ops, rec = hostside
+    x = torch.zeros(2, 64).half()
+    values, scales = torch.zeros(8, 32, dtype=torch.uint8), lambda: torch.zeros(8, 2).half()
+    with torch.no_grad():
+        first = ops.Q4Weight(values, scales().requires_grad_())
+    later = ops.Q4Weight(values, scales(), scales())
+    later.mins.requires_grad_()
+    for w in (first, later):
+        with pytest.raises(ge.GemmaEmbedError) as e:
+            ops.linear_q4(x, w)
+        assert e.value.case == "invalidOptions" and "gradient" in str(e.value) and not rec.calls
+    with torch.no_grad():
+        ops.linear_q4(x, first)
+        ops.linear_q4(x, later)
+    assert len(rec.calls) == 2
