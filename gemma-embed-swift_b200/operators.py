@@ -149,6 +149,11 @@ def _in_use(s, *tensors):
                 t.record_stream(s)
 
 
+def _written(out):
+    """Tells autograd that a caller's tensor changed: the kernels write through its pointer."""
+    _torch()[0].autograd.graph.increment_version(out)
+
+
 @functools.lru_cache(maxsize=1024)
 def _workspace_bytes(device: int, dtype: int, heads: int, kv_heads: int, dim: int, scale: float, window: int, ntok: int,
                      prefix: int) -> int:
@@ -189,8 +194,9 @@ def _attention(q, k, v, prefix_k, prefix_v, q_seqs, kv_seqs, scale, window, out,
         raise _invalid("window must not be negative")
     handle, side = _stream(stream, device)
     nbytes = _workspace_bytes(device, code, heads, kv_heads, dim, scale, window, ntok, prefix)
+    given = out is not None
     with _on(side):
-        if out is None:
+        if not given:
             out = q.new_empty((ntok, heads, dim))
             out_stride = heads * dim
         else:
@@ -209,6 +215,8 @@ def _attention(q, k, v, prefix_k, prefix_v, q_seqs, kv_seqs, scale, window, out,
                                    prefix_v.data_ptr(), prefix, q_seqs.data_ptr(), kv_seqs.data_ptr(), nseq, out.data_ptr(),
                                    ws.data_ptr(), nbytes, handle)
     _call(rc)
+    if given:
+        _written(out)
     _in_use(side, q, k, v, prefix_k, prefix_v, q_seqs, kv_seqs, out)
     return out
 
@@ -324,7 +332,8 @@ def linear_q4(x, weight: Q4Weight, out=None, stream=None):
                 _no_gradient(name, t)
     handle, side = _stream(stream, device)
     out_stride = n
-    if out is None:
+    given = out is not None
+    if not given:
         with _on(side):
             out = x.new_empty((rows, n))
     else:
@@ -337,5 +346,7 @@ def linear_q4(x, weight: Q4Weight, out=None, stream=None):
     _call(_lib.lib().ge_linear_q4(device, dtype, x.data_ptr(), x_stride if rows > 1 else k, rows, k, values.data_ptr(),
                                   weight.scales.data_ptr(), None if mins is None else mins.data_ptr(), weight.group, n,
                                   out.data_ptr(), out_stride, handle))
+    if given:
+        _written(out)
     _in_use(side, x, values, weight.scales, mins, out)
     return out

@@ -284,3 +284,29 @@ def test_scales_that_require_a_gradient_by_the_call_are_refused(hostside, ge):
         ops.linear_q4(x, first)
         ops.linear_q4(x, later)
     assert len(rec.calls) == 2
+
+
+def test_a_given_out_counts_as_changed(hostside):
+    """Autograd's saved values: an `out` that another operation kept for its backward pass is known to have changed,
+    views and their base alike; inference tensors, which count nothing, pass."""
+    import torch
+    ops, _ = hostside
+    q, k, s = torch.zeros(4, 2, 64).half(), torch.zeros(4, 1, 64).half(), torch.zeros(1, 2, dtype=torch.int32)
+    x = torch.zeros(2, 64).half()
+    w = ops.Q4Weight(torch.zeros(8, 32, dtype=torch.uint8), torch.zeros(8, 2).half())
+    wide, o = torch.zeros(2, 16).half(), torch.zeros(4, 2, 64).half()
+    for call, out, base in ((lambda t: ops.linear_q4(x, w, out=t), wide[:, 8:], wide),
+                            (lambda t: ops.attention_causal(q, k, k, s, out=t), o, o),
+                            (lambda t: ops.attention_prefix(q, k, k, s, s, k, k, out=t), o, o)):
+        p = torch.ones(out.shape, requires_grad=True)
+        y = (p.half() * out).sum()
+        before = base._version
+        assert call(out) is out
+        assert base._version == before + 1
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.backward()
+        with torch.inference_mode():
+            call(out.clone())
+    with torch.inference_mode():
+        held = torch.zeros(2, 8).half()
+    ops.linear_q4(x, w, out=held)
