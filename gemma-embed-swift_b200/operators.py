@@ -149,6 +149,13 @@ def _in_use(s, *tensors):
                 t.record_stream(s)
 
 
+def _made_on(s, out, device: int):
+    """An output allocated on stream `s` for the current one: dropped while work there still reads it, its memory
+    is not given out again on `s` before that work has ended."""
+    if s is not None:
+        out.record_stream(_torch()[0].cuda.current_stream(device))
+
+
 def _written(out):
     """Tells autograd that a caller's tensor changed: the kernels write through its pointer."""
     _torch()[0].autograd.graph.increment_version(out)
@@ -217,6 +224,8 @@ def _attention(q, k, v, prefix_k, prefix_v, q_seqs, kv_seqs, scale, window, out,
     _call(rc)
     if given:
         _written(out)
+    else:
+        _made_on(side, out, device)
     _in_use(side, q, k, v, prefix_k, prefix_v, q_seqs, kv_seqs, out)
     return out
 
@@ -348,5 +357,7 @@ def linear_q4(x, weight: Q4Weight, out=None, stream=None):
                                   out.data_ptr(), out_stride, handle))
     if given:
         _written(out)
+    else:
+        _made_on(side, out, device)
     _in_use(side, x, values, weight.scales, mins, out)
     return out

@@ -169,3 +169,33 @@ def test_scores_of_minus_infinity_alone_in_a_cut_prompt(ge, torch, heads, kvh, d
     end = 1000 + window if window else n
     assert torch.isnan(got[:1000]).all() and torch.isnan(got[end:]).all()
     assert torch.equal(got[1000:end], v[1000].repeat_interleave(heads // kvh, 0)[None].expand(end - 1000, -1, -1))
+
+
+# ---------------------------------------------------------------------------- what a caller relies on around a call
+def test_outputs_dropped_while_the_current_stream_reads_them(ge, torch):
+    """An output made on another stream and dropped while the current one still reads it: the next call on that
+    stream does not get its memory."""
+    w = q4(torch, ge, 5000, 512, 32, False)
+    x = normal(torch, 9, (4, 512), "f16")
+    q, k, v = (normal(torch, 50 + i, (700, h, 128), "bf16") for i, h in enumerate((8, 2, 2)))
+    s = dev(torch, [(0, 700)])
+    xs, vs = [x * i for i in range(1, 5)], [v * i for i in range(1, 5)]
+    calls = [lambda i, stream=None: ge.linear_q4(xs[i], w, stream=stream),
+             lambda i, stream=None: ge.attention_causal(q, k, vs[i], s, stream=stream),
+             lambda i, stream=None: ge.attention_prefix(q, k, vs[i], s, s, k, v, stream=stream)]
+    for call in calls:
+        want = call(0)
+        side = torch.cuda.Stream()
+        torch.cuda.synchronize()
+        call(0, side)  # kernels loaded, memory of the stream's own
+        torch.cuda.synchronize()
+        made = call(0, side)
+        torch.cuda.current_stream().wait_stream(side)
+        torch.cuda._sleep(100_000_000)
+        read = made.clone()
+        del made
+        with torch.cuda.stream(side):  # not behind the sleeping stream
+            others = [call(i) for i in range(1, 4)]
+        torch.cuda.synchronize()
+        assert torch.equal(read, want)
+        del others
