@@ -90,6 +90,25 @@ int check_tensor(const char* name, const void* p, int32_t rows, int64_t stride, 
     return GE_OK;
 }
 
+// Rows of `width` bytes, `stride` bytes apart.
+struct Rows {
+    const void* p;
+    int64_t rows, stride, width;
+};
+// Whether two arrays share a byte.  Columns of the same wide rows do not; arrays of different strides whose spans
+// meet count as sharing one.
+bool overlap(const Rows& a, const Rows& b) {
+    if (!a.p || !b.p || a.rows <= 0 || b.rows <= 0 || a.width <= 0 || b.width <= 0) return false;
+    const uint64_t a0 = reinterpret_cast<uintptr_t>(a.p), b0 = reinterpret_cast<uintptr_t>(b.p);
+    const auto end = [](uint64_t at, const Rows& r) { return __int128(at) + __int128(r.rows - 1) * r.stride + r.width; };
+    if (end(a0, a) <= __int128(b0) || end(b0, b) <= __int128(a0)) return false;
+    if (a.rows > 1 && b.rows > 1 && a.stride != b.stride) return true;
+    const uint64_t s = uint64_t(a.rows > 1 ? a.stride : b.rows > 1 ? b.stride : 0);
+    if (s == 0) return true;
+    const uint64_t d = (b0 % s + s - a0 % s) % s;  // b's columns behind a's in a row
+    return d < uint64_t(a.width) || d + uint64_t(b.width) > s;
+}
+
 void fill_shape(ge::CausalLaunch& a, const ge_attention_shape* s) {
     a.bf16 = s->dtype == GE_BF16;
     a.heads = s->heads;
@@ -121,6 +140,11 @@ int run_attention(int device, const ge_attention_shape* s, ge::CausalLaunch& a, 
         return rc;
     if (!a.q_seqs || !a.kv_seqs || (reinterpret_cast<uintptr_t>(a.q_seqs) & 3) || (reinterpret_cast<uintptr_t>(a.kv_seqs) & 3))
         return invalid("sequence ranges are NULL or not 4-byte aligned");
+    const Rows out{a.out, a.ntok, 2 * a.out_stride, 2 * qw};
+    if (overlap(out, {a.q, a.ntok, 2 * a.q_stride, 2 * qw}) || overlap(out, {a.k, a.nkv, 2 * a.k_stride, 2 * kw}) ||
+        overlap(out, {a.v, a.nkv, 2 * a.v_stride, 2 * kw}) || overlap(out, {a.pk, a.prefix, 2 * a.pk_stride, 2 * kw}) ||
+        overlap(out, {a.pv, a.prefix, 2 * a.pv_stride, 2 * kw}))
+        return invalid("out must not overlap q, k, v or the prefix");
     DeviceGuard keep;
     a.num_sms = use_device(keep, device, &rc);
     if (!a.num_sms) return rc;
@@ -223,8 +247,14 @@ int ge_linear_q4(int32_t device_ordinal, int32_t dtype, const void* d_x, int64_t
     if (!aligned16(d_x) || !aligned16(d_values) || (reinterpret_cast<uintptr_t>(d_scales) & 1) ||
         (reinterpret_cast<uintptr_t>(d_mins) & 1) || (reinterpret_cast<uintptr_t>(d_out) & 1))
         return invalid("x and values must be 16-byte aligned");
-    if (x_stride < k || x_stride % 8 || out_stride < n)
-        return invalid("x's row stride must be a multiple of 8 elements and at least k, out's at least n");
+    constexpr int64_t kMaxStride = int64_t(1) << 38;
+    if (x_stride < k || x_stride % 8 || out_stride < n || x_stride > kMaxStride || out_stride > kMaxStride)
+        return invalid("x's row stride must be a multiple of 8 elements and at least k, out's at least n, both at most 2^38");
+    const Rows out{d_out, rows, 2 * out_stride, 2 * int64_t(n)};
+    const int64_t groups = int64_t(n) * (k / group);
+    if (overlap(out, {d_x, rows, 2 * x_stride, 2 * int64_t(k)}) || overlap(out, {d_values, 1, 0, int64_t(n) * (k / 2)}) ||
+        overlap(out, {d_scales, 1, 0, 2 * groups}) || overlap(out, {d_mins, 1, 0, 2 * groups}))
+        return invalid("out must not overlap x or the weights");
     DeviceGuard keep;
     int rc = GE_OK;
     ge::Q4Launch a;

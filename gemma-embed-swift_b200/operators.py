@@ -236,7 +236,8 @@ def attention_causal(q, k, v, seqs, scale: Optional[float] = None, window: int =
 
     q [T, H, D], k and v [T, KV, D], float16 or bfloat16, D 64, 128 or 256, H a multiple of KV;
     rows may be column ranges of a wider tensor.  `seqs` [n, 2] int32 on the device: (start, length)
-    of each sequence.  `scale` defaults to 1 / sqrt(D).  Returns `out` [T, H, D], made when None;
+    of each sequence, neither negative.  `scale` defaults to 1 / sqrt(D).  Returns `out` [T, H, D], made when
+    None (a given one must not overlap the inputs, or is refused);
     rows outside every sequence are left as they were (of a new output: unset)."""
     return _attention(q, k, v, None, None, seqs, seqs, scale, window, out, stream)
 
@@ -316,7 +317,7 @@ class Q4Weight:
 
 def linear_q4(x, weight: Q4Weight, out=None, stream=None):
     """x [rows, k] times the 4-bit weights (ge_linear_q4): out [rows, n] in x's type (float16 or
-    bfloat16), for 0 to 64 rows.  x's rows may be a column range of a wider tensor."""
+    bfloat16), for 0 to 64 rows; a given `out` must not overlap x or the weights.  x's rows may be a column range of a wider tensor."""
     torch = _torch()[0]
     values, mins = weight.values, weight.mins
     device = _on_device("x", x)

@@ -555,7 +555,7 @@ GE_API int ge_q4_repack(const uint8_t* blocks, int32_t type, int64_t n, int64_t 
  * 2 j in the low half of byte j) and scale and min those of group j / group (32, 64 or 128 weights).
  * x is [rows][k] of `dtype` (16-byte aligned, row stride a multiple of 8), d_values [n][k / 2]
  * (16-byte aligned), d_scales and d_mins [n][k / group] fp16, out [rows][n] of `dtype`.  Sums are
- * fp32 over exact products, the result is rounded once.  Where they are not finite (an infinite or NaN x, scale or
+ * fp32 over exact products, the result is rounded once; `out` must not overlap the inputs.  Where they are not finite (an infinite or NaN x, scale or
  * minimum, bf16 values above 1e35), the result is summed again from the definition in 64 bits, which costs time: up to
  * 100 times a call's where every row has such a value.  k is a multiple of group, at most 65536. */
 GE_API int ge_linear_q4(int32_t device_ordinal, int32_t dtype, const void* d_x, int64_t x_stride, int32_t rows, int32_t k,

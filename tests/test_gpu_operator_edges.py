@@ -199,3 +199,24 @@ def test_outputs_dropped_while_the_current_stream_reads_them(ge, torch):
         torch.cuda.synchronize()
         assert torch.equal(read, want)
         del others
+
+
+def test_outputs_beside_inputs_in_the_same_rows(ge, torch):
+    """`out` as columns of the rows that q, k and v are columns of: allowed, and nothing else changes; over any of
+    them it is refused."""
+    heads, kvh, dim, n = 4, 2, 64, 150
+    wide = normal(torch, 60, (n, (2 * heads + 2 * kvh) * dim), "f16")
+    q, k, v, out = (t.unflatten(1, (-1, dim)) for t in wide.split([heads * dim, kvh * dim, kvh * dim, heads * dim], 1))
+    s = dev(torch, [(0, n)])
+    want, before = ge.attention_causal(q, k, v, s), wide[:, :(heads + 2 * kvh) * dim].clone()
+    ge.attention_causal(q, k, v, s, out=out)
+    assert torch.equal(out, want) and torch.equal(wide[:, :(heads + 2 * kvh) * dim], before)
+    w = q4(torch, ge, 64, 64, 32, False)
+    x = normal(torch, 61, (5, 128), "f16")
+    y = ge.linear_q4(x[:, :64], w)
+    assert torch.equal(ge.linear_q4(x[:, :64], w, out=x[:, 64:]), y)
+    for call in (lambda: ge.attention_causal(q, k, v, s, out=q), lambda: ge.attention_prefix(q, k, v, s, s, k, v, out=q),
+                 lambda: ge.linear_q4(x[:, :64], w, out=x[:, 32:96]), lambda: ge.linear_q4(x[:, :64], w, out=x[:, :64])):
+        with pytest.raises(ge.GemmaEmbedError) as e:
+            call()
+        assert e.value.case == "invalidOptions" and "overlap" in str(e.value)

@@ -310,3 +310,73 @@ def test_a_given_out_counts_as_changed(hostside):
     with torch.inference_mode():
         held = torch.zeros(2, 8).half()
     ops.linear_q4(x, w, out=held)
+
+
+def q4_call(lib, device=-1, **over):
+    a = dict(dtype=0, x=FAKE, x_stride=64, rows=2, k=64, values=FAKE << 1, scales=FAKE << 2, mins=None, group=32, n=8, out=FAKE << 3,
+             out_stride=8)
+    a.update(over)
+    L = lib.lib()
+    rc = L.ge_linear_q4(device, a["dtype"], a["x"], a["x_stride"], a["rows"], a["k"], a["values"], a["scales"], a["mins"], a["group"],
+                        a["n"], a["out"], a["out_stride"], None)
+    return rc, (L.ge_last_error(None) or b"").decode()
+
+
+# Addresses of arrays far apart; of the calls below those that are not refused for their arguments name no device.
+Q, K, V, PK, PV, OUT = (FAKE << i for i in range(1, 7))
+ROW = 2 * 256  # bytes of a row of 4 heads of 64
+WIDE = {n + "_stride": 1 << 38 for n in ("q", "k", "v", "prefix_k", "prefix_v", "out")}
+
+
+def apart(call, lib, s, **over):
+    L = lib.lib()
+    a = dict(q=Q, k=K, v=V, out=OUT, ntok=8, nkv=8, pk=PK, pv=PV, plen=4)
+    a.update(over)
+    if call == "causal":
+        rc = L.ge_attention_causal(-1, ctypes.byref(s), a["q"], a["k"], a["v"], a["ntok"], FAKE, 1, a["out"], FAKE, 1 << 30, None)
+    else:
+        rc = L.ge_attention_prefix(-1, ctypes.byref(s), a["q"], a["ntok"], a["k"], a["v"], a["nkv"], a["pk"], a["pv"], a["plen"], FAKE,
+                                   FAKE, 1, a["out"], FAKE, 1 << 30, None)
+    return rc, (L.ge_last_error(None) or b"").decode()
+
+
+@pytest.mark.parametrize("over,strides,refused", [
+    (dict(), {}, False),
+    (dict(out=Q), {}, True),                                  # in place
+    (dict(out=Q + 8 * ROW), {}, False),                       # right behind q
+    (dict(out=Q + 8 * ROW - 16), {}, True),                   # its last 16 bytes
+    (dict(q=OUT + 8 * ROW), {}, False),
+    (dict(q=OUT + 8 * ROW - 16), {}, True),
+    (dict(out=K), {}, True), (dict(out=V), {}, True),
+    (dict(out=K - 8 * ROW), {}, False), (dict(out=V - 8 * ROW + 16), {}, True),
+    (dict(out=Q + ROW), dict(q_stride=512, out_stride=512), False),       # columns of the same wide rows
+    (dict(out=Q + ROW - 16), dict(q_stride=512, out_stride=512), True),   # one column in common
+    (dict(out=Q + ROW + 16), dict(q_stride=512, out_stride=512), True),   # into q's next row
+    (dict(q=OUT + ROW), dict(q_stride=512, out_stride=512), False),
+    (dict(out=Q + ROW), dict(q_stride=512, out_stride=768), True),        # spans that meet, strides that do not
+    (dict(ntok=1, out=Q + ROW), {}, False), (dict(ntok=1, out=Q + ROW - 16), {}, True),
+    (dict(ntok=1, out=Q), dict(q_stride=4096), True),
+    (dict(ntok=1 << 30, out=Q - ROW), WIDE, False),
+    (dict(ntok=1 << 30, out=Q - 16), WIDE, True)])
+def test_outputs_over_inputs_are_refused(lib, over, strides, refused):
+    for call in ("causal", "prefix"):
+        rc, msg = apart(call, lib, shape(lib, **strides), **over)
+        assert (rc == 9 and "overlap" in msg) if refused else rc == 8, msg
+
+
+@pytest.mark.parametrize("over,refused", [(dict(out=PK), True), (dict(out=PV + 16), True), (dict(plen=0, pk=OUT, pv=OUT), False),
+                                          (dict(nkv=0, k=OUT, v=OUT), False), (dict(nkv=2, out=K + 512), False),
+                                          (dict(nkv=2, out=K + 512 - 16), True)])
+def test_outputs_over_the_prefix_or_keys_are_refused(lib, over, refused):
+    rc, msg = apart("prefix", lib, shape(lib), **over)
+    assert (rc == 9 and "overlap" in msg) if refused else rc == 8, msg
+
+
+@pytest.mark.parametrize("over,refused", [
+    (dict(), False), (dict(out=FAKE, n=64, out_stride=64), True), (dict(out=FAKE + 2 * 128), False), (dict(out=FAKE + 2 * 128 - 2), True),
+    (dict(x_stride=128, out=FAKE + 128, out_stride=128), False), (dict(x_stride=128, out=FAKE + 126, out_stride=128), True),
+    (dict(out=FAKE << 1), True), (dict(out=(FAKE << 1) + 8 * 32), False), (dict(out=(FAKE << 2) + 30), True), (dict(out=(FAKE << 2) + 32), False),
+    (dict(mins=FAKE << 3), True), (dict(mins=(FAKE << 3) + 32), False), (dict(mins=(FAKE << 3) + 30), True)])
+def test_linear_q4_outputs_over_inputs_are_refused(lib, over, refused):
+    rc, msg = q4_call(lib, **over)
+    assert (rc == 9 and "overlap" in msg) if refused else rc == 8, msg
