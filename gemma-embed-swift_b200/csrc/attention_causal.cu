@@ -52,6 +52,8 @@
 //   2 x 8192 tokens, 12 heads of 64            0.285 ms,  722 TFLOP/s (a 64 wide S costs half the product, the
 //                                              same softmax)
 //   64 x 300 tokens, 32 heads of 128 on 8      0.129 ms,  367 TFLOP/s; 394 MB of tensors, 3.0 TB/s
+#include <stdlib.h>
+
 #include <algorithm>
 
 #include "attention_rows.cuh"
@@ -578,30 +580,39 @@ template <bool kSleep>
 __device__ __forceinline__ bool wait_on(uint64_t* bar, uint32_t parity, int* err, int64_t limit) {
     if (mbar_test(bar, parity)) return true;
     const int64_t t0 = clock64();
-    while (!mbar_test(bar, parity)) {
-        if (kSleep) __nanosleep(32);
-        if (clock64() - t0 > limit) {
+    do {
+        if (clock64() - t0 >= limit) {
             *err = kErrTimeout;
             return false;
         }
-    }
+        if (kSleep) __nanosleep(32);
+    } while (!mbar_test(bar, parity));
     return true;
 }
 // The same by a whole warp, whose lanes agree.
 __device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t parity, int* err, int64_t limit) {
     if (__all_sync(0xffffffffu, mbar_poll(bar, parity))) return true;
     const int64_t t0 = clock64();
-    while (!__all_sync(0xffffffffu, mbar_test(bar, parity)))
-        if (__any_sync(0xffffffffu, clock64() - t0 > limit)) {
+    do {
+        if (__any_sync(0xffffffffu, clock64() - t0 >= limit)) {
             *err = kErrTimeout;
             return false;
         }
+    } while (!__all_sync(0xffffffffu, mbar_test(bar, parity)));
     return true;
 }
 // kWaitLimitNs at 2 GHz, and more over many keys: a warp recomputes 32 rows over all of them at most, at about 0.25 us
 // for a key of a row (8 heads of 128 wide, 8192 rows that all see an infinite value: 69 ms, 0.13 ms without it); 1 us
 // is allowed.
-constexpr int64_t wait_limit(int64_t keys) { return 2 * (int64_t(kWaitLimitNs) + keys * 32 * 1000); }
+// GE_ATTENTION_WAIT_NS in the environment of the process' first call stands in its place (0: whatever is not there
+// at the first look has run out).
+int64_t wait_limit(int64_t keys) {
+    static const int64_t given = [] {
+        const char* ns = getenv("GE_ATTENTION_WAIT_NS");
+        return ns ? int64_t(std::max(0LL, std::min(atoll(ns), 1LL << 60))) : int64_t(-1);
+    }();
+    return 2 * (given >= 0 ? given : int64_t(kWaitLimitNs) + keys * 32 * 1000);
+}
 // 32 bytes at once, to a 32-byte boundary: a store touches a line for every lane's row, so half as many go out.
 __device__ __forceinline__ void store32(void* p, const uint32_t (&w)[8]) {
     asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]),
@@ -768,6 +779,28 @@ __device__ __forceinline__ void exact_row(const TcParams& p, int id, int row, in
     }
 }
 
+// Where a wait of a CTA's softmax warps ran out: the rows of all its pieces become NaN, so that what `out` held before
+// cannot pass for a result.  By the softmax warps (others may not have the registers), a row a thread.  Rows done
+// before go too: to know how far each warp came would hold registers throughout (200 bytes of spills).
+template <typename E, int D>
+__device__ __noinline__ void rows_lost(const TcParams& p) {
+    const int i = int(threadIdx.x) - 128, x = i >> 7, r = i & 127, token = r / p.group, total = p.head->nwork * p.kv_heads;
+#pragma unroll 1
+    for (int round = 0; piece_id(round) < total; round++) {
+        const Piece s = piece_of(p, fetch_piece(p, piece_id(round), total));
+        const int row = s.tile * p.TI + x * p.T + token, head = s.kvh * p.group + (r - token * p.group);
+        if (r >= p.group * p.T || row >= p.ntok || (!(s.flags & 4) && p.rng[row].y < 0)) continue;
+        if (s.piece >= 0) {  // the merge makes the row of it
+            p.ml[(int64_t(s.piece) * p.ntok + row) * p.heads + head] = make_float2(0.f, NAN);
+            continue;
+        }
+        const uint32_t nan = float_to_pair<E>(NAN, NAN);
+        uint4* dst = reinterpret_cast<uint4*>(static_cast<E*>(p.out) + row * p.out_stride + int64_t(head) * D);
+#pragma unroll 1
+        for (int c = 0; c < D / 8; c++) dst[c] = make_uint4(nan, nan, nan, nan);
+    }
+}
+
 template <typename E, int D>
 __global__ void __launch_bounds__(Cfg<D>::kThreads, 1)
     k_causal_tc(const __grid_constant__ CUtensorMap mapQ, const __grid_constant__ CUtensorMap mapK,
@@ -785,6 +818,7 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1)
     uint64_t *o_full = p_full + 2, *o_empty = o_full + 2;   // per tile
     uint64_t *pv_done = o_empty + 2, *idle = pv_done + 1;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(idle + 1);
+    volatile uint32_t* lost = tmem_slot + 1;
     int* err = &p.head->err;
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -806,6 +840,7 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1)
         }
         mbar_init(pv_done, 1);
         mbar_init(idle, 1);
+        *lost = 0;
         fence_mbar_init();
     }
     if (warp == 0 && lane == 0) {
@@ -1291,6 +1326,7 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1)
                 exact_row<E, D>(p, id, __shfl_sync(0xffffffffu, row, src), __shfl_sync(0xffffffffu, head, src), g);
             }
         }
+        if (!ok) *lost = 1;
     }
 
     if (C::kBoxes && warp >= 4 && lane == 0) bulk_wait_all();
@@ -1300,6 +1336,7 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1)
         tc_fence_after();
         tmem_dealloc(tmem, 512);
     }
+    if (warp >= 4 && *lost) rows_lost<E, D>(p);
 }
 
 // ------------------------------------------------------------------------------------ merge

@@ -6,7 +6,8 @@ ge_attention_prefix and ge_linear_q4 of include/gemma_embed.h).  Every call enqu
 `stream` -- a torch stream, a raw cudaStream_t, or None for torch's current stream of the
 tensors' device -- and returns without synchronising; it may be captured into a CUDA graph.  A stream
 other than the current one has to be behind the work that fills the inputs; their memory is not reused
-before the call's work there has ended.  There is no derivative: inputs that require a gradient are
+before the call's work there has ended.  A wait inside the attention kernels that ran out (2 s and more,
+which no argument can bring about) leaves NaN in the rows it kept from being finished.  There is no derivative: inputs that require a gradient are
 refused while gradients are recorded, dual tensors of forward-mode differentiation always.
 
     out = attention_causal(q, k, v, seqs)               # q [T, H, D], k and v [T, KV, D]

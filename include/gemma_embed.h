@@ -511,7 +511,9 @@ typedef struct ge_attention_shape {
  * holds is free again once the call's work has completed, and calls that may overlap on the GPU
  * (other streams, captured graphs replayed at the same time) need one each.  Its first 32-bit word is 0
  * after a call's work, or GE_ERR_TIMEOUT where a wait inside the kernel ran out (2 s and more, which no
- * argument can bring about); `out` is then not to be used. */
+ * argument can bring about; GE_ATTENTION_WAIT_NS in the environment of the process' first call sets another limit,
+ * in nanoseconds); `out` is then not to be used, and rows that were not finished hold NaN.  A call without rows or
+ * sequences does no work and leaves the word as it was. */
 GE_API int ge_attention_workspace(int32_t device_ordinal, const ge_attention_shape* shape, int32_t ntok,
                                   int32_t prefix_len, int64_t* bytes);
 

@@ -1,6 +1,9 @@
 """The operators on device tensors at the edges of what their calls allow, on a B200: infinities and sums past
 the types, and what a caller relies on around a call."""
 import math
+import os
+import subprocess
+import sys
 
 import numpy as np
 import pytest
@@ -220,3 +223,56 @@ def test_outputs_beside_inputs_in_the_same_rows(ge, torch):
         with pytest.raises(ge.GemmaEmbedError) as e:
             call()
         assert e.value.case == "invalidOptions" and "overlap" in str(e.value)
+
+
+WAITS_RUN_OUT = """
+import ctypes, importlib, sys
+import torch
+ge = importlib.import_module("gemma-embed-swift_b200")
+lib = importlib.import_module("gemma-embed-swift_b200._lib")
+expect_lost = sys.argv[1] == "lost"
+for heads, kvh, dim in ((8, 2, 128), (3, 1, 256), (2, 2, 64), (6, 2, 128)):
+    for lens, gap in (([5, 40, 9], 3), ([700, 20, 300], 7), ([90] * 60, 1), ([3000], 2)):
+        total = sum(lens) + gap * len(lens)
+        seqs, inside, at = [], torch.zeros(total, dtype=torch.bool, device="cuda"), 0
+        for n in lens:
+            seqs.append((at, n))
+            inside[at:at + n] = True
+            at += n + gap
+        s = torch.tensor(seqs, dtype=torch.int32, device="cuda")
+        q, k = (torch.randn(total, h, dim, device="cuda").to(torch.bfloat16) for h in (heads, kvh))
+        pk = torch.randn(600, kvh, dim, device="cuda").to(torch.bfloat16)
+        for call in (lambda o: ge.attention_causal(q, k, k, s, out=o), lambda o: ge.attention_prefix(q, k, k, s, s, pk, pk, out=o)):
+            out = call(torch.full_like(q, 7.0))
+            assert (out[~inside] == 7.0).all(), "rows of no sequence"
+            if expect_lost:
+                assert torch.isnan(out[inside]).all(), (heads, dim, lens)
+            else:
+                assert torch.isfinite(out[inside]).all()
+# The status a C caller finds in the workspace's first word.
+q = torch.randn(900, 4, 64, device="cuda").half()
+s = torch.tensor([[0, 900]], dtype=torch.int32, device="cuda")
+shape = lib.GeAttentionShape(0, 4, 4, 64, 0.125, 0, 256, 256, 256, 0, 0, 256)
+n = ctypes.c_int64(0)
+assert lib.lib().ge_attention_workspace(0, ctypes.byref(shape), 900, 0, ctypes.byref(n)) == 0
+ws, out = torch.full((n.value,), 255, dtype=torch.uint8, device="cuda"), torch.empty_like(q)
+torch.cuda.synchronize()
+assert lib.lib().ge_attention_causal(0, shape, q.data_ptr(), q.data_ptr(), q.data_ptr(), 900, s.data_ptr(), 1, out.data_ptr(),
+                                     ws.data_ptr(), n.value, None) == 0
+torch.cuda.synchronize()
+assert ws[:4].view(torch.int32).item() == (12 if expect_lost else 0)
+print("as expected")
+"""
+
+
+@pytest.mark.parametrize("limit,outcome", [("0", "lost"), (None, "kept"), ("1000000000", "kept")])
+def test_rows_of_a_wait_that_ran_out_are_nan(cuda_device, limit, outcome):
+    """With no time to wait every wait of the attention kernels runs out: its rows are NaN, no other row is
+    touched, the status says so, and the process goes on."""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    env = {k: v for k, v in os.environ.items() if k != "GE_ATTENTION_WAIT_NS"}
+    if limit is not None:
+        env["GE_ATTENTION_WAIT_NS"] = limit
+    r = subprocess.run([sys.executable, "-c", WAITS_RUN_OUT, outcome], cwd=root, env={**env, "PYTHONPATH": root}, capture_output=True,
+                       text=True, timeout=200)
+    assert r.returncode == 0 and "as expected" in r.stdout, r.stderr[-2000:]
