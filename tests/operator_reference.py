@@ -91,3 +91,41 @@ def linear_q4(x, values, scales, mins):
     mag = x64.abs() @ (q * s.abs() + lo.abs()).T
     tiny = 2.0 ** -25 if x.dtype == torch.float16 else 0.0
     return want, (2 * half + 16) * 2.0 ** -23 * mag + torch.finfo(x.dtype).eps / 2 * want.abs() + tiny
+
+
+def linear_q4_by_steps(x, values, scales, mins):
+    """(want, bound) of linear_q4 in float64, the bound by the steps a sum passes through.
+
+    A group's products with the 4-bit integers are summed by 16-wide tensor products, `group / 16` in a row: each
+    aligns its 16 products and the sum so far to the largest and truncates, 18 terms of 2^-23 of what the group
+    holds.  The groups' sums are then scaled into a running sum, one or two roundings (2^-24) a group of whatever
+    that sum holds by then; the 16 parts of k it may be split into are joined in order.  Partial sums of any run of
+    groups are at most twice the largest prefix, plus one group's part before its minimum joins it."""
+    n, half = values.shape
+    groups = scales.shape[1]
+    group = 2 * half // groups
+    q = torch.stack([values & 15, values >> 4], -1).double().view(n, groups, group)
+    if mins is None:
+        q = q - 8
+    xg = x.double().view(x.shape[0], groups, group)
+    want = torch.empty((x.shape[0], n), dtype=torch.float64, device=x.device)
+    bound = torch.empty_like(want)
+    sums, mags = xg.sum(2), xg.abs().sum(2)
+    step = max(1, (1 << 26) // max(1, x.shape[0] * groups))
+    for a in range(0, n, step):
+        s = scales[a:a + step].double()[None]
+        part = torch.einsum("rgk,ngk->rng", xg, q[a:a + step]) * s
+        mag = torch.einsum("rgk,ngk->rng", xg.abs(), q[a:a + step].abs()) * s.abs()
+        whole, low = part, 0.0
+        if mins is not None:
+            m = mins[a:a + step].double()[None]
+            whole = part + sums[:, None] * m
+            low = (mags[:, None] * m.abs()).sum(2)
+        run = whole.cumsum(2)
+        most = 2 * run.abs().amax(2) + mag.amax(2)
+        want[:, a:a + step] = run[..., -1]
+        # A sum of x over a group: at most 16 roundings of half a step, and its product's own.
+        bound[:, a:a + step] = (18 * group / 16 * 2.0 ** -23 * mag.sum(2) + 18 * 2.0 ** -24 * low
+                                + (2 * groups + 16) * 2.0 ** -24 * most)
+    tiny = 2.0 ** -25 if x.dtype == torch.float16 else 0.0
+    return want, bound + torch.finfo(x.dtype).eps / 2 * (want.abs() + bound) + tiny

@@ -276,3 +276,158 @@ def test_rows_of_a_wait_that_ran_out_are_nan(cuda_device, limit, outcome):
     r = subprocess.run([sys.executable, "-c", WAITS_RUN_OUT, outcome], cwd=root, env={**env, "PYTHONPATH": root}, capture_output=True,
                        text=True, timeout=200)
     assert r.returncode == 0 and "as expected" in r.stdout, r.stderr[-2000:]
+
+
+# ---------------------------------------------------------------------------- nothing lost, nothing twice
+@pytest.mark.parametrize("mins", [False, True])
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("rows,n,k,dtype", [(1, 300, 65536, "f16"), (12, 300, 65536, "bf16"), (40, 130, 65536, "f16"), (1, 2500, 8192, "bf16"),
+                                            (9, 5003, 8192, "f16"), (17, 41003, 8192, "bf16"), (32, 41003, 8192, "f16"),
+                                            (12, 38001, 8192 + 384, "f16"), (5, 768, 1152, "bf16"), (64, 2400, 4096, "f16")])
+def test_linear_q4_by_steps(ge, torch, rows, n, k, dtype, group, mins):
+    """Against the bound that sees a lost stage, unit or minimum: long sums of many chunks of x, several passes over
+    the column tiles, every number of rows to a launch."""
+    w = q4(torch, ge, n, k, group, mins, seed=rows + k)
+    x = normal(torch, rows, (rows, k), dtype)
+    want, bound = ref.linear_q4_by_steps(x, w.values, w.scales, w.mins)
+    ref.check(ge.linear_q4(x, w), want, bound)
+
+
+@pytest.mark.parametrize("mins", [False, True])
+@pytest.mark.parametrize("group", [32, 128])
+@pytest.mark.parametrize("n,k", [(50, 256), (300, 1152), (41003, 2048), (70, 8192 + 128), (300, 65536)])
+def test_linear_q4_single_weights(ge, torch, n, k, group, mins):
+    """Rows of x with one 1 give the weights themselves: at the borders of units, stages, chunks of x and parts of k,
+    for every number of rows to a launch."""
+    w = q4(torch, ge, n, k, group, mins, seed=7)
+    table = dense(torch, w)
+    places = sorted({p for at in (0, 32, 128, 256, 512, 1024, 4096, 8192, 16384, 32768, k // 3 // 256 * 256, k // 2 // 256 * 256, k)
+                     for p in (at - 1, at, at + 7, at + 8) if 0 <= p < k})
+    for rows in (1, 8, 13, 32, 64):
+        for first in range(0, len(places), rows):
+            at = torch.tensor(places[first:first + rows], device="cuda")
+            x = torch.zeros((len(at), k), dtype=torch.float16, device="cuda")
+            x[torch.arange(len(at), device="cuda"), at] = 1.0
+            want = table[:, at].T
+            # scale q (or q - 8) is exact in 32 bits; the minimum's product and the result round once each.
+            ref.check(ge.linear_q4(x, w), want, (2.0 ** -11 + 2.0 ** -23) * want.abs() + 2.0 ** -25)
+
+
+def marked(torch, rows, kvh, dim, dtype, keys, value):
+    """Values of 0 but for keys[c] in column c, of every head."""
+    v = torch.zeros((rows, kvh, dim), dtype=dt(torch, dtype), device="cuda")
+    c = torch.arange(len(keys), device="cuda")
+    v[torch.as_tensor(keys, device="cuda"), :, c] = value
+    return v
+
+
+def each_key(ge, torch, heads, kvh, dim, dtype, qr, kr, nkv, plen=None, window=0, keys=None):
+    """Uniform weights (q = 0): a row that sees n keys gives value / n in the column of every key it sees, once,
+    and 0 in the others'.  `keys`: which of the prefix' and own rows to mark (all)."""
+    ntok, pre, value = max(s + n for s, n in qr), plen or 0, 1024.0
+    q = torch.zeros((ntok, heads, dim), dtype=dt(torch, dtype), device="cuda")
+    k = normal(torch, 1, (nkv, kvh, dim), dtype)
+    pk = normal(torch, 2, (pre, kvh, dim), dtype)
+    place = torch.full((ntok,), -1, device="cuda")  # of a row among its sequence's keys
+    start, lost = torch.zeros(ntok, dtype=torch.long, device="cuda"), torch.ones(ntok, dtype=torch.bool, device="cuda")
+    for (s, n), (ks, m) in zip(qr, kr):
+        place[s:s + n] = torch.arange(n, device="cuda") + m - n
+        start[s:s + n] = ks
+        lost[s:s + n] = False
+    lo = (place - window + 1).clamp_min(0) if window else torch.zeros_like(place)
+    count = pre + (place + 1 - lo).clamp_min(0)
+    keys = list(range(pre + nkv)) if keys is None else keys
+    u = torch.finfo(q.dtype).eps / 2
+    qs, ks = dev(torch, qr), dev(torch, kr)
+    for first in range(0, len(keys), dim):
+        part = keys[first:first + dim]
+        both = marked(torch, pre + nkv, kvh, dim, dtype, part, value)
+        pv, v = both[:pre], both[pre:]
+        if plen is None:
+            got = ge.attention_causal(q, k, v, qs, window=window)
+        else:
+            got = ge.attention_prefix(q, k, v, qs, ks, pk, pv)
+        key = torch.as_tensor(part, device="cuda")[None] - pre
+        own = key - start[:, None]
+        seen = (key < 0) | ((own >= lo[:, None]) & (own <= place[:, None]) & (place >= 0)[:, None])
+        want = torch.zeros((ntok, dim), dtype=torch.float64, device="cuda")
+        want[:, :len(part)] = seen * value / count.clamp_min(1)[:, None].double()
+        # Exponentials of 0 and the sums of their equals (2^-20 together), the result's rounding.
+        bound = (u + 2.0 ** -20) * want + (2.0 ** -25 if dtype == "f16" else 0.0) * (want > 0)
+        err = (got.double() - want[:, None]).abs()
+        bad = (err > bound[:, None]) & ~lost[:, None, None]
+        assert not bad.any(), (first, bad.nonzero()[:3].tolist())
+
+
+SHAPES = [(8, 2, 128, "bf16"), (3, 1, 256, "f16"), (4, 4, 64, "f16"), (2, 1, 64, "bf16")]
+
+
+@pytest.mark.parametrize("heads,kvh,dim,dtype", SHAPES)
+@pytest.mark.parametrize("plen,n", [(8000, 1), (4097, 3), (127, 2), (128, 2), (129, 2), (1, 5), (0, 2)])
+def test_prefix_every_key_once(ge, torch, heads, kvh, dim, dtype, plen, n):
+    """Single tokens whose keys are cut into pieces: every prefix and own key counts once."""
+    kr = []
+    for i in range(n):
+        kr.append((sum(m for _, m in kr), 1500 + 389 * i))
+    each_key(ge, torch, heads, kvh, dim, dtype, [(i, 1) for i in range(n)], kr, sum(m for _, m in kr), plen)
+
+
+@pytest.mark.parametrize("heads,kvh,dim,dtype", SHAPES)
+def test_prefix_every_key_once_in_scattered_slots(ge, torch, heads, kvh, dim, dtype):
+    """Slots in no order with keys of no row between them, some ranges shared, some empty; last tokens and texts."""
+    slot, rng = 400, np.random.default_rng(3)
+    order = [int(i) for i in rng.permutation(24)[:14]]
+    kr = [(slot * i, int(m)) for i, m in zip(order, rng.integers(0, 300, 14))]
+    kr[5], kr[9] = kr[2], (17, 0)
+    qr, at = [], 0
+    for n in rng.integers(0, 9, 14):
+        qr.append((at, int(n)))
+        at += int(n)
+    qr[3] = (qr[3][0], 0)
+    for plen in (0, 257):
+        each_key(ge, torch, heads, kvh, dim, dtype, qr, kr, slot * 24, plen)
+
+
+@pytest.mark.parametrize("heads,kvh,dim,dtype", SHAPES)
+@pytest.mark.parametrize("window", [0, 1, 127, 128, 129, 700])
+def test_causal_every_key_once(ge, torch, heads, kvh, dim, dtype, window):
+    """A cut prompt beside short ones, and a batch whose sequences share tiles."""
+    for lens in ([2500, 33], [1, 130, 300, 77, 513, 0, 128]):
+        r = []
+        for n in lens:
+            r.append((sum(m for _, m in r), n))
+        keys = None if len(lens) == 2 else list(range(0, sum(lens), 3)) + [sum(lens) - 1]
+        each_key(ge, torch, heads, kvh, dim, dtype, r, r, sum(lens), window=window, keys=keys)
+
+
+@pytest.mark.parametrize("heads,kvh,dim,dtype", SHAPES)
+@pytest.mark.parametrize("plen,own", [(8000, 2500), (4097, 1), (0, 3000), (300, 64)])
+def test_one_key_holds_all_the_weight(ge, torch, heads, kvh, dim, dtype, plen, own):
+    """Each row asks for one key, which scores far above all others: its value comes back, from either side of
+    every border of blocks and pieces."""
+    rows = dim
+    total = plen + own
+    step = max(1, total // 700)
+    keys = sorted({p for p in list(range(0, total, step)) + [plen - 1, plen, plen + 1, plen - 2, total - 1, total - 2]
+                   + [b + d for b in range(0, total, 128) for d in (-1, 0)] if 0 <= p < total})
+    both_v = normal(torch, 5, (total, kvh, dim), dtype)
+    s = dev(torch, [(i, 1) for i in range(rows)])
+    ks = dev(torch, [(0, own)] * rows)
+    q = torch.zeros((rows, heads, dim), dtype=dt(torch, dtype), device="cuda")
+    for h in range(heads):
+        q[torch.arange(rows, device="cuda"), h, (torch.arange(rows, device="cuda") + h) % dim] = 8.0
+    group = heads // kvh
+    u = torch.finfo(q.dtype).eps / 2
+    for first in range(0, len(keys), dim):
+        part = (keys[first:first + dim] * dim)[:dim]
+        both_k = torch.zeros((total, kvh, dim), dtype=q.dtype, device="cuda")
+        both_k[torch.as_tensor(part, device="cuda"), :, torch.arange(dim, device="cuda")] = 8.0
+        got = ge.attention_prefix(q, both_k[plen:], both_v[plen:], s, ks, both_k[:plen], both_v[:plen], scale=1.0).double()
+        for h in range(heads):
+            column = (torch.arange(rows, device="cuda") + h) % dim
+            # A key may be marked in several columns where there are fewer keys than columns: still one key a row.
+            key = torch.as_tensor(part, device="cuda")[column]
+            want = both_v[key, h // group].double()
+            # The other keys' weights: e^-64 each, below 2^-25 of fp16 and 2^-60 of bf16 in all.
+            err = (got[:, h] - want).abs()
+            assert (err <= (u + 2.0 ** -20) * want.abs() + 2.0 ** -24 * both_v.abs().max()).all(), (first, h)

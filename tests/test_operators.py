@@ -380,3 +380,39 @@ def test_outputs_over_the_prefix_or_keys_are_refused(lib, over, refused):
 def test_linear_q4_outputs_over_inputs_are_refused(lib, over, refused):
     rc, msg = q4_call(lib, **over)
     assert (rc == 9 and "overlap" in msg) if refused else rc == 8, msg
+
+
+@pytest.mark.parametrize("mins", [False, True])
+@pytest.mark.parametrize("group", [32, 128])
+@pytest.mark.parametrize("k", [1152, 8192, 65536])
+def test_the_4bit_bound_sees_what_is_lost(k, group, mins):
+    """The bound that the GPU results are held to leaves no room for a stage of 256 weights, a group's minimum, one
+    32-weight unit or another row's x."""
+    import torch
+
+    import operator_reference as ref
+    g = torch.Generator().manual_seed(k + group)
+    n, rows = 24, 3
+    values = torch.randint(0, 256, (n, k // 2), generator=g, dtype=torch.uint8)
+    scales = (torch.rand((n, k // group), generator=g) * 0.02 + 1e-3).half()
+    lows = (torch.randn((n, k // group), generator=g) * 0.05).half() if mins else None
+    x = torch.randn((rows, k), generator=g).half()
+    want, bound = ref.linear_q4_by_steps(x, values, scales, lows)
+    same, loose = ref.linear_q4(x, values, scales, lows)
+    assert torch.allclose(want, same, rtol=0, atol=1e-9 * float(same.abs().max())) and (bound <= loose).all()
+
+    def off(x=x, scales=scales, lows=lows):  # the share of outputs past the bound
+        wrong, _ = ref.linear_q4(x, values, scales, lows)
+        return float(((wrong - want).abs() > bound).double().mean())
+    for at in (0, k // 2 // 256 * 256, (k - 1) // 256 * 256):
+        lost = x.clone()
+        lost[:, at:at + 256] = 0
+        assert off(x=lost) > 0.8
+        lost = x.clone()
+        lost[:, at:at + 32] = 0
+        assert off(x=lost) > 0.5
+        if mins:
+            less = lows.clone()
+            less[:, at // group] = 0
+            assert off(lows=less) > 0.25  # some minima are near 0, some sums of x too
+    assert off(x=x[[1, 2, 0]]) > 0.9
