@@ -4,6 +4,7 @@ import math
 import os
 import subprocess
 import sys
+import threading
 
 import numpy as np
 import pytest
@@ -431,3 +432,148 @@ def test_one_key_holds_all_the_weight(ge, torch, heads, kvh, dim, dtype, plen, o
             # The other keys' weights: e^-64 each, below 2^-25 of fp16 and 2^-60 of bf16 in all.
             err = (got[:, h] - want).abs()
             assert (err <= (u + 2.0 ** -20) * want.abs() + 2.0 ** -24 * both_v.abs().max()).all(), (first, h)
+
+
+# ---------------------------------------------------------------------------- how calls are made
+FIRST_CALL_IN_A_CAPTURE = """
+import importlib
+import torch
+ge = importlib.import_module("gemma-embed-swift_b200")
+dev = "cuda"
+q, k = (torch.randn(300, h, 128, device=dev).half() for h in (8, 2))
+s = torch.tensor([[0, 200], [200, 100]], dtype=torch.int32, device=dev)
+one = torch.tensor([[0, 1], [1, 1]], dtype=torch.int32, device=dev)
+w = ge.Q4Weight(torch.randint(0, 256, (500, 256), dtype=torch.uint8, device=dev), torch.rand(500, 16, device=dev).half())
+x = torch.randn(3, 512, device=dev).half()
+big = torch.randn(3000, 2, 128, device=dev).half()
+torch.cuda.synchronize()
+calls = [lambda: ge.attention_causal(q, k, k, s), lambda: ge.attention_prefix(q[:2], k, k, one, s, big, big), lambda: ge.linear_q4(x, w)]
+held = []
+for call in calls:
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = call()
+    held.append((g, out))
+for (g, out), call in zip(held, calls):
+    out.fill_(7.0)
+    g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, call())
+print("as expected")
+"""
+
+
+def test_the_first_call_of_a_process_may_be_captured(cuda_device):
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", FIRST_CALL_IN_A_CAPTURE], cwd=root, env={**os.environ, "PYTHONPATH": root}, capture_output=True,
+                       text=True, timeout=200)
+    assert r.returncode == 0 and "as expected" in r.stdout, r.stderr[-2000:]
+
+
+def test_a_side_stream_within_a_capture(ge, torch):
+    """Calls on a forked stream inside a capture, joined before its end: replays give the eager results."""
+    w = q4(torch, ge, 900, 256, 64, True)
+    x = normal(torch, 1, (7, 256), "bf16")
+    q, k, v = (normal(torch, 2 + i, (400, h, 64), "bf16") for i, h in enumerate((4, 2, 2)))
+    s = dev(torch, [(0, 150), (150, 250)])
+    want = [ge.linear_q4(x, w), ge.attention_causal(q, k, v, s), ge.attention_prefix(q, k, v, s, s, k, v)]
+    torch.cuda.synchronize()
+    side, g = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        side.wait_stream(torch.cuda.current_stream())
+        got = [ge.linear_q4(x, w, stream=side), ge.attention_causal(q, k, v, s, stream=side)]
+        got.append(ge.attention_prefix(q, k, v, s, s, k, v))  # beside them
+        torch.cuda.current_stream().wait_stream(side)
+    for _ in range(3):
+        for t in got:
+            t.fill_(7.0)
+        g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_calls_of_several_threads(ge, torch):
+    """Threads with streams of their own, a launch policy and an error message each."""
+    w = q4(torch, ge, 900, 256, 64, True)
+    xs = [normal(torch, i, (7, 256), "f16") for i in range(4)]
+    q, k = (normal(torch, 20 + i, (700, h, 128), "f16") for i, h in enumerate((8, 2)))
+    s = dev(torch, [(0, 500), (500, 200)])
+    wants = [(ge.linear_q4(x, w), ge.attention_causal(q * (i + 1), k, k, s)) for i, x in enumerate(xs)]
+    qs = [q * (i + 1) for i in range(4)]
+    torch.cuda.synchronize()
+    failed = []
+
+    def work(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(60):
+                    y, o = ge.linear_q4(xs[i], w), ge.attention_causal(qs[i], k, k, s)
+                    with pytest.raises(ge.GemmaEmbedError) as e:
+                        ge.attention_causal(q, k, k, s, scale=-1.0) if i % 2 else ge.linear_q4(xs[i][:, :32], w)
+                    assert ("scale" if i % 2 else "x must be") in str(e.value)
+                torch.cuda.current_stream().synchronize()
+                assert torch.equal(y, wants[i][0]) and torch.equal(o, wants[i][1])
+        except BaseException as e:
+            failed.append((i, e))
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed, failed
+
+
+@pytest.mark.parametrize("heads,kvh,dim", [(4, 1, 128), (3, 1, 256), (2, 2, 64), (3, 1, 64)])
+def test_causal_across_32_bit_offsets(ge, torch, heads, kvh, dim):
+    """q, k, v and out as columns of rows whose element offsets pass 2^31, whole items, pieces and recomputed rows."""
+    width, rows = 1 << 16, 34000  # 4.5 GB of fp16
+    cache = torch.empty((rows, width), dtype=torch.float16, device="cuda")
+    part = lambda at, h: cache[:, at:at + h * dim].unflatten(1, (h, dim))
+    q, k, v, out = part(0, heads), part(8192, kvh), part(20000, kvh), part(width - heads * dim, heads)
+    for lens in ([900], [60] * 15):
+        r = ranges_from(rows - sum(lens) - 3, lens)
+        a, b = rows - sum(lens) - 10, rows
+        for i, t in enumerate((q, k, v)):
+            t[a:] = normal(torch, i, tuple(t[a:].shape), "f16")
+        for bad in (None, math.inf):
+            out[a:] = 7.0
+            if bad is not None:
+                v[r[0][0], :, 3] = bad
+            ge.attention_causal(q, k, v, dev(torch, r), out=out)
+            own = [(s - a, n) for s, n in r]
+            want, bound, touched = ref.attention(q[a:b].contiguous(), k[a:b].contiguous(), v[a:b].contiguous(), own, own, 1 / math.sqrt(dim))
+            keep = [c for c in range(dim) if bad is None or c != 3]
+            got = out[a:b][..., keep]
+            ref.check(got[touched], want[touched][..., keep], bound[touched][..., keep])
+            assert (got[~touched] == 7.0).all()
+
+
+def ranges_from(at, lens):
+    out = []
+    for n in lens:
+        out.append((at, n))
+        at += n
+    return out
+
+
+def test_linear_q4_across_32_bit_offsets(ge, torch):
+    """Weights of more than 2^32 bytes, x and out as columns of rows further apart than 2^31 elements."""
+    n, k = 140_003, 65536
+    values = torch.randint(0, 256, (n, k // 2), dtype=torch.uint8, device="cuda")
+    scales = (torch.rand((n, k // 32), device="cuda") * 0.02 + 1e-3).half()
+    w = ge.Q4Weight(values, scales)
+    x = normal(torch, 1, (2, k), "f16", 0.1)
+    got = ge.linear_q4(x, w)
+    for at in (0, 65530, 131064, n - 20):
+        want, bound = ref.linear_q4_by_steps(x, values[at:at + 20].contiguous(), scales[at:at + 20].contiguous(), None)
+        ref.check(got[:, at:at + 20], want, bound)
+    del w, values, scales
+    stride = (1 << 31) + 64
+    far = torch.empty(stride + 2048, dtype=torch.float16, device="cuda")
+    w = q4(torch, ge, 500, 512, 32, True)
+    x = far.as_strided((2, 512), (stride, 1))
+    x.copy_(normal(torch, 2, (2, 512), "f16"))
+    out = far.as_strided((2, 500), (stride, 1), 1024)
+    want, bound = ref.linear_q4_by_steps(x.contiguous(), w.values, w.scales, w.mins)
+    ref.check(ge.linear_q4(x, w, out=out), want, bound)
