@@ -766,13 +766,13 @@ __device__ __forceinline__ void exact_row(const TcParams& p, int id, int row, in
                        p.scale_log2e, lane);
     }
     if (s.piece < 0) {
-        const float inv = inverse_sum(st.l, p.prefix > 0 || rg.y > rg.x);
+        const float inv = st.l != 0.f ? 1.0f : inverse_sum(0.f, p.prefix > 0 || rg.y > rg.x);
         uint32_t* o = reinterpret_cast<uint32_t*>(static_cast<E*>(p.out) + row * p.out_stride + int64_t(head) * D + lane * (D / 32));
 #pragma unroll
         for (int i = 0; i < D / 64; i++) o[i] = float_to_pair<E>(st.o[2 * i] * inv, st.o[2 * i + 1] * inv);
     } else {
         const int64_t at = (int64_t(s.piece) * p.ntok + row) * p.heads + head;
-        if (lane == 0) p.ml[at] = make_float2(st.m, st.l);
+        if (lane == 0) p.ml[at] = make_float2(st.m, -st.l);  // a negative sum: divided by it already
         float2* o = reinterpret_cast<float2*>(p.o + at * D + lane * (D / 32));
 #pragma unroll
         for (int i = 0; i < D / 64; i++) o[i] = make_float2(st.o[2 * i], st.o[2 * i + 1]);
@@ -1351,7 +1351,7 @@ struct MergeParams {
 };
 
 // One CTA of W warps per (row, head): out = sum_c 2^(m_c - m) O_c / sum_c 2^(m_c - m) l_c, m the
-// largest m_c.  Thread c weighs piece c; the warps add every W-th piece each, joined in order.  The
+// largest m_c (O_c l_c in O_c's place for recomputed rows, which come divided, their sums negative).  Thread c weighs piece c; the warps add every W-th piece each, joined in order.  The
 // loads that say whether and how many pieces there are go out together with the pieces' maxima.
 template <typename E, int D, int W>
 __global__ void __launch_bounds__(32 * W) k_causal_merge(MergeParams p) {
@@ -1378,17 +1378,28 @@ __global__ void __launch_bounds__(32 * W) k_causal_merge(MergeParams p) {
 #pragma unroll
     for (int i = 1; i < W; i++) m = fmaxf(m, red_m[i]);
     const float wt = ml.x == -INFINITY ? 0.f : ex2_approx(ml.x - m);  // 0: no visible key, and no row was left
-    if (tid < n) w[tid] = wt;
-    const float l = warp_sum(wt * ml.y);
+    const float part_l = wt * fabsf(ml.y);
+    if (tid < n) w[tid] = ml.y < 0.f ? part_l : wt;  // of a recomputed row, which is a mean, and of a sum
+    const float l = warp_sum(part_l);
     if (lane == 0) red_l[warp] = l;
     __syncthreads();
+    // Weights over the whole sum before they meet the pieces: no partial sum of means passes the largest value.
+    float lt = 0.f;
+#pragma unroll
+    for (int i = 0; i < W; i++) lt += red_l[i];
+    bool sees = p.prefix > 0;
+    if (lt == 0.f && !sees) {
+        const int2 own = simple ? own_range(f->see + (row - row / p.TI * p.TI), f->ks, f->ke, p.window) : rng;
+        sees = own.y > own.x;
+    }
+    const float inv = nan ? NAN : inverse_sum(lt, sees);
     constexpr int P = D / 32;
     float acc[P];
 #pragma unroll
     for (int i = 0; i < P; i++) acc[i] = 0.f;
 #pragma unroll 4
     for (int c = warp; c < n; c += W) {
-        const float wc = w[c];
+        const float wc = w[c] * inv;
         const float2* src = reinterpret_cast<const float2*>(p.o + (c * step + id) * D + lane * P);
 #pragma unroll
         for (int i = 0; i < P / 2; i++) {
@@ -1401,21 +1412,14 @@ __global__ void __launch_bounds__(32 * W) k_causal_merge(MergeParams p) {
     for (int i = 0; i < P; i++) part[warp][lane * P + i] = acc[i];
     __syncthreads();
     if (tid < D / 2) {
-        float lt = 0.f, v[2] = {0.f, 0.f};
+        float v[2] = {0.f, 0.f};
 #pragma unroll
         for (int i = 0; i < W; i++) {
-            lt += red_l[i];
             v[0] += part[i][2 * tid];
             v[1] += part[i][2 * tid + 1];
         }
-        bool sees = p.prefix > 0;
-        if (lt == 0.f && !sees) {
-            const int2 own = simple ? own_range(f->see + (row - row / p.TI * p.TI), f->ks, f->ke, p.window) : rng;
-            sees = own.y > own.x;
-        }
-        const float inv = nan ? NAN : inverse_sum(lt, sees);
         reinterpret_cast<uint32_t*>(static_cast<E*>(p.out) + row * p.out_stride + int64_t(head) * D)[tid] =
-            float_to_pair<E>(v[0] * inv, v[1] * inv);
+            float_to_pair<E>(v[0], v[1]);
     }
 }
 

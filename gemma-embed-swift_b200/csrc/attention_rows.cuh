@@ -1,8 +1,9 @@
 // attention_rows.cuh -- one attention row of ge_attention_causal / ge_attention_prefix by one warp,
 // straight from the definition: lane l holds dims [l * D / 32, (l + 1) * D / 32) of the row, and the
-// running maximum m (log2 units), sum l and unnormalised output of a softmax are kept in fp32
-// over its keys.  It reads the visible keys and values only, so nothing a masked place
-// holds can reach the row.
+// running maximum m (log2 units), sum l and output of a softmax are kept in fp32 over its keys.  The output is
+// a mean of the values so far throughout, weights summing to 1, so that values up to the type's largest
+// do not overflow on the way.  It reads the visible keys and values only, so nothing a masked place holds can
+// reach the row.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -94,18 +95,23 @@ __device__ void row_keys(RowState<D>& s, const T* k, const T* v, int64_t k_strid
             d[b] = warp_sum(d[b]) * scale_log2e;
             m = fmaxf(m, d[b]);
         }
-        const float alpha = s.m == m ? 1.0f : ex2_approx(s.m - m);
+        const float before = s.m == m ? s.l : s.l * ex2_approx(s.m - m);  // the sum so far, under the new maximum
         s.m = m;
-        s.l *= alpha;
+        s.l = before;
 #pragma unroll
-        for (int i = 0; i < D / 32; i++) s.o[i] *= alpha;
+        for (int b = 0; b < B; b++) {
+            // A score of -inf under a finite maximum weighs 0; with no finite score yet it counts nothing either
+            // (m stays -inf).  A NaN score, which the maximum passes over, makes the sum NaN.
+            d[b] = b >= count || (m == -INFINITY && !isnan(d[b])) ? 0.f : ex2_approx(d[b] - m);
+            s.l += d[b];
+        }
+        const float inv = s.l == 0.f ? 0.f : 1.0f / s.l, keep = before * inv;
+#pragma unroll
+        for (int i = 0; i < D / 32; i++) s.o[i] *= keep;
 #pragma unroll
         for (int b = 0; b < B; b++) {
             if (b >= count) break;
-            // A score of -inf under a finite maximum weighs 0; with no finite score yet it counts nothing either
-            // (m stays -inf).  A NaN score, which the maximum passes over, makes the sum NaN.
-            const float p = m == -INFINITY && !isnan(d[b]) ? 0.f : ex2_approx(d[b] - m);
-            s.l += p;
+            const float p = d[b] * inv;
 #pragma unroll
             for (int i = 0; i < W; i++) {
                 const float2 x = pair_to_float<T>(vw[b][i]);

@@ -577,3 +577,44 @@ def test_linear_q4_across_32_bit_offsets(ge, torch):
     out = far.as_strided((2, 500), (stride, 1), 1024)
     want, bound = ref.linear_q4_by_steps(x.contiguous(), w.values, w.scales, w.mins)
     ref.check(ge.linear_q4(x, w, out=out), want, bound)
+
+
+# ---------------------------------------------------------------------------- values up to the type's largest
+@pytest.mark.parametrize("heads,kvh,dim", [(4, 1, 128), (2, 2, 64), (3, 1, 256)])
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+def test_causal_values_at_the_types_limits(ge, torch, heads, kvh, dim, sign):
+    """A row's result is a mean of values: bf16's largest, in columns beside ordinary and tiny ones, do not overflow
+    on the way, in whole items and in pieces."""
+    top = sign * torch.finfo(torch.bfloat16).max
+    for lens in ([40, 300, 7], [2600]):
+        n = sum(lens)
+        q, k, v = (normal(torch, 30 + i, (n, h, dim), "bf16") for i, h in enumerate((heads, kvh, kvh)))
+        v[..., 0] = top                                             # in every key
+        v[..., 1] = torch.where(torch.arange(n, device="cuda") % 2 == 0, top, -top)[:, None]
+        v[::3, :, 2] = top
+        v[..., 3] = 1e-36 * v[..., 4].float()
+        r = ranges_from(0, lens)
+        got = ge.attention_causal(q, k, v, dev(torch, r))
+        want, bound, _ = ref.attention(q, k, v, r, r, 1 / math.sqrt(dim))
+        assert torch.isfinite(got).all()
+        ref.check(got, want, bound)
+
+
+@pytest.mark.parametrize("heads,kvh,dim", [(8, 2, 128), (3, 1, 256), (2, 2, 64)])
+@pytest.mark.parametrize("plen,own", [(6000, 900), (0, 5000), (300, 50)])
+def test_prefix_values_at_the_types_limits(ge, torch, heads, kvh, dim, plen, own):
+    """The same where pieces are joined: the largest values in all pieces, or in one."""
+    top = torch.finfo(torch.bfloat16).max
+    rows = 5
+    q = normal(torch, 1, (rows, heads, dim), "bf16")
+    k, v = normal(torch, 2, (own, kvh, dim), "bf16"), normal(torch, 3, (own, kvh, dim), "bf16")
+    pk, pv = normal(torch, 4, (plen, kvh, dim), "bf16"), normal(torch, 5, (plen, kvh, dim), "bf16")
+    v[..., 0] = pv[..., 0] = top
+    v[..., 1] = -top
+    v[own // 2:, :, 2] = top
+    pv[plen // 3:plen // 2, :, 3] = -top
+    qr, kr = [(i, 1) for i in range(rows)], [(0, own - i) for i in range(rows)]
+    got = ge.attention_prefix(q, k, v, dev(torch, qr), dev(torch, kr), pk, pv)
+    want, bound, _ = ref.attention(q, k, v, qr, kr, 1 / math.sqrt(dim), prefix_k=pk, prefix_v=pv)
+    assert torch.isfinite(got).all()
+    ref.check(got, want, bound)
