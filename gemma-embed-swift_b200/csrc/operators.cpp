@@ -128,7 +128,8 @@ int run_attention(int device, const ge_attention_shape* s, ge::CausalLaunch& a, 
                   bool prefix) {
     int rc = check_shape(s, prefix);
     if (rc) return rc;
-    if (a.ntok < 0 || a.nkv < 0 || a.prefix < 0 || a.nseq < 0 || a.ntok > kMaxRows || a.nkv > kMaxRows || a.prefix > kMaxRows)
+    if (a.ntok < 0 || a.nkv < 0 || a.prefix < 0 || a.nseq < 0 || a.ntok > kMaxRows || a.nkv > kMaxRows || a.prefix > kMaxRows ||
+        a.nseq > kMaxRows)
         return invalid("row and sequence counts must be from 0 to 2^30");
     fill_shape(a, s);
     if (a.ntok == 0 || a.nseq == 0) return GE_OK;

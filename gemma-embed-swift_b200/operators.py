@@ -31,7 +31,7 @@ __all__ = ["attention_causal", "attention_prefix", "linear_q4", "Q4Weight"]
 
 _HERE = contextlib.nullcontext()
 # What the entry points take, checked here where a larger number would reach them as its lowest 32 bits.
-MAX_ROWS, MAX_HEADS, MAX_SEQUENCES, MAX_WINDOW = 1 << 30, 65535, (1 << 31) - 1, (1 << 31) - 1
+MAX_ROWS, MAX_HEADS, MAX_SEQUENCES, MAX_WINDOW = 1 << 30, 65535, 1 << 30, (1 << 31) - 1
 Q4_MAX_ROWS, Q4_MAX_N, Q4_MAX_K = 64, 1 << 30, 65536
 Q4_TYPES = {"Q4_0": 2, "Q4_1": 3}  # GGUF tensor type ids (ge_q4_type)
 
@@ -115,7 +115,7 @@ def _ranges(name: str, t, device: int) -> int:
     if t.dtype not in (torch.int32, torch.uint32) or t.dim() != 2 or t.shape[1] != 2 or not t.is_contiguous():
         raise _invalid(f"{name} must be a contiguous [sequences, 2] int32 tensor of (start, length)")
     if t.shape[0] > MAX_SEQUENCES:
-        raise _invalid(f"{name} names {t.shape[0]} sequences, past 2^31 - 1")
+        raise _invalid(f"{name} names {t.shape[0]} sequences, past 2^30")
     return t.shape[0]
 
 

@@ -416,3 +416,12 @@ def test_the_4bit_bound_sees_what_is_lost(k, group, mins):
             less[:, at // group] = 0
             assert off(lows=less) > 0.25  # some minima are near 0, some sums of x too
     assert off(x=x[[1, 2, 0]]) > 0.9
+
+
+def test_more_sequences_than_32_bit_offsets_reach_are_refused(lib):
+    """(start, length) words are indexed in 32 bits: 2^30 sequences at most."""
+    L = lib.lib()
+    s = shape(lib)
+    for nseq, code in ((1 << 30, 8), ((1 << 30) + 1, 9), ((1 << 31) - 1, 9)):  # 8: the device, which comes later
+        assert L.ge_attention_causal(-1, ctypes.byref(s), Q, K, V, 8, FAKE, nseq, OUT, FAKE, 1 << 30, None) == code
+        assert L.ge_attention_prefix(-1, ctypes.byref(s), Q, 8, K, V, 8, PK, PV, 4, FAKE, FAKE, nseq, OUT, FAKE, 1 << 30, None) == code
