@@ -10,7 +10,8 @@
 // t * G + g of its 128, whatever sequences its rows belong to.  Short texts fill a tile together, and
 // the prefix' tiles serve the rows of many sequences at once.
 //
-// Three kernels, each waiting for the one before (programmatic dependent launch):
+// Kernels, each waiting for the one before (programmatic dependent launch):
+//   k_rows_*        only for more than kPlanSeqs sequences: (lo, hi) of every row ahead of the plan
 //   k_causal_plan   (lo, hi) per row where a tile mixes sequences, per item (below) the disjoint key segments its
 //                   rows see, and the list of work pieces.  A warp plans an item; one CTA up to 64 items, which
 //                   hand their results on through shared memory, else a cluster of 4 or 8.  Items that fill the
@@ -152,6 +153,7 @@ struct PlanParams {
     const uint32_t* q_seqs;
     const uint32_t* kv_seqs;
     int nseq, ntok, nkv, window, T, TI, tiles, kv_heads, prefix_blocks, lmax, sms;
+    bool by_rows;  // rng is there already (k_rows_range)
     Header* head;
     int2 *rng, *segs;
     TileInfo* info;
@@ -184,29 +186,24 @@ __device__ __forceinline__ Seq seq_of(const PlanParams& p, int s) {
     return r;
 }
 
-// Sequences in shared memory (those past kPlanSeqs are read from global memory every time).
-constexpr int kPlanSeqs = 4096, kMaxItemRows = 256, kPlanItems = 64;  // items planned by one CTA
+// Up to kPlanSeqs sequences are kept in shared memory, where every item looks through them all.  Texts of 20 tokens, 4
+// heads of 64 / 32 of 128: 600 of them 23.5 / 68 us so and 27 / 72 by rows (below); 1000 29 / 112 and 31 / 104; 2000
+// 68 / 232 and 44 / 187; 4000 167 / 538 and 71 / 354.
+constexpr int kPlanSeqs = 1024, kMaxItemRows = 256, kPlanItems = 64;  // items planned by one CTA
 struct Seqs {
     int4* range;  // q0, q1, ks, ke
     int* see;
 };
-constexpr size_t plan_smem(int nseq) {
-    return size_t(((nseq < kPlanSeqs ? nseq : kPlanSeqs) + 3) / 4 * 4) * (sizeof(int4) + sizeof(int)) + 32 * 2 * kMaxItemRows * sizeof(int2);
+constexpr size_t plan_smem(int kept) {
+    return size_t((kept + 3) / 4 * 4) * (sizeof(int4) + sizeof(int)) + 32 * 2 * kMaxItemRows * sizeof(int2);
 }
-__device__ __forceinline__ Seq seq_at(const PlanParams& p, const Seqs& seqs, int s) {
-    if (s >= kPlanSeqs) return seq_of(p, s);
+__device__ __forceinline__ Seq seq_at(const Seqs& seqs, int s) {
     const int4 r = seqs.range[s];
     return Seq{r.x, r.y, r.z, r.w, seqs.see[s]};
 }
 // Rows sequence s has among [r0, r1), as offsets from r0: [x, y), empty unless x < y.
 __device__ __forceinline__ int2 rows_within(const PlanParams& p, const Seqs& seqs, int s, int r0, int r1) {
-    int2 q = make_int2(0, 0);
-    if (s < kPlanSeqs) {
-        if (s < p.nseq) q = *reinterpret_cast<const int2*>(&seqs.range[s]);
-    } else if (s < p.nseq) {
-        const Seq r = seq_of(p, s);
-        q = make_int2(r.q0, r.q1);
-    }
+    const int2 q = s < p.nseq ? *reinterpret_cast<const int2*>(&seqs.range[s]) : make_int2(0, 0);
     return make_int2(max(q.x, r0) - r0, min(q.y, r1) - r0);
 }
 
@@ -274,19 +271,128 @@ __device__ void sort_ranges(const int2* rng, int2* seg, int n, int lane) {
         }
 }
 
+// More sequences: the rows' ranges are written to rng before the plan, so that the time is that of the rows and
+// sequences, not of the product of items and sequences (4 heads of 64: 10,000 texts of 20 tokens 0.15 ms, 100,000 of
+// them 1.4, a million of 2 tokens 1.1; looking through all of them took 1.36 ms for 10,000 and 100 times that for
+// each ten times more).  Every sequence s adds (1, s + 1) where it starts and takes
+// it away where it ends, in 64 bits; the sum up to a row then holds how many sequences have it and, where that is
+// one, which.  Rows of several are left out like rows of none.  Sums of whole numbers: the atomics' order is free.
+constexpr int kRowBlock = 1024;  // rows of a CTA
+__device__ __forceinline__ uint64_t* row_marks(const PlanParams& p) { return reinterpret_cast<uint64_t*>(p.rng); }
+__device__ __forceinline__ uint64_t* block_sums(const PlanParams& p) { return reinterpret_cast<uint64_t*>(p.segs); }
+
+__global__ void __launch_bounds__(256) k_rows_clear(PlanParams p) {
+    pdl_wait();
+    pdl_launch();
+    for (int row = int(blockIdx.x) * 256 + int(threadIdx.x); row < p.ntok; row += int(gridDim.x) * 256) row_marks(p)[row] = 0;
+}
+
+__global__ void __launch_bounds__(256) k_rows_mark(PlanParams p) {
+    pdl_wait();
+    pdl_launch();
+    unsigned long long* marks = reinterpret_cast<unsigned long long*>(row_marks(p));
+    for (int s = int(blockIdx.x) * 256 + int(threadIdx.x); s < p.nseq; s += int(gridDim.x) * 256) {
+        const Seq q = seq_of(p, s);
+        if (q.q0 >= q.q1) continue;
+        const unsigned long long one = (1ull << 32) + uint32_t(s + 1);
+        atomicAdd(&marks[q.q0], one);
+        if (q.q1 < p.ntok) atomicAdd(&marks[q.q1], 0ull - one);
+    }
+}
+
+// The exclusive sum of v over the CTA's 32 W threads, and in `all` the whole.
+template <int W>
+__device__ __forceinline__ uint64_t block_scan(uint64_t v, uint64_t& all) {
+    __shared__ uint64_t warps[W];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    uint64_t inc = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const uint64_t u = __shfl_up_sync(0xffffffffu, inc, o);
+        if (lane >= o) inc += u;
+    }
+    if (lane == 31) warps[warp] = inc;
+    __syncthreads();
+    uint64_t before = 0;
+    all = 0;
+#pragma unroll
+    for (int w = 0; w < W; w++) {
+        if (w < warp) before += warps[w];
+        all += warps[w];
+    }
+    __syncthreads();
+    return before + inc - v;
+}
+
+__device__ __forceinline__ void load_marks(const PlanParams& p, int row, uint64_t (&v)[4]) {
+#pragma unroll
+    for (int i = 0; i < 4; i++) v[i] = row + i < p.ntok ? row_marks(p)[row + i] : 0;
+}
+
+__global__ void __launch_bounds__(256) k_rows_sum(PlanParams p) {
+    pdl_wait();
+    pdl_launch();
+    uint64_t v[4], all;
+    load_marks(p, int(blockIdx.x) * kRowBlock + int(threadIdx.x) * 4, v);
+    block_scan<8>(v[0] + v[1] + v[2] + v[3], all);
+    if (threadIdx.x == 0) block_sums(p)[blockIdx.x] = all;
+}
+
+__global__ void __launch_bounds__(1024) k_rows_scan(PlanParams p) {
+    pdl_wait();
+    pdl_launch();
+    const int blocks = (p.ntok + kRowBlock - 1) / kRowBlock;
+    uint64_t carry = 0, all;
+    for (int b0 = 0; b0 < blocks; b0 += 1024) {
+        const int b = b0 + int(threadIdx.x);
+        const uint64_t at = carry + block_scan<32>(b < blocks ? block_sums(p)[b] : 0, all);
+        if (b < blocks) block_sums(p)[b] = at;
+        carry += all;
+    }
+}
+
+__global__ void __launch_bounds__(256) k_rows_range(PlanParams p) {
+    pdl_wait();
+    pdl_launch();
+    const int row = int(blockIdx.x) * kRowBlock + int(threadIdx.x) * 4;
+    uint64_t v[4], all;
+    load_marks(p, row, v);
+    uint64_t at = block_sums(p)[blockIdx.x] + block_scan<8>(v[0] + v[1] + v[2] + v[3], all);
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        at += v[i];
+        if (row + i >= p.ntok) break;
+        int2 rg = make_int2(0, -1);
+        if (at >> 32 == 1) {
+            const Seq q = seq_of(p, int(uint32_t(at)) - 1);
+            rg = own_range(q.see + (row + i - q.q0), q.ks, q.ke, p.window);
+        }
+        p.rng[row + i] = rg;
+    }
+}
+
 // One item, by one warp: rng and seg are the warp's own shared memory.  Its segments and (mixed) rows go to the
 // workspace.
 __device__ TileInfo plan_item(const PlanParams& p, const Seqs& seqs, int2* rng, int2* seg, int t, int lane) {
     const int r0 = t * p.TI, n = min(p.TI, p.ntok - r0);
     TileInfo f{};
     bool any = false;
+    const int scan = p.by_rows ? 0 : p.nseq;
+    if (p.by_rows) {
 #pragma unroll 1
-    for (int s0 = 0; s0 < p.nseq; s0 += 32) {
+        for (int i = lane; i < p.TI; i += 32) {
+            rng[i] = i < n ? p.rng[r0 + i] : make_int2(0, -1);
+            any |= rng[i].y >= 0;
+        }
+        __syncwarp();
+    }
+#pragma unroll 1
+    for (int s0 = 0; s0 < scan; s0 += 32) {
         const int2 in = rows_within(p, seqs, s0 + lane, r0, r0 + n);
         any |= in.x < in.y;
         const unsigned whole = __ballot_sync(0xffffffffu, in.x == 0 && in.y == n);
         if (whole) {  // the item lies inside one sequence
-            const Seq q = seq_at(p, seqs, s0 + __ffs(whole) - 1);
+            const Seq q = seq_at(seqs, s0 + __ffs(whole) - 1);
             const int see = q.see + (r0 - q.q0), n0 = min(p.T, n);
             const int2 a = own_range(see, q.ks, q.ke, p.window), b = own_range(see + n0 - 1, q.ks, q.ke, p.window);
             const int2 e = own_range(see + n - 1, q.ks, q.ke, p.window);
@@ -304,15 +410,15 @@ __device__ TileInfo plan_item(const PlanParams& p, const Seqs& seqs, int2* rng, 
     }
     if (!__any_sync(0xffffffffu, any)) return f;  // live 0: no row of a sequence, no work
 #pragma unroll 1
-    for (int i = lane; i < p.TI; i += 32) rng[i] = make_int2(0, -1);
+    for (int i = p.by_rows ? p.TI : lane; i < p.TI; i += 32) rng[i] = make_int2(0, -1);
     __syncwarp();
 #pragma unroll 1
-    for (int s0 = 0; s0 < p.nseq; s0 += 32) {
+    for (int s0 = 0; s0 < scan; s0 += 32) {
         const int2 in = rows_within(p, seqs, s0 + lane, r0, r0 + n);
         unsigned m = __ballot_sync(0xffffffffu, in.x < in.y);
         if (__popc(m) > 4) {  // many short ones: a lane each
             if (in.x < in.y) {
-                const Seq q = seq_at(p, seqs, s0 + lane);
+                const Seq q = seq_at(seqs, s0 + lane);
 #pragma unroll 1
                 for (int i = in.x; i < in.y; i++) rng[i] = own_range(q.see + (r0 + i - q.q0), q.ks, q.ke, p.window);
             }
@@ -321,7 +427,7 @@ __device__ TileInfo plan_item(const PlanParams& p, const Seqs& seqs, int2* rng, 
             while (m) {
                 const int src = __ffs(m) - 1;
                 m &= m - 1;
-                const Seq q = seq_at(p, seqs, s0 + src);
+                const Seq q = seq_at(seqs, s0 + src);
                 const int x = __shfl_sync(0xffffffffu, in.x, src), y = __shfl_sync(0xffffffffu, in.y, src);
 #pragma unroll 1
                 for (int i = x + lane; i < y; i += 32) rng[i] = own_range(q.see + (r0 + i - q.q0), q.ks, q.ke, p.window);
@@ -358,7 +464,7 @@ __device__ TileInfo plan_item(const PlanParams& p, const Seqs& seqs, int2* rng, 
         p.segs[int64_t(t) * p.TI + i] = seg[i];
     }
 #pragma unroll 1
-    for (int i = lane; i < n; i += 32) p.rng[r0 + i] = rng[i];
+    for (int i = p.by_rows ? n : lane; i < n; i += 32) p.rng[r0 + i] = rng[i];
     if (f.nseg > 0) f.pos = seg[0].x, f.end = seg[0].y;
     f.nblk = __reduce_add_sync(0xffffffffu, nblk) + p.prefix_blocks;
     f.pieces = 1;
@@ -373,7 +479,7 @@ __global__ void __launch_bounds__(1024) k_causal_plan(PlanParams p) {
     __shared__ TileInfo s_info[kPlanItems];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int ctas = int(gridDim.x);
-    const int kept = min(p.nseq, kPlanSeqs), room = (kept + 3) / 4 * 4;
+    const int kept = p.by_rows ? 0 : p.nseq, room = (kept + 3) / 4 * 4;
     const Seqs seqs{reinterpret_cast<int4*>(plan_shared), reinterpret_cast<int*>(plan_shared + size_t(room) * sizeof(int4))};
     int2* rng = reinterpret_cast<int2*>(seqs.see + room) + warp * 2 * kMaxItemRows;
     hist[tid] = 0;
@@ -1483,13 +1589,26 @@ cudaError_t launch_causal(const CausalLaunch& a, cudaStream_t stream) {
     const Sizes s = sizes_of(a);
     const Layout l = layout_of(a, s);
     const int window = std::min(a.window, 1 << 30);  // no range is longer
+    const bool by_rows = a.nseq > kPlanSeqs;
     PlanParams pp{a.q_seqs, a.kv_seqs, a.nseq, a.ntok, a.nkv, window, s.T, s.TI, s.tiles, a.kv_heads,
-                  (a.prefix + kKeys - 1) / kKeys, s.lmax, a.num_sms, l.head, l.rng, l.segs, l.info, l.work};
+                  (a.prefix + kKeys - 1) / kKeys, s.lmax, a.num_sms, by_rows, l.head, l.rng, l.segs, l.info, l.work};
     // A warp plans an item; up to 8 CTAs share them.
     const int ctas = s.tiles <= kPlanItems ? 1 : s.tiles <= 128 ? 4 : 8;
     static std::atomic<uint64_t> devices{0};
     cudaError_t e = allow_smem(k_causal_plan, int(plan_smem(kPlanSeqs)), devices);
-    if (e == cudaSuccess) e = launch_pdl(k_causal_plan, unsigned(ctas), 1024, plan_smem(a.nseq), stream, ctas, pp);
+    if (by_rows) {
+        const unsigned blocks = unsigned((a.ntok + kRowBlock - 1) / kRowBlock);
+        const auto some = [&](int n) { return unsigned(std::min((n + 255) / 256, 8 * a.num_sms)); };
+        const auto next = [&](void (*kern)(PlanParams), unsigned grid, unsigned threads) {
+            if (e == cudaSuccess) e = launch_pdl(kern, grid, threads, 0, stream, 1, pp);
+        };
+        next(k_rows_clear, some(a.ntok), 256);
+        next(k_rows_mark, some(a.nseq), 256);
+        next(k_rows_sum, blocks, 256);
+        next(k_rows_scan, 1, 1024);
+        next(k_rows_range, blocks, 256);
+    }
+    if (e == cudaSuccess) e = launch_pdl(k_causal_plan, unsigned(ctas), 1024, plan_smem(by_rows ? 0 : a.nseq), stream, ctas, pp);
     if (e != cudaSuccess) return e;
     return a.bf16 ? launch_e<__nv_bfloat16>(a, s, l, stream) : launch_e<__half>(a, s, l, stream);
 }

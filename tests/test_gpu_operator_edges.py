@@ -618,3 +618,70 @@ def test_prefix_values_at_the_types_limits(ge, torch, heads, kvh, dim, plen, own
     want, bound, _ = ref.attention(q, k, v, qr, kr, 1 / math.sqrt(dim), prefix_k=pk, prefix_v=pv)
     assert torch.isfinite(got).all()
     ref.check(got, want, bound)
+
+
+# ---------------------------------------------------------------------------- thousands of sequences
+def shuffled(rng, lens, gap=0):
+    """Ranges of these lengths in memory order, named in another."""
+    r = []
+    at = 0
+    for n in lens:
+        r.append((at, int(n)))
+        at += int(n) + gap
+    return [r[i] for i in rng.permutation(len(r))], max(a + n for a, n in r)
+
+
+@pytest.mark.parametrize("heads,kvh,dim,dtype", SHAPES)
+@pytest.mark.parametrize("window,gap", [(0, 0), (3, 2)])
+def test_thousands_of_sequences_every_key_once(ge, torch, heads, kvh, dim, dtype, window, gap):
+    """Short texts, empty ones among them, beside a few long ones, in no order."""
+    rng = np.random.default_rng(7)
+    lens = rng.integers(0, 4, 1500)
+    lens[[100, 900]] = 700, 300
+    r, total = shuffled(rng, lens, gap)
+    each_key(ge, torch, heads, kvh, dim, dtype, r, r, total, window=window, keys=list(range(0, total, 5)))
+
+
+@pytest.mark.parametrize("heads,kvh,dim,dtype", SHAPES)
+def test_thousands_of_last_tokens_every_key_once(ge, torch, heads, kvh, dim, dtype):
+    rng = np.random.default_rng(8)
+    kr, nkv = shuffled(rng, rng.integers(0, 6, 1300), 1)
+    kr[7], kr[8] = kr[1200], (3, 500)
+    qr, ntok = shuffled(rng, rng.integers(0, 3, 1300))
+    each_key(ge, torch, heads, kvh, dim, dtype, qr, kr, nkv + 600, 130, keys=list(range(0, 130 + nkv, 7)))
+
+
+def test_thousands_of_ranges_that_share_rows_or_leave_the_tensors(ge, torch):
+    """Rows of one range alone are right, rows of none untouched, whatever the others name: the same range many
+    times, ranges within ranges, starts and ends past the last row."""
+    n, rng = 4000, np.random.default_rng(9)
+    q, k, v = (normal(torch, 31 + i, (n, h, 64), "f16") for i, h in enumerate((2, 1, 1)))
+    r = [(int(i) * 2, 2) for i in rng.permutation(900)]              # [0, 1800): two rows each
+    r += [(2000, 40)] * 300 + [(2100, 200), (2150, 10), (2200, 300)] + [(2900 + i, 3) for i in range(50)]
+    r += [(3000, 500), (3900, 1 << 30), (4000, 5), (1 << 30, 7), (-3, 2), (3700, 0), (3701, 0)]
+    r = [r[i] for i in rng.permutation(len(r))]
+    out = torch.full_like(q, 7.0)
+    ge.attention_causal(q, k, v, dev(torch, r), out=out)
+    cover = torch.zeros(n, dtype=torch.int32, device="cuda")
+    cut = [(s, min(m, n - s)) for s, m in r if 0 <= s < n and m > 0]
+    for s, m in cut:
+        cover[s:s + m] += 1
+    assert (out[cover == 0] == 7.0).all() and (cover > 1).sum() > 100
+    want, bound, _ = ref.attention(q, k, v, cut, cut, 0.125)  # shared rows hold the last range's: not looked at
+    alone = cover == 1
+    ref.check(out[alone], want[alone], bound[alone])
+
+
+def test_time_of_many_sequences_grows_with_their_number(ge, torch):
+    """300,000 single tokens: a few ms, where a look through all sequences for every tile would take 100 times that."""
+    n = 300_000
+    q, k = normal(torch, 1, (n, 4, 64), "f16"), normal(torch, 2, (n, 1, 64), "f16")
+    s = torch.stack([torch.arange(n, device="cuda"), torch.ones(n, device="cuda")], 1).int()
+    for _ in range(2):
+        a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+        a.record()
+        got = ge.attention_causal(q, k, k, s)
+        b.record()
+        torch.cuda.synchronize()
+    assert torch.equal(got, k.expand(-1, 4, -1))
+    assert a.elapsed_time(b) < 50
