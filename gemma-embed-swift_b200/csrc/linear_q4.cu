@@ -57,7 +57,7 @@ static_assert(kSmem <= 227 * 1024, "shared memory");
 struct Q4Params {
     const void* x;
     int64_t x_stride;
-    int rows, n, k, group;
+    int rows, n, k;
     const uint8_t* values;
     const __half *scales, *mins;
     void* out;
@@ -440,7 +440,7 @@ cudaError_t launch_t(const Q4Launch& a, cudaStream_t stream) {
     static std::atomic<uint64_t> devices{0};
     cudaError_t e = allow_smem(k_linear_q4<T, NB, kMins, kPer>, kSmem, devices);
     if (e != cudaSuccess) return e;
-    Q4Params p{a.x, a.x_stride, a.rows, a.n, a.k, a.group, a.values, a.scales, a.mins, a.out, a.out_stride, 0, 0, 0, 0};
+    Q4Params p{a.x, a.x_stride, a.rows, a.n, a.k, a.values, a.scales, a.mins, a.out, a.out_stride, 0, 0, 0, 0};
     p.tiles = (a.n + 15) / 16;
     const int grid = std::min(p.tiles, a.num_sms);
     p.R = std::min(kWarps, (p.tiles + grid - 1) / grid);
