@@ -48,11 +48,12 @@
 // What bounds it: on long sequences the softmax beside the products (of a tile's block, about 1350 cycles for a warp
 // that has the scheduler to itself, for 1090 of the tensor core); on texts of a few hundred tokens the turn from one
 // item to the next (Q's load, the first softmax and the epilogue have nothing beside them).  Measured:
-//   2 x 4096 tokens, 32 heads of 128 on 8      0.239 ms, 1150 TFLOP/s
-//   4 x 4096 tokens, 4 heads of 256 on 2       0.119 ms, 1155 TFLOP/s
-//   2 x 8192 tokens, 12 heads of 64            0.285 ms,  722 TFLOP/s (a 64 wide S costs half the product, the
+//   2 x 4096 tokens, 32 heads of 128 on 8      0.243 ms, 1131 TFLOP/s
+//   4 x 8000 tokens, 32 heads of 128 on 8       2.04 ms, 1028 TFLOP/s (runs long enough for the power limit's clock)
+//   4 x 4096 tokens, 4 heads of 256 on 2       0.122 ms, 1131 TFLOP/s
+//   2 x 8192 tokens, 12 heads of 64            0.282 ms,  731 TFLOP/s (a 64 wide S costs half the product, the
 //                                              same softmax)
-//   64 x 300 tokens, 32 heads of 128 on 8      0.129 ms,  367 TFLOP/s; 394 MB of tensors, 3.0 TB/s
+//   64 x 300 tokens, 32 heads of 128 on 8      0.125 ms,  379 TFLOP/s; 394 MB of tensors, 3.1 TB/s
 #include <stdlib.h>
 
 #include <algorithm>
@@ -707,8 +708,8 @@ __device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t parity, int* e
     } while (!__all_sync(0xffffffffu, mbar_test(bar, parity)));
     return true;
 }
-// kWaitLimitNs at 2 GHz, and more over many keys: a warp recomputes 32 rows over all of them at most, at about 0.25 us
-// for a key of a row (8 heads of 128 wide, 8192 rows that all see an infinite value: 69 ms, 0.13 ms without it); 1 us
+// kWaitLimitNs at 2 GHz, and more over many keys: a warp recomputes 32 rows over all of them at most, at about 0.1 us
+// for a key of a row (8 heads of 128 wide, 8192 rows that all see an infinite value: 27 ms, 0.13 ms without it); 1 us
 // is allowed.
 // GE_ATTENTION_WAIT_NS in the environment of the process' first call stands in its place (0: whatever is not there
 // at the first look has run out).

@@ -15,7 +15,8 @@
 // 32-bit reads of a fragment hit 32 banks).  The lane's word of a 32-weight group holds the group's
 // elements 8 c .. 8 c + 7; their nibbles come out as pairs (0, 4), (1, 5), (2, 6), (3, 7), which x is
 // stored to match: the products' k order is permuted the same on both sides.  A stage's scales and minima
-// come along in its slot.
+// come along in its slot, by cp.async where k is a multiple of the stage and the planes start on 16 bytes; else by
+// loads the warp waits for (below).
 // x is staged for all warps in two buffers of kXElems elements (all of it where it fits, so that the
 // warps never meet while they stream).
 //
@@ -26,10 +27,13 @@
 // (16384 x 8192, 1 row: 7 tiles at once 21.4 us, 4 + 3 24.7, one by one 34.5; 28671 x 8192, 12 rows: 13 at once 64,
 // 7 + 6 67, 5 + 5 + 3 76), and sharing a chunk's stages of all tiles out evenly, up to two tiles a warp, won nothing
 // either (23.3 and 67).  Measured, weights from memory:
-//   16384 x 8192, groups of 32, 1 row, fp16              21.4 us, 3.5 TB/s
-//   28671 x 8192, groups of 128 with mins, 12 rows, bf16   64 us, 2.0 TB/s
-//   41003 x 4096, groups of 32, 4 rows, fp16               33 us, 2.9 TB/s
-//    2304 x 768, groups of 32, 1 row, fp16                3.0 us (a launch and one trip to memory)
+//   16384 x 8192, groups of 32, 1 row, fp16              22.0 us, 3.4 TB/s
+//   16384 x 8224, the same, k no multiple of 256         32.0 us, 2.4 TB/s
+//   28671 x 8192, groups of 128 with mins, 12 rows, bf16   63 us, 2.0 TB/s
+//   28671 x 8320, the same, k no multiple of 256           71 us, 1.8 TB/s
+//   41003 x 4096, groups of 32, 4 rows, fp16               33 us, 2.8 TB/s
+//    2304 x 768, groups of 32, 1 row, fp16                3.1 us (a launch and one trip to memory)
+//     768 x 1152, the same                                3.6 us
 #include <algorithm>
 
 #include "attention_rows.cuh"
@@ -471,7 +475,7 @@ cudaError_t launch_e(const Q4Launch& a, cudaStream_t stream) {
     if (a.rows <= 16) return launch_m<T, 2>(a, stream);
     if (a.rows <= kRows) return launch_m<T, 4>(a, stream);
     // More rows in two halves, each over all weights (the second from the L2 cache where they fit): sums of 64 rows
-    // spill, and their x leaves room for one stage at a time, which only one part of k works on (16384 x 4096, groups of
+    // spill into local memory in earnest (those of 32 store 32 to 52 bytes a thread, next to nothing), and their x leaves room for one stage at a time, which only one part of k works on (16384 x 4096, groups of
     // 64 with mins, bf16, 64 rows: 115 us at once, 72 in halves; 33 rows of groups of 32: 78 and 45).
     Q4Launch half = a;
     half.rows = (a.rows + 1) / 2;
