@@ -1486,7 +1486,10 @@ __global__ void __launch_bounds__(32 * W) k_causal_merge(MergeParams p) {
     for (int i = 1; i < W; i++) m = fmaxf(m, red_m[i]);
     const float wt = ml.x == -INFINITY ? 0.f : ex2_approx(ml.x - m);  // 0: no visible key, and no row was left
     const float part_l = wt * fabsf(ml.y);
-    if (tid < n) w[tid] = ml.y < 0.f ? part_l : wt;  // of a recomputed row, which is a mean, and of a sum
+    // Of a recomputed row, which is a mean, and of a sum; -1: no score of the piece is finite, and its row is 0.  Any
+    // other meets its weight, also one that is 0 beside a far larger one, and so does a recomputed row without a finite
+    // score: 0 times an infinite value is NaN, in pieces as in one row.
+    if (tid < n) w[tid] = signbit(ml.y) ? part_l : ml.x == -INFINITY ? -1.f : wt;
     const float l = warp_sum(part_l);
     if (lane == 0) red_l[warp] = l;
     __syncthreads();
@@ -1506,11 +1509,12 @@ __global__ void __launch_bounds__(32 * W) k_causal_merge(MergeParams p) {
     for (int i = 0; i < P; i++) acc[i] = 0.f;
 #pragma unroll 4
     for (int c = warp; c < n; c += W) {
-        const float wc = w[c] * inv;
+        const bool none = w[c] < 0.f;
+        const float wc = (none ? 0.f : w[c]) * inv;
         const float2* src = reinterpret_cast<const float2*>(p.o + (c * step + id) * D + lane * P);
 #pragma unroll
         for (int i = 0; i < P / 2; i++) {
-            const float2 v = wc != 0.f ? src[i] : make_float2(0.f, 0.f);
+            const float2 v = none ? make_float2(0.f, 0.f) : src[i];
             acc[2 * i] = fmaf(wc, v.x, acc[2 * i]);
             acc[2 * i + 1] = fmaf(wc, v.y, acc[2 * i + 1]);
         }

@@ -685,3 +685,28 @@ def test_time_of_many_sequences_grows_with_their_number(ge, torch):
         torch.cuda.synchronize()
     assert torch.equal(got, k.expand(-1, 4, -1))
     assert a.elapsed_time(b) < 50
+
+
+@pytest.mark.parametrize("heads,kvh,dim", [(4, 1, 128), (2, 2, 64), (3, 1, 256)])
+@pytest.mark.parametrize("plen,own", [(3000, 500), (0, 2500), (40, 60)])
+@pytest.mark.parametrize("weight", ["underflows", "none"])
+def test_no_weight_times_an_infinite_value(ge, torch, heads, kvh, dim, plen, own, weight):
+    """A key with an infinite value whose weight is 0 -- far below another's, or a score of -infinity -- gives NaN in
+    that column, wherever the keys are cut, and the others' mean in the other columns."""
+    total, dtype = plen + own, torch.float16
+    q = torch.zeros((3, heads, dim), dtype=dtype, device="cuda")
+    q[..., 0] = 1.0
+    ks, vs = normal(torch, 1, (total, kvh, dim), "f16"), normal(torch, 2, (total, kvh, dim), "f16")
+    ks[..., 0] = -2000.0  # e^-4000 beside a key of 2000
+    ks[total - 5, :, 0] = 2000.0
+    for at in (0, total // 3, total - 1):
+        k, v = ks.clone(), vs.clone()
+        if weight == "none":
+            k[at, :, 0] = -math.inf
+        v[at, :, 7] = math.inf
+        qr, kr = [(i, 1) for i in range(3)], [(0, own)] * 3
+        got = ge.attention_prefix(q, k[plen:], v[plen:], dev(torch, qr), dev(torch, kr), k[:plen], v[:plen], scale=1.0)
+        want = vs[total - 5].repeat_interleave(heads // kvh, 0)[None].expand(3, -1, -1)
+        assert torch.isnan(got[..., 7]).all()
+        rest = [c for c in range(dim) if c != 7]
+        assert torch.equal(got[..., rest], want[..., rest])
