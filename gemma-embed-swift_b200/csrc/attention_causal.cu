@@ -43,7 +43,7 @@
 // segment never meets the product.  Keys masked for some rows of a tile only (later tokens, other
 // sequences) do meet it, with P = 0: where their values are infinite or NaN, 0 x V leaves NaN in rows that
 // must not see it, and the epilogue recomputes rows with non-finite outputs from the definition
-// (attention_rows.cuh), which reads a row's own keys only.
+// (attention_rows.cuh), which reads a row's own keys only, as it does rows with scores past kFar.
 //
 // What bounds it: on long sequences the softmax beside the products (of a tile's block, about 1350 cycles for a warp
 // that has the scheduler to itself, for 1090 of the tensor core); on texts of a few hundred tokens the turn from one
@@ -67,6 +67,9 @@ namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kGrow = 8.0f;  // log2 units a row's maximum may grow before it is moved
+// Row maxima (log2 units) from which on a row is recomputed: scores times scale are rounded there to steps that an
+// exponent feels (1/8; from 2^23 on 1, where 2^(S scale - m) of the largest key itself would be 0 or infinite).
+constexpr float kFar = 1048576.0f;
 constexpr int kKeys = 128;     // keys of a block
 // Probabilities are held times 2^kRaise: fp16's smallest numbers then stand for probabilities of 2^-31, not 2^-24,
 // so that many small ones beside a large one keep their sum (P stays within 2^(kGrow + 7), below fp16's largest).
@@ -1353,7 +1356,7 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1)
             const int64_t at = (int64_t(s.piece) * p.ntok + row) * p.heads + head;  // of a partial row
             const float inv = s.piece >= 0 ? 1.0f : inverse_sum(l, p.prefix > 0 || rg.y > rg.x);
             if (in && s.piece >= 0) p.ml[at] = make_float2(m - kRaise<E>, l);
-            bool bad = false;
+            bool bad = fabsf(m) >= kFar && m != -INFINITY;
             // Whole rows of head dim 128 leave as boxes through shared memory, where all of the warp's belong to a sequence:
             // the threads do not wait for the stores (64 texts of 300 tokens, 32 heads: 129 us, by stores 140).  Head dim
             // 64 gains nothing (88 us both ways), 256 loses with its four warps (148 us for 141).

@@ -710,3 +710,33 @@ def test_no_weight_times_an_infinite_value(ge, torch, heads, kvh, dim, plen, own
         assert torch.isnan(got[..., 7]).all()
         rest = [c for c in range(dim) if c != 7]
         assert torch.equal(got[..., rest], want[..., rest])
+
+
+@pytest.mark.parametrize("heads,kvh,dim", [(4, 1, 128), (2, 2, 64), (3, 1, 256)])
+@pytest.mark.parametrize("dtype,size", [("f16", 60000.0), ("bf16", 3e9), ("bf16", 1e18), ("f16", 3000.0)])
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+def test_scores_whose_steps_an_exponent_feels(ge, torch, heads, kvh, dim, dtype, size, sign):
+    """Scores of 10^7 to 10^36, all positive or all negative: the largest of a row holds all the weight, in whole
+    items and where the keys are cut."""
+    for lens in ([40, 200, 7], [2300]):
+        n = sum(lens)
+        g = torch.Generator(device="cuda").manual_seed(n)
+        q, v = torch.zeros((n, heads, dim), device="cuda"), normal(torch, 3, (n, kvh, dim), dtype)
+        q[..., 1] = size
+        k = torch.zeros((n, kvh, dim), device="cuda")
+        # From size / 2 on in steps of size / 128: equal, or far apart.
+        k[..., 1] = sign * size * (64 + torch.randint(0, 30, (n, kvh), generator=g, device="cuda")) / 128
+        q, k = q.to(v.dtype), k.to(v.dtype)
+        r = ranges_from(0, lens)
+        got = ge.attention_causal(q, k, v, dev(torch, r), scale=1.0).double()
+        group, u = heads // kvh, torch.finfo(v.dtype).eps / 2
+        for s, m in r:
+            for h in range(heads):
+                score = k[s:s + m, h // group, 1].double()
+                top = torch.cummax(score, 0).values
+                at = (score[None] == top[:, None]) & (torch.arange(m, device="cuda")[None] <= torch.arange(m, device="cuda")[:, None])
+                w = at.double() / at.sum(1, keepdim=True)
+                vals = v[s:s + m, h // group].double()
+                err = (got[s:s + m, h] - w @ vals).abs()
+                # Weights of 1 / ties in 32 bits, then the result's rounding.
+                assert (err <= (u + 2.0 ** -18) * (w @ vals.abs()) + 2.0 ** -24).all()
