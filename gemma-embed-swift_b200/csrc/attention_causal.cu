@@ -1394,7 +1394,7 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1)
                         uint32_t w[4];
 #pragma unroll
                         for (int f = 0; f < 4; f++)
-                            w[f] = float_to_pair<E>(__uint_as_float(o[8 * e + 2 * f]) * inv, __uint_as_float(o[8 * e + 2 * f + 1]) * inv);
+                            w[f] = mean_to_pair<E>(__uint_as_float(o[8 * e + 2 * f]) * inv, __uint_as_float(o[8 * e + 2 * f + 1]) * inv);
                         *reinterpret_cast<uint4*>(buf + lane * 64 + ((e ^ ((lane >> 1) & 3)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
                     }
                     fence_proxy_async_smem();
@@ -1410,7 +1410,7 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1)
                         uint32_t w[8];
 #pragma unroll
                         for (int f = 0; f < 8; f++)
-                            w[f] = float_to_pair<E>(__uint_as_float(o[16 * e + 2 * f]) * inv, __uint_as_float(o[16 * e + 2 * f + 1]) * inv);
+                            w[f] = mean_to_pair<E>(__uint_as_float(o[16 * e + 2 * f]) * inv, __uint_as_float(o[16 * e + 2 * f + 1]) * inv);
                         if (p.out_wide) {
                             store32(dst + 8 * e, w);
                         } else {
@@ -1532,8 +1532,11 @@ __global__ void __launch_bounds__(32 * W) k_causal_merge(MergeParams p) {
             v[0] += part[i][2 * tid];
             v[1] += part[i][2 * tid + 1];
         }
-        reinterpret_cast<uint32_t*>(static_cast<E*>(p.out) + row * p.out_stride + int64_t(head) * D)[tid] =
-            float_to_pair<E>(v[0], v[1]);
+        uint32_t pair = mean_to_pair<E>(v[0], v[1]);
+        const uint32_t plain = float_to_pair<E>(v[0], v[1]);  // of infinite values
+        if (isinf(v[0])) pair = (pair & 0xffff0000u) | (plain & 0xffffu);
+        if (isinf(v[1])) pair = (pair & 0xffffu) | (plain & 0xffff0000u);
+        reinterpret_cast<uint32_t*>(static_cast<E*>(p.out) + row * p.out_stride + int64_t(head) * D)[tid] = pair;
     }
 }
 

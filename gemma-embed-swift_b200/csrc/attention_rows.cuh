@@ -36,6 +36,23 @@ __device__ __forceinline__ uint32_t float_to_pair<__nv_bfloat16>(float a, float 
     return *reinterpret_cast<const uint32_t*>(&h);
 }
 
+// The same, finite values past the type's largest as that: a mean whose weights were rounded may pass it, the values'
+// own mean cannot.
+template <typename T>
+__device__ __forceinline__ uint32_t mean_to_pair(float a, float b);
+template <>
+__device__ __forceinline__ uint32_t mean_to_pair<__half>(float a, float b) {
+    uint32_t r;
+    asm("cvt.rn.satfinite.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
+    return r;
+}
+template <>
+__device__ __forceinline__ uint32_t mean_to_pair<__nv_bfloat16>(float a, float b) {
+    uint32_t r;
+    asm("cvt.rn.satfinite.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
+    return r;
+}
+
 template <int D>
 struct RowState {
     static constexpr int kPer = D / 32;  // dims of one lane

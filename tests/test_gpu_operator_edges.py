@@ -740,3 +740,26 @@ def test_scores_whose_steps_an_exponent_feels(ge, torch, heads, kvh, dim, dtype,
                 err = (got[s:s + m, h] - w @ vals).abs()
                 # Weights of 1 / ties in 32 bits, then the result's rounding.
                 assert (err <= (u + 2.0 ** -18) * (w @ vals.abs()) + 2.0 ** -24).all()
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("heads,kvh,dim", [(4, 1, 128), (2, 2, 64), (3, 1, 256), (6, 2, 128)])
+@pytest.mark.parametrize("lens", [[1, 2, 3, 40, 90], [700, 33], [2600]])
+def test_means_of_the_largest_value_are_finite(ge, torch, dtype, heads, kvh, dim, lens):
+    """Every key has the type's largest (or lowest) value in some columns: so has every row, whatever its weights
+    were rounded to."""
+    n = sum(lens)
+    top = torch.finfo(dt(torch, dtype)).max
+    q, k, v = (normal(torch, 30 + i, (n, h, dim), dtype) for i, h in enumerate((heads, kvh, kvh)))
+    v[..., 5], v[..., 6] = top, -top
+    r = ranges_from(0, lens)
+    got = ge.attention_causal(q, k, v, dev(torch, r)).double()
+    u = torch.finfo(dt(torch, dtype)).eps / 2
+    assert torch.isfinite(got).all()
+    # A probability's rounding, exponentials and sums.
+    assert ((got[..., 5] - top).abs() <= (2 * u + 2.0 ** -18) * top).all() and ((got[..., 6] + top).abs() <= (2 * u + 2.0 ** -18) * top).all()
+    want, bound, _ = ref.attention(q, k, v, r, r, 1 / math.sqrt(dim))
+    ref.check(got, want, bound)
+    v[0, :, 5] = math.inf  # an infinity stays one
+    got = ge.attention_causal(q, k, v, dev(torch, r))
+    assert torch.isinf(got[:lens[0], :, 5]).all() and torch.isfinite(got[lens[0]:]).all()
