@@ -1461,7 +1461,8 @@ struct MergeParams {
 };
 
 // One CTA of W warps per (row, head): out = sum_c 2^(m_c - m) O_c / sum_c 2^(m_c - m) l_c, m the
-// largest m_c (O_c l_c in O_c's place for recomputed rows, which come divided, their sums negative).  Thread c weighs piece c; the warps add every W-th piece each, joined in order.  The
+// largest m_c (O_c l_c in O_c's place for recomputed rows, which come divided, their sums negative).
+// Thread c weighs piece c; the warps add every W-th piece each, joined in order.  The
 // loads that say whether and how many pieces there are go out together with the pieces' maxima.
 template <typename E, int D, int W>
 __global__ void __launch_bounds__(32 * W) k_causal_merge(MergeParams p) {

@@ -475,8 +475,9 @@ cudaError_t launch_e(const Q4Launch& a, cudaStream_t stream) {
     if (a.rows <= 16) return launch_m<T, 2>(a, stream);
     if (a.rows <= kRows) return launch_m<T, 4>(a, stream);
     // More rows in two halves, each over all weights (the second from the L2 cache where they fit): sums of 64 rows
-    // spill into local memory in earnest (those of 32 store 32 to 52 bytes a thread, next to nothing), and their x leaves room for one stage at a time, which only one part of k works on (16384 x 4096, groups of
-    // 64 with mins, bf16, 64 rows: 115 us at once, 72 in halves; 33 rows of groups of 32: 78 and 45).
+    // spill into local memory in earnest (those of 32 store 32 to 52 bytes a thread, next to nothing), and their x leaves
+    // room for one stage at a time, which only one part of k works on (16384 x 4096, groups of 64 with mins, bf16, 64
+    // rows: 115 us at once, 72 in halves; 33 rows of groups of 32: 78 and 45).
     Q4Launch half = a;
     half.rows = (a.rows + 1) / 2;
     cudaError_t e = launch_e<T>(half, stream);

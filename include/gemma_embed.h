@@ -524,8 +524,8 @@ GE_API int ge_attention_workspace(int32_t device_ordinal, const ge_attention_sha
  * at ntok and may be empty; query rows that two ranges share hold unspecified values.  Rows of `out` in
  * no range are left as they were; `out` must not overlap the inputs.  Scores, sums and maxima are fp32,
  * probabilities are rounded to dtype before their product with v, the result once to dtype.  What masked
- * places hold never reaches a row; infinite or NaN values among the keys near a row cost time, since such
- * rows are computed again one by one. */
+ * places hold never reaches a row; infinite or NaN values among the keys near a row and scores (times scale)
+ * past 10^6 cost time, since such rows are computed again one by one (up to 200 times a call's where all are). */
 GE_API int ge_attention_causal(int32_t device_ordinal, const ge_attention_shape* shape, const void* d_q, const void* d_k,
                                const void* d_v, int32_t ntok, const uint32_t* d_seqs, int32_t nseq, void* d_out,
                                void* workspace, int64_t workspace_bytes, void* stream);

@@ -763,3 +763,35 @@ def test_means_of_the_largest_value_are_finite(ge, torch, dtype, heads, kvh, dim
     v[0, :, 5] = math.inf  # an infinity stays one
     got = ge.attention_causal(q, k, v, dev(torch, r))
     assert torch.isinf(got[:lens[0], :, 5]).all() and torch.isfinite(got[lens[0]:]).all()
+
+
+@pytest.mark.parametrize("ntok", [1, 5, 1023, 1024, 1025, 3000])
+def test_thousands_of_sequences_over_few_rows(ge, torch, ntok):
+    """More sequences than rows: nearly all are empty, or lie past the last row."""
+    q, k, v = (normal(torch, 31 + i, (ntok, h, 64), "f16") for i, h in enumerate((2, 1, 1)))
+    out = torch.full_like(q, 7.0)
+    ge.attention_causal(q, k, v, torch.zeros((5000, 2), dtype=torch.int32, device="cuda"), out=out)
+    assert (out == 7.0).all()
+    s = torch.zeros((5000, 2), dtype=torch.int32, device="cuda")
+    s[1200:2400, 0], s[1200:2400, 1] = ntok, 9
+    s[4999] = torch.tensor([ntok // 2, ntok - ntok // 2])
+    ge.attention_causal(q, k, v, s, out=out)
+    r = [(ntok // 2, ntok - ntok // 2)]
+    want, bound, touched = ref.attention(q, k, v, r, r, 0.125)
+    ref.check(out[touched], want[touched], bound[touched])
+    assert (out[~touched] == 7.0).all()
+
+
+@pytest.mark.parametrize("heads,kvh,dim", [(65535, 65535, 64), (65408, 511, 64), (6000, 6000, 256), (12800, 100, 128)])
+def test_many_heads_few_rows(ge, torch, heads, kvh, dim):
+    """The most heads there may be, with one of their own and with 128 to a KV head."""
+    n = 3
+    q, k, v = (normal(torch, 31 + i, (n, h, dim), "bf16") for i, h in enumerate((heads, kvh, kvh)))
+    r = [(0, 1), (1, 2)]
+    got = ge.attention_causal(q, k, v, dev(torch, r))
+    want, bound, _ = ref.attention(q, k, v, r, r, 1 / math.sqrt(dim))
+    ref.check(got, want, bound)
+    pk = normal(torch, 5, (150, kvh, dim), "bf16")
+    got = ge.attention_prefix(q, k, v, dev(torch, r), dev(torch, r), pk, pk)
+    want, bound, _ = ref.attention(q, k, v, r, r, 1 / math.sqrt(dim), prefix_k=pk, prefix_v=pk)
+    ref.check(got, want, bound)
