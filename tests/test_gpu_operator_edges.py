@@ -795,3 +795,25 @@ def test_many_heads_few_rows(ge, torch, heads, kvh, dim):
     got = ge.attention_prefix(q, k, v, dev(torch, r), dev(torch, r), pk, pk)
     want, bound, _ = ref.attention(q, k, v, r, r, 1 / math.sqrt(dim), prefix_k=pk, prefix_v=pk)
     ref.check(got, want, bound)
+
+
+def test_thousands_of_sequences_in_a_graph(ge, torch):
+    """Captured, and replayed with other ranges in the same tensor, bit for bit as outside."""
+    rng = np.random.default_rng(4)
+    lens = rng.integers(0, 5, 2500)
+    lens[3] = 900
+    r, n = shuffled(rng, lens)
+    other, m = shuffled(rng, lens[::-1].copy())
+    assert n == m
+    q, k, v = (normal(torch, 31 + i, (n, h, 128), "bf16") for i, h in enumerate((8, 2, 2)))
+    s = dev(torch, r)
+    wants = [ge.attention_causal(q, k, v, dev(torch, t)) for t in (r, other)]
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        got = ge.attention_causal(q, k, v, s)
+    for t, want in ((r, wants[0]), (other, wants[1]), (r, wants[0])):
+        s.copy_(dev(torch, t))
+        got.fill_(7.0)
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got, want)
