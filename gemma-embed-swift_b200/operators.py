@@ -7,8 +7,9 @@ ge_attention_prefix and ge_linear_q4 of include/gemma_embed.h).  Every call enqu
 tensors' device -- and returns without synchronising; it may be captured into a CUDA graph.  A stream
 other than the current one has to be behind the work that fills the inputs; their memory is not reused
 before the call's work there has ended.  A wait inside the attention kernels that ran out (2 s and more,
-which no argument can bring about) leaves NaN in the rows it kept from being finished.  There is no derivative: inputs that require a gradient are
-refused while gradients are recorded, dual tensors of forward-mode differentiation always.
+which no argument can bring about) leaves NaN in the rows it kept from being finished.  There is no
+derivative: inputs that require a gradient are refused while gradients are recorded, dual tensors of
+forward-mode differentiation always.
 
     out = attention_causal(q, k, v, seqs)               # q [T, H, D], k and v [T, KV, D]
     last = attention_prefix(q, k, v, q_seqs, kv_seqs, prefix_k, prefix_v)
@@ -318,7 +319,8 @@ class Q4Weight:
 
 def linear_q4(x, weight: Q4Weight, out=None, stream=None):
     """x [rows, k] times the 4-bit weights (ge_linear_q4): out [rows, n] in x's type (float16 or
-    bfloat16), for 0 to 64 rows; a given `out` must not overlap x or the weights.  x's rows may be a column range of a wider tensor."""
+    bfloat16), for 0 to 64 rows.  x's rows may be a column range of a wider tensor; a given `out` must not
+    overlap x or the weights."""
     torch = _torch()[0]
     values, mins = weight.values, weight.mins
     device = _on_device("x", x)
